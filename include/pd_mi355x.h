@@ -667,6 +667,72 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
                         const float* delta, const float* V, const float* U, const float* w_sq_norms, float scale,
                         const float* d_loss, float* dV, float* dU, void* stream);
 
+/* ---- causal attention over packed sequences -------------------------------------------
+ * The attention of a language-model target around its decomposed projections
+ * (pd/attention.py:26-130), for tokens of several sequences in one axis. q [rows, n_head,
+ * head_dim], k and v [rows, n_kv_head, head_dim] in `dtype` (bf16 or fp32) with the given
+ * row and head strides in elements (last axis dense; strides whole 16-byte words, tensors
+ * 16-byte aligned: views of one projection's output will do). Query head h reads key head
+ * h / (n_head / n_kv_head). head_dim: a multiple of 8 up to 128. offsets int32
+ * [n_seq + 1] in device memory, not decreasing: sequence s is rows [offsets[s],
+ * offsets[s+1]) (empty ones allowed); row i of it sees rows offsets[s] .. i. Rows that no
+ * sequence holds (before offsets[0], from offsets[n_seq] on) get zeros (fill = 1) or are
+ * left as they were (fill = 0); what they, other sequences and later rows hold, NaN and
+ * infinities included, reaches no other row. Offsets outside [0, rows] or out of order
+ * give wrong rows but no access outside the tensors.
+ *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, fp32 statistics;
+ *   stats fp32 [n_head, rows] (nullable) log2 of the rows' softmax sums, for the backward.
+ * The backward gives dq [rows, n_head, head_dim], dk and dv [rows, n_kv_head, head_dim]
+ * (summed over the query heads that share a key head) from the forward's out and stats and
+ * d_out [rows, n_head, head_dim]. out, d_out, dq, dk, dv are dense. Bit-identical from
+ * call to call. */
+int pd_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                            const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
+                            int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
+                            void* out, float* stats, void* stream);
+size_t pd_packed_attention_bwd_workspace_size(int64_t rows, int n_head);
+int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                            const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
+                            int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
+                            const void* out, const float* stats, const void* d_out, void* dq, void* dk, void* dv,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- layer norm -------------------------------------------------------------------------
+ * The norm of targets and CI functions whose blocks centre their activations (the stack
+ * steps hold the RMS form inside). x, y, d_y, d_x [rows, d] in `dtype` (bf16 or fp32);
+ * weight and bias fp32 [d], NULL = 1 and 0.
+ *   y = (x - mean) / sqrt(var + eps) weight + bias, mean and (biased) var over d;
+ *   stats fp32 [rows, 3] (nullable): the mean as a base and its distance from it, and
+ *   1 / sqrt(var + eps), for the backward.
+ * The backward: d_x; d_weight = sum_rows d_y (x - mean) / sqrt(var + eps) and d_bias =
+ * sum_rows d_y, fp32 [d], overwritten; each of the three may be NULL. workspace: needed
+ * with d_weight or d_bias. Fixed-order sums: bit-identical from call to call. */
+int pd_layer_norm_fwd(const void* x, int dtype, int64_t rows, int64_t d, const float* weight, const float* bias,
+                      float eps, void* y, float* stats, void* stream);
+size_t pd_layer_norm_bwd_workspace_size(int64_t rows, int64_t d);
+int pd_layer_norm_bwd(const void* x, const void* d_y, int dtype, int64_t rows, int64_t d, const float* weight,
+                      const float* stats, void* d_x, float* d_weight, float* d_bias, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---- KL to a teacher's top logits --------------------------------------------------------
+ * pd_kl with the clean side kept as k logits per position (pd/core/losses.py:80-92 is the
+ * form over all of them). z [rows, vocab] in `dtype` (bf16 or fp32) the masked logits; top
+ * [rows, k] (top_dtype bf16 or fp32) the clean logits listed, idx [rows, k] (idx_bits 32
+ * or 64) their vocabulary indices in any order; an index outside [0, vocab) is padding and
+ * its entry absent, repeated indices add their probabilities. With q = softmax(z /
+ * temperature):
+ *   clean_lse NULL: p = softmax(top / temperature) over the listed entries,
+ *     kl = sum p (log p - log q); no entry at all: kl = 0;
+ *   clean_lse fp32 [rows] (the clean row's logsumexp of logits / temperature): p =
+ *     exp(top / temperature - clean_lse), and the mass they leave (below 2^-20: none) is
+ *     compared as one entry with the mass q gives all entries not listed.
+ * kl fp32 [rows] (nullable); grad [rows, vocab] in `dtype` (nullable) = row_weight (fp32
+ * [rows], NULL = 1) times d kl / d z; a row of weight 0 gets zeros whatever it holds.
+ * vocab up to 2^19, k up to 1024. */
+int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void* top, int top_dtype, const void* idx,
+              int idx_bits, int k, const float* clean_lse, float temperature, const float* row_weight, float* kl,
+              void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,493 @@
+// Layer norm over the last axis, forward and backward, with the reduction of the weight's
+// and bias's gradients.
+//
+//   mean = sum(x) / d, var = sum((x - mean)^2) / d, rstd = 1 / sqrt(var + eps)
+//   xh = (x - mean) rstd, y = xh w + b
+//   backward, a = dy w: dx = rstd (a - mean(a) - xh mean(a xh)), dw = sum_rows dy xh,
+//   db = sum_rows dy
+//
+// Memory bound: the forward reads x and writes y, the backward reads x and dy and writes dx.
+// A row is held in registers by NT threads of E elements each, so it is read once; blocks
+// walk over rows with the next row's loads issued before this row's reductions. A wave's
+// residuals around its own mean give the variance and the mean's own rounding; waves are
+// joined relative to the first one's mean (the base), and the mean is kept as base + delta
+// (stats: base, delta, rstd), so an offset far above the spread costs no digits and a row
+// takes one barrier. Weight and bias gradients are summed over a block's rows in registers (columns
+// are fixed per thread), written as one partial row per block and added in block order by a
+// second kernel: results are the same on every run.
+#include <initializer_list>
+#include <type_traits>
+
+#include "pd_common.hpp"
+
+namespace pd {
+namespace {
+
+constexpr int LN_MAX_D = 16384;   // largest row held in registers
+constexpr int LN_BLOCKS = 1024;   // most blocks of a launch that walks over rows
+constexpr int LN_GRAD_BLOCKS = 512;  // the same where each block leaves a partial row of gradients
+
+struct LnStat {
+  float base, delta, rstd;  // mean = base + delta
+};
+
+template <typename T, int VEC>
+struct Pack {
+  T v[VEC];
+};
+template <>
+struct alignas(16) Pack<bf16_t, 8> {
+  bf16_t v[8];
+};
+template <>
+struct alignas(16) Pack<float, 4> {
+  float v[4];
+};
+
+// This thread's columns: chunk c covers columns VEC (tid + c NT) .. + VEC.
+template <typename T, int VEC, int NT, int CH>
+__device__ inline void ln_load(const T* __restrict__ row, int tid, int d, Pack<T, VEC> (&p)[CH]) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = VEC * (tid + c * NT);
+    if (col < d) p[c] = *(const Pack<T, VEC>*)(row + col);
+    else p[c] = Pack<T, VEC>{};
+  }
+}
+template <int VEC, int NT, int CH>
+__device__ inline void ln_load_param(const float* __restrict__ w, float none, int tid, int d, float (&v)[CH * VEC]) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = VEC * (tid + c * NT);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[c * VEC + e] = w && col < d ? w[col + e] : none;
+  }
+}
+template <typename T>
+__device__ inline float ln_f(T v);
+template <>
+__device__ inline float ln_f<float>(float v) {
+  return v;
+}
+template <>
+__device__ inline float ln_f<bf16_t>(bf16_t v) {
+  return bf16_to_f32(v);
+}
+template <typename T, int VEC>
+__device__ inline Pack<T, VEC> ln_pack(const float* v) {
+  Pack<T, VEC> p;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    if constexpr (sizeof(T) == 2) p.v[e] = f32_to_bf16(v[e]);
+    else p.v[e] = v[e];
+  }
+  return p;
+}
+
+// Columns below d that wave w of the row holds.
+template <int VEC, int NT, int CH>
+__device__ inline int ln_wave_count(int w, int d) {
+  int n = 0;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) n += min(max(d - VEC * (64 * w + c * NT), 0), 64 * VEC);
+  return n;
+}
+
+// Forward. Grid: row groups; a block holds RPB rows at a time (one per wave where NT = 64).
+template <typename T, int VEC, int NT, int CH>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_fwd(const T* __restrict__ x, int64_t rows, int d,
+                                                               const float* __restrict__ w,
+                                                               const float* __restrict__ b, float eps,
+                                                               T* __restrict__ y, LnStat* __restrict__ stats) {
+  constexpr int E = CH * VEC, RPB = NT == 64 ? 4 : 1, NW = NT / 64;
+  __shared__ float4 part[2][NW];
+  const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x, wv = tid >> 6, lane = threadIdx.x & 63;
+  int64_t r = (int64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0);
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  if (NT == 64 && r >= rows) return;
+  float wr[E], br[E];
+  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr);
+  ln_load_param<VEC, NT, CH>(b, 0.f, tid, d, br);
+  Pack<T, VEC> cur[CH], nxt[CH];
+  ln_load<T, VEC, NT, CH>(x + r * d, tid, d, cur);
+  const int nw = ln_wave_count<VEC, NT, CH>(wv, d);
+  for (int it = 0; r < rows; r += step, it ^= 1) {
+    if (r + step < rows) ln_load<T, VEC, NT, CH>(x + (r + step) * d, tid, d, nxt);
+    float v[E], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += v[i] = ln_f<T>(cur[i / VEC].v[i % VEC]);  // columns past d hold 0
+    s = wave_sum(s);
+    float base = nw ? s / (float)nw : 0.f, q = 0.f, res = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (VEC * (tid + (i / VEC) * NT) < d) {
+        const float t = v[i] - base;
+        res += t;
+        q = fmaf(t, t, q);
+      }
+    }
+    q = wave_sum(q);
+    res = wave_sum(res);
+    float delta, var;
+    if constexpr (NT == 64) {
+      delta = res / (float)d;
+      var = fmaxf(q / (float)d - delta * delta, 0.f);
+    } else {
+      if (lane == 0) part[it][wv] = make_float4(base, res, q, (float)nw);
+      __syncthreads();  // the other buffer is rewritten behind the next row's barrier
+      base = part[it][0].x;
+      delta = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) delta += fmaf(part[it][i].w, part[it][i].x - base, part[it][i].y);
+      delta /= (float)d;
+      float Q = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {  // sum (t - u)^2 = q - 2 u res + n u^2, u = (base - own) + delta
+        const float4 p = part[it][i];
+        const float u = (base - p.x) + delta;
+        if (p.w > 0.f) Q += p.z + u * fmaf(p.w, u, -2.f * p.y);
+      }
+      var = fmaxf(Q / (float)d, 0.f);
+    }
+    const float rstd = 1.f / sqrtf(var + eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = VEC * (tid + c * NT);
+      if (col >= d) continue;
+      float o[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int i = c * VEC + e;
+        o[e] = fmaf(((v[i] - base) - delta) * rstd, wr[i], br[i]);
+      }
+      *(Pack<T, VEC>*)(y + r * d + col) = ln_pack<T, VEC>(o);
+    }
+    if (stats && tid == 0) stats[r] = LnStat{base, delta, rstd};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) cur[c] = nxt[c];
+  }
+}
+
+// Backward. dwdb [gridDim.x][2][d]: each block's sums of dy xh and dy over its rows (NULL:
+// not wanted).
+template <typename T, int VEC, int NT, int CH>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
+                                                               int64_t rows, int d, const float* __restrict__ w,
+                                                               const LnStat* __restrict__ stats, T* __restrict__ dx,
+                                                               float* __restrict__ dwdb) {
+  constexpr int E = CH * VEC, RPB = NT == 64 ? 4 : 1, NW = NT / 64;
+  __shared__ float2 part[2][NW];
+  extern __shared__ float cols[];  // [2][d] where NT = 64 and gradients are wanted
+  const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x, wv = tid >> 6, lane = threadIdx.x & 63;
+  int64_t r = (int64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0);
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  float wr[E];
+  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr);
+  float dw[E], db[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.f;
+  Pack<T, VEC> cx[CH], cg[CH], nx[CH], ng[CH];
+  LnStat st = {}, nst = {};
+  if (r < rows) {
+    ln_load<T, VEC, NT, CH>(x + r * d, tid, d, cx);
+    ln_load<T, VEC, NT, CH>(dy + r * d, tid, d, cg);
+    st = stats[r];
+  }
+  const float invd = 1.f / (float)d;
+  for (int it = 0; r < rows; r += step, it ^= 1) {
+    if (r + step < rows) {
+      ln_load<T, VEC, NT, CH>(x + (r + step) * d, tid, d, nx);
+      ln_load<T, VEC, NT, CH>(dy + (r + step) * d, tid, d, ng);
+      nst = stats[r + step];
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int col = VEC * (tid + (i / VEC) * NT);
+      const float g = ln_f<T>(cg[i / VEC].v[i % VEC]);  // 0 past d
+      const float xh = ((ln_f<T>(cx[i / VEC].v[i % VEC]) - st.base) - st.delta) * st.rstd;
+      if (col < d) {
+        const float a = g * wr[i];
+        s1 += a;
+        s2 = fmaf(a, xh, s2);
+        dw[i] = fmaf(g, xh, dw[i]);
+        db[i] += g;
+      }
+    }
+    if (dx) {
+      s1 = wave_sum(s1);
+      s2 = wave_sum(s2);
+      if constexpr (NT > 64) {
+        if (lane == 0) part[it][wv] = make_float2(s1, s2);
+        __syncthreads();
+        s1 = s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) s1 += part[it][i].x, s2 += part[it][i].y;
+      }
+      const float m1 = s1 * invd, m2 = s2 * invd;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = VEC * (tid + c * NT);
+        if (col >= d) continue;
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int i = c * VEC + e;
+          const float xh = ((ln_f<T>(cx[c].v[e]) - st.base) - st.delta) * st.rstd;
+          const float a = ln_f<T>(cg[c].v[e]) * wr[i];
+          o[e] = st.rstd * (a - m1 - xh * m2);
+        }
+        *(Pack<T, VEC>*)(dx + r * d + col) = ln_pack<T, VEC>(o);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) cx[c] = nx[c], cg[c] = ng[c];
+    st = nst;
+  }
+  if (!dwdb) return;
+  float* dst = dwdb + (int64_t)blockIdx.x * 2 * d;
+  if constexpr (NT == 64) {  // the four waves' sums in wave order
+    for (int wave = 0; wave < RPB; ++wave) {
+      if ((int)(threadIdx.x >> 6) == wave) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int col = VEC * (tid + (i / VEC) * NT) + i % VEC;
+          if (col < d) {
+            cols[col] = wave ? cols[col] + dw[i] : dw[i];
+            cols[d + col] = wave ? cols[d + col] + db[i] : db[i];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 2 * d; i += 256) dst[i] = cols[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int col = VEC * (tid + (i / VEC) * NT) + i % VEC;
+      if (col < d) dst[col] = dw[i], dst[d + col] = db[i];
+    }
+  }
+}
+
+// dw, db = the partial rows [n][2][d] added in order: 16 columns by 16 slices of the rows
+// per block, the slices' sums joined in order. n = 0 (no rows) gives zeros.
+__global__ __launch_bounds__(256) void k_ln_cols(const float* __restrict__ part, int n, int64_t d,
+                                                 float* __restrict__ dw, float* __restrict__ db) {
+  __shared__ float red[16][17];
+  const int c = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  const int per = (n + 15) / 16, lo = min(sl * per, n), hi = min(lo + per, n);
+  red[sl][c] = col < 2 * d && hi > lo ? pd_ordered_sum(part + lo * 2 * d + col, hi - lo, 2 * d) : 0.f;
+  __syncthreads();
+  if (sl || col >= 2 * d) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += red[i][c];
+  float* out = col < d ? dw : db;
+  if (out) out[col < d ? col : col - d] = s;
+}
+
+// ---------------------------------------------------------------- rows beyond the registers
+// One block of 1024 threads per row; the row is read again for each of its passes.
+__device__ inline float2 block_sum2(float a, float b, float2* red) {
+  a = wave_sum(a), b = wave_sum(b);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(a, b);
+  __syncthreads();
+  a = b = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a += red[i].x, b += red[i].y;
+  return make_float2(a, b);
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ln_fwd_long(const T* __restrict__ x, int64_t d, const float* __restrict__ w,
+                                                      const float* __restrict__ b, float eps, T* __restrict__ y,
+                                                      LnStat* __restrict__ stats) {
+  __shared__ float2 red[16];
+  const T* row = x + (int64_t)blockIdx.x * d;
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < d; i += 1024) s += load_f<T>(row, i);
+  const float base = block_sum2(s, 0.f, red).x / (float)d;
+  float q = 0.f, res = 0.f;
+  for (int64_t i = threadIdx.x; i < d; i += 1024) {
+    const float t = load_f<T>(row, i) - base;
+    res += t;
+    q = fmaf(t, t, q);
+  }
+  const float2 rq = block_sum2(res, q, red);
+  const float delta = rq.x / (float)d;
+  const float rstd = 1.f / sqrtf(fmaxf(rq.y / (float)d - delta * delta, 0.f) + eps);
+  for (int64_t i = threadIdx.x; i < d; i += 1024)
+    store_f<T>(y + (int64_t)blockIdx.x * d, i,
+               fmaf(((load_f<T>(row, i) - base) - delta) * rstd, w ? w[i] : 1.f, b ? b[i] : 0.f));
+  if (stats && threadIdx.x == 0) stats[blockIdx.x] = LnStat{base, delta, rstd};
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_ln_dx_long(const T* __restrict__ x, const T* __restrict__ dy, int64_t d,
+                                                     const float* __restrict__ w, const LnStat* __restrict__ stats,
+                                                     T* __restrict__ dx) {
+  __shared__ float2 red[16];
+  const int64_t r = blockIdx.x;
+  const LnStat st = stats[r];
+  float s1 = 0.f, s2 = 0.f;
+  for (int64_t i = threadIdx.x; i < d; i += 1024) {
+    const float a = load_f<T>(dy + r * d, i) * (w ? w[i] : 1.f);
+    s1 += a;
+    s2 = fmaf(a, ((load_f<T>(x + r * d, i) - st.base) - st.delta) * st.rstd, s2);
+  }
+  const float2 s = block_sum2(s1, s2, red);
+  const float m1 = s.x / (float)d, m2 = s.y / (float)d;
+  for (int64_t i = threadIdx.x; i < d; i += 1024) {
+    const float a = load_f<T>(dy + r * d, i) * (w ? w[i] : 1.f);
+    store_f<T>(dx + r * d, i, st.rstd * (a - m1 - ((load_f<T>(x + r * d, i) - st.base) - st.delta) * st.rstd * m2));
+  }
+}
+
+// Columns 256 blockIdx.x .. of slice blockIdx.y of the rows, into partial row blockIdx.y.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ln_dw_long(const T* __restrict__ x, const T* __restrict__ dy, int64_t rows,
+                                                    int64_t d, const LnStat* __restrict__ stats,
+                                                    float* __restrict__ dwdb) {
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = (rows + gridDim.y - 1) / gridDim.y, lo = per * blockIdx.y;
+  const int64_t hi = lo + per < rows ? lo + per : rows;
+  if (col >= d) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t r = lo; r < hi; ++r) {
+    const float g = load_f<T>(dy, r * d + col);
+    const LnStat st = stats[r];
+    dw = fmaf(g, ((load_f<T>(x, r * d + col) - st.base) - st.delta) * st.rstd, dw);
+    db += g;
+  }
+  dwdb[(int64_t)blockIdx.y * 2 * d + col] = dw;
+  dwdb[(int64_t)blockIdx.y * 2 * d + d + col] = db;
+}
+
+constexpr int LN_LONG_SLICES = 16;
+
+// Threads and elements a row is held in: the smallest of the built forms that covers d.
+// F is called with (NT, E) as integral constants.
+template <typename F>
+void ln_form(int64_t d, F&& f) {
+  using std::integral_constant;
+  if (d <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  else if (d <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+  else if (d <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
+  else if (d <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
+  else if (d <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
+  else f(integral_constant<int, 512>{}, integral_constant<int, 32>{});
+}
+
+int64_t ln_blocks(int64_t rows, int64_t d, int64_t most) {
+  const int64_t groups = d <= 2048 ? cdiv(rows, 4) : rows;
+  return groups < most ? groups : most;
+}
+int64_t ln_partials(int64_t rows, int64_t d) {
+  if (d > LN_MAX_D) return rows < LN_LONG_SLICES ? rows : LN_LONG_SLICES;
+  return ln_blocks(rows, d, LN_GRAD_BLOCKS);
+}
+bool ln_aligned(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (p && ((uintptr_t)p & 15)) return false;
+  return true;
+}
+
+int ln_check(const char* what, int dtype, int64_t rows, int64_t d, std::initializer_list<const void*> needed) {
+  if (dtype != PD_DTYPE_F32 && dtype != PD_DTYPE_BF16)
+    return fail(PD_EUNSUPPORTED, std::string(what) + ": dtype must be fp32 or bf16");
+  if (rows < 0 || d <= 0) return fail(PD_EINVAL, std::string(what) + ": rows >= 0 and d >= 1");
+  if (rows > 0x7FFFFFFF || d > 0x7FFFFFFF / 2) return fail(PD_EUNSUPPORTED, std::string(what) + ": rows or d too large");
+  if (rows)
+    for (const void* p : needed)
+      if (!p) return fail(PD_EINVAL, std::string(what) + ": null pointer");
+  return PD_OK;
+}
+
+template <typename T>
+void ln_fwd(const T* x, int64_t rows, int64_t d, const float* w, const float* b, float eps, T* y, LnStat* stats,
+            hipStream_t s) {
+  if (d > LN_MAX_D) {
+    hipLaunchKernelGGL(k_ln_fwd_long<T>, dim3((unsigned)rows), dim3(1024), 0, s, x, d, w, b, eps, y, stats);
+    return;
+  }
+  const unsigned grid = (unsigned)ln_blocks(rows, d, LN_BLOCKS);
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = d % V == 0 && ln_aligned({x, y});
+  ln_form(d, [&](auto nt, auto e) {
+    constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+    const dim3 block(NT < 256 ? 256 : NT);
+    if (vec) hipLaunchKernelGGL((k_ln_fwd<T, V, NT, E / V>), dim3(grid), block, 0, s, x, rows, (int)d, w, b, eps, y, stats);
+    else hipLaunchKernelGGL((k_ln_fwd<T, 1, NT, E>), dim3(grid), block, 0, s, x, rows, (int)d, w, b, eps, y, stats);
+  });
+}
+
+template <typename T>
+void ln_bwd(const T* x, const T* dy, int64_t rows, int64_t d, const float* w, const LnStat* stats, T* dx, float* part,
+            hipStream_t s) {
+  if (d > LN_MAX_D) {
+    if (dx) hipLaunchKernelGGL(k_ln_dx_long<T>, dim3((unsigned)rows), dim3(1024), 0, s, x, dy, d, w, stats, dx);
+    if (part)
+      hipLaunchKernelGGL(k_ln_dw_long<T>, dim3((unsigned)cdiv(d, 256), (unsigned)ln_partials(rows, d)), dim3(256), 0, s,
+                         x, dy, rows, d, stats, part);
+    return;
+  }
+  const unsigned grid = (unsigned)(part ? ln_partials(rows, d) : ln_blocks(rows, d, LN_BLOCKS));
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = d % V == 0 && ln_aligned({x, dy, dx});
+  ln_form(d, [&](auto nt, auto e) {
+    constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
+    const dim3 block(NT < 256 ? 256 : NT);
+    const size_t lds = NT == 64 && part ? (size_t)2 * d * sizeof(float) : 0;
+    if (vec) hipLaunchKernelGGL((k_ln_bwd<T, V, NT, E / V>), dim3(grid), block, lds, s, x, dy, rows, (int)d, w, stats, dx, part);
+    else hipLaunchKernelGGL((k_ln_bwd<T, 1, NT, E>), dim3(grid), block, lds, s, x, dy, rows, (int)d, w, stats, dx, part);
+  });
+}
+
+}  // namespace
+}  // namespace pd
+
+using namespace pd;
+
+extern "C" {
+
+int pd_layer_norm_fwd(const void* x, int dtype, int64_t rows, int64_t d, const float* weight, const float* bias,
+                      float eps, void* y, float* stats, void* stream) {
+  if (int rc = ln_check("pd_layer_norm_fwd", dtype, rows, d, {x, y})) return rc;
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(PD_EINVAL, "pd_layer_norm_fwd: eps must be finite and >= 0");
+  if (!rows) return PD_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PD_DTYPE_F32) ln_fwd<float>((const float*)x, rows, d, weight, bias, eps, (float*)y, (LnStat*)stats, s);
+  else ln_fwd<bf16_t>((const bf16_t*)x, rows, d, weight, bias, eps, (bf16_t*)y, (LnStat*)stats, s);
+  return check_launch("pd_layer_norm_fwd");
+}
+
+size_t pd_layer_norm_bwd_workspace_size(int64_t rows, int64_t d) {
+  if (rows <= 0 || d <= 0) return 0;
+  return (size_t)ln_partials(rows, d) * 2 * (size_t)d * sizeof(float);
+}
+
+int pd_layer_norm_bwd(const void* x, const void* d_y, int dtype, int64_t rows, int64_t d, const float* weight,
+                      const float* stats, void* d_x, float* d_weight, float* d_bias, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  if (int rc = ln_check("pd_layer_norm_bwd", dtype, rows, d, {x, d_y, stats})) return rc;
+  const bool params = d_weight || d_bias;
+  if (params && rows && (!workspace || workspace_bytes < pd_layer_norm_bwd_workspace_size(rows, d)))
+    return fail(PD_EWORKSPACE, "pd_layer_norm_bwd: workspace");
+  hipStream_t s = (hipStream_t)stream;
+  float* part = params ? (float*)workspace : nullptr;
+  if (rows && (d_x || params)) {
+    if (dtype == PD_DTYPE_F32)
+      ln_bwd<float>((const float*)x, (const float*)d_y, rows, d, weight, (const LnStat*)stats, (float*)d_x, part, s);
+    else
+      ln_bwd<bf16_t>((const bf16_t*)x, (const bf16_t*)d_y, rows, d, weight, (const LnStat*)stats, (bf16_t*)d_x, part, s);
+  }
+  if (params)
+    hipLaunchKernelGGL(k_ln_cols, dim3((unsigned)cdiv(2 * d, 16)), dim3(256), 0, s, part,
+                       rows ? (int)ln_partials(rows, d) : 0, d, d_weight, d_bias);
+  return check_launch("pd_layer_norm_bwd");
+}
+
+}  // extern "C"

@@ -15,6 +15,8 @@ Mirrors:
   clean frozen (`pd/core/losses.py:80-92`).
 - `streamed_position_kl` / `streamed_kl_per_position` — the same KL over the factored
   lm-head edge, streamed over vocab chunks (`pd/targets/losses.py:101-170`).
+- `top_logits_position_kl` / `top_logits_kl` — the KL of `categorical_kl_from_logits` with
+  the clean side kept as its top logits (no reference counterpart).
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ from dataclasses import dataclass
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from param_decomp_amd import _lib as L
 from param_decomp_amd import ops
@@ -286,3 +289,46 @@ def streamed_position_kl(act_masked: torch.Tensor, head_masked: torch.Tensor, ac
 def streamed_kl_per_position(act_masked, head_masked, act_clean, head_clean, n_chunks: int) -> torch.Tensor:
     """`streamed_kl_per_position` (`targets/losses.py:166-170`): the mean over positions."""
     return streamed_position_kl(act_masked, head_masked, act_clean, head_clean, n_chunks).mean()
+
+
+class _TopLogitsKL(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, masked, top, indices, clean_lse, temperature):
+        ctx.save_for_backward(masked, top, indices, clean_lse)
+        ctx.temperature = temperature
+        return ops.top_logits_kl(masked, top, indices, clean_lse=clean_lse, temperature=temperature)[0]
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        masked, top, indices, clean_lse = ctx.saved_tensors
+        _, grad = ops.top_logits_kl(masked, top, indices, clean_lse=clean_lse, temperature=ctx.temperature,
+                                    row_weight=g.contiguous(), want_kl=False, want_grad=True)
+        return grad, None, None, None, None
+
+
+def top_logits_position_kl(masked_logits: torch.Tensor, top_logits: torch.Tensor, top_indices: torch.Tensor, *,
+                           clean_lse: torch.Tensor | None = None, temperature: float = 1.0) -> torch.Tensor:
+    """Per-position KL(clean || masked) from the clean side's k largest (or any k) logits
+    per position in place of all of them: `clean_logits.topk(k)` stored once, or a teacher
+    run elsewhere. masked_logits [..., V]; top_logits, top_indices [..., k] (bf16 or fp32;
+    int32 or int64; an index outside [0, V) is padding). Without `clean_lse` the clean
+    probabilities are the softmax of the listed logits alone. With `clean_lse` (fp32 [...],
+    `torch.logsumexp(clean_logits / temperature, -1)`) they are the clean model's own, and
+    the mass of the entries not listed is compared as one: a lower bound of
+    `categorical_kl_from_logits`'s KL that it meets at k = V. Returns fp32 [...];
+    differentiable in the masked logits. `ops.top_logits_kl` gives the loss and its weighted
+    gradient from one read of the logits."""
+    masked = masked_logits.contiguous()
+    top, indices = top_logits.detach().contiguous(), top_indices.contiguous()
+    lse = None if clean_lse is None else clean_lse.detach().contiguous()
+    if torch.is_grad_enabled() and masked.requires_grad:
+        return _TopLogitsKL.apply(masked, top, indices, lse, float(temperature))
+    return ops.top_logits_kl(masked, top, indices, clean_lse=lse, temperature=float(temperature))[0]
+
+
+def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, temperature: float = 1.0) -> torch.Tensor:
+    """The mean of `top_logits_position_kl` over positions, as `categorical_kl_from_logits`
+    is over all logits."""
+    return top_logits_position_kl(masked_logits, top_logits, top_indices, clean_lse=clean_lse,
+                                  temperature=temperature).mean()

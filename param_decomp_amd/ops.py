@@ -365,3 +365,161 @@ def source_ascend(opt: int, sources, grad, state_a=None, state_b=None, *, step_c
            L.ptr(state_a), L.ptr(state_b), step_count, lr, beta1, beta2, eps, momentum, key[0], key[1], layout,
            L.stream())
     return sources
+
+# ------------------------------------------------- around a language model's decomposed sites
+def _on(name: str, first: torch.Tensor, **others: torch.Tensor | None):
+    """Every tensor on the first one's GPU, which is current for the call."""
+    for label, t in others.items():
+        if t is not None and t.device != first.device:
+            raise L.PDError(f"{name}: {label} is on {t.device}, not {first.device}")
+    return L.on_device(first)
+
+
+def _strides(name: str, label: str, t: torch.Tensor) -> tuple[int, int]:
+    """Row and head strides of [rows, heads, head_dim] as the attention kernels take them."""
+    rows, heads, D = t.shape
+    per = 16 // t.element_size()
+    row = t.stride(0) if rows > 1 else heads * D
+    head = t.stride(1) if heads > 1 else D
+    if (D > 1 and t.stride(2) != 1) or row % per or head % per or t.data_ptr() % 16:
+        raise L.PDError(f"{name}: {label} needs a dense last axis and 16-byte aligned rows and heads")
+    return row, head
+
+
+def _attention_checks(name: str, q, k, v, offsets, scale):
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise L.PDError(f"{name}: q [rows, heads, head_dim], k and v [rows, kv heads, head_dim], got "
+                        f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise L.PDError(f"{name}: q, k and v share one dtype, float32 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise L.PDError(f"{name}: {q.shape[1]} query heads are no multiple of {k.shape[1]} key heads")
+    if q.shape[2] % 8 or not 8 <= q.shape[2] <= 128:
+        raise L.PDError(f"{name}: head_dim is a multiple of 8 up to 128, got {q.shape[2]}")
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+        raise L.PDError(f"{name}: offsets is a dense int32 vector of sequences + 1 row numbers")
+    return q.shape[2]**-0.5 if scale is None else float(scale)
+
+
+def _attention_args(name: str, q, k, v, offsets, scale: float, fill: bool) -> list:
+    N, H, D = q.shape
+    args = []
+    for label, t in (("q", q), ("k", k), ("v", v)):
+        args += [t.data_ptr(), *_strides(name, label, t)]
+    return args + [L.dtype_code(q.dtype), N, H, k.shape[1], D, L.ptr(offsets), offsets.numel() - 1, scale, int(fill)]
+
+
+def _like_rows(name: str, label: str, t: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
+    if t.shape != q.shape or t.dtype != q.dtype:
+        raise L.PDError(f"{name}: {label} is {tuple(t.shape)} {t.dtype}, not {tuple(q.shape)} {q.dtype}")
+    return t
+
+
+def packed_attention_fwd(q, k, v, offsets, *, scale: float | None = None, out: torch.Tensor | None = None,
+                         want_stats: bool = False):
+    """(out, stats) of causal attention over packed sequences: q [rows, H, head_dim], k and v
+    [rows, KV, head_dim] (strided views will do), sequence s in rows offsets[s] ..
+    offsets[s + 1] (int32, on the device). `scale`: head_dim^-0.5 by default. Rows of no
+    sequence are zeros, or left as they were in an `out` that is given. stats: fp32
+    [H, rows], None unless wanted."""
+    name = "packed_attention_fwd"
+    scale = _attention_checks(name, q, k, v, offsets, scale)
+    with _on(name, q, k=k, v=v, offsets=offsets, out=out):
+        fill = out is None
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if fill else _like_rows(name, "out", out, q)
+        stats = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_stats else None
+        L.call("pd_packed_attention_fwd", *_attention_args(name, q, k, v, offsets, scale, fill), L.ptr(out), L.ptr(stats),
+               L.stream())
+    return out, stats
+
+
+def packed_attention_bwd(q, k, v, offsets, out, stats, d_out, *, scale: float | None = None):
+    """(dq, dk, dv) from the forward's inputs, `out` and `stats`; zeros in rows of no
+    sequence."""
+    name = "packed_attention_bwd"
+    scale = _attention_checks(name, q, k, v, offsets, scale)
+    _like_rows(name, "out", out, q)
+    _like_rows(name, "d_out", d_out, q)
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (q.shape[1], q.shape[0]):
+        raise L.PDError(f"{name}: stats is the forward's, float32 [heads, rows]")
+    with _on(name, q, k=k, v=v, offsets=offsets, out=out, stats=stats, d_out=d_out):
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        ws = L.workspace(L.load().pd_packed_attention_bwd_workspace_size(q.shape[0], q.shape[1]), q.device)
+        L.call("pd_packed_attention_bwd", *_attention_args(name, q, k, v, offsets, scale, True), L.ptr(out), L.ptr(stats),
+               L.ptr(d_out), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(ws), ws.numel(), L.stream())
+    return dq, dk, dv
+
+
+def _norm_checks(name: str, x, weight, bias=None) -> tuple[int, int]:
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise L.PDError(f"{name}: x has no last axis to norm: {tuple(x.shape)}")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise L.PDError(f"{name}: x is float32 or bfloat16, got {x.dtype}")
+    for label, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (x.shape[-1],)):
+            raise L.PDError(f"{name}: {label} is float32 [{x.shape[-1]}], got {t.dtype} {tuple(t.shape)}")
+    return _flat_rows(x)
+
+
+def layer_norm_fwd(x, weight=None, bias=None, *, eps: float = 1e-5, want_stats: bool = False):
+    """(y, stats) over the last axis; stats fp32 [rows, 3] for the backward, None unless
+    wanted."""
+    rows, d = _norm_checks("layer_norm_fwd", x, weight, bias)
+    with _on("layer_norm_fwd", x, weight=weight, bias=bias):
+        y = torch.empty_like(x)
+        stats = torch.empty((rows, 3), dtype=torch.float32, device=x.device) if want_stats else None
+        L.call("pd_layer_norm_fwd", L.ptr(x), L.dtype_code(x.dtype), rows, d, L.ptr(weight), L.ptr(bias), eps, L.ptr(y),
+               L.ptr(stats), L.stream())
+    return y, stats
+
+
+def layer_norm_bwd(x, d_y, weight, stats, *, want_dx: bool = True, want_dweight: bool = True, want_dbias: bool = True):
+    """(dx, dweight, dbias) from the forward's input and stats; None for those not wanted."""
+    name = "layer_norm_bwd"
+    rows, d = _norm_checks(name, x, weight)
+    if d_y.shape != x.shape or d_y.dtype != x.dtype:
+        raise L.PDError(f"{name}: d_y is {tuple(d_y.shape)} {d_y.dtype}, not {tuple(x.shape)} {x.dtype}")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 3):
+        raise L.PDError(f"{name}: stats is the forward's, float32 [rows, 3]")
+    with _on(name, x, d_y=d_y, weight=weight, stats=stats):
+        dx = torch.empty_like(x) if want_dx else None
+        dw, db = (torch.empty(d, dtype=torch.float32, device=x.device) if want else None
+                  for want in (want_dweight, want_dbias))
+        params = want_dweight or want_dbias
+        ws = L.workspace(L.load().pd_layer_norm_bwd_workspace_size(rows, d), x.device) if params else None
+        L.call("pd_layer_norm_bwd", L.ptr(x), L.ptr(d_y), L.dtype_code(x.dtype), rows, d, L.ptr(weight), L.ptr(stats),
+               L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), ws.numel() if params else 0, L.stream())
+    return dx, dw, db
+
+
+def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, temperature: float = 1.0,
+                  row_weight=None, want_kl: bool = True, want_grad: bool = False):
+    """(kl, grad): per-position KL from the clean side's listed logits to the masked logits
+    [..., V] (see `losses.top_logits_position_kl`), and row_weight (fp32 [...]; None: 1)
+    times its gradient, from one read of the logits. None for those not wanted."""
+    name = "top_logits_kl"
+    z = masked_logits
+    lead, V = z.shape[:-1], z.shape[-1] if z.dim() else 0
+    if z.dtype not in (torch.float32, torch.bfloat16) or top_logits.dtype not in (torch.float32, torch.bfloat16):
+        raise L.PDError(f"{name}: logits are float32 or bfloat16, got {z.dtype} and {top_logits.dtype}")
+    if top_indices.dtype not in (torch.int32, torch.int64):
+        raise L.PDError(f"{name}: indices are int32 or int64, got {top_indices.dtype}")
+    k = top_logits.shape[-1] if top_logits.dim() else 0
+    if top_logits.shape[:-1] != lead or top_indices.shape != top_logits.shape or not 1 <= k <= 1024:
+        raise L.PDError(f"{name}: top logits and indices are [..., k], 1 <= k <= 1024, beside logits [..., V]; got "
+                        f"{tuple(top_logits.shape)}, {tuple(top_indices.shape)}, {tuple(z.shape)}")
+    if not 1 <= V <= 1 << 19:
+        raise L.PDError(f"{name}: 1 to 2^19 logits a position, got {V}")
+    for label, t in (("clean_lse", clean_lse), ("row_weight", row_weight)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != lead):
+            raise L.PDError(f"{name}: {label} is float32 {tuple(lead)}, got {t.dtype} {tuple(t.shape)}")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise L.PDError(f"{name}: temperature must be positive and finite, got {temperature}")
+    with _on(name, z, top_logits=top_logits, top_indices=top_indices, clean_lse=clean_lse, row_weight=row_weight):
+        kl = torch.empty(lead, dtype=torch.float32, device=z.device) if want_kl else None
+        grad = torch.empty_like(z) if want_grad else None
+        if want_kl or want_grad:
+            L.call("pd_top_kl", L.ptr(z), L.dtype_code(z.dtype), math.prod(lead), V, L.ptr(top_logits),
+                   L.dtype_code(top_logits.dtype), L.ptr(top_indices), 8 * top_indices.element_size(), k,
+                   L.ptr(clean_lse), temperature, L.ptr(row_weight), L.ptr(kl), L.ptr(grad), L.stream())
+    return kl, grad
