@@ -671,8 +671,8 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
  * The attention of a language-model target around its decomposed projections
  * (pd/attention.py:26-130), for tokens of several sequences in one axis. q [rows, n_head,
  * head_dim], k and v [rows, n_kv_head, head_dim] in `dtype` (bf16 or fp32) with the given
- * row and head strides in elements (last axis dense; strides whole 16-byte words, tensors
- * 16-byte aligned: views of one projection's output will do). Query head h reads key head
+ * row and head strides in elements (last axis dense; strides whole 16-byte words, a row's
+ * at most 8 MiB, tensors 16-byte aligned: views of one projection's output will do). Query head h reads key head
  * h / (n_head / n_kv_head). head_dim: a multiple of 8 up to 128. offsets int32
  * [n_seq + 1] in device memory, not decreasing: sequence s is rows [offsets[s],
  * offsets[s+1]) (empty ones allowed); row i of it sees rows offsets[s] .. i. Rows that no
@@ -681,21 +681,23 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
  * infinities included, reaches no other row. Offsets outside [0, rows] or out of order
  * give wrong rows but no access outside the tensors.
  *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, fp32 statistics;
- *   stats fp32 [n_head, rows] (nullable) log2 of the rows' softmax sums, for the backward.
+ * For the backward (nullable): stats, log2 of the rows' softmax sums, fp32 [n_head, rows]
+ * (with fp32 tensors [2, n_head, rows]: then what rounding took off them), and with bf16
+ * tensors out_rest [rows, n_head, head_dim] bf16, what rounding took off out.
  * The backward gives dq [rows, n_head, head_dim], dk and dv [rows, n_kv_head, head_dim]
- * (summed over the query heads that share a key head) from the forward's out and stats and
- * d_out [rows, n_head, head_dim]. out, d_out, dq, dk, dv are dense. Bit-identical from
- * call to call. */
+ * (summed over the query heads that share a key head) from the forward's out, out_rest
+ * (NULL with fp32) and stats and d_out [rows, n_head, head_dim]. out, d_out, dq, dk, dv are
+ * dense. Bit-identical from call to call. */
 int pd_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                             const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
                             int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
-                            void* out, float* stats, void* stream);
-size_t pd_packed_attention_bwd_workspace_size(int64_t rows, int n_head);
+                            void* out, void* out_rest, float* stats, void* stream);
+size_t pd_packed_attention_bwd_workspace_size(int64_t rows, int n_head, int n_kv_head, int head_dim);
 int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                             const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
                             int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
-                            const void* out, const float* stats, const void* d_out, void* dq, void* dk, void* dv,
-                            void* workspace, size_t workspace_bytes, void* stream);
+                            const void* out, const void* out_rest, const float* stats, const void* d_out, void* dq,
+                            void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- layer norm -------------------------------------------------------------------------
  * The norm of targets and CI functions whose blocks centre their activations (the stack

@@ -7,7 +7,6 @@ tensor raises.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -126,10 +125,10 @@ _SIGNATURES = {
     "pd_source_ascend": (_c_i32, [_c_i32, _c_i32, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_f32, _c_f32, ctypes.c_double,
                                   ctypes.c_double, _c_f32, _c_f32, _c_u32, _c_u32, _c_i32, _c_p]),
     "pd_packed_attention_fwd": (_c_i32, [_c_p, _c_i64, _c_i64] * 3 + [_c_i32, _c_i64] + [_c_i32] * 3 +
-                                [_c_p, _c_i64, _c_f32, _c_i32, _c_p, _c_p, _c_p]),
-    "pd_packed_attention_bwd_workspace_size": (_c_sz, [_c_i64, _c_i32]),
+                                [_c_p, _c_i64, _c_f32, _c_i32] + [_c_p] * 4),
+    "pd_packed_attention_bwd_workspace_size": (_c_sz, [_c_i64, _c_i32, _c_i32, _c_i32]),
     "pd_packed_attention_bwd": (_c_i32, [_c_p, _c_i64, _c_i64] * 3 + [_c_i32, _c_i64] + [_c_i32] * 3 +
-                                [_c_p, _c_i64, _c_f32, _c_i32] + [_c_p] * 6 + [_c_p, _c_sz, _c_p]),
+                                [_c_p, _c_i64, _c_f32, _c_i32] + [_c_p] * 8 + [_c_sz, _c_p]),
     "pd_layer_norm_fwd": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_p, _c_f32, _c_p, _c_p, _c_p]),
     "pd_layer_norm_bwd_workspace_size": (_c_sz, [_c_i64, _c_i64]),
     "pd_layer_norm_bwd": (_c_i32, [_c_p, _c_p, _c_i32, _c_i64, _c_i64] + [_c_p] * 6 + [_c_sz, _c_p]),
@@ -201,15 +200,17 @@ def host_array(ctype, values):
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-def on_device(t: torch.Tensor):
-    """Makes the tensor's device current for a call (its current stream is then the one
-    used); costs nothing where it is already."""
-    if not t.is_cuda:
-        raise PDError("pd kernels take GPU tensors")
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def launch(name: str, device: torch.device, *args) -> None:
+    """`call` with the device's current stream as the last argument, the device made current
+    for it where it is not."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream())
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream())
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:

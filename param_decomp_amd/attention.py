@@ -16,9 +16,11 @@ from param_decomp_amd import ops
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
-    """The tensor, or a dense copy where its rows or heads are not 16-byte aligned."""
+    """The tensor, or a dense copy where its rows or heads are not 16-byte aligned or its
+    rows are more than 8 MiB apart."""
     per = 16 // t.element_size()
-    if t.dim() == 3 and t.numel() and (t.stride(2) != 1 or t.stride(0) % per or t.stride(1) % per or t.data_ptr() % 16):
+    if t.dim() == 3 and t.numel() and (t.stride(2) != 1 or t.stride(0) % per or t.stride(1) % per or
+                                       t.data_ptr() % 16 or t.stride(0) * t.element_size() > 1 << 23):
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -26,16 +28,17 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, scale):
-        out, stats = ops.packed_attention_fwd(q, k, v, offsets, scale=scale, want_stats=True)
-        ctx.save_for_backward(q, k, v, offsets, out, stats)
+        out, (stats, rest) = ops.packed_attention_fwd(q, k, v, offsets, scale=scale, want_saved=True)
+        ctx.save_for_backward(q, k, v, offsets, out, stats, rest)
         ctx.scale = scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, offsets, out, stats = ctx.saved_tensors
-        dq, dk, dv = ops.packed_attention_bwd(q, k, v, offsets, out, stats, _dense(g.contiguous()), scale=ctx.scale)
+        q, k, v, offsets, out, stats, rest = ctx.saved_tensors
+        dq, dk, dv = ops.packed_attention_bwd(q, k, v, offsets, out, (stats, rest), _dense(g.contiguous()),
+                                              scale=ctx.scale)
         return dq, dk, dv, None, None
 
 

@@ -34,10 +34,12 @@ typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned at_u32x4
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short at_i16x4;
 typedef __attribute__((address_space(3))) at_i16x4* at_lds_i16x4;
 
-constexpr int AT_THREADS = 256;  // 4 waves of 32 rows
-constexpr int AT_ROWS = 128;
+constexpr int AT_THREADS = 256;  // 4 waves
+constexpr int AT_ROWS = 128;     // rows of a block whose waves own 32 each
+constexpr int AT_SPLIT = 32;     // rows of a block whose waves share them
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float AT_NONE = -1e38f;  // a row's maximum before its first key (base-2 units)
+constexpr float AT_NONE = -1e30f;  // a row's reference score before its first key
+constexpr float AT_SLACK = 8.f;    // a row is rescaled once its maximum has grown past 2^this
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -48,10 +50,13 @@ struct AttnArgs {
   float scale, c2;  // c2 = scale log2 e
   int fill;         // rows of no sequence: 1 zeros, 0 left as they are
   void* out;        // [N, H, D]
-  float* stats;     // [H, N]: L_i / ln 2
+  void* rest;       // bf16 [N, H, D]: what rounding took off out (NULL: not kept; fp32: none)
+  float* stats;     // [H, N]: L_i / ln 2; fp32: then [H, N] what rounding took off it
   const void* d_out;
   float* rowdot;  // [H, N]: D_i
   void *dq, *dk, *dv;
+  float* part;  // [hs][2][N, KV, D]: dk and dv over a share of a group's heads (hs > 1)
+  int hs;       // shares
 };
 
 // ---------------------------------------------------------------- operand fragments
@@ -66,9 +71,18 @@ struct Op<bf16_t> {
   static __device__ inline f32x16 mma(const Frag& x, const Frag& y, f32x16 acc) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
   }
-  static __device__ inline Frag pack(const float* v) {
-    return (Frag)(at_u32x4){pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                            pack_bf16x2(v[6], v[7])};
+  // Accumulator registers 8 kk .. 8 kk + 7 as an operand.
+  static __device__ inline Frag pack(const f32x16& v, int kk) {
+    return (Frag)(at_u32x4){pack_bf16x2(v[8 * kk], v[8 * kk + 1]), pack_bf16x2(v[8 * kk + 2], v[8 * kk + 3]),
+                            pack_bf16x2(v[8 * kk + 4], v[8 * kk + 5]), pack_bf16x2(v[8 * kk + 6], v[8 * kk + 7])};
+  }
+  static __device__ inline Frag scaled(const Frag& a, float f) {  // f = -1 or 0
+    const at_u32x4 x = (at_u32x4)a;
+    at_u32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      y[i] = pack_bf16x2(__uint_as_float(x[i] << 16) * f, __uint_as_float(x[i] & 0xFFFF0000u) * f);
+    return (Frag)y;
   }
   static __device__ inline float dot(const Frag& a, const Frag& b, float s) {
     const at_u32x4 x = (at_u32x4)a, y = (at_u32x4)b;
@@ -99,8 +113,17 @@ struct Op<float> {
     for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x.v[j], y.v[j], acc, 0, 0, 0);
     return acc;
   }
-  static __device__ inline Frag pack(const float* v) {
-    return Frag{{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}};
+  static __device__ inline Frag pack(const f32x16& v, int kk) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f.v[i] = v[8 * kk + i];
+    return f;
+  }
+  static __device__ inline Frag scaled(const Frag& a, float f) {
+    Frag y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] = a.v[i] * f;
+    return y;
   }
   static __device__ inline float dot(const Frag& a, const Frag& b, float s) {
 #pragma unroll
@@ -120,7 +143,8 @@ struct Op<float> {
 // rows p and p + 4 at 8 consecutive chunks (the fp32 transposed reads).
 template <typename T, int DP>
 struct Img {
-  static constexpr int ROWB = DP * (int)sizeof(T), CHUNKS = ROWB / 16, EPC = 16 / (int)sizeof(T);
+  // bytes a row takes: a power of two (rows of 96 elements leave a quarter of it unused)
+  static constexpr int ROWB = (DP <= 64 ? 64 : 128) * (int)sizeof(T), EPC = 16 / (int)sizeof(T);
   static __device__ inline int swz(int R) {
     if constexpr (sizeof(T) == 4) return ((R & 4) << 1) | (R & 3) | ((R >> 1) & 4);
     else if constexpr (ROWB == 128) return (((R >> 1) & 1) << 2) | ((R >> 2) & 3);
@@ -160,32 +184,58 @@ struct Img {
   }
 };
 
-// Rows of one operand on their way from memory into an image of ROWS rows: each thread
-// carries ROWS * CHUNKS / 256 chunks. Row j of the image is row `first + j` of the operand,
-// held inside [lo, hi] (a row beyond them repeats the edge: masked where it is used);
-// columns from D on are zeros.
-template <typename T, int DP, int ROWS>
-struct Stage {
-  static constexpr int CH = Img<T, DP>::CHUNKS, PER = ROWS * CH / AT_THREADS;
-  static_assert(PER * AT_THREADS == ROWS * CH, "whole chunks per thread");
-  uint4 w[PER];
-  __device__ inline void load(const T* base, int64_t stride, int first, int lo, int hi, int D, int tid) {
+// Rows of one operand into an image of ROWS rows by buffer loads straight to LDS, 1 KB an
+// instruction, shared by NW waves. Lane l of a load writes 16 bytes at 16 l, so it fetches
+// the chunk that the swizzle puts there. The descriptor ends behind row `hi`: later rows,
+// and columns from D on (lanes with an offset no descriptor reaches), arrive as zeros.
+template <typename T, int DP, int ROWS, int NW>
+struct Loader {
+  typedef Img<T, DP> I;
+  static constexpr int RPI = 1024 / I::ROWB, NI = ROWS / RPI / NW;
+  static_assert(NI * NW * RPI == ROWS, "whole loads per wave");
+  uint32_t voff[NI];
+  __device__ inline void init(int64_t stride, int D, int wave, int lane) {
+    constexpr int C = I::ROWB / 16;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = tid + i * AT_THREADS, c = at % CH;
-      const int row = min(max(first + at / CH, lo), hi);
-      w[i] = c * Img<T, DP>::EPC < D ? *(const uint4*)(base + row * stride + c * Img<T, DP>::EPC)
-                                     : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < NI; ++i) {
+      const int R = (wave + NW * i) * RPI + lane / C, c = (lane % C) ^ I::swz(R);
+      voff[i] = c * I::EPC < D ? (uint32_t)(R * stride * (int64_t)sizeof(T)) + 16 * c : 0x80000000u;
     }
   }
-  __device__ inline void store(char* img, int tid) const {
+  // Image row 0 is row `first` (first <= hi) of the operand at `base`. (The host pass does
+  // not know the descriptor's type: a body it parsed would leave the kernels without stubs.)
+  __device__ inline void issue(const T* base, int64_t stride, int first, int hi, int D, char* img, int wave) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const int64_t bytes = ((hi - first) * stride + D) * (int64_t)sizeof(T);
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + first * stride), (short)0,
+                                                        (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int at = tid + i * AT_THREADS;
-      *(uint4*)(img + Img<T, DP>::off(at / CH, at % CH)) = w[i];
-    }
+    for (int i = 0; i < NI; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (wave + NW * i) * 1024), 16, voff[i], 0, 0, 0);
+#endif
   }
 };
+
+// Waits for this wave's LDS reads, so that loads issued next may overwrite what they read.
+__device__ inline void at_lds_free() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// Waits until at most `left` of the wave's loads are in flight.
+template <int LEFT>
+__device__ inline void at_landed(bool more) {
+  asm volatile("" ::: "memory");
+  if (more) wait_vmcnt<LEFT>();
+  else wait_vmcnt<0>();
+  asm volatile("" ::: "memory");
+}
+// Every wave's loads have landed and every wave's LDS reads are done.
+__device__ inline void at_exchange() {
+  asm volatile("" ::: "memory");
+  wait_loads_and_lds<0>();
+  lds_barrier();
+}
 
 // Fragments of one row of an operand in memory (zeros from column D on).
 template <typename T, int DP>
@@ -268,7 +318,16 @@ __device__ __attribute__((noinline)) void at_fwd_row(const AttnArgs* a, int h, i
   T* o = (T*)a->out + ((int64_t)row * a->H + h) * D;
   if (lane < D) store_f<T>(o, lane, o0 / l);
   if (lane + 64 < D) store_f<T>(o, lane + 64, o1 / l);
-  if (a->stats && lane == 0) a->stats[(int64_t)h * a->N + row] = m + log2f(l);
+  if constexpr (sizeof(T) == 2) {
+    T* rest = (T*)a->rest + ((int64_t)row * a->H + h) * D;
+    if (a->rest && lane < D) store_f<T>(rest, lane, o0 / l - at_f<T>(o[lane]));
+    if (a->rest && lane + 64 < D) store_f<T>(rest, lane + 64, o1 / l - at_f<T>(o[lane + 64]));
+  }
+  if (a->stats && lane == 0) {
+    const float L = m + log2f(l);
+    a->stats[(int64_t)h * a->N + row] = L;
+    if (sizeof(T) == 4) a->stats[((int64_t)a->H + h) * a->N + row] = (m - L) + log2f(l);
+  }
 }
 
 template <typename T>
@@ -279,7 +338,8 @@ __device__ __attribute__((noinline)) void at_dq_row(const AttnArgs* a, int h, in
   const T* k = (const T*)a->k + hk * a->k_head;
   const T* v = (const T*)a->v + hk * a->v_head;
   const float L = a->stats[(int64_t)h * a->N + row];
-  const float dot = at_dot<T>(g, (const T*)a->out + ((int64_t)row * a->H + h) * D, D);
+  float dot = at_dot<T>(g, (const T*)a->out + ((int64_t)row * a->H + h) * D, D);
+  if (sizeof(T) == 2) dot += at_dot<T>(g, (const T*)a->rest + ((int64_t)row * a->H + h) * D, D);
   float o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 64) {
     const int j = j0 + lane;
@@ -299,12 +359,13 @@ __device__ __attribute__((noinline)) void at_dq_row(const AttnArgs* a, int h, in
 }
 
 template <typename T>
-__device__ __attribute__((noinline)) void at_dkv_row(const AttnArgs* a, int hk, int row, int end, int lane) {
-  const int D = a->D, rep = a->H / a->KV;
+__device__ __attribute__((noinline)) void at_dkv_row(const AttnArgs* a, int hk, int share, int row, int end,
+                                                         int lane) {
+  const int D = a->D, rep = a->H / a->KV, nh = rep / a->hs, h0 = hk * rep + share * nh;
   const T* k = (const T*)a->k + row * a->k_row + hk * a->k_head;
   const T* v = (const T*)a->v + row * a->v_row + hk * a->v_head;
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int h = hk * rep; h < (hk + 1) * rep; ++h)
+  for (int h = h0; h < h0 + nh; ++h)
     for (int i0 = row; i0 < end; i0 += 64) {
       const int i = i0 + lane;
       float p = 0.f, ds = 0.f;
@@ -322,8 +383,16 @@ __device__ __attribute__((noinline)) void at_dkv_row(const AttnArgs* a, int hk, 
         if (lane + 64 < D) k1 = fmaf(ws, at_f<T>(q[lane + 64]), k1), v1 = fmaf(wp, at_f<T>(g[lane + 64]), v1);
       }
     }
-  T* dk = (T*)a->dk + ((int64_t)row * a->KV + hk) * D;
-  T* dv = (T*)a->dv + ((int64_t)row * a->KV + hk) * D;
+  const int64_t at = ((int64_t)row * a->KV + hk) * D, plane = (int64_t)a->N * a->KV * D;
+  if (a->hs > 1) {
+    float* pk = a->part + 2 * share * plane + at;
+    float* pv = pk + plane;
+    if (lane < D) pk[lane] = k0, pv[lane] = v0;
+    if (lane + 64 < D) pk[lane + 64] = k1, pv[lane + 64] = v1;
+    return;
+  }
+  T* dk = (T*)a->dk + at;
+  T* dv = (T*)a->dv + at;
   if (lane < D) store_f<T>(dk, lane, k0), store_f<T>(dv, lane, v0);
   if (lane + 64 < D) store_f<T>(dk, lane + 64, k1), store_f<T>(dv, lane + 64, v1);
 }
@@ -333,60 +402,169 @@ __device__ inline const AttnArgs* at_args() { return (const AttnArgs*)__builtin_
 
 // Query tile and head of a block: the heads of one key head on one XCD (blocks go round
 // the 8 XCDs in turn), tiles with the most keys behind a long sequence's start first.
+template <int ROWS>
 __device__ inline void at_query_tile(const AttnArgs& a, int& h, int& q0) {
-  const int nt = (a.N + AT_ROWS - 1) / AT_ROWS, rep = a.H / a.KV;
+  const int nt = (a.N + ROWS - 1) / ROWS, rep = a.H / a.KV;
   const int id = blockIdx.x, x = id % a.H;
   h = (x % a.KV) * rep + x / a.KV;
-  q0 = (nt - 1 - id / a.H) * AT_ROWS;
+  q0 = (nt - 1 - id / a.H) * ROWS;
+}
+
+// A lane's query row, its sequence, and the keys its wave meets.
+struct Rows {
+  int row, start, end;
+  bool in;       // the row is in a sequence
+  int lo, hi;    // keys the wave meets: [lo, hi)
+  int inner_lo;  // largest start of the wave's rows
+  bool whole;    // every row of the wave is in a sequence
+  __device__ inline void init(const AttnArgs& a, int r) {
+    row = r;
+    at_sequence(a.off, a.S, a.N, row, start, end);
+    in = start <= row;
+    lo = at_wave_min(in ? start : 0x7FFFFFFF);
+    hi = at_wave_max(in ? row + 1 : -1);
+    inner_lo = at_wave_max(in ? start : -1);
+    whole = __all(in);
+  }
+  // No key of [j, j + n) is hidden from any row of the wave (its first row is row0).
+  __device__ inline bool inner(int j, int n, int row0) const { return whole && j >= inner_lo && j + n <= row0 + 1; }
+};
+
+// Keys the block's four waves meet.
+__device__ inline void at_block_range(int lo, int hi, int lane, int w, int (&ends)[2][4], int& blo, int& bhi) {
+  if (lane == 0) ends[0][w] = lo, ends[1][w] = hi;
+  __syncthreads();
+  blo = __builtin_amdgcn_readfirstlane(min(min(ends[0][0], ends[0][1]), min(ends[0][2], ends[0][3])));
+  bhi = __builtin_amdgcn_readfirstlane(max(max(ends[1][0], ends[1][1]), max(ends[1][2], ends[1][3])));
+}
+
+// Stores a lane's row from its accumulators (times f; zeros where the row has no sequence)
+// and tells whether a value is a NaN or infinite.
+template <typename T, int NC>
+__device__ inline bool at_store_row(T* orow, T* rest, const f32x16 (&o)[NC], float f, bool in, int D, int hh) {
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int ch = 32 * c + 8 * g + 4 * hh;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = in ? o[c][4 * g + e] * f : 0.f;
+        sum = fmaf(v[e], 0.f, sum);
+      }
+      if (ch < D) {
+        Op<T>::store4(orow + ch, v[0], v[1], v[2], v[3]);
+        if constexpr (sizeof(T) == 2)
+          if (rest) {
+            float l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) l[e] = v[e] - bf16_to_f32(f32_to_bf16(v[e]));
+            Op<T>::store4(rest + ch, l[0], l[1], l[2], l[3]);
+          }
+      }
+    }
+  return in && sum != 0.f;
+}
+
+// Row stats of one query: L and what rounding takes off it.
+template <typename T>
+__device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float mc, float l) {
+  const float ll = log2f(l), L = mc + ll;
+  a.stats[(int64_t)h * a.N + row] = L;
+  if constexpr (sizeof(T) == 4) a.stats[((int64_t)a.H + h) * a.N + row] = (mc - L) + ll;
 }
 
 // ---------------------------------------------------------------- forward
-// Grid: query tiles x heads. Keys come through LDS BK rows at a time, the next tile's loads
-// in flight during this one's products.
-template <typename T, int DP, int BK>
+// One row block's online softmax over a tile of NB key blocks: scores sc (raw, masked ones
+// -inf) to weights in place, the running reference m (raw), the lane's own part of the sum l,
+// and the accumulators rescaled where a maximum has grown by more than the slack: weights
+// stay below 2^8 and a tile without growth costs no pass over the accumulators.
+template <int NB, int NC>
+__device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], float& m, float& l, f32x16 (&o)[NC], float c2) {
+  float mt = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[b][i]);
+  mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+  if (__any((mt - m) * c2 > AT_SLACK)) {
+    const float mn = fmaxf(m, mt), al = at_exp2((m - mn) * c2);
+    m = mn;
+    l *= al;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[c][i] *= al;
+  }
+  const float mc = -m * c2;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      sc[b][i] = at_exp2(fmaf(sc[b][i], c2, mc));
+      l += sc[b][i];
+    }
+}
+
+// Query fragments with the scale's sign: c2 is positive then. (Scale 0: zeros, c2 = 1.)
+template <typename T, int DP>
+__device__ inline float at_query(const AttnArgs& a, int h, int row, int hh, typename Op<T>::Frag (&f)[DP / 16]) {
+  at_row<T, DP>((const T*)a.q + (int64_t)min(row, a.N - 1) * a.q_row + h * a.q_head, a.D, hh, f);
+  if (a.c2 > 0.f) return a.c2;
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) f[s] = Op<T>::scaled(f[s], a.c2 < 0.f ? -1.f : 0.f);
+  return a.c2 < 0.f ? -a.c2 : 1.f;
+}
+
+// Two LDS buffers that loads and reads alternate between. They are two variables, and the
+// loops run two tiles a turn, so that the compiler can tell a load into one from a read of
+// the other: where it cannot, it waits for every load in flight before the read.
+#define AT_TWO_BUFFERS(bytes)                                   \
+  __shared__ __attribute__((aligned(1024))) char ldsA[bytes]; \
+  __shared__ __attribute__((aligned(1024))) char ldsB[bytes]
+
+// A block of 128 query rows, 32 a wave. Grid: query tiles x heads. Keys and values come
+// through LDS BK rows at a time in two buffers: one barrier a tile, behind it the next
+// tile's loads go out and have this tile's products to land.
+template <typename T, int DP>
+struct FwdCfg {
+  static constexpr int BK = Img<T, DP>::ROWB == 512 ? 32 : 64, TILE = BK * Img<T, DP>::ROWB;
+};
+template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   typedef Img<T, DP> I;
   typedef typename Op<T>::Frag Frag;
-  constexpr int NS = DP / 16, NB = BK / 32, NC = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char Kl[BK * I::ROWB];
-  __shared__ __attribute__((aligned(1024))) char Vl[BK * I::ROWB];
+  constexpr int BK = FwdCfg<T, DP>::BK, TILE = FwdCfg<T, DP>::TILE, NS = DP / 16, NB = BK / 32, NC = DP / 32;
+  AT_TWO_BUFFERS(2 * TILE);
   __shared__ int ends[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   int h, q0;
-  at_query_tile(a, h, q0);
-  const int hk = h / (a.H / a.KV), row = q0 + 32 * w + r;
+  at_query_tile<AT_ROWS>(a, h, q0);
+  const int hk = h / (a.H / a.KV), row0 = q0 + 32 * w;
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   Frag qf[NS];
-  at_row<T, DP>((const T*)a.q + (int64_t)min(row, a.N - 1) * a.q_row + h * a.q_head, a.D, hh, qf);
-  int start, end;
-  at_sequence(a.off, a.S, a.N, row, start, end);
-  const bool in = start <= row;
-  const int lo = at_wave_min(in ? start : 0x7FFFFFFF), hi = at_wave_max(in ? row + 1 : -1);
-  const int inner_lo = at_wave_max(in ? start : -1);
-  const bool whole = __all(in);
-  if (lane == 0) ends[0][w] = lo, ends[1][w] = hi;
-  __syncthreads();
-  const int blo = min(min(ends[0][0], ends[0][1]), min(ends[0][2], ends[0][3]));
-  const int bhi = max(max(ends[1][0], ends[1][1]), max(ends[1][2], ends[1][3]));
-
+  const float c2 = at_query<T, DP>(a, h, row0 + r, hh, qf);
+  Rows R;
+  R.init(a, row0 + r);
+  int blo, bhi;
+  at_block_range(R.lo, R.hi, lane, w, ends, blo, bhi);
+  Loader<T, DP, BK, 4> lk, lv;
+  lk.init(a.k_row, a.D, w, lane);
+  lv.init(a.v_row, a.D, w, lane);
   float m = AT_NONE, l = 0.f;
   f32x16 o[NC] = {};
-  Stage<T, DP, BK> sk, sv;
-  if (blo < bhi) {
-    sk.load(kb, a.k_row, blo, blo, bhi - 1, a.D, tid);
-    sv.load(vb, a.v_row, blo, blo, bhi - 1, a.D, tid);
-  }
-  for (int j0 = blo; j0 < bhi; j0 += BK) {
-    __syncthreads();
-    sk.store(Kl, tid);
-    sv.store(Vl, tid);
-    __syncthreads();
-    if (j0 + BK < bhi) {
-      sk.load(kb, a.k_row, j0 + BK, blo, bhi - 1, a.D, tid);
-      sv.load(vb, a.v_row, j0 + BK, blo, bhi - 1, a.D, tid);
-    }
-    if (j0 >= hi || j0 + BK <= lo) continue;
+  auto issue = [&](int j0, char* img) {
+    lk.issue(kb, a.k_row, j0, bhi - 1, a.D, img, w);
+    lv.issue(vb, a.v_row, j0, bhi - 1, a.D, img + TILE, w);
+  };
+  auto tile = [&](int j0, const char* Kl, char* next) {
+    at_exchange();
+    if (j0 + BK < bhi) issue(j0 + BK, next);
+    if (j0 >= R.hi || j0 + BK <= R.lo) return;
+    const char* Vl = Kl + TILE;
     f32x16 sc[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -394,308 +572,664 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) sc[b] = Op<T>::mma(I::rows(Kl, 32 * b + r, s, hh), qf[s], sc[b]);
     }
-    // scores in base-2 units; masked ones are -inf whatever their keys hold
-    const bool inner = whole && j0 >= inner_lo && j0 + BK <= q0 + 32 * w + 1;
-    float mt = -INFINITY;
+    if (!R.inner(j0, BK, row0)) {  // hidden scores are -inf whatever their keys hold
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + 32 * b + at_pos(i, hh);
+          sc[b][i] = j >= R.start && j <= R.row ? sc[b][i] : -INFINITY;
+        }
+    }
+    at_softmax<NB, NC>(sc, m, l, o, c2);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float t = sc[b][i] * a.c2;
-        if (!inner) {
-          const int j = j0 + 32 * b + at_pos(i, hh);
-          t = j >= start && j <= row ? t : -INFINITY;
-        }
-        sc[b][i] = t;
-        mt = fmaxf(mt, t);
-      }
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    if (__any(mt > m)) {
-      const float mn = fmaxf(m, mt), al = at_exp2(m - mn);
-      m = mn;
-      l *= al;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[c][i] *= al;
-    }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = at_exp2(sc[b][i] - m);
-        l += p[i];
-      }
-#pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        const Frag pf = Op<T>::pack(p + 8 * kk);
+        const Frag pf = Op<T>::pack(sc[b], kk);
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[c] = Op<T>::mma(I::cols(Vl, 32 * b, kk, c, lane), pf, o[c]);
       }
-    }
+  };
+  if (blo < bhi) issue(blo, ldsA);
+  for (int j0 = blo; j0 < bhi; j0 += 2 * BK) {
+    tile(j0, ldsA, ldsB);
+    if (j0 + BK < bhi) tile(j0 + BK, ldsB, ldsA);
   }
   l += __shfl_xor(l, 32, 64);
-  const float il = in ? 1.f / l : 0.f;
-  float sum = 0.f;  // NaN where any of the row's outputs is
-  if (row < a.N && (in || a.fill)) {
-    T* orow = (T*)a.out + ((int64_t)row * a.H + h) * a.D;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int ch = 32 * c + 8 * g + 4 * hh;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = in ? o[c][4 * g + e] * il : 0.f;
-          sum = fmaf(v[e], 0.f, sum);
-        }
-        if (ch < a.D) Op<T>::store4(orow + ch, v[0], v[1], v[2], v[3]);
-      }
-    if (in && a.stats && hh == 0) a.stats[(int64_t)h * a.N + row] = m + log2f(l);
+  bool odd = false;
+  if (R.row < a.N && (R.in || a.fill)) {
+    const int64_t at = ((int64_t)R.row * a.H + h) * a.D;
+    odd = at_store_row<T, NC>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, o, 1.f / l, R.in, a.D, hh);
+    if (R.in && a.stats && hh == 0) at_store_stats<T>(a, h, R.row, m * c2, l);
   }
   // infinities count too: 0 times one is a NaN in another row's product
-  unsigned long long bad = __ballot(in && sum != 0.f);
+  unsigned long long bad = __ballot(odd);
   bad = (bad | bad >> 32) & 0xFFFFFFFFull;
   while (bad) {
     const int i = __builtin_ctzll(bad);
     bad &= bad - 1;
-    at_fwd_row<T>(at_args(), h, q0 + 32 * w + i, __shfl(start, i, 64), lane);
+    at_fwd_row<T>(at_args(), h, row0 + i, __shfl(R.start, i, 64), lane);
+  }
+}
+
+// fp32 rows of four waves for a join, two waves in each of two LDS regions: value v of row r
+// at chunk (v / 4) ^ (r & 15).
+template <int DP>
+struct Join {
+  static constexpr int SHARE = 32 * (DP <= 64 ? 64 : 128) * 4;
+  char *a, *b;
+  __device__ inline float4* at(int w, int r, int ch) const {
+    return (float4*)((w < 2 ? a : b) + (w & 1) * SHARE + ((r * (DP <= 64 ? 16 : 32) + ((ch >> 2) ^ (r & 15))) << 4));
+  }
+  // Writes a wave's accumulators into its share, times f.
+  __device__ inline void put(int w, int r, int hh, const f32x16 (&o)[DP / 32], float f) const {
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *at(w, r, 32 * c + 8 * g + 4 * hh) =
+            make_float4(o[c][4 * g] * f, o[c][4 * g + 1] * f, o[c][4 * g + 2] * f, o[c][4 * g + 3] * f);
+  }
+  // The four waves' values ch .. ch + 3 of row r, added in wave order.
+  __device__ inline float4 sum(int r, int ch) const {
+    float4 s = *at(0, r, ch);
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 v = *at(w, r, ch);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    return s;
+  }
+};
+// Marks rows with a NaN or an infinity among the values this thread stored of row r
+// (the 8 threads of a row are neighbours).
+__device__ inline unsigned at_join_odd(float sum, bool in) {
+  const unsigned long long b = __ballot(in && sum != 0.f);
+  unsigned rows = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rows |= (b >> (8 * i) & 0xFF ? 1u : 0u) << i;
+  return rows;  // of the wave's 8 rows
+}
+
+// The same for grids too small to fill the GPU: a block of 32 query rows whose four waves
+// take every fourth block of 32 keys each, through LDS of their own (no barrier in the
+// loop: a block's keys come in while the last one's weights are used, its values while its
+// scores are formed), and join their sums at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename Op<T>::Frag Frag;
+  constexpr int TILE = 32 * I::ROWB, NS = DP / 16, NC = DP / 32;
+  typedef Loader<T, DP, 32, 1> Ld;
+  static_assert(4 * TILE >= 2 * Join<DP>::SHARE, "a region holds two waves' rows");
+  AT_TWO_BUFFERS(4 * TILE);  // the waves' keys, and their values
+  __shared__ float ml[2][4][32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  int h, q0;
+  at_query_tile<AT_SPLIT>(a, h, q0);
+  const int hk = h / (a.H / a.KV);
+  const T* kb = (const T*)a.k + hk * a.k_head;
+  const T* vb = (const T*)a.v + hk * a.v_head;
+  Frag qf[NS];
+  const float c2 = at_query<T, DP>(a, h, q0 + r, hh, qf);
+  Rows R;
+  R.init(a, q0 + r);
+  Ld lk, lv;
+  lk.init(a.k_row, a.D, 0, lane);
+  lv.init(a.v_row, a.D, 0, lane);
+  char* Kl = ldsA + w * TILE;
+  char* Vl = ldsB + w * TILE;
+  float m = AT_NONE, l = 0.f;
+  f32x16 o[NC] = {};
+  int j0 = R.lo < R.hi ? R.lo + 32 * w : R.hi;
+  if (j0 < R.hi) {
+    lk.issue(kb, a.k_row, j0, R.hi - 1, a.D, Kl, 0);
+    lv.issue(vb, a.v_row, j0, R.hi - 1, a.D, Vl, 0);
+  }
+  for (; j0 < R.hi; j0 += 128) {
+    const bool more = j0 + 128 < R.hi;
+    at_landed<Ld::NI>(true);  // the keys; the values may still be on their way
+    f32x16 sc[1] = {};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) sc[0] = Op<T>::mma(I::rows(Kl, r, s, hh), qf[s], sc[0]);
+    at_lds_free();
+    if (more) lk.issue(kb, a.k_row, j0 + 128, R.hi - 1, a.D, Kl, 0);
+    if (!R.inner(j0, 32, q0)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = j0 + at_pos(i, hh);
+        sc[0][i] = j >= R.start && j <= R.row ? sc[0][i] : -INFINITY;
+      }
+    }
+    at_softmax<1, NC>(sc, m, l, o, c2);
+    at_landed<Ld::NI>(more);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const Frag pf = Op<T>::pack(sc[0], kk);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[c] = Op<T>::mma(I::cols(Vl, 0, kk, c, lane), pf, o[c]);
+    }
+    at_lds_free();
+    if (more) lv.issue(vb, a.v_row, j0 + 128, R.hi - 1, a.D, Vl, 0);
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (hh == 0) ml[0][w][r] = m, ml[1][w][r] = l;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(ml[0][0][r], ml[0][1][r]), fmaxf(ml[0][2][r], ml[0][3][r]));
+  float sum_l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2((ml[0][i][r] - M) * c2);
+  const Join<DP> join = {ldsA, ldsB};
+  join.put(w, r, hh, o, at_exp2((m - M) * c2) / sum_l);
+  if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats<T>(a, h, R.row, M * c2, sum_l);
+  __syncthreads();
+  const int rr = tid >> 3, row = q0 + rr;
+  const int start = __shfl(R.start, rr, 64);
+  const bool in = start <= row;
+  float odd = 0.f;
+  if (row < a.N && (in || a.fill)) {
+    const int64_t at = ((int64_t)row * a.H + h) * a.D;
+#pragma unroll
+    for (int q = 0; q < DP / 32; ++q) {
+      const int ch = 4 * ((tid & 7) + 8 * q);
+      float4 v = join.sum(rr, ch);
+      if (!in) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      odd = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, odd))));
+      if (ch >= a.D) continue;
+      Op<T>::store4((T*)a.out + at + ch, v.x, v.y, v.z, v.w);
+      if constexpr (sizeof(T) == 2)
+        if (a.rest)
+          Op<T>::store4((T*)a.rest + at + ch, v.x - bf16_to_f32(f32_to_bf16(v.x)), v.y - bf16_to_f32(f32_to_bf16(v.y)),
+                        v.z - bf16_to_f32(f32_to_bf16(v.z)), v.w - bf16_to_f32(f32_to_bf16(v.w)));
+    }
+  }
+  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
+    const int i = 8 * w + __builtin_ctz(bad);
+    at_fwd_row<T>(at_args(), h, q0 + i, __shfl(R.start, i, 64), lane);
   }
 }
 
 // ---------------------------------------------------------------- backward: queries
-// dq, and D_i for the key side. Tiles and waves as the forward's.
-template <typename T, int DP, int BK>
-__global__ __launch_bounds__(AT_THREADS, 2) void k_attn_dq(AttnArgs a) {
+// The row's operands: q and do fragments, L, and D = do . out from the stored out and what
+// rounding took off it (from the rounded out alone, D's error weighs on every key of a row
+// alike and was the largest of dq's), written for the key side.
+template <typename T, int DP>
+struct QueryRow {
+  typename Op<T>::Frag q[DP / 16], g[DP / 16];
+  float L = 0.f, Lr = 0.f, dot = 0.f;
+  __device__ inline void init(const AttnArgs& a, int h, const Rows& R, int hh, bool write) {
+    const int rc = min(R.row, a.N - 1);
+    const int64_t at = ((int64_t)rc * a.H + h) * a.D;
+    at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, q);
+    at_row<T, DP>((const T*)a.d_out + at, a.D, hh, g);
+    if (R.in) {
+      typename Op<T>::Frag o[DP / 16];
+      at_row<T, DP>((const T*)a.out + at, a.D, hh, o);
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) dot = Op<T>::dot(g[s], o[s], dot);
+      if constexpr (sizeof(T) == 2) {
+        at_row<T, DP>((const T*)a.rest + at, a.D, hh, o);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) dot = Op<T>::dot(g[s], o[s], dot);
+      }
+      L = a.stats[(int64_t)h * a.N + R.row];
+      if constexpr (sizeof(T) == 4) Lr = a.stats[((int64_t)a.H + h) * a.N + R.row];
+    }
+    dot += __shfl_xor(dot, 32, 64);
+    if (write && R.in && hh == 0) a.rowdot[(int64_t)h * a.N + R.row] = dot;
+  }
+  __device__ inline float p(float s, float c2) const {
+    const float t = fmaf(s, c2, -L);
+    return at_exp2(sizeof(T) == 4 ? t - Lr : t);
+  }
+};
+
+// ds / scale of one block (images of its 32 keys and values at row R0), and dq += ds k.
+template <typename T, int DP>
+__device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int R0, int j0, bool inner, const Rows& R,
+                                   const QueryRow<T, DP>& Q, float c2, int lane, f32x16 (&dq)[DP / 32]) {
   typedef Img<T, DP> I;
-  typedef typename Op<T>::Frag Frag;
-  constexpr int NS = DP / 16, NB = BK / 32, NC = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char Kl[BK * I::ROWB];
-  __shared__ __attribute__((aligned(1024))) char Vl[BK * I::ROWB];
+  const int r = lane & 31, hh = lane >> 5;
+  f32x16 sc = {}, dp = {};
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    sc = Op<T>::mma(I::rows(Kl, R0 + r, s, hh), Q.q[s], sc);
+    dp = Op<T>::mma(I::rows(Vl, R0 + r, s, hh), Q.g[s], dp);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sc[i] = Q.p(sc[i], c2) * (dp[i] - Q.dot);
+  if (!inner) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int j = j0 + at_pos(i, hh);
+      sc[i] = j >= R.start && j <= R.row ? sc[i] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    const typename Op<T>::Frag sf = Op<T>::pack(sc, kk);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) dq[c] = Op<T>::mma(I::cols(Kl, R0, kk, c, lane), sf, dq[c]);
+  }
+}
+
+// dq, and D_i for the key side. Tiles and waves as the forward's.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS, 2) void k_attn_dq(AttnArgs a) {
+  constexpr int BK = FwdCfg<T, DP>::BK, TILE = FwdCfg<T, DP>::TILE, NC = DP / 32;
+  AT_TWO_BUFFERS(2 * TILE);
   __shared__ int ends[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   int h, q0;
-  at_query_tile(a, h, q0);
-  const int hk = h / (a.H / a.KV), row = q0 + 32 * w + r, rc = min(row, a.N - 1);
+  at_query_tile<AT_ROWS>(a, h, q0);
+  const int hk = h / (a.H / a.KV), row0 = q0 + 32 * w;
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
-  Frag qf[NS], gf[NS];
-  at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, qf);
-  at_row<T, DP>((const T*)a.d_out + ((int64_t)rc * a.H + h) * a.D, a.D, hh, gf);
-  int start, end;
-  at_sequence(a.off, a.S, a.N, row, start, end);
-  const bool in = start <= row;
-  const int lo = at_wave_min(in ? start : 0x7FFFFFFF), hi = at_wave_max(in ? row + 1 : -1);
-  const int inner_lo = at_wave_max(in ? start : -1);
-  const bool whole = __all(in);
-  if (lane == 0) ends[0][w] = lo, ends[1][w] = hi;
-  float dot = 0.f, L = 0.f;
-  if (in) {
-    Frag of[NS];
-    at_row<T, DP>((const T*)a.out + ((int64_t)rc * a.H + h) * a.D, a.D, hh, of);
-#pragma unroll
-    for (int s = 0; s < NS; ++s) dot = Op<T>::dot(gf[s], of[s], dot);
-    L = a.stats[(int64_t)h * a.N + row];
-  }
-  dot += __shfl_xor(dot, 32, 64);
-  if (in && hh == 0) a.rowdot[(int64_t)h * a.N + row] = dot;
-  __syncthreads();
-  const int blo = min(min(ends[0][0], ends[0][1]), min(ends[0][2], ends[0][3]));
-  const int bhi = max(max(ends[1][0], ends[1][1]), max(ends[1][2], ends[1][3]));
-
+  Rows R;
+  R.init(a, row0 + r);
+  QueryRow<T, DP> Q;
+  Q.init(a, h, R, hh, true);
+  int blo, bhi;
+  at_block_range(R.lo, R.hi, lane, w, ends, blo, bhi);
+  Loader<T, DP, BK, 4> lk, lv;
+  lk.init(a.k_row, a.D, w, lane);
+  lv.init(a.v_row, a.D, w, lane);
   f32x16 dq[NC] = {};
-  Stage<T, DP, BK> sk, sv;
-  if (blo < bhi) {
-    sk.load(kb, a.k_row, blo, blo, bhi - 1, a.D, tid);
-    sv.load(vb, a.v_row, blo, blo, bhi - 1, a.D, tid);
+  auto issue = [&](int j0, char* img) {
+    lk.issue(kb, a.k_row, j0, bhi - 1, a.D, img, w);
+    lv.issue(vb, a.v_row, j0, bhi - 1, a.D, img + TILE, w);
+  };
+  auto tile = [&](int j0, const char* Kl, char* next) {
+    at_exchange();
+    if (j0 + BK < bhi) issue(j0 + BK, next);
+    if (j0 >= R.hi || j0 + BK <= R.lo) return;
+    const bool inner = R.inner(j0, BK, row0);
+#pragma unroll
+    for (int b = 0; b < BK / 32; ++b)
+      at_dq_block<T, DP>(Kl, Kl + TILE, 32 * b, j0 + 32 * b, inner, R, Q, a.c2, lane, dq);
+  };
+  if (blo < bhi) issue(blo, ldsA);
+  for (int j0 = blo; j0 < bhi; j0 += 2 * BK) {
+    tile(j0, ldsA, ldsB);
+    if (j0 + BK < bhi) tile(j0 + BK, ldsB, ldsA);
   }
-  for (int j0 = blo; j0 < bhi; j0 += BK) {
-    __syncthreads();
-    sk.store(Kl, tid);
-    sv.store(Vl, tid);
-    __syncthreads();
-    if (j0 + BK < bhi) {
-      sk.load(kb, a.k_row, j0 + BK, blo, bhi - 1, a.D, tid);
-      sv.load(vb, a.v_row, j0 + BK, blo, bhi - 1, a.D, tid);
-    }
-    if (j0 >= hi || j0 + BK <= lo) continue;
-    const bool inner = whole && j0 >= inner_lo && j0 + BK <= q0 + 32 * w + 1;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      f32x16 sc = {}, dp = {};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        sc = Op<T>::mma(I::rows(Kl, 32 * b + r, s, hh), qf[s], sc);
-        dp = Op<T>::mma(I::rows(Vl, 32 * b + r, s, hh), gf[s], dp);
-      }
-      float ds[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        ds[i] = at_exp2(fmaf(sc[i], a.c2, -L)) * (dp[i] - dot);
-        if (!inner) {
-          const int j = j0 + 32 * b + at_pos(i, hh);
-          ds[i] = j >= start && j <= row ? ds[i] : 0.f;
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const Frag sf = Op<T>::pack(ds + 8 * kk);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) dq[c] = Op<T>::mma(I::cols(Kl, 32 * b, kk, c, lane), sf, dq[c]);
-      }
-    }
-  }
-  float sum = 0.f;
-  if (row < a.N && (in || a.fill)) {
-    T* orow = (T*)a.dq + ((int64_t)row * a.H + h) * a.D;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int ch = 32 * c + 8 * g + 4 * hh;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = in ? dq[c][4 * g + e] * a.scale : 0.f;
-          sum = fmaf(v[e], 0.f, sum);
-        }
-        if (ch < a.D) Op<T>::store4(orow + ch, v[0], v[1], v[2], v[3]);
-      }
-  }
-  unsigned long long bad = __ballot(in && sum != 0.f);
+  bool odd = false;
+  if (R.row < a.N && (R.in || a.fill))
+    odd = at_store_row<T, NC>((T*)a.dq + ((int64_t)R.row * a.H + h) * a.D, nullptr, dq, a.scale, R.in, a.D, hh);
+  unsigned long long bad = __ballot(odd);
   bad = (bad | bad >> 32) & 0xFFFFFFFFull;
   while (bad) {
     const int i = __builtin_ctzll(bad);
     bad &= bad - 1;
-    at_dq_row<T>(at_args(), h, q0 + 32 * w + i, __shfl(start, i, 64), lane);
+    at_dq_row<T>(at_args(), h, row0 + i, __shfl(R.start, i, 64), lane);
+  }
+}
+
+// The form for small grids, as the forward's, but a block's keys are read to the end of it:
+// with bf16 the next block has a buffer of its own, with fp32 it is loaded behind this one
+// (its products take eight times as long, the loads' latency is small beside them).
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
+  typedef Img<T, DP> I;
+  constexpr int TILE = 32 * I::ROWB, NC = DP / 32, NBUF = sizeof(T) == 2 ? 2 : 1;
+  typedef Loader<T, DP, 32, 1> Ld;
+  constexpr int MINE = 2 * TILE;
+  static_assert(4 * MINE >= 4 * Join<DP>::SHARE, "a buffer holds the waves' rows");
+  AT_TWO_BUFFERS(4 * MINE);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  int h, q0;
+  at_query_tile<AT_SPLIT>(a, h, q0);
+  const int hk = h / (a.H / a.KV);
+  const T* kb = (const T*)a.k + hk * a.k_head;
+  const T* vb = (const T*)a.v + hk * a.v_head;
+  Rows R;
+  R.init(a, q0 + r);
+  QueryRow<T, DP> Q;
+  Q.init(a, h, R, hh, w == 0);
+  Ld lk, lv;
+  lk.init(a.k_row, a.D, 0, lane);
+  lv.init(a.v_row, a.D, 0, lane);
+  f32x16 dq[NC] = {};
+  auto issue = [&](int j, char* img) {
+    lk.issue(kb, a.k_row, j, R.hi - 1, a.D, img, 0);
+    lv.issue(vb, a.v_row, j, R.hi - 1, a.D, img + TILE, 0);
+  };
+  auto block = [&](int j0, char* Kl, char* next) {
+    const bool more = j0 + 128 < R.hi;
+    if (NBUF == 2 && more) issue(j0 + 128, next);  // its last reads were waited for
+    at_landed<2 * Ld::NI>(NBUF == 2 && more);
+    at_dq_block<T, DP>(Kl, Kl + TILE, 0, j0, R.inner(j0, 32, q0), R, Q, a.c2, lane, dq);
+    at_lds_free();
+    if (NBUF == 1 && more) issue(j0 + 128, next);
+  };
+  char* mineA = ldsA + w * MINE;
+  char* mineB = NBUF == 2 ? ldsB + w * MINE : mineA;
+  const int first = R.lo < R.hi ? R.lo + 32 * w : R.hi;
+  if (first < R.hi) issue(first, mineA);
+  for (int j0 = first; j0 < R.hi; j0 += 256) {
+    block(j0, mineA, mineB);
+    if (j0 + 128 < R.hi) block(j0 + 128, mineB, mineA);
+  }
+  __syncthreads();
+  const Join<DP> join = {ldsA, ldsA + 2 * Join<DP>::SHARE};
+  join.put(w, r, hh, dq, a.scale);
+  __syncthreads();
+  const int rr = tid >> 3, row = q0 + rr;
+  const bool in = __shfl(R.start, rr, 64) <= row;
+  float odd = 0.f;
+  if (row < a.N && (in || a.fill)) {
+#pragma unroll
+    for (int q = 0; q < DP / 32; ++q) {
+      const int ch = 4 * ((tid & 7) + 8 * q);
+      float4 v = join.sum(rr, ch);
+      if (!in) v = make_float4(0.f, 0.f, 0.f, 0.f);
+      odd = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, odd))));
+      if (ch < a.D) Op<T>::store4((T*)a.dq + ((int64_t)row * a.H + h) * a.D + ch, v.x, v.y, v.z, v.w);
+    }
+  }
+  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
+    const int i = 8 * w + __builtin_ctz(bad);
+    at_dq_row<T>(at_args(), h, q0 + i, __shfl(R.start, i, 64), lane);
   }
 }
 
 // ---------------------------------------------------------------- backward: keys
-// dk and dv of a tile of 128 keys and one key head: every query head of the group, and the
-// queries from the tile's first row to the last row of its rows' sequences, BQ at a time.
-// The accumulators hold dk^T and dv^T (a lane one key row); shared key heads are summed
-// here, in head order, so the result is the same on every run. Grid: key tiles x key heads,
-// the tiles with the most queries (a long sequence's first) first.
-template <typename T, int DP, int BQ>
-__global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv(AttnArgs a) {
+// A lane's key row and the queries that its wave meets.
+struct Keys {
+  int row, start, end;
+  bool in;
+  int lo, hi;    // queries the wave meets: [lo, hi)
+  int inner_hi;  // smallest end of the wave's rows
+  bool whole;
+  __device__ inline void init(const AttnArgs& a, int r) {
+    row = r;
+    at_sequence(a.off, a.S, a.N, row, start, end);
+    in = start <= row;
+    lo = at_wave_min(in ? row : 0x7FFFFFFF);
+    hi = at_wave_max(in ? end : -1);
+    inner_hi = at_wave_min(in ? end : 0x7FFFFFFF);
+    whole = __all(in);
+  }
+  // Every query of [i, i + n) sees every key of the wave (its first row is row0).
+  __device__ inline bool inner(int i, int n, int row0) const { return whole && i >= row0 + 31 && i + n <= inner_hi; }
+};
+
+// One block of 32 queries (images at Ql, Gl; L, D and L's remainder in qs): dv += p do,
+// dk += ds / scale q. vf(s) gives fragment s of the lane's value row.
+template <typename T, int DP, typename VF>
+__device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, const float (*qs)[32], int i0, bool inner,
+                                    const Keys& K, const typename Op<T>::Frag (&kf)[DP / 16], VF&& vf, float c2,
+                                    int lane, f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32]) {
   typedef Img<T, DP> I;
   typedef typename Op<T>::Frag Frag;
-  constexpr int NS = DP / 16, NB = BQ / 32, NC = DP / 32;
-  __shared__ __attribute__((aligned(1024))) char Ql[BQ * I::ROWB];
-  __shared__ __attribute__((aligned(1024))) char Gl[BQ * I::ROWB];
-  __shared__ __attribute__((aligned(16))) float qs[2][BQ];  // L and D of the staged queries
-  __shared__ int ends[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 31, hh = lane >> 5;
-  const int hk = blockIdx.x % a.KV, k0 = blockIdx.x / a.KV * AT_ROWS, rep = a.H / a.KV;
-  const int row = k0 + 32 * w + r, rc = min(row, a.N - 1);
-  Frag kf[NS], vf[NS];
-  at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + hk * a.k_head, a.D, hh, kf);
-  at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + hk * a.v_head, a.D, hh, vf);
-  int start, end;
-  at_sequence(a.off, a.S, a.N, row, start, end);
-  const bool in = start <= row;
-  const int lo = at_wave_min(in ? row : 0x7FFFFFFF), hi = at_wave_max(in ? end : -1);
-  const int inner_hi = at_wave_min(in ? end : 0x7FFFFFFF);  // smallest end of the wave's rows
-  const bool whole = __all(in);
-  if (lane == 0) ends[w] = hi;
-  // the block's first row in a sequence: rows of none come before the first sequence or
-  // behind the last, so it is the tile's first row or the first sequence's
-  const int blo = max(k0, a.S > 0 ? max(a.off[0], 0) : 0);
-  __syncthreads();
-  const int bhi = max(max(ends[0], ends[1]), max(ends[2], ends[3]));
-
-  f32x16 dk[NC] = {}, dv[NC] = {};
-  Stage<T, DP, BQ> sq, sg;
-  float st = 0.f;  // L (threads below BQ) or D (the next BQ) of one staged query
-  const int nq = blo < bhi ? (bhi - blo + BQ - 1) / BQ : 0, total = nq * rep;
-  auto load = [&](int t) {
-    const int h = hk * rep + t / nq, i0 = blo + t % nq * BQ;
-    sq.load((const T*)a.q + h * a.q_head, a.q_row, i0, blo, bhi - 1, a.D, tid);
-    sg.load((const T*)a.d_out + (int64_t)h * a.D, (int64_t)a.H * a.D, i0, blo, bhi - 1, a.D, tid);
-    const int64_t at = (int64_t)h * a.N + min(i0 + tid % BQ, bhi - 1);
-    if (tid < 2 * BQ) st = tid < BQ ? a.stats[at] : a.rowdot[at];
-  };
-  if (total) load(0);
-  for (int t = 0; t < total; ++t) {
-    const int i0 = blo + t % nq * BQ;
-    __syncthreads();
-    sq.store(Ql, tid);
-    sg.store(Gl, tid);
-    if (tid < 2 * BQ) qs[tid / BQ][tid % BQ] = st;
-    __syncthreads();
-    if (t + 1 < total) load(t + 1);
-    if (i0 >= hi || i0 + BQ <= lo) continue;
-    const bool inner = whole && i0 >= k0 + 32 * w + 31 && i0 + BQ <= inner_hi;
+  const int r = lane & 31, hh = lane >> 5;
+  f32x16 p = {}, ds = {};
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      f32x16 sc = {}, dp = {};
+  for (int s = 0; s < DP / 16; ++s) {
+    p = Op<T>::mma(I::rows(Ql, r, s, hh), kf[s], p);
+    ds = Op<T>::mma(I::rows(Gl, r, s, hh), vf(s), ds);
+  }
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        sc = Op<T>::mma(I::rows(Ql, 32 * b + r, s, hh), kf[s], sc);
-        dp = Op<T>::mma(I::rows(Gl, 32 * b + r, s, hh), vf[s], dp);
-      }
-      float p[16], ds[16];
+  for (int g = 0; g < 4; ++g) {
+    const float4 L = *(const float4*)&qs[0][8 * g + 4 * hh], D = *(const float4*)&qs[1][8 * g + 4 * hh];
+    const float Lv[4] = {L.x, L.y, L.z, L.w}, Dv[4] = {D.x, D.y, D.z, D.w};
+    float Rv[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(T) == 4) {
+      const float4 Lr = *(const float4*)&qs[2][8 * g + 4 * hh];
+      Rv[0] = Lr.x, Rv[1] = Lr.y, Rv[2] = Lr.z, Rv[3] = Lr.w;
+    }
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4 L = *(const float4*)&qs[0][32 * b + 8 * g + 4 * hh];
-        const float4 Dt = *(const float4*)&qs[1][32 * b + 8 * g + 4 * hh];
-        const float Lv[4] = {L.x, L.y, L.z, L.w}, Dv[4] = {Dt.x, Dt.y, Dt.z, Dt.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * g + e;
-          p[i] = at_exp2(fmaf(sc[i], a.c2, -Lv[e]));
-          ds[i] = p[i] * (dp[i] - Dv[e]);
-          if (!inner) {
-            const int qi = i0 + 32 * b + at_pos(i, hh);
-            const bool ok = qi >= row && qi < end;
-            p[i] = ok ? p[i] : 0.f;
-            ds[i] = ok ? ds[i] : 0.f;
-          }
-        }
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const Frag pf = Op<T>::pack(p + 8 * kk), sf = Op<T>::pack(ds + 8 * kk);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          dv[c] = Op<T>::mma(I::cols(Gl, 32 * b, kk, c, lane), pf, dv[c]);
-          dk[c] = Op<T>::mma(I::cols(Ql, 32 * b, kk, c, lane), sf, dk[c]);
-        }
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int i = 4 * g + e;
+      float t = fmaf(p[i], c2, -Lv[e]);
+      if constexpr (sizeof(T) == 4) t -= Rv[e];
+      p[i] = at_exp2(t);
+      ds[i] = p[i] * (ds[i] - Dv[e]);
     }
   }
-  float sum = 0.f;
-  if (row < a.N && (in || a.fill)) {
-    T* krow = (T*)a.dk + ((int64_t)row * a.KV + hk) * a.D;
-    T* vrow = (T*)a.dv + ((int64_t)row * a.KV + hk) * a.D;
+  if (!inner) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int ch = 32 * c + 8 * g + 4 * hh;
-        float x[4], y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = in ? dk[c][4 * g + e] * a.scale : 0.f;
-          y[e] = in ? dv[c][4 * g + e] : 0.f;
-          sum = fmaf(x[e], 0.f, fmaf(y[e], 0.f, sum));
-        }
-        if (ch < a.D) {
-          Op<T>::store4(krow + ch, x[0], x[1], x[2], x[3]);
-          Op<T>::store4(vrow + ch, y[0], y[1], y[2], y[3]);
-        }
-      }
+    for (int i = 0; i < 16; ++i) {
+      const int q = i0 + at_pos(i, hh);
+      const bool ok = q >= K.row && q < K.end;
+      p[i] = ok ? p[i] : 0.f;
+      ds[i] = ok ? ds[i] : 0.f;
+    }
   }
-  unsigned long long bad = __ballot(in && sum != 0.f);
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) {
+    const Frag pf = Op<T>::pack(p, kk), sf = Op<T>::pack(ds, kk);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      dv[c] = Op<T>::mma(I::cols(Gl, 0, kk, c, lane), pf, dv[c]);
+      dk[c] = Op<T>::mma(I::cols(Ql, 0, kk, c, lane), sf, dk[c]);
+    }
+  }
+}
+
+// Key tile, key head and share of its query heads of a block: the tiles with the most
+// queries (a long sequence's first) first.
+struct KeyTile {
+  int hk, k0, share, h0, nh;
+  __device__ inline KeyTile(const AttnArgs& a, int rows) {
+    const int id = blockIdx.x, x = id % (a.KV * a.hs), rep = a.H / a.KV;
+    hk = x % a.KV;
+    share = x / a.KV;
+    k0 = id / (a.KV * a.hs) * rows;
+    nh = rep / a.hs;
+    h0 = hk * rep + share * nh;
+  }
+};
+
+// L, D (and L's remainder) of one query, for thread q of a block of 32.
+template <typename T>
+struct QueryStats {
+  float L, D, R;
+  __device__ inline void load(const AttnArgs& a, int h, int row) {
+    const int64_t at = (int64_t)h * a.N + row;
+    L = a.stats[at], D = a.rowdot[at];
+    if constexpr (sizeof(T) == 4) R = a.stats[at + (int64_t)a.H * a.N];
+  }
+  __device__ inline void store(float (*qs)[32], int q) const {
+    qs[0][q] = L, qs[1][q] = D;
+    if constexpr (sizeof(T) == 4) qs[2][q] = R;
+  }
+};
+
+// Stores a lane's dk and dv rows, or its share's fp32 sums.
+template <typename T, int DP>
+__device__ inline bool at_store_keys(const AttnArgs& a, const KeyTile& t, const Keys& K, const f32x16 (&dk)[DP / 32],
+                                     const f32x16 (&dv)[DP / 32], int hh) {
+  if (K.row >= a.N) return false;
+  const int64_t at = ((int64_t)K.row * a.KV + t.hk) * a.D;
+  if (a.hs > 1) {
+    if (!K.in) return false;  // the sum over shares knows
+    const int64_t plane = (int64_t)a.N * a.KV * a.D;
+    float* pk = a.part + 2 * t.share * plane + at;
+    const bool x = at_store_row<float, DP / 32>(pk, nullptr, dk, a.scale, true, a.D, hh);
+    const bool y = at_store_row<float, DP / 32>(pk + plane, nullptr, dv, 1.f, true, a.D, hh);
+    return x || y;
+  }
+  if (!K.in && !a.fill) return false;
+  const bool x = at_store_row<T, DP / 32>((T*)a.dk + at, nullptr, dk, a.scale, K.in, a.D, hh);
+  const bool y = at_store_row<T, DP / 32>((T*)a.dv + at, nullptr, dv, 1.f, K.in, a.D, hh);
+  return x || y;
+}
+
+// dk and dv of a tile of 128 keys, 32 a wave, over a share of its group's query heads: the
+// queries from the tile's first row to the end of its rows' sequences, 32 at a time in two
+// buffers. The accumulators hold dk^T and dv^T (a lane one key row); heads are added in
+// order, so the result is the same on every run. The keys' fragments stay in registers and
+// the values' in LDS: with both in registers a wave takes more than 256 and a SIMD holds
+// one, with nothing beside it while it waits.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename Op<T>::Frag Frag;
+  constexpr int TILE = 32 * I::ROWB, NS = DP / 16, NC = DP / 32;
+  constexpr int VLDS = sizeof(T) == 2 ? AT_ROWS * I::ROWB : 16;
+  AT_TWO_BUFFERS(2 * TILE);
+  __shared__ __attribute__((aligned(1024))) char Vl[VLDS];
+  __shared__ __attribute__((aligned(16))) float qs[2][3][32];
+  __shared__ int ends[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  const KeyTile t(a, AT_ROWS);
+  const int row0 = t.k0 + 32 * w, rc = min(row0 + r, a.N - 1);
+  Frag kf[NS], vf[sizeof(T) == 2 ? 1 : NS];
+  at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
+  if constexpr (sizeof(T) == 2) {
+    Loader<T, DP, AT_ROWS, 4> lv;
+    lv.init(a.v_row, a.D, w, lane);
+    lv.issue((const T*)a.v + t.hk * a.v_head, a.v_row, t.k0, a.N - 1, a.D, Vl, w);
+  } else {
+    at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
+  }
+  auto value = [&](int s) -> Frag {
+    if constexpr (sizeof(T) == 2) return I::rows(Vl, 32 * w + r, s, hh);
+    else return vf[s];
+  };
+  Keys K;
+  K.init(a, row0 + r);
+  int blo, bhi;
+  at_block_range(K.lo, K.hi, lane, w, ends, blo, bhi);
+  Loader<T, DP, 32, 4> lq, lg;
+  lq.init(a.q_row, a.D, w, lane);
+  lg.init((int64_t)a.H * a.D, a.D, w, lane);
+  const int nq = blo < bhi ? (bhi - blo + 31) / 32 : 0, total = nq * t.nh;
+  QueryStats<T> st;
+  int nh = t.h0, ni = blo;  // the next block to load
+  auto issue = [&](char* img) {
+    lq.issue((const T*)a.q + nh * a.q_head, a.q_row, ni, bhi - 1, a.D, img, w);
+    lg.issue((const T*)a.d_out + (int64_t)nh * a.D, (int64_t)a.H * a.D, ni, bhi - 1, a.D, img + TILE, w);
+    if (tid < 32) st.load(a, nh, min(ni + tid, bhi - 1));
+    ni += 32;
+    if (ni >= bhi) ni = blo, ++nh;
+  };
+  f32x16 dk[NC] = {}, dv[NC] = {};
+  if (total) issue(ldsA);
+  int i0 = blo;
+  auto block = [&](int n, const char* Ql, char* next) {
+    if (tid < 32) st.store(qs[n & 1], tid);
+    at_exchange();
+    if (n + 1 < total) issue(next);
+    if (i0 < K.hi && i0 + 32 > K.lo)
+      at_dkv_block<T, DP>(Ql, Ql + TILE, qs[n & 1], i0, K.inner(i0, 32, row0), K, kf, value, a.c2, lane, dk, dv);
+    i0 += 32;
+    if (i0 >= bhi) i0 = blo;
+  };
+  for (int n = 0; n < total; n += 2) {
+    block(n, ldsA, ldsB);
+    if (n + 1 < total) block(n + 1, ldsB, ldsA);
+  }
+  unsigned long long bad = __ballot(at_store_keys<T, DP>(a, t, K, dk, dv, hh));
   bad = (bad | bad >> 32) & 0xFFFFFFFFull;
   while (bad) {
     const int i = __builtin_ctzll(bad);
     bad &= bad - 1;
-    at_dkv_row<T>(at_args(), hk, k0 + 32 * w + i, __shfl(end, i, 64), lane);
+    at_dkv_row<T>(at_args(), t.hk, t.share, row0 + i, __shfl(K.end, i, 64), lane);
   }
+}
+
+// The form for small grids: a block of 32 keys whose four waves take every fourth block of
+// 32 queries (over the share's heads), and join their sums at the end.
+template <typename T, int DP>
+__global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
+  typedef Img<T, DP> I;
+  typedef typename Op<T>::Frag Frag;
+  constexpr int TILE = 32 * I::ROWB, NS = DP / 16, NC = DP / 32, NBUF = sizeof(T) == 2 ? 2 : 1;
+  typedef Loader<T, DP, 32, 1> Ld;
+  constexpr int MINE = 2 * TILE;
+  AT_TWO_BUFFERS(4 * MINE);
+  __shared__ __attribute__((aligned(16))) float qs[4][3][32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
+  const KeyTile t(a, AT_SPLIT);
+  const int rc = min(t.k0 + r, a.N - 1);
+  Frag kf[NS], vf[NS];
+  at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
+  at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
+  auto value = [&](int s) -> const Frag& { return vf[s]; };
+  Keys K;
+  K.init(a, t.k0 + r);
+  Ld lq, lg;
+  lq.init(a.q_row, a.D, 0, lane);
+  lg.init((int64_t)a.H * a.D, a.D, 0, lane);
+  const int nq = K.lo < K.hi ? (K.hi - K.lo + 31) / 32 : 0, total = nq * t.nh;
+  QueryStats<T> st;
+  auto issue = [&](int n, char* img) {
+    const int h = t.h0 + n / nq, i = K.lo + n % nq * 32;
+    lq.issue((const T*)a.q + h * a.q_head, a.q_row, i, K.hi - 1, a.D, img, 0);
+    lg.issue((const T*)a.d_out + (int64_t)h * a.D, (int64_t)a.H * a.D, i, K.hi - 1, a.D, img + TILE, 0);
+    if (lane < 32) st.load(a, h, min(i + lane, K.hi - 1));
+  };
+  f32x16 dk[NC] = {}, dv[NC] = {};
+  auto block = [&](int n, const char* Ql, char* next) {
+    const int i0 = K.lo + n % nq * 32;
+    const bool more = n + 4 < total;
+    if (lane < 32) st.store(qs[w], lane);
+    at_landed<0>(false);
+    if (NBUF == 2 && more) issue(n + 4, next);
+    at_dkv_block<T, DP>(Ql, Ql + TILE, qs[w], i0, K.inner(i0, 32, t.k0), K, kf, value, a.c2, lane, dk, dv);
+    at_lds_free();
+    if (NBUF == 1 && more) issue(n + 4, next);
+  };
+  char* mineA = ldsA + w * MINE;
+  char* mineB = NBUF == 2 ? ldsB + w * MINE : mineA;
+  if (w < total) issue(w, mineA);
+  for (int n = w; n < total; n += 8) {
+    block(n, mineA, mineB);
+    if (n + 4 < total) block(n + 4, mineB, mineA);
+  }
+  // dk, then dv, through the same LDS
+  const Join<DP> join = {ldsA, ldsA + 2 * Join<DP>::SHARE};
+  float odd = 0.f;
+  const int rr = tid >> 3, row = t.k0 + rr;
+  const bool in = __shfl(K.start, rr, 64) <= row;
+  const int64_t at = ((int64_t)row * a.KV + t.hk) * a.D, plane = (int64_t)a.N * a.KV * a.D;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+    join.put(w, r, hh, which ? dv : dk, which ? 1.f : a.scale);
+    __syncthreads();
+    if (row < a.N && (in || (a.fill && a.hs == 1))) {
+#pragma unroll
+      for (int q = 0; q < DP / 32; ++q) {
+        const int ch = 4 * ((tid & 7) + 8 * q);
+        float4 v = join.sum(rr, ch);
+        if (!in) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        odd = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, odd))));
+        if (ch >= a.D) continue;
+        if (a.hs > 1) *(float4*)(a.part + (2 * t.share + which) * plane + at + ch) = v;
+        else Op<T>::store4((T*)(which ? a.dv : a.dk) + at + ch, v.x, v.y, v.z, v.w);
+      }
+    }
+  }
+  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
+    const int i = 8 * w + __builtin_ctz(bad);
+    at_dkv_row<T>(at_args(), t.hk, t.share, t.k0 + i, __shfl(K.end, i, 64), lane);
+  }
+}
+
+// dk and dv as the shares' sums in share order; rows of no sequence as `fill` says. One
+// thread per four values.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_dkv_sum(AttnArgs a) {
+  const int64_t plane = (int64_t)a.N * a.KV * a.D;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * plane) return;
+  const int which = i >= plane;
+  const int64_t at = i - which * plane;
+  int start, end;
+  at_sequence(a.off, a.S, a.N, (int)(at / ((int64_t)a.KV * a.D)), start, end);
+  const bool in = end > start;
+  if (!in && !a.fill) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (in)
+    for (int h = 0; h < a.hs; ++h) {
+      const float4 v = *(const float4*)(a.part + (2 * h + which) * plane + at);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+  Op<T>::store4((T*)(which ? a.dv : a.dk) + at, s.x, s.y, s.z, s.w);
 }
 
 // ---------------------------------------------------------------- host side
@@ -706,7 +1240,7 @@ int at_check(const char* what, int dtype, int64_t rows, int H, int KV, int D, co
   if (rows < 0 || n_seq < 0) return fail(PD_EINVAL, w + ": rows and sequences must be >= 0");
   if (H <= 0 || KV <= 0 || H % KV) return fail(PD_EINVAL, w + ": n_head must be a multiple of n_kv_head");
   if (D <= 0 || D % 8 || D > 128) return fail(PD_EUNSUPPORTED, w + ": head_dim must be a multiple of 8 up to 128");
-  if (rows > (1 << 30) || n_seq > (1 << 30) || cdiv(rows, AT_ROWS) * H > 0x7FFFFFFF)
+  if (rows > (1 << 30) || n_seq > (1 << 30) || cdiv(rows, AT_SPLIT) * H > 0x7FFFFFFF)
     return fail(PD_EUNSUPPORTED, w + ": rows too many");
   if (!std::isfinite(scale)) return fail(PD_EINVAL, w + ": scale must be finite");
   if (!rows) return PD_OK;
@@ -714,6 +1248,10 @@ int at_check(const char* what, int dtype, int64_t rows, int H, int KV, int D, co
   const int per = dtype == PD_DTYPE_F32 ? 4 : 8;
   for (int i = 0; i < 6; ++i)
     if (strides[i] % per) return fail(PD_EUNSUPPORTED, w + ": strides must be whole 16-byte words");
+  for (int i = 0; i < 6; i += 2)  // a tile's 128 rows within a 31-bit offset
+    if (strides[i] < 0 || strides[i] * (per == 4 ? 4 : 2) > (1 << 23))
+      return fail(PD_EUNSUPPORTED, w + ": row strides of at most 8 MiB");
+  if ((int64_t)H * D * (per == 4 ? 4 : 2) > (1 << 23)) return fail(PD_EUNSUPPORTED, w + ": rows of at most 8 MiB");
   for (int i = 0; i < n_tensors; ++i) {
     if (!tensors[i]) return fail(PD_EINVAL, w + ": null pointer");
     if ((uintptr_t)tensors[i] & 15) return fail(PD_EUNSUPPORTED, w + ": tensors must be 16-byte aligned");
@@ -721,17 +1259,47 @@ int at_check(const char* what, int dtype, int64_t rows, int H, int KV, int D, co
   return PD_OK;
 }
 
-// F(T, DP, rows a stage of LDS holds): 64 rows, 32 where a row is 512 bytes.
+// F(T, DP): the widths the kernels are built for.
 template <typename F>
 void at_form(int dtype, int D, F&& f) {
   using std::integral_constant;
-  if (dtype == PD_DTYPE_BF16) {
-    if (D <= 64) f(bf16_t(0), integral_constant<int, 64>{}, integral_constant<int, 64>{});
-    else f(bf16_t(0), integral_constant<int, 128>{}, integral_constant<int, 64>{});
-  } else {
-    if (D <= 64) f(0.f, integral_constant<int, 64>{}, integral_constant<int, 64>{});
-    else f(0.f, integral_constant<int, 128>{}, integral_constant<int, 32>{});
-  }
+  auto width = [&](auto t) {
+    if (D <= 64) f(t, integral_constant<int, 64>{});
+    else if (D <= 96) f(t, integral_constant<int, 96>{});
+    else f(t, integral_constant<int, 128>{});
+  };
+  if (dtype == PD_DTYPE_BF16) width(bf16_t(0));
+  else width(0.f);
+}
+
+// Blocks below which a launch leaves CUs without one of the two it holds.
+constexpr int64_t AT_FULL = 512;
+
+bool at_query_split(int64_t rows, int H) { return cdiv(rows, AT_ROWS) * H < AT_FULL; }
+
+// Shares of a group's heads and the tile of the key side: as few shares as fill the GPU
+// with 128-key tiles, else 32-key tiles whose waves share the queries.
+struct KeyPlan {
+  int hs;
+  bool split;
+};
+KeyPlan at_key_plan(int64_t rows, int H, int KV) {
+  const int rep = H / KV;
+  for (int hs = 1; hs <= rep; ++hs)
+    if (rep % hs == 0 && cdiv(rows, AT_ROWS) * KV * hs >= 4 * AT_FULL) return {hs, false};
+  if (cdiv(rows, AT_ROWS) * KV * rep >= AT_FULL) return {rep, false};
+  for (int hs = 1; hs <= rep; ++hs)
+    if (rep % hs == 0 && cdiv(rows, AT_SPLIT) * KV * hs >= AT_FULL) return {hs, true};
+  return {rep, true};
+}
+
+void at_fill_args(AttnArgs& a, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                  const void* v, int64_t v_row, int64_t v_head, int64_t rows, int H, int KV, int D, const int32_t* off,
+                  int64_t n_seq, float scale, int fill) {
+  a.q = q, a.k = k, a.v = v;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.N = (int)rows, a.H = H, a.KV = KV, a.D = D, a.off = off, a.S = (int)n_seq;
+  a.scale = scale, a.c2 = scale * LOG2E, a.fill = fill != 0, a.hs = 1;
 }
 
 }  // namespace
@@ -744,56 +1312,74 @@ extern "C" {
 int pd_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                             const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
                             int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
-                            void* out, float* stats, void* stream) {
+                            void* out, void* out_rest, float* stats, void* stream) {
   const int64_t st[6] = {q_row, q_head, k_row, k_head, v_row, v_head};
   const void* ts[4] = {q, k, v, out};
   if (int rc = at_check("pd_packed_attention_fwd", dtype, rows, n_head, n_kv_head, head_dim, offsets, n_seq, scale, st, ts, 4))
     return rc;
   if (!rows) return PD_OK;
+  if (dtype == PD_DTYPE_F32 && out_rest) return fail(PD_EINVAL, "pd_packed_attention_fwd: out_rest goes with bf16");
+  if ((uintptr_t)out_rest & 15) return fail(PD_EUNSUPPORTED, "pd_packed_attention_fwd: tensors must be 16-byte aligned");
   AttnArgs a = {};
-  a.q = q, a.k = k, a.v = v;
-  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.N = (int)rows, a.H = n_head, a.KV = n_kv_head, a.D = head_dim, a.off = offsets, a.S = (int)n_seq;
-  a.scale = scale, a.c2 = scale * LOG2E, a.fill = fill != 0, a.out = out, a.stats = stats;
-  const unsigned grid = (unsigned)(cdiv(rows, AT_ROWS) * n_head);
-  at_form(dtype, head_dim, [&](auto t, auto dp, auto bk) {
-    hipLaunchKernelGGL((k_attn_fwd<decltype(t), decltype(dp)::value, decltype(bk)::value>), dim3(grid), dim3(AT_THREADS), 0,
-                       (hipStream_t)stream, a);
+  at_fill_args(a, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, rows, n_head, n_kv_head, head_dim, offsets, n_seq,
+               scale, fill);
+  a.out = out, a.rest = out_rest, a.stats = stats;
+  const bool split = at_query_split(rows, n_head);
+  const unsigned grid = (unsigned)(cdiv(rows, split ? AT_SPLIT : AT_ROWS) * n_head);
+  at_form(dtype, head_dim, [&](auto t, auto dp) {
+    typedef decltype(t) T;
+    constexpr int DP = decltype(dp)::value;
+    if (split) hipLaunchKernelGGL((k_attn_fwd_split<T, DP>), dim3(grid), dim3(AT_THREADS), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((k_attn_fwd<T, DP>), dim3(grid), dim3(AT_THREADS), 0, (hipStream_t)stream, a);
   });
   return check_launch("pd_packed_attention_fwd");
 }
 
-size_t pd_packed_attention_bwd_workspace_size(int64_t rows, int n_head) {
-  return rows > 0 && n_head > 0 ? (size_t)rows * n_head * sizeof(float) : 0;
+size_t pd_packed_attention_bwd_workspace_size(int64_t rows, int n_head, int n_kv_head, int head_dim) {
+  if (rows <= 0 || n_head <= 0 || n_kv_head <= 0 || head_dim <= 0 || n_head % n_kv_head) return 0;
+  const int hs = at_key_plan(rows, n_head, n_kv_head).hs;
+  const size_t dots = (size_t)cdiv(rows * n_head, 4) * 16;
+  return dots + (hs > 1 ? (size_t)hs * 2 * rows * n_kv_head * head_dim * sizeof(float) : 0);
 }
 
 int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                             const void* v, int64_t v_row, int64_t v_head, int dtype, int64_t rows, int n_head,
                             int n_kv_head, int head_dim, const int32_t* offsets, int64_t n_seq, float scale, int fill,
-                            const void* out, const float* stats, const void* d_out, void* dq, void* dk, void* dv,
-                            void* workspace, size_t workspace_bytes, void* stream) {
+                            const void* out, const void* out_rest, const float* stats, const void* d_out, void* dq,
+                            void* dk, void* dv, void* workspace, size_t workspace_bytes, void* stream) {
   const int64_t st[6] = {q_row, q_head, k_row, k_head, v_row, v_head};
   const void* ts[8] = {q, k, v, out, d_out, dq, dk, dv};
   if (int rc = at_check("pd_packed_attention_bwd", dtype, rows, n_head, n_kv_head, head_dim, offsets, n_seq, scale, st, ts, 8))
     return rc;
   if (!rows) return PD_OK;
-  if (!stats) return fail(PD_EINVAL, "pd_packed_attention_bwd: null stats");
+  if (!stats || (dtype == PD_DTYPE_BF16 && !out_rest))
+    return fail(PD_EINVAL, "pd_packed_attention_bwd: the forward's stats (and out_rest with bf16) are needed");
+  if (dtype == PD_DTYPE_F32 && out_rest) return fail(PD_EINVAL, "pd_packed_attention_bwd: out_rest goes with bf16");
+  if ((uintptr_t)out_rest & 15) return fail(PD_EUNSUPPORTED, "pd_packed_attention_bwd: tensors must be 16-byte aligned");
   if (!workspace || ((uintptr_t)workspace & 15) ||
-      workspace_bytes < pd_packed_attention_bwd_workspace_size(rows, n_head))
+      workspace_bytes < pd_packed_attention_bwd_workspace_size(rows, n_head, n_kv_head, head_dim))
     return fail(PD_EWORKSPACE, "pd_packed_attention_bwd: workspace");
   AttnArgs a = {};
-  a.q = q, a.k = k, a.v = v;
-  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
-  a.N = (int)rows, a.H = n_head, a.KV = n_kv_head, a.D = head_dim, a.off = offsets, a.S = (int)n_seq;
-  a.scale = scale, a.c2 = scale * LOG2E, a.fill = fill != 0;
-  a.out = const_cast<void*>(out), a.stats = const_cast<float*>(stats);
+  at_fill_args(a, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, rows, n_head, n_kv_head, head_dim, offsets, n_seq,
+               scale, fill);
+  a.out = const_cast<void*>(out), a.rest = const_cast<void*>(out_rest), a.stats = const_cast<float*>(stats);
   a.d_out = d_out, a.dq = dq, a.dk = dk, a.dv = dv, a.rowdot = (float*)workspace;
+  const KeyPlan plan = at_key_plan(rows, n_head, n_kv_head);
+  a.hs = plan.hs;
+  a.part = (float*)((char*)workspace + (size_t)cdiv(rows * n_head, 4) * 16);
   hipStream_t s = (hipStream_t)stream;
-  at_form(dtype, head_dim, [&](auto t, auto dp, auto bk) {
+  const bool split = at_query_split(rows, n_head);
+  const dim3 block(AT_THREADS), gq((unsigned)(cdiv(rows, split ? AT_SPLIT : AT_ROWS) * n_head)),
+      gk((unsigned)(cdiv(rows, plan.split ? AT_SPLIT : AT_ROWS) * n_kv_head * plan.hs)),
+      gs((unsigned)cdiv(2 * rows * n_kv_head * head_dim, 1024));
+  at_form(dtype, head_dim, [&](auto t, auto dp) {
     typedef decltype(t) T;
-    constexpr int DP = decltype(dp)::value, BK = decltype(bk)::value;
-    hipLaunchKernelGGL((k_attn_dq<T, DP, BK>), dim3((unsigned)(cdiv(rows, AT_ROWS) * n_head)), dim3(AT_THREADS), 0, s, a);
-    hipLaunchKernelGGL((k_attn_dkv<T, DP, BK>), dim3((unsigned)(cdiv(rows, AT_ROWS) * n_kv_head)), dim3(AT_THREADS), 0, s, a);
+    constexpr int DP = decltype(dp)::value;
+    if (split) hipLaunchKernelGGL((k_attn_dq_split<T, DP>), gq, block, 0, s, a);
+    else hipLaunchKernelGGL((k_attn_dq<T, DP>), gq, block, 0, s, a);
+    if (plan.split) hipLaunchKernelGGL((k_attn_dkv_split<T, DP>), gk, block, 0, s, a);
+    else hipLaunchKernelGGL((k_attn_dkv<T, DP>), gk, block, 0, s, a);
+    if (plan.hs > 1) hipLaunchKernelGGL((k_attn_dkv_sum<T>), gs, block, 0, s, a);
   });
   return check_launch("pd_packed_attention_bwd");
 }

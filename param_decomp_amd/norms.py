@@ -30,7 +30,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     [..., d], weight and bias fp32 [d] (None: 1 and 0), as the stack steps keep norm weights.
     Differentiable in all three."""
     x = x.contiguous()
-    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return ops.layer_norm_fwd(x, weight, bias, eps=eps)[0]

@@ -367,12 +367,15 @@ def source_ascend(opt: int, sources, grad, state_a=None, state_b=None, *, step_c
     return sources
 
 # ------------------------------------------------- around a language model's decomposed sites
-def _on(name: str, first: torch.Tensor, **others: torch.Tensor | None):
-    """Every tensor on the first one's GPU, which is current for the call."""
-    for label, t in others.items():
-        if t is not None and t.device != first.device:
-            raise L.PDError(f"{name}: {label} is on {t.device}, not {first.device}")
-    return L.on_device(first)
+def _one_device(name: str, first: torch.Tensor, labels: str, *others: torch.Tensor | None) -> torch.device:
+    """The first tensor's device, which the others (named in `labels`) have to share."""
+    device = first.device
+    for i, t in enumerate(others):
+        if t is not None and t.device != device:
+            raise L.PDError(f"{name}: {labels.split()[i]} is on {t.device}, not {device}")
+    if device.type != "cuda":
+        raise L.PDError("pd kernels take GPU tensors")
+    return device
 
 
 def _strides(name: str, label: str, t: torch.Tensor) -> tuple[int, int]:
@@ -381,8 +384,8 @@ def _strides(name: str, label: str, t: torch.Tensor) -> tuple[int, int]:
     per = 16 // t.element_size()
     row = t.stride(0) if rows > 1 else heads * D
     head = t.stride(1) if heads > 1 else D
-    if (D > 1 and t.stride(2) != 1) or row % per or head % per or t.data_ptr() % 16:
-        raise L.PDError(f"{name}: {label} needs a dense last axis and 16-byte aligned rows and heads")
+    if (D > 1 and t.stride(2) != 1) or row % per or head % per or t.data_ptr() % 16 or row * t.element_size() > 1 << 23:
+        raise L.PDError(f"{name}: {label} needs a dense last axis and 16-byte aligned rows (8 MiB apart at most) and heads")
     return row, head
 
 
@@ -409,6 +412,10 @@ def _attention_args(name: str, q, k, v, offsets, scale: float, fill: bool) -> li
     return args + [L.dtype_code(q.dtype), N, H, k.shape[1], D, L.ptr(offsets), offsets.numel() - 1, scale, int(fill)]
 
 
+def _stats_shape(q: torch.Tensor) -> tuple:
+    return (2, q.shape[1], q.shape[0]) if q.dtype == torch.float32 else (q.shape[1], q.shape[0])
+
+
 def _like_rows(name: str, label: str, t: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
     if t.shape != q.shape or t.dtype != q.dtype:
         raise L.PDError(f"{name}: {label} is {tuple(t.shape)} {t.dtype}, not {tuple(q.shape)} {q.dtype}")
@@ -416,37 +423,46 @@ def _like_rows(name: str, label: str, t: torch.Tensor, q: torch.Tensor) -> torch
 
 
 def packed_attention_fwd(q, k, v, offsets, *, scale: float | None = None, out: torch.Tensor | None = None,
-                         want_stats: bool = False):
-    """(out, stats) of causal attention over packed sequences: q [rows, H, head_dim], k and v
+                         want_saved: bool = False):
+    """(out, saved) of causal attention over packed sequences: q [rows, H, head_dim], k and v
     [rows, KV, head_dim] (strided views will do), sequence s in rows offsets[s] ..
     offsets[s + 1] (int32, on the device). `scale`: head_dim^-0.5 by default. Rows of no
-    sequence are zeros, or left as they were in an `out` that is given. stats: fp32
-    [H, rows], None unless wanted."""
+    sequence are zeros, or left as they were in an `out` that is given. saved: what the
+    backward takes, (stats, out_rest), None unless wanted."""
     name = "packed_attention_fwd"
     scale = _attention_checks(name, q, k, v, offsets, scale)
-    with _on(name, q, k=k, v=v, offsets=offsets, out=out):
-        fill = out is None
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if fill else _like_rows(name, "out", out, q)
-        stats = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device) if want_stats else None
-        L.call("pd_packed_attention_fwd", *_attention_args(name, q, k, v, offsets, scale, fill), L.ptr(out), L.ptr(stats),
-               L.stream())
-    return out, stats
+    device = _one_device(name, q, "k v offsets out", k, v, offsets, out)
+    fill = out is None
+    out = torch.empty(q.shape, dtype=q.dtype, device=device) if fill else _like_rows(name, "out", out, q)
+    stats = rest = None
+    if want_saved:
+        stats = torch.empty(_stats_shape(q), dtype=torch.float32, device=device)
+        rest = torch.empty(q.shape, dtype=q.dtype, device=device) if q.dtype == torch.bfloat16 else None
+    L.launch("pd_packed_attention_fwd", device, *_attention_args(name, q, k, v, offsets, scale, fill), L.ptr(out),
+             L.ptr(rest), L.ptr(stats))
+    return out, (stats, rest) if want_saved else None
 
 
-def packed_attention_bwd(q, k, v, offsets, out, stats, d_out, *, scale: float | None = None):
-    """(dq, dk, dv) from the forward's inputs, `out` and `stats`; zeros in rows of no
+def packed_attention_bwd(q, k, v, offsets, out, saved, d_out, *, scale: float | None = None):
+    """(dq, dk, dv) from the forward's inputs, `out` and `saved`; zeros in rows of no
     sequence."""
     name = "packed_attention_bwd"
     scale = _attention_checks(name, q, k, v, offsets, scale)
     _like_rows(name, "out", out, q)
     _like_rows(name, "d_out", d_out, q)
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (q.shape[1], q.shape[0]):
-        raise L.PDError(f"{name}: stats is the forward's, float32 [heads, rows]")
-    with _on(name, q, k=k, v=v, offsets=offsets, out=out, stats=stats, d_out=d_out):
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        ws = L.workspace(L.load().pd_packed_attention_bwd_workspace_size(q.shape[0], q.shape[1]), q.device)
-        L.call("pd_packed_attention_bwd", *_attention_args(name, q, k, v, offsets, scale, True), L.ptr(out), L.ptr(stats),
-               L.ptr(d_out), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(ws), ws.numel(), L.stream())
+    stats, rest = saved
+    if stats.dtype != torch.float32 or tuple(stats.shape) != _stats_shape(q):
+        raise L.PDError(f"{name}: saved stats are the forward's, float32 {_stats_shape(q)}")
+    if (rest is None) != (q.dtype == torch.float32):
+        raise L.PDError(f"{name}: the forward saves out_rest for bfloat16")
+    if rest is not None:
+        _like_rows(name, "out_rest", rest, q)
+    device = _one_device(name, q, "k v offsets out stats out_rest d_out", k, v, offsets, out, stats, rest, d_out)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+    ws = L.workspace(L.load().pd_packed_attention_bwd_workspace_size(q.shape[0], q.shape[1], k.shape[1], q.shape[2]),
+                     device)
+    L.launch("pd_packed_attention_bwd", device, *_attention_args(name, q, k, v, offsets, scale, True), L.ptr(out),
+             L.ptr(rest), L.ptr(stats), L.ptr(d_out), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(ws), ws.numel())
     return dq, dk, dv
 
 
@@ -465,11 +481,11 @@ def layer_norm_fwd(x, weight=None, bias=None, *, eps: float = 1e-5, want_stats: 
     """(y, stats) over the last axis; stats fp32 [rows, 3] for the backward, None unless
     wanted."""
     rows, d = _norm_checks("layer_norm_fwd", x, weight, bias)
-    with _on("layer_norm_fwd", x, weight=weight, bias=bias):
-        y = torch.empty_like(x)
-        stats = torch.empty((rows, 3), dtype=torch.float32, device=x.device) if want_stats else None
-        L.call("pd_layer_norm_fwd", L.ptr(x), L.dtype_code(x.dtype), rows, d, L.ptr(weight), L.ptr(bias), eps, L.ptr(y),
-               L.ptr(stats), L.stream())
+    device = _one_device("layer_norm_fwd", x, "weight bias", weight, bias)
+    y = torch.empty_like(x)
+    stats = torch.empty((rows, 3), dtype=torch.float32, device=device) if want_stats else None
+    L.launch("pd_layer_norm_fwd", device, L.ptr(x), L.dtype_code(x.dtype), rows, d, L.ptr(weight), L.ptr(bias), eps,
+             L.ptr(y), L.ptr(stats))
     return y, stats
 
 
@@ -481,14 +497,13 @@ def layer_norm_bwd(x, d_y, weight, stats, *, want_dx: bool = True, want_dweight:
         raise L.PDError(f"{name}: d_y is {tuple(d_y.shape)} {d_y.dtype}, not {tuple(x.shape)} {x.dtype}")
     if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 3):
         raise L.PDError(f"{name}: stats is the forward's, float32 [rows, 3]")
-    with _on(name, x, d_y=d_y, weight=weight, stats=stats):
-        dx = torch.empty_like(x) if want_dx else None
-        dw, db = (torch.empty(d, dtype=torch.float32, device=x.device) if want else None
-                  for want in (want_dweight, want_dbias))
-        params = want_dweight or want_dbias
-        ws = L.workspace(L.load().pd_layer_norm_bwd_workspace_size(rows, d), x.device) if params else None
-        L.call("pd_layer_norm_bwd", L.ptr(x), L.ptr(d_y), L.dtype_code(x.dtype), rows, d, L.ptr(weight), L.ptr(stats),
-               L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), ws.numel() if params else 0, L.stream())
+    device = _one_device(name, x, "d_y weight stats", d_y, weight, stats)
+    dx = torch.empty_like(x) if want_dx else None
+    dw, db = (torch.empty(d, dtype=torch.float32, device=device) if want else None for want in (want_dweight, want_dbias))
+    params = want_dweight or want_dbias
+    ws = L.workspace(L.load().pd_layer_norm_bwd_workspace_size(rows, d), device) if params else None
+    L.launch("pd_layer_norm_bwd", device, L.ptr(x), L.ptr(d_y), L.dtype_code(x.dtype), rows, d, L.ptr(weight),
+             L.ptr(stats), L.ptr(dx), L.ptr(dw), L.ptr(db), L.ptr(ws), ws.numel() if params else 0)
     return dx, dw, db
 
 
@@ -515,11 +530,12 @@ def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, tem
             raise L.PDError(f"{name}: {label} is float32 {tuple(lead)}, got {t.dtype} {tuple(t.shape)}")
     if not (math.isfinite(temperature) and temperature > 0):
         raise L.PDError(f"{name}: temperature must be positive and finite, got {temperature}")
-    with _on(name, z, top_logits=top_logits, top_indices=top_indices, clean_lse=clean_lse, row_weight=row_weight):
-        kl = torch.empty(lead, dtype=torch.float32, device=z.device) if want_kl else None
-        grad = torch.empty_like(z) if want_grad else None
-        if want_kl or want_grad:
-            L.call("pd_top_kl", L.ptr(z), L.dtype_code(z.dtype), math.prod(lead), V, L.ptr(top_logits),
-                   L.dtype_code(top_logits.dtype), L.ptr(top_indices), 8 * top_indices.element_size(), k,
-                   L.ptr(clean_lse), temperature, L.ptr(row_weight), L.ptr(kl), L.ptr(grad), L.stream())
+    device = _one_device(name, z, "top_logits top_indices clean_lse row_weight", top_logits, top_indices, clean_lse,
+                         row_weight)
+    kl = torch.empty(lead, dtype=torch.float32, device=device) if want_kl else None
+    grad = torch.empty_like(z) if want_grad else None
+    if want_kl or want_grad:
+        L.launch("pd_top_kl", device, L.ptr(z), L.dtype_code(z.dtype), math.prod(lead), V, L.ptr(top_logits),
+                 L.dtype_code(top_logits.dtype), L.ptr(top_indices), 8 * top_indices.element_size(), k,
+                 L.ptr(clean_lse), temperature, L.ptr(row_weight), L.ptr(kl), L.ptr(grad))
     return kl, grad

@@ -136,6 +136,35 @@ def test_long_sequence_of_many_tiles(device, dtype):
     _check(_grads(q, k, v, g, _offsets(device, lengths)), *_definition(q, k, v, g, lengths))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("H, KV, D", [(32, 32, 64), (36, 36, 80), (32, 8, 128), (32, 4, 96), (64, 1, 64)])
+def test_grids_that_fill_the_gpu(device, dtype, H, KV, D):
+    """Enough rows and heads for 128-row tiles, shared key heads over one and several shares
+    of their query heads, a tile that ends a sequence inside, rows behind the last."""
+    N, lengths, first = 2100, [1, 700, 31, 1200, 100], 3
+    q, k, v, g = _inputs(device, N, H, KV, D, dtype, seed=D)
+    got = _grads(q, k, v, g, _offsets(device, lengths, first))
+    _check(got, *_definition(q, k, v, g, lengths, first))
+    rest = torch.ones(N, dtype=torch.bool, device=device)
+    rest[first:first + sum(lengths)] = False
+    for t in got:
+        assert (t[rest] == 0).all()
+    for x, y in zip(_grads(q, k, v, g, _offsets(device, lengths, first)), got):
+        assert torch.equal(x, y)
+    # NaN behind the last sequence and in one of them
+    for t in (q, k, v, g):
+        t[first + sum(lengths):] = math.nan
+    for x, y in zip(_grads(q, k, v, g, _offsets(device, lengths, first)), got):
+        assert torch.equal(x, y)
+    k[first + 720] = v[first + 720] = math.inf  # inside the third sequence
+    q[first + 715, H // 2], g[first + 716, 0] = math.nan, -math.inf
+    val, tol = _definition(q.nan_to_num(0), k.nan_to_num(0), v.nan_to_num(0), g.nan_to_num(0), lengths, first)
+    keep = ~rest
+    keep[first + 701:first + 732] = False
+    for x, y, e in zip(_grads(q, k, v, g, _offsets(device, lengths, first)), val, tol):
+        assert ((x.double() - y).abs() <= e)[keep].all()
+
+
 @pytest.mark.parametrize("scale", [0.5, 0.0, -0.3])
 def test_scale(device, scale):
     q, k, v, g = _inputs(device, 100, 2, 1, 64, BF16, seed=3)
@@ -283,8 +312,8 @@ def test_out_keeps_rows_of_no_sequence(device):
     q, k, v, _ = _inputs(device, 300, 2, 2, 64, BF16)
     off = _offsets(device, [10, 200], first=20)
     out = torch.full_like(q, 7.0)
-    same, stats = ops.packed_attention_fwd(q, k, v, off, out=out)
-    assert same is out and stats is None
+    same, saved = ops.packed_attention_fwd(q, k, v, off, out=out)
+    assert same is out and saved is None
     assert (out[:20] == 7).all() and (out[230:] == 7).all()
     assert torch.equal(out[20:230], packed_attention(q, k, v, off)[20:230])
 
@@ -304,12 +333,17 @@ def test_offsets_that_are_out_of_order_stay_inside(device):
 
 
 def test_rows_past_32_bit_offsets(device):
-    """Row strides that put the last rows beyond 2^31 elements and 2^32 bytes."""
-    N, D = 140, 64
+    """Row strides that put the last rows beyond 2^31 elements and 2^32 bytes; rows further
+    apart than the kernels reach are copied."""
+    for N, stride in ((140, 1 << 24), (600, 1 << 22)):
+        _far_rows(device, N, stride)
+
+
+def _far_rows(device, N, stride):
+    D = 64
     q, k, v, g = _inputs(device, N, 1, 1, D, BF16, seed=9)
-    off = _offsets(device, [139], first=1)
-    wide = torch.empty(N * (1 << 24), dtype=BF16, device=device)
-    far = wide.view(N, 1 << 24)
+    off = _offsets(device, [N - 1], first=1)
+    far = torch.empty(N * stride, dtype=BF16, device=device).view(N, stride)
     far[:, :D], far[:, D:2 * D], far[:, 2 * D:3 * D] = q[:, 0], k[:, 0], v[:, 0]
     views = [far[:, i * D:(i + 1) * D].view(N, 1, D) for i in range(3)]
     for x, y in zip(_grads2(views, g, off), _grads(q, k, v, g, off)):
@@ -380,8 +414,8 @@ def test_graph_replays(device):
     off = _offsets(device, [100, 300])
 
     def calls(q, k, v, g, off):
-        out, stats = ops.packed_attention_fwd(q, k, v, off, want_stats=True)
-        return (out, *ops.packed_attention_bwd(q, k, v, off, out, stats, g))
+        out, saved = ops.packed_attention_fwd(q, k, v, off, want_saved=True)
+        return (out, *ops.packed_attention_bwd(q, k, v, off, out, saved, g))
 
     calls(*static, off)
     torch.cuda.synchronize()

@@ -67,11 +67,13 @@ def test_attention_backward_refuses():
     q, k, v = _qkv()
     stats = torch.zeros(4, 6)
     with pytest.raises(L.PDError, match="d_out"):
-        ops.packed_attention_bwd(q, k, v, OFF, q, stats, q.float())
+        ops.packed_attention_bwd(q, k, v, OFF, q, (stats, q), q.float())
     with pytest.raises(L.PDError, match="stats"):
-        ops.packed_attention_bwd(q, k, v, OFF, q, stats[:, :5], q)
+        ops.packed_attention_bwd(q, k, v, OFF, q, (stats[:, :5], q), q)
+    with pytest.raises(L.PDError, match="out_rest"):
+        ops.packed_attention_bwd(q, k, v, OFF, q, (stats, None), q)
     with pytest.raises(L.PDError, match="out is"):
-        ops.packed_attention_bwd(q, k, v, OFF, q[:, :2], stats, q)
+        ops.packed_attention_bwd(q, k, v, OFF, q[:, :2], (stats, q), q)
 
 
 def test_layer_norm_refuses():
@@ -134,7 +136,7 @@ def _buffer():
     (dict(D=12), "head_dim"), (dict(D=0), "head_dim"), (dict(D=136), "head_dim"), (dict(rows=-1), ">= 0"),
     (dict(n_seq=-1), ">= 0"), (dict(rows=1 << 31), "too many"), (dict(n_seq=1 << 31), "too many"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(q_row=1), "strides"),
-    (dict(v_head=4), "strides"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(off=None), "offsets"),
+    (dict(v_head=4), "strides"), (dict(q_row=1 << 23), "row strides"), (dict(q_row=-64), "row strides"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(off=None), "offsets"),
     (dict(shift=8), "aligned"),
 ])
 def test_attention_entry_points_refuse(kw, message):
@@ -145,23 +147,29 @@ def test_attention_entry_points_refuse(kw, message):
     head = [q, d["q_row"], 16, p, 32, 16, p, 32, d["v_head"], d["dtype"], d["rows"], d["H"], d["KV"], d["D"], d["off"],
             d["n_seq"], d["scale"], 1]
     with pytest.raises(L.PDError, match=message):
-        L.call("pd_packed_attention_fwd", *head, d["out"], p, None)
+        L.call("pd_packed_attention_fwd", *head, d["out"], None, p, None)
     with pytest.raises(L.PDError, match=message):
-        L.call("pd_packed_attention_bwd", *head, d["out"], p, p, p, p, p, p, 1 << 30, None)
+        L.call("pd_packed_attention_bwd", *head, d["out"], p, p, p, p, p, p, p, 1 << 30, None)
 
 
 @built
 def test_entry_points_refuse_workspaces_and_stats():
     keep, p = _buffer()
     head = [p, 64, 16, p, 32, 16, p, 32, 16, 1, 4, 4, 2, 16, p, 1, 1.0, 1]
-    need = L.load().pd_packed_attention_bwd_workspace_size(4, 4)
-    assert need == 4 * 4 * 4
+    need = L.load().pd_packed_attention_bwd_workspace_size(4, 4, 2, 16)
+    assert need == 4 * 4 * 4 + 2 * 2 * 4 * 2 * 16 * 4  # D of every row; dk and dv of two shares of the heads
+    assert L.load().pd_packed_attention_bwd_workspace_size(65536, 4, 4, 16) == 65536 * 4 * 4
     with pytest.raises(L.PDError, match="workspace"):
-        L.call("pd_packed_attention_bwd", *head, p, p, p, p, p, p, p, need - 1, None)
+        L.call("pd_packed_attention_bwd", *head, p, p, p, p, p, p, p, p, need - 1, None)
     with pytest.raises(L.PDError, match="workspace"):
-        L.call("pd_packed_attention_bwd", *head, p, p, p, p, p, p, None, need, None)
+        L.call("pd_packed_attention_bwd", *head, p, p, p, p, p, p, p, None, need, None)
     with pytest.raises(L.PDError, match="stats"):
-        L.call("pd_packed_attention_bwd", *head, p, None, p, p, p, p, p, need, None)
+        L.call("pd_packed_attention_bwd", *head, p, p, None, p, p, p, p, p, need, None)
+    with pytest.raises(L.PDError, match="out_rest"):
+        L.call("pd_packed_attention_bwd", *head, p, None, p, p, p, p, p, p, need, None)
+    head[9] = 0
+    with pytest.raises(L.PDError, match="out_rest"):
+        L.call("pd_packed_attention_fwd", *head, p, p, p, None)
     need = L.load().pd_layer_norm_bwd_workspace_size(4, 8)
     with pytest.raises(L.PDError, match="workspace"):
         L.call("pd_layer_norm_bwd", p, p, 1, 4, 8, None, p, p, p, None, p, need - 1, None)
@@ -196,8 +204,8 @@ def test_norm_and_kl_entry_points_refuse():
 @built
 def test_no_rows_is_no_launch():
     """Without rows nothing is read, written or launched (no GPU is needed)."""
-    L.call("pd_packed_attention_fwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, None, None, None)
-    L.call("pd_packed_attention_bwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, *[None] * 6, None, 0, None)
+    L.call("pd_packed_attention_fwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, None, None, None, None)
+    L.call("pd_packed_attention_bwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, *[None] * 8, 0, None)
     L.call("pd_layer_norm_fwd", None, 1, 0, 8, None, None, 1e-5, None, None, None)
     L.call("pd_top_kl", None, 1, 0, 10, None, 0, None, 32, 3, None, 1.0, None, None, None, None)
     assert ctypes.sizeof(ctypes.c_size_t) == 8
