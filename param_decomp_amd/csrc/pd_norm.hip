@@ -270,18 +270,29 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restr
   }
 }
 
-// dw, db = the partial rows [n][2][d] added in order: 16 columns by 16 slices of the rows
-// per block, the slices' sums joined in order. n = 0 (no rows) gives zeros.
-__global__ __launch_bounds__(256) void k_ln_cols(const float* __restrict__ part, int n, int64_t d,
-                                                 float* __restrict__ dw, float* __restrict__ db) {
+// dw, db = the partial rows [n][2][d] added in a fixed order: 16 columns by 64 slices of the
+// rows per block, a slice's loads in batches of 8. n = 0 (no rows) gives zeros.
+__global__ __launch_bounds__(1024) void k_ln_cols(const float* __restrict__ part, int n, int64_t d,
+                                                  float* __restrict__ dw, float* __restrict__ db) {
   __shared__ float red[16][17];
-  const int c = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const int c = threadIdx.x & 15, sl = threadIdx.x >> 4, wv = threadIdx.x >> 6;
   const int64_t col = (int64_t)blockIdx.x * 16 + c;
-  const int per = (n + 15) / 16, lo = min(sl * per, n), hi = min(lo + per, n);
-  red[sl][c] = col < 2 * d && hi > lo ? pd_ordered_sum(part + lo * 2 * d + col, hi - lo, 2 * d) : 0.f;
-  __syncthreads();
-  if (sl || col >= 2 * d) return;
+  const int per = (n + 63) / 64, lo = min(sl * per, n), hi = col < 2 * d ? min(lo + per, n) : lo;
+  const float* p = part + col;
   float s = 0.f;
+  for (int i = lo; i < hi; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = i + j < hi ? p[(i + j) * 2 * d] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += v[j];
+  }
+  s += __shfl_xor(s, 16, 64);
+  s += __shfl_xor(s, 32, 64);
+  if ((threadIdx.x & 63) < 16) red[wv][c] = s;
+  __syncthreads();
+  if (threadIdx.x >= 16 || col >= 2 * d) return;
+  s = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s += red[i][c];
   float* out = col < d ? dw : db;
@@ -485,7 +496,7 @@ int pd_layer_norm_bwd(const void* x, const void* d_y, int dtype, int64_t rows, i
       ln_bwd<bf16_t>((const bf16_t*)x, (const bf16_t*)d_y, rows, d, weight, (const LnStat*)stats, (bf16_t*)d_x, part, s);
   }
   if (params)
-    hipLaunchKernelGGL(k_ln_cols, dim3((unsigned)cdiv(2 * d, 16)), dim3(256), 0, s, part,
+    hipLaunchKernelGGL(k_ln_cols, dim3((unsigned)cdiv(2 * d, 16)), dim3(1024), 0, s, part,
                        rows ? (int)ln_partials(rows, d) : 0, d, d_weight, d_bias);
   return check_launch("pd_layer_norm_bwd");
 }

@@ -189,13 +189,14 @@ def test_norm_and_kl_entry_points_refuse():
         with pytest.raises(L.PDError, match="eps"):
             L.call("pd_layer_norm_fwd", p, 1, 4, 8, None, None, eps, p, None, None)
 
-    def kl(z=p, dtype=1, rows=2, V=10, top_dtype=0, bits=32, k=3, tau=1.0, out=p):
-        L.call("pd_top_kl", z, dtype, rows, V, p, top_dtype, p, bits, k, None, tau, None, out, None, None)
+    def kl(z=p, dtype=1, rows=2, V=10, top_dtype=0, bits=32, k=3, tau=1.0, out=p, ws=p):
+        L.call("pd_top_kl", z, dtype, rows, V, p, top_dtype, p, bits, k, None, tau, None, out, None, ws, 64, None)
 
     for kw, message in ((dict(dtype=2), "fp32 or bf16"), (dict(top_dtype=2), "fp32 or bf16"), (dict(bits=16), "indices"),
                         (dict(rows=-1), "rows"), (dict(V=0), "vocab"), (dict(k=0), "k >= 1"), (dict(k=1025), "1024"),
                         (dict(V=(1 << 19) + 1), "2\\^19"), (dict(tau=0.0), "temperature"),
                         (dict(tau=float("nan")), "temperature"), (dict(z=None), "null"), (dict(out=None), "null"),
+                        (dict(ws=None), "workspace"), (dict(ws=p + 8), "workspace"), (dict(rows=3), "workspace"),
                         (dict(rows=1 << 31), "rows")):
         with pytest.raises(L.PDError, match=message):
             kl(**kw)
@@ -207,5 +208,5 @@ def test_no_rows_is_no_launch():
     L.call("pd_packed_attention_fwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, None, None, None, None)
     L.call("pd_packed_attention_bwd", *[None, 64, 16] * 3, 1, 0, 4, 2, 16, None, 0, 1.0, 1, *[None] * 8, 0, None)
     L.call("pd_layer_norm_fwd", None, 1, 0, 8, None, None, 1e-5, None, None, None)
-    L.call("pd_top_kl", None, 1, 0, 10, None, 0, None, 32, 3, None, 1.0, None, None, None, None)
+    L.call("pd_top_kl", None, 1, 0, 10, None, 0, None, 32, 3, None, 1.0, None, None, None, None, 0, None)
     assert ctypes.sizeof(ctypes.c_size_t) == 8
