@@ -15,6 +15,7 @@
 // takes one barrier. Weight and bias gradients are summed over a block's rows in registers (columns
 // are fixed per thread), written as one partial row per block and added in block order by a
 // second kernel: results are the same on every run.
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -24,112 +25,116 @@ namespace pd {
 namespace {
 
 constexpr int LN_MAX_D = 16384;   // largest row held in registers
-constexpr int LN_BLOCKS = 1024;   // most blocks of a launch that walks over rows
-constexpr int LN_GRAD_BLOCKS = 512;  // the same where each block leaves a partial row of gradients
+constexpr int LN_THREADS = 256 * 1024;  // most threads of a launch that walks over rows
+constexpr int LN_GRAD_THREADS = 256 * 512;  // the same where each block leaves a row of partial gradients
 
 struct LnStat {
   float base, delta, rstd;  // mean = base + delta
 };
 
-template <typename T, int VEC>
-struct Pack {
-  T v[VEC];
-};
-template <>
-struct alignas(16) Pack<bf16_t, 8> {
-  bf16_t v[8];
-};
-template <>
-struct alignas(16) Pack<float, 4> {
-  float v[4];
+// 16 bytes of a row, at any element's boundary (the hardware takes them as one access), and
+// kept packed in registers.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) LnWord {
+  uint32_t v[4];
+  __device__ inline float operator[](int e) const {
+    if constexpr (sizeof(T) == 2) return __uint_as_float((e & 1) ? v[e >> 1] & 0xFFFF0000u : v[e >> 1] << 16);
+    else return __uint_as_float(v[e]);
+  }
 };
 
-// This thread's columns: chunk c covers columns VEC (tid + c NT) .. + VEC.
-template <typename T, int VEC, int NT, int CH>
-__device__ inline void ln_load(const T* __restrict__ row, int tid, int d, Pack<T, VEC> (&p)[CH]) {
+// This thread's columns: word c covers columns VEC (tid + c NT) .. + VEC where those are
+// below d, and threads 0, 1, .. have one column each behind the last whole word.
+template <typename T, int NT, int CH>
+__device__ inline void ln_load(const T* __restrict__ row, int tid, int d, LnWord<T> (&p)[CH], float& pt) {
+  constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int col = VEC * (tid + c * NT);
-    if (col < d) p[c] = *(const Pack<T, VEC>*)(row + col);
-    else p[c] = Pack<T, VEC>{};
+    if (col + VEC <= d) p[c] = *(const LnWord<T>*)(row + col);
+    else p[c] = LnWord<T>{};
   }
-}
-template <int VEC, int NT, int CH>
-__device__ inline void ln_load_param(const float* __restrict__ w, float none, int tid, int d, float (&v)[CH * VEC]) {
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const int col = VEC * (tid + c * NT);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[c * VEC + e] = w && col < d ? w[col + e] : none;
-  }
+  if (tid < d % VEC) pt = load_f<T>(row, d - d % VEC + tid);
 }
 template <typename T>
-__device__ inline float ln_f(T v);
-template <>
-__device__ inline float ln_f<float>(float v) {
+__device__ inline void ln_store(T* __restrict__ row, const float* v) {
+  LnWord<T> p;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 2) p.v[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
+    else p.v[e] = __float_as_uint(v[e]);
+  }
+  *(LnWord<T>*)row = p;
+}
+template <int VEC, int NT, int CH>
+__device__ inline void ln_load_param(const float* __restrict__ w, float none, int tid, int d, float (&v)[CH * VEC],
+                                     float& vt) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = VEC * (tid + c * NT);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[c * VEC + e] = w && col + VEC <= d ? w[col + e] : none;
+  }
+  vt = w && tid < d % VEC ? w[d - d % VEC + tid] : none;
+}
+// Sum over the NT threads of a row, or over the wave where a row has more.
+template <int NT>
+__device__ inline float ln_sum(float v) {
+#pragma unroll
+  for (int off = (NT < 64 ? NT : 64) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
 }
-template <>
-__device__ inline float ln_f<bf16_t>(bf16_t v) {
-  return bf16_to_f32(v);
-}
-template <typename T, int VEC>
-__device__ inline Pack<T, VEC> ln_pack(const float* v) {
-  Pack<T, VEC> p;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if constexpr (sizeof(T) == 2) p.v[e] = f32_to_bf16(v[e]);
-    else p.v[e] = v[e];
-  }
-  return p;
-}
 
-// Columns below d that wave w of the row holds.
+// Columns below d that wave w of the row holds (the row's all threads where it has one).
 template <int VEC, int NT, int CH>
 __device__ inline int ln_wave_count(int w, int d) {
+  if (NT <= 64) return d;
   int n = 0;
 #pragma unroll
-  for (int c = 0; c < CH; ++c) n += min(max(d - VEC * (64 * w + c * NT), 0), 64 * VEC);
-  return n;
+  for (int c = 0; c < CH; ++c) n += min(max(d / VEC - (64 * w + c * NT), 0), 64) * VEC;
+  return n + (w == 0 ? d % VEC : 0);
 }
+constexpr int ln_threads(int nt) { return nt <= 64 ? 256 : nt; }
 
-// Forward. Grid: row groups; a block holds RPB rows at a time (one per wave where NT = 64).
-template <typename T, int VEC, int NT, int CH>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_fwd(const T* __restrict__ x, int64_t rows, int d,
-                                                               const float* __restrict__ w,
-                                                               const float* __restrict__ b, float eps,
-                                                               T* __restrict__ y, LnStat* __restrict__ stats) {
-  constexpr int E = CH * VEC, RPB = NT == 64 ? 4 : 1, NW = NT / 64;
+// Forward. Grid: row groups; a block holds RPB rows at a time (NT <= 64: rows share waves or
+// have one each, with no barrier).
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(ln_threads(NT)) void k_ln_fwd(const T* __restrict__ x, int64_t rows, int d,
+                                                           const float* __restrict__ w, const float* __restrict__ b,
+                                                           float eps, T* __restrict__ y, LnStat* __restrict__ stats) {
+  constexpr int VEC = 16 / sizeof(T), CH = E / VEC, RPB = ln_threads(NT) / NT, NW = NT <= 64 ? 1 : NT / 64;
   __shared__ float4 part[2][NW];
-  const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x, wv = tid >> 6, lane = threadIdx.x & 63;
-  int64_t r = (int64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0);
+  const int tid = threadIdx.x % NT, wv = tid >> 6, lane = threadIdx.x & 63;
+  int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  if (NT == 64 && r >= rows) return;
-  float wr[E], br[E];
-  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr);
-  ln_load_param<VEC, NT, CH>(b, 0.f, tid, d, br);
-  Pack<T, VEC> cur[CH], nxt[CH];
-  ln_load<T, VEC, NT, CH>(x + r * d, tid, d, cur);
+  if (NT <= 64 && r >= rows) return;
+  const bool tail = tid < d % VEC;
+  float wr[E], br[E], wt, bt;
+  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr, wt);
+  ln_load_param<VEC, NT, CH>(b, 0.f, tid, d, br, bt);
+  LnWord<T> cur[CH], nxt[CH];
+  float vt = 0.f, nt = 0.f;
+  ln_load<T, NT, CH>(x + r * d, tid, d, cur, vt);
   const int nw = ln_wave_count<VEC, NT, CH>(wv, d);
   for (int it = 0; r < rows; r += step, it ^= 1) {
-    if (r + step < rows) ln_load<T, VEC, NT, CH>(x + (r + step) * d, tid, d, nxt);
-    float v[E], s = 0.f;
+    if (r + step < rows) ln_load<T, NT, CH>(x + (r + step) * d, tid, d, nxt, nt);
+    float v[E], s = vt;
 #pragma unroll
-    for (int i = 0; i < E; ++i) s += v[i] = ln_f<T>(cur[i / VEC].v[i % VEC]);  // columns past d hold 0
-    s = wave_sum(s);
-    float base = nw ? s / (float)nw : 0.f, q = 0.f, res = 0.f;
+    for (int i = 0; i < E; ++i) s += v[i] = cur[i / VEC][i % VEC];
+    s = ln_sum<NT>(s);
+    float base = nw ? s / (float)nw : 0.f, res = tail ? vt - base : 0.f, q = res * res;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      if (VEC * (tid + (i / VEC) * NT) < d) {
+      if (VEC * (tid + (i / VEC) * NT) + VEC <= d) {
         const float t = v[i] - base;
         res += t;
         q = fmaf(t, t, q);
       }
     }
-    q = wave_sum(q);
-    res = wave_sum(res);
+    q = ln_sum<NT>(q);
+    res = ln_sum<NT>(res);
     float delta, var;
-    if constexpr (NT == 64) {
+    if constexpr (NT <= 64) {
       delta = res / (float)d;
       var = fmaxf(q / (float)d - delta * delta, 0.f);
     } else {
@@ -153,60 +158,69 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_fwd(const T* __restr
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = VEC * (tid + c * NT);
-      if (col >= d) continue;
+      if (col + VEC > d) continue;
       float o[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int i = c * VEC + e;
         o[e] = fmaf(((v[i] - base) - delta) * rstd, wr[i], br[i]);
       }
-      *(Pack<T, VEC>*)(y + r * d + col) = ln_pack<T, VEC>(o);
+      ln_store<T>(y + r * d + col, o);
     }
+    if (tail) store_f<T>(y + r * d, d - d % VEC + tid, fmaf(((vt - base) - delta) * rstd, wt, bt));
     if (stats && tid == 0) stats[r] = LnStat{base, delta, rstd};
 #pragma unroll
     for (int c = 0; c < CH; ++c) cur[c] = nxt[c];
+    vt = nt;
   }
 }
 
 // Backward. dwdb [gridDim.x][2][d]: each block's sums of dy xh and dy over its rows (NULL:
 // not wanted).
-template <typename T, int VEC, int NT, int CH>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
-                                                               int64_t rows, int d, const float* __restrict__ w,
-                                                               const LnStat* __restrict__ stats, T* __restrict__ dx,
-                                                               float* __restrict__ dwdb) {
-  constexpr int E = CH * VEC, RPB = NT == 64 ? 4 : 1, NW = NT / 64;
+template <typename T, int NT, int E>
+__global__ __launch_bounds__(ln_threads(NT)) void k_ln_bwd(const T* __restrict__ x, const T* __restrict__ dy,
+                                                           int64_t rows, int d, const float* __restrict__ w,
+                                                           const LnStat* __restrict__ stats, T* __restrict__ dx,
+                                                           float* __restrict__ dwdb) {
+  constexpr int VEC = 16 / sizeof(T), CH = E / VEC, RPB = ln_threads(NT) / NT, NW = NT <= 64 ? 1 : NT / 64;
   __shared__ float2 part[2][NW];
-  extern __shared__ float cols[];  // [2][d] where NT = 64 and gradients are wanted
-  const int tid = NT == 64 ? threadIdx.x & 63 : threadIdx.x, wv = tid >> 6, lane = threadIdx.x & 63;
-  int64_t r = (int64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0);
+  extern __shared__ float cols[];  // [2][d] where NT <= 64 and gradients are wanted
+  const int tid = threadIdx.x % NT, wv = tid >> 6, lane = threadIdx.x & 63;
+  int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  float wr[E];
-  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr);
-  float dw[E], db[E];
+  const bool tail = tid < d % VEC;
+  float wr[E], wt;
+  ln_load_param<VEC, NT, CH>(w, 1.f, tid, d, wr, wt);
+  float dw[E], db[E], dwt = 0.f, dbt = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.f;
-  Pack<T, VEC> cx[CH], cg[CH], nx[CH], ng[CH];
+  LnWord<T> cx[CH], cg[CH], nx[CH], ng[CH];
+  float xt = 0.f, gt = 0.f, nxt = 0.f, ngt = 0.f;
   LnStat st = {}, nst = {};
   if (r < rows) {
-    ln_load<T, VEC, NT, CH>(x + r * d, tid, d, cx);
-    ln_load<T, VEC, NT, CH>(dy + r * d, tid, d, cg);
+    ln_load<T, NT, CH>(x + r * d, tid, d, cx, xt);
+    ln_load<T, NT, CH>(dy + r * d, tid, d, cg, gt);
     st = stats[r];
   }
   const float invd = 1.f / (float)d;
   for (int it = 0; r < rows; r += step, it ^= 1) {
     if (r + step < rows) {
-      ln_load<T, VEC, NT, CH>(x + (r + step) * d, tid, d, nx);
-      ln_load<T, VEC, NT, CH>(dy + (r + step) * d, tid, d, ng);
+      ln_load<T, NT, CH>(x + (r + step) * d, tid, d, nx, nxt);
+      ln_load<T, NT, CH>(dy + (r + step) * d, tid, d, ng, ngt);
       nst = stats[r + step];
     }
+    const float xht = ((xt - st.base) - st.delta) * st.rstd, at = gt * wt;
     float s1 = 0.f, s2 = 0.f;
+    if (tail) {
+      s1 = at, s2 = at * xht;
+      dwt = fmaf(gt, xht, dwt);
+      dbt += gt;
+    }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int col = VEC * (tid + (i / VEC) * NT);
-      const float g = ln_f<T>(cg[i / VEC].v[i % VEC]);  // 0 past d
-      const float xh = ((ln_f<T>(cx[i / VEC].v[i % VEC]) - st.base) - st.delta) * st.rstd;
-      if (col < d) {
+      const float g = cg[i / VEC][i % VEC];
+      const float xh = ((cx[i / VEC][i % VEC] - st.base) - st.delta) * st.rstd;
+      if (VEC * (tid + (i / VEC) * NT) + VEC <= d) {
         const float a = g * wr[i];
         s1 += a;
         s2 = fmaf(a, xh, s2);
@@ -215,8 +229,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restr
       }
     }
     if (dx) {
-      s1 = wave_sum(s1);
-      s2 = wave_sum(s2);
+      s1 = ln_sum<NT>(s1);
+      s2 = ln_sum<NT>(s2);
       if constexpr (NT > 64) {
         if (lane == 0) part[it][wv] = make_float2(s1, s2);
         __syncthreads();
@@ -228,34 +242,46 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restr
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = VEC * (tid + c * NT);
-        if (col >= d) continue;
+        if (col + VEC > d) continue;
         float o[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           const int i = c * VEC + e;
-          const float xh = ((ln_f<T>(cx[c].v[e]) - st.base) - st.delta) * st.rstd;
-          const float a = ln_f<T>(cg[c].v[e]) * wr[i];
-          o[e] = st.rstd * (a - m1 - xh * m2);
+          const float xh = ((cx[c][e] - st.base) - st.delta) * st.rstd;
+          o[e] = st.rstd * (cg[c][e] * wr[i] - m1 - xh * m2);
         }
-        *(Pack<T, VEC>*)(dx + r * d + col) = ln_pack<T, VEC>(o);
+        ln_store<T>(dx + r * d + col, o);
       }
+      if (tail) store_f<T>(dx + r * d, d - d % VEC + tid, st.rstd * (at - m1 - xht * m2));
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) cx[c] = nx[c], cg[c] = ng[c];
+    xt = nxt, gt = ngt;
     st = nst;
   }
   if (!dwdb) return;
   float* dst = dwdb + (int64_t)blockIdx.x * 2 * d;
-  if constexpr (NT == 64) {  // the four waves' sums in wave order
-    for (int wave = 0; wave < RPB; ++wave) {
-      if ((int)(threadIdx.x >> 6) == wave) {
+  if constexpr (NT <= 64) {  // the rows that share a wave, then the four waves' sums in order
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int off = 32; off >= NT; off >>= 1) dw[i] += __shfl_xor(dw[i], off, 64), db[i] += __shfl_xor(db[i], off, 64);
+#pragma unroll
+    for (int off = 32; off >= NT; off >>= 1) dwt += __shfl_xor(dwt, off, 64), dbt += __shfl_xor(dbt, off, 64);
+    for (int wave = 0; wave < 4; ++wave) {
+      if ((int)(threadIdx.x >> 6) == wave && lane < NT) {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-          const int col = VEC * (tid + (i / VEC) * NT) + i % VEC;
-          if (col < d) {
+          const int word = VEC * (tid + (i / VEC) * NT), col = word + i % VEC;
+          if (word + VEC <= d) {
             cols[col] = wave ? cols[col] + dw[i] : dw[i];
             cols[d + col] = wave ? cols[d + col] + db[i] : db[i];
           }
+        }
+        if (tail) {
+          const int col = d - d % VEC + tid;
+          cols[col] = wave ? cols[col] + dwt : dwt;
+          cols[d + col] = wave ? cols[d + col] + dbt : dbt;
         }
       }
       __syncthreads();
@@ -264,9 +290,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_ln_bwd(const T* __restr
   } else {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int col = VEC * (tid + (i / VEC) * NT) + i % VEC;
-      if (col < d) dst[col] = dw[i], dst[d + col] = db[i];
+      const int word = VEC * (tid + (i / VEC) * NT), col = word + i % VEC;
+      if (word + VEC <= d) dst[col] = dw[i], dst[d + col] = db[i];
     }
+    if (tail) dst[d - d % VEC + tid] = dwt, dst[d + d - d % VEC + tid] = dbt;
   }
 }
 
@@ -384,26 +411,33 @@ constexpr int LN_LONG_SLICES = 16;
 template <typename F>
 void ln_form(int64_t d, F&& f) {
   using std::integral_constant;
-  if (d <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  auto form = [&](auto nt) {
+    constexpr int NT = decltype(nt)::value;
+    f(nt, integral_constant<int, NT <= 64 ? 8 : 16>{});
+  };
+  if (d <= 64) form(integral_constant<int, 8>{});
+  else if (d <= 128) form(integral_constant<int, 16>{});
+  else if (d <= 256) form(integral_constant<int, 32>{});
+  else if (d <= 512) form(integral_constant<int, 64>{});
   else if (d <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
-  else if (d <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 32>{});
-  else if (d <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-  else if (d <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 32>{});
-  else f(integral_constant<int, 512>{}, integral_constant<int, 32>{});
+  else if (d <= 2048) form(integral_constant<int, 128>{});
+  else if (d <= 4096) form(integral_constant<int, 256>{});
+  else if (d <= 8192) form(integral_constant<int, 512>{});
+  else form(integral_constant<int, 1024>{});
 }
 
-int64_t ln_blocks(int64_t rows, int64_t d, int64_t most) {
-  const int64_t groups = d <= 2048 ? cdiv(rows, 4) : rows;
-  return groups < most ? groups : most;
+// Blocks of a launch that walks over rows: `threads` threads in all at most.
+int64_t ln_blocks(int64_t rows, int64_t d, int64_t threads) {
+  int64_t n = 0;
+  ln_form(d, [&](auto nt, auto) {
+    constexpr int NT = decltype(nt)::value;
+    n = std::min(cdiv(rows, ln_threads(NT) / NT), threads / ln_threads(NT));
+  });
+  return n;
 }
 int64_t ln_partials(int64_t rows, int64_t d) {
   if (d > LN_MAX_D) return rows < LN_LONG_SLICES ? rows : LN_LONG_SLICES;
-  return ln_blocks(rows, d, LN_GRAD_BLOCKS);
-}
-bool ln_aligned(std::initializer_list<const void*> ps) {
-  for (const void* p : ps)
-    if (p && ((uintptr_t)p & 15)) return false;
-  return true;
+  return ln_blocks(rows, d, LN_GRAD_THREADS);
 }
 
 int ln_check(const char* what, int dtype, int64_t rows, int64_t d, std::initializer_list<const void*> needed) {
@@ -424,14 +458,10 @@ void ln_fwd(const T* x, int64_t rows, int64_t d, const float* w, const float* b,
     hipLaunchKernelGGL(k_ln_fwd_long<T>, dim3((unsigned)rows), dim3(1024), 0, s, x, d, w, b, eps, y, stats);
     return;
   }
-  const unsigned grid = (unsigned)ln_blocks(rows, d, LN_BLOCKS);
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = d % V == 0 && ln_aligned({x, y});
+  const unsigned grid = (unsigned)ln_blocks(rows, d, LN_THREADS);
   ln_form(d, [&](auto nt, auto e) {
     constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
-    const dim3 block(NT < 256 ? 256 : NT);
-    if (vec) hipLaunchKernelGGL((k_ln_fwd<T, V, NT, E / V>), dim3(grid), block, 0, s, x, rows, (int)d, w, b, eps, y, stats);
-    else hipLaunchKernelGGL((k_ln_fwd<T, 1, NT, E>), dim3(grid), block, 0, s, x, rows, (int)d, w, b, eps, y, stats);
+    hipLaunchKernelGGL((k_ln_fwd<T, NT, E>), dim3(grid), dim3(ln_threads(NT)), 0, s, x, rows, (int)d, w, b, eps, y, stats);
   });
 }
 
@@ -445,15 +475,12 @@ void ln_bwd(const T* x, const T* dy, int64_t rows, int64_t d, const float* w, co
                          x, dy, rows, d, stats, part);
     return;
   }
-  const unsigned grid = (unsigned)(part ? ln_partials(rows, d) : ln_blocks(rows, d, LN_BLOCKS));
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = d % V == 0 && ln_aligned({x, dy, dx});
+  const unsigned grid = (unsigned)(part ? ln_partials(rows, d) : ln_blocks(rows, d, LN_THREADS));
   ln_form(d, [&](auto nt, auto e) {
     constexpr int NT = decltype(nt)::value, E = decltype(e)::value;
-    const dim3 block(NT < 256 ? 256 : NT);
-    const size_t lds = NT == 64 && part ? (size_t)2 * d * sizeof(float) : 0;
-    if (vec) hipLaunchKernelGGL((k_ln_bwd<T, V, NT, E / V>), dim3(grid), block, lds, s, x, dy, rows, (int)d, w, stats, dx, part);
-    else hipLaunchKernelGGL((k_ln_bwd<T, 1, NT, E>), dim3(grid), block, lds, s, x, dy, rows, (int)d, w, stats, dx, part);
+    const size_t lds = NT <= 64 && part ? (size_t)2 * d * sizeof(float) : 0;
+    hipLaunchKernelGGL((k_ln_bwd<T, NT, E>), dim3(grid), dim3(ln_threads(NT)), lds, s, x, dy, rows, (int)d, w, stats, dx,
+                       part);
   });
 }
 

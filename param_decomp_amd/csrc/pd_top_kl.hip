@@ -58,7 +58,7 @@ struct TopKLArgs {
 
 // 16 bytes of a row, at any element's boundary (the hardware takes them as one access).
 template <typename T>
-struct __attribute__((aligned(sizeof(T)))) KLWord {
+struct __attribute__((packed, aligned(sizeof(T)))) KLWord {
   uint32_t v[4];
 };
 template <typename T>
