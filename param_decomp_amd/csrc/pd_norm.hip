@@ -426,12 +426,12 @@ void ln_form(int64_t d, F&& f) {
   else form(integral_constant<int, 1024>{});
 }
 
-// Blocks of a launch that walks over rows: `threads` threads in all at most.
+// Blocks of a launch that walks over rows: `threads` threads in all at most, or a block a CU.
 int64_t ln_blocks(int64_t rows, int64_t d, int64_t threads) {
   int64_t n = 0;
   ln_form(d, [&](auto nt, auto) {
     constexpr int NT = decltype(nt)::value;
-    n = std::min(cdiv(rows, ln_threads(NT) / NT), threads / ln_threads(NT));
+    n = std::min(cdiv(rows, ln_threads(NT) / NT), std::max<int64_t>(threads / ln_threads(NT), 256));
   });
   return n;
 }
