@@ -165,6 +165,15 @@ def test_grids_that_fill_the_gpu(device, dtype, H, KV, D):
         assert ((x.double() - y).abs() <= e)[keep].all()
 
 
+@pytest.mark.parametrize("H, KV", [(2, 1), (32, 32)])
+def test_more_sequences_than_a_block_holds_offsets_of(device, H, KV):
+    lengths = ([1, 2, 0, 3, 1] * 500)[:2300]
+    N = sum(lengths) + 7
+    q, k, v, g = _inputs(device, N, H, KV, 64, BF16, seed=12)
+    got = _grads(q, k, v, g, _offsets(device, lengths, 4))
+    _check(got, *_definition(q, k, v, g, lengths, 4))
+
+
 @pytest.mark.parametrize("scale", [0.5, 0.0, -0.3])
 def test_scale(device, scale):
     q, k, v, g = _inputs(device, 100, 2, 1, 64, BF16, seed=3)
