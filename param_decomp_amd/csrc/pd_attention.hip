@@ -502,6 +502,12 @@ __device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float m
   if constexpr (sizeof(T) == 4) a.stats[((int64_t)a.H + h) * a.N + row] = (mc - L) + ll;
 }
 
+// The larger of a lane's value and its partner's in the wave's other half.
+__device__ inline float at_halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // ---------------------------------------------------------------- forward
 // One row block's online softmax over a tile of NB key blocks: scores sc (raw, masked ones
 // -inf) to weights in place, the running reference m (raw), the lane's own part of the sum l,
@@ -509,12 +515,13 @@ __device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float m
 // stay below 2^8 and a tile without growth costs no pass over the accumulators.
 template <int NB, int NC>
 __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], float& m, float& l, f32x16 (&o)[NC], float c2) {
-  float mt = -INFINITY;
+  // four chains of maxima and of sums: one would be a wait for each of its steps
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mt = fmaxf(mt, sc[b][i]);
-  mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    for (int i = 0; i < 16; ++i) x[i & 3] = fmaxf(x[i & 3], sc[b][i]);
+  const float mt = at_halves_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   if (__any((mt - m) * c2 > AT_SLACK)) {
     const float mn = fmaxf(m, mt), al = at_exp2((m - mn) * c2);
     m = mn;
@@ -525,13 +532,15 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], float& m, float& l,
       for (int i = 0; i < 16; ++i) o[c][i] *= al;
   }
   const float mc = -m * c2;
+  float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       sc[b][i] = at_exp2(fmaf(sc[b][i], c2, mc));
-      l += sc[b][i];
+      y[i & 3] += sc[b][i];
     }
+  l += (y[0] + y[1]) + (y[2] + y[3]);
 }
 
 // Query fragments with the scale's sign: c2 is positive then. (Scale 0: zeros, c2 = 1.)
@@ -1115,24 +1124,24 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
   const SeqTable table(a, seq, tid);
   const KeyTile t(a, AT_ROWS);
   const int row0 = t.k0 + 32 * w, rc = min(row0 + r, a.N - 1);
-  Frag kf[NS], vf[sizeof(T) == 2 ? 1 : NS];
-  at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
   if constexpr (sizeof(T) == 2) {
     Loader<T, DP, AT_ROWS, 4> lv;
     lv.init(a.v_row, a.D, w, lane);
     lv.issue((const T*)a.v + t.hk * a.v_head, a.v_row, t.k0, a.N - 1, a.D, Vl, w);
-  } else {
-    at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
   }
-  auto value = [&](int s) -> Frag {
-    if constexpr (sizeof(T) == 2) return I::rows(Vl, 32 * w + r, s, hh);
-    else return vf[s];
-  };
   __syncthreads();
   Keys K;
   K.init(table, row0 + r);
   int blo, bhi;
   at_block_range(K.lo, K.hi, lane, w, ends, blo, bhi);
+  Frag kf[NS], vf[sizeof(T) == 2 ? 1 : NS];
+  at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
+  if constexpr (sizeof(T) == 4)
+    at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
+  auto value = [&](int s) -> Frag {
+    if constexpr (sizeof(T) == 2) return I::rows(Vl, 32 * w + r, s, hh);
+    else return vf[s];
+  };
   Loader<T, DP, 32, 4> lq, lg;
   lq.init(a.q_row, a.D, w, lane);
   lg.init((int64_t)a.H * a.D, a.D, w, lane);
