@@ -249,8 +249,7 @@ __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i 
 __device__ inline float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The offsets in LDS, every step-th of them where there are more than the table holds: one
-// round trip to memory for a block, where a search in memory takes one for each halving
-// (8192 tokens in 128 sequences, 8 heads of 64: forward 13.6 us).
+// round trip to memory for a block, where a search in memory takes one for each halving.
 struct SeqTable {
   static constexpr int SIZE = 1024;
   int* tab;
@@ -426,34 +425,89 @@ __device__ __attribute__((noinline)) void at_dkv_row(const AttnArgs* a, int hk, 
 // The kernel's own arguments, where they lie (a copy of them would live in scratch).
 __device__ inline const AttnArgs* at_args() { return (const AttnArgs*)__builtin_amdgcn_kernarg_segment_ptr(); }
 
-// Query tile and head of a block: the heads of one key head on one XCD (blocks go round
-// the 8 XCDs in turn), tiles with the most keys behind a long sequence's start first.
-template <int ROWS>
-__device__ inline void at_query_tile(const AttnArgs& a, int& h, int& q0) {
-  const int nt = (a.N + ROWS - 1) / ROWS, rep = a.H / a.KV;
-  const int id = blockIdx.x, x = id % a.H;
-  h = (x % a.KV) * rep + x / a.KV;
-  q0 = (nt - 1 - id / a.H) * ROWS;
+// The order of a grid's blocks, `per` of them (heads) to a tile of ROWS rows. Blocks go to the
+// CUs in turn, id mod 256, so with the tiles in order of their work, most first, and the
+// first 256 turned around (by eights: the 8 XCDs keep their heads), the longest blocks share
+// a CU with the shortest ones, or with none, and where they do not all fit at once the short
+// ones come last. Every block forms the order itself from the offsets: thread t a key
+// of tile t (its work in units of 32 rows, then t), and its rank. Up to 256 blocks a CU holds
+// one and no order is better than another; beyond 256 tiles the ranks would cost more than
+// the order gives, and there the tiles at the sequences' long side simply come first.
+// Starts with a barrier behind which the table is whole.
+template <int ROWS, bool QUERIES>
+__device__ inline void at_order(const AttnArgs& a, const SeqTable& table, int (&keys)[260], int per, int tid, int& x,
+                                int& first) {
+  const int nt = (a.N + ROWS - 1) / ROWS, total = nt * per, id = blockIdx.x;
+  __syncthreads();
+  if (nt > 256 || total <= 256) {
+    x = id % per;
+    first = (QUERIES ? nt - 1 - id / per : id / per) * ROWS;
+    return;
+  }
+  int c = id & 255;
+  const int round = id - c;
+  if (round == 0) c = (248 - (c & 248)) | (c & 7);
+  const int want = (round + c) / per;
+  x = (round + c) % per;
+  int mine = -1;
+  if (tid < nt) {
+    const int lo = tid * ROWS, hi = min(lo + ROWS, a.N);
+    int start, end, work = 0;
+    table.find(QUERIES ? lo : hi - 1, start, end);
+    if (start < end) work = QUERIES ? hi - start : end - lo;
+    mine = (work + 31) >> 5 << 8 | tid;
+  }
+  keys[tid] = mine;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < nt; j += 4) {
+    const int4 k = *(const int4*)&keys[j];
+    rank += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+  }
+  if (tid < nt && rank == want) keys[256] = tid;
+  __syncthreads();
+  first = __builtin_amdgcn_readfirstlane(keys[256]) * ROWS;
 }
 
-// A lane's query row, its sequence, and the keys its wave meets.
+// Query tile and head of a block: the heads of one key head on one XCD.
+template <int ROWS>
+__device__ inline void at_query_tile(const AttnArgs& a, const SeqTable& table, int (&keys)[260], int tid, int& h, int& q0) {
+  int x;
+  at_order<ROWS, true>(a, table, keys, a.H, tid, x, q0);
+  h = x % a.KV * (a.H / a.KV) + x / a.KV;
+}
+
+// The positions that a lane's row sees: `width` of them from `first` on (none: width 0).
+struct Span {
+  int first, width;
+  __device__ inline bool sees(int j) const { return (unsigned)(j - first) < (unsigned)width; }
+  // Whether any lane of the wave sees a part of [j, j + n). Where none does, a lane sees all
+  // of it, or it is `hidden` from it: one value, a row's infinite L or no maximum, hides it,
+  // where a part takes a comparison an entry. A wave that holds a sequence's end and the next
+  // one's start meets such blocks from the one's start on.
+  __device__ inline bool some(int j, int n, bool& hidden) const {
+    const int b = j - first;
+    hidden = b + n <= 0 || b >= width;
+    return !__all(hidden || (b >= 0 && b + n <= width));
+  }
+};
+
+// A lane's query row, the keys it sees, and the keys its wave meets.
 struct Rows {
-  int row, start, end;
-  bool in;       // the row is in a sequence
-  int lo, hi;    // keys the wave meets: [lo, hi)
-  int inner_lo;  // largest start of the wave's rows
-  bool whole;    // every row of the wave is in a sequence
+  int row, start;  // start: of the row's sequence, behind the row where it has none
+  bool in;         // the row is in a sequence
+  int lo, hi;      // keys the wave meets: [lo, hi)
+  Span sees;
   __device__ inline void init(const SeqTable& t, int r) {
+    int end;
     row = r;
     t.find(row, start, end);
     in = start <= row;
     lo = at_wave_min(in ? start : 0x7FFFFFFF);
     hi = at_wave_max(in ? row + 1 : -1);
-    inner_lo = at_wave_max(in ? start : -1);
-    whole = __all(in);
+    sees = {start, in ? row + 1 - start : 0};
   }
-  // No key of [j, j + n) is hidden from any row of the wave (its first row is row0).
-  __device__ inline bool inner(int j, int n, int row0) const { return whole && j >= inner_lo && j + n <= row0 + 1; }
 };
 
 // Keys the block's four waves meet.
@@ -514,14 +568,15 @@ __device__ inline float at_halves_max(float v) {
 // and the accumulators rescaled where a maximum has grown by more than the slack: weights
 // stay below 2^8 and a tile without growth costs no pass over the accumulators.
 template <int NB, int NC>
-__device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], float& m, float& l, f32x16 (&o)[NC], float c2) {
+__device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float& m, float& l, f32x16 (&o)[NC],
+                                           float c2) {
   // four chains of maxima and of sums: one would be a wait for each of its steps
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i & 3] = fmaxf(x[i & 3], sc[b][i]);
-  const float mt = at_halves_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+  const float mt = hidden ? -INFINITY : at_halves_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   if (__any((mt - m) * c2 > AT_SLACK)) {
     const float mn = fmaxf(m, mt), al = at_exp2((m - mn) * c2);
     m = mn;
@@ -531,7 +586,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], float& m, float& l,
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[c][i] *= al;
   }
-  const float mc = -m * c2;
+  const float mc = hidden ? -INFINITY : -m * c2;
   float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -576,15 +631,15 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   __shared__ int ends[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
   int h, q0;
-  at_query_tile<AT_ROWS>(a, h, q0);
+  at_query_tile<AT_ROWS>(a, table, keys, tid, h, q0);
   const int hk = h / (a.H / a.KV), row0 = q0 + 32 * w;
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   Frag qf[NS];
   const float c2 = at_query<T, DP>(a, h, row0 + r, hh, qf);
-  __syncthreads();
   Rows R;
   R.init(table, row0 + r);
   int blo, bhi;
@@ -610,16 +665,14 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) sc[b] = Op<T>::mma(I::rows(Kl, 32 * b + r, s, hh), qf[s], sc[b]);
     }
-    if (!R.inner(j0, BK, row0)) {  // hidden scores are -inf whatever their keys hold
+    bool hidden;
+    if (R.sees.some(j0, BK, hidden)) {  // hidden scores are -inf whatever their keys hold
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * b + at_pos(i, hh);
-          sc[b][i] = j >= R.start && j <= R.row ? sc[b][i] : -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i) sc[b][i] = R.sees.sees(j0 + 32 * b + at_pos(i, hh)) ? sc[b][i] : -INFINITY;
     }
-    at_softmax<NB, NC>(sc, m, l, o, c2);
+    at_softmax<NB, NC>(sc, hidden, m, l, o, c2);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -705,15 +758,15 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   __shared__ float ml[2][4][32];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
   int h, q0;
-  at_query_tile<AT_SPLIT>(a, h, q0);
+  at_query_tile<AT_SPLIT>(a, table, keys, tid, h, q0);
   const int hk = h / (a.H / a.KV);
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   Frag qf[NS];
   const float c2 = at_query<T, DP>(a, h, q0 + r, hh, qf);
-  __syncthreads();
   Rows R;
   R.init(table, q0 + r);
   Ld lk, lv;
@@ -736,14 +789,12 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
     for (int s = 0; s < NS; ++s) sc[0] = Op<T>::mma(I::rows(Kl, r, s, hh), qf[s], sc[0]);
     at_lds_free();
     if (more) lk.issue(kb, a.k_row, j0 + 128, R.hi - 1, a.D, Kl, 0);
-    if (!R.inner(j0, 32, q0)) {
+    bool hidden;
+    if (R.sees.some(j0, 32, hidden)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int j = j0 + at_pos(i, hh);
-        sc[0][i] = j >= R.start && j <= R.row ? sc[0][i] : -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i) sc[0][i] = R.sees.sees(j0 + at_pos(i, hh)) ? sc[0][i] : -INFINITY;
     }
-    at_softmax<1, NC>(sc, m, l, o, c2);
+    at_softmax<1, NC>(sc, hidden, m, l, o, c2);
     at_landed<Ld::NI>(more);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
@@ -817,7 +868,7 @@ struct QueryRow {
     at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, q);
     dot += __shfl_xor(dot, 32, 64);
   }
-  __device__ inline float p(float s, float c2) const {
+  __device__ inline float p(float s, float c2, float L) const {
     const float t = fmaf(s, c2, -L);
     return at_exp2(sizeof(T) == 4 ? t - Lr : t);
   }
@@ -825,7 +876,7 @@ struct QueryRow {
 
 // ds / scale of one block (images of its 32 keys and values at row R0), and dq += ds k.
 template <typename T, int DP>
-__device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int R0, int j0, bool inner, const Rows& R,
+__device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int R0, int j0, const Rows& R,
                                    const QueryRow<T, DP>& Q, float c2, int lane, f32x16 (&dq)[DP / 32]) {
   typedef Img<T, DP> I;
   const int r = lane & 31, hh = lane >> 5;
@@ -835,14 +886,14 @@ __device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int 
     sc = Op<T>::mma(I::rows(Kl, R0 + r, s, hh), Q.q[s], sc);
     dp = Op<T>::mma(I::rows(Vl, R0 + r, s, hh), Q.g[s], dp);
   }
+  bool hidden;
+  const bool some = R.sees.some(j0, 32, hidden);
+  const float L = hidden ? INFINITY : Q.L;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sc[i] = Q.p(sc[i], c2) * (dp[i] - Q.dot);
-  if (!inner) {
+  for (int i = 0; i < 16; ++i) sc[i] = Q.p(sc[i], c2, L) * (dp[i] - Q.dot);
+  if (some) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int j = j0 + at_pos(i, hh);
-      sc[i] = j >= R.start && j <= R.row ? sc[i] : 0.f;
-    }
+    for (int i = 0; i < 16; ++i) sc[i] = R.sees.sees(j0 + at_pos(i, hh)) ? sc[i] : 0.f;
   }
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
@@ -860,15 +911,15 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_dq(AttnArgs a) {
   __shared__ int ends[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
   int h, q0;
-  at_query_tile<AT_ROWS>(a, h, q0);
+  at_query_tile<AT_ROWS>(a, table, keys, tid, h, q0);
   const int hk = h / (a.H / a.KV), row0 = q0 + 32 * w;
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   QueryRow<T, DP> Q;
   Q.load(a, h, row0 + r, hh);
-  __syncthreads();
   Rows R;
   R.init(table, row0 + r);
   if (R.in && hh == 0) a.rowdot[(int64_t)h * a.N + R.row] = Q.dot;
@@ -886,10 +937,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_dq(AttnArgs a) {
     at_exchange();
     if (j0 + BK < bhi) issue(j0 + BK, next);
     if (j0 >= R.hi || j0 + BK <= R.lo) return;
-    const bool inner = R.inner(j0, BK, row0);
 #pragma unroll
     for (int b = 0; b < BK / 32; ++b)
-      at_dq_block<T, DP>(Kl, Kl + TILE, 32 * b, j0 + 32 * b, inner, R, Q, a.c2, lane, dq);
+      at_dq_block<T, DP>(Kl, Kl + TILE, 32 * b, j0 + 32 * b, R, Q, a.c2, lane, dq);
   };
   if (blo < bhi) issue(blo, ldsA);
   for (int j0 = blo; j0 < bhi; j0 += 2 * BK) {
@@ -921,15 +971,15 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
   AT_TWO_BUFFERS(4 * MINE);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
   int h, q0;
-  at_query_tile<AT_SPLIT>(a, h, q0);
+  at_query_tile<AT_SPLIT>(a, table, keys, tid, h, q0);
   const int hk = h / (a.H / a.KV);
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   QueryRow<T, DP> Q;
   Q.load(a, h, q0 + r, hh);
-  __syncthreads();
   Rows R;
   R.init(table, q0 + r);
   if (R.in && hh == 0 && w == 0) a.rowdot[(int64_t)h * a.N + R.row] = Q.dot;
@@ -945,7 +995,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
     const bool more = j0 + 128 < R.hi;
     if (NBUF == 2 && more) issue(j0 + 128, next);  // its last reads were waited for
     at_landed<2 * Ld::NI>(NBUF == 2 && more);
-    at_dq_block<T, DP>(Kl, Kl + TILE, 0, j0, R.inner(j0, 32, q0), R, Q, a.c2, lane, dq);
+    at_dq_block<T, DP>(Kl, Kl + TILE, 0, j0, R, Q, a.c2, lane, dq);
     at_lds_free();
     if (NBUF == 1 && more) issue(j0 + 128, next);
   };
@@ -981,30 +1031,27 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------- backward: keys
-// A lane's key row and the queries that its wave meets.
+// A lane's key row, the queries that see it, and the queries that its wave meets.
 struct Keys {
   int row, start, end;
   bool in;
-  int lo, hi;    // queries the wave meets: [lo, hi)
-  int inner_hi;  // smallest end of the wave's rows
-  bool whole;
+  int lo, hi;  // queries the wave meets: [lo, hi)
+  Span seen;
   __device__ inline void init(const SeqTable& t, int r) {
     row = r;
     t.find(row, start, end);
     in = start <= row;
     lo = at_wave_min(in ? row : 0x7FFFFFFF);
     hi = at_wave_max(in ? end : -1);
-    inner_hi = at_wave_min(in ? end : 0x7FFFFFFF);
-    whole = __all(in);
+    seen = {row, in ? end - row : 0};
   }
-  // Every query of [i, i + n) sees every key of the wave (its first row is row0).
-  __device__ inline bool inner(int i, int n, int row0) const { return whole && i >= row0 + 31 && i + n <= inner_hi; }
 };
 
-// One block of 32 queries (images at Ql, Gl; L, D and L's remainder in qs): dv += p do,
-// dk += ds / scale q. vf(s) gives fragment s of the lane's value row.
+// One block of 32 queries (images at Ql, Gl; L, D, L's remainder and, for lanes that the
+// queries do not see, infinite L in qs): dv += p do, dk += ds / scale q. vf(s) gives
+// fragment s of the lane's value row.
 template <typename T, int DP, typename VF>
-__device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, const float (*qs)[32], int i0, bool inner,
+__device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, const float (*qs)[32], int i0,
                                     const Keys& K, const typename Op<T>::Frag (&kf)[DP / 16], VF&& vf, float c2,
                                     int lane, f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32]) {
   typedef Img<T, DP> I;
@@ -1016,9 +1063,12 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
     p = Op<T>::mma(I::rows(Ql, r, s, hh), kf[s], p);
     ds = Op<T>::mma(I::rows(Gl, r, s, hh), vf(s), ds);
   }
+  bool hidden;
+  const bool some = K.seen.some(i0, 32, hidden);
+  const float* ql = qs[hidden ? 3 : 0];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const float4 L = *(const float4*)&qs[0][8 * g + 4 * hh], D = *(const float4*)&qs[1][8 * g + 4 * hh];
+    const float4 L = *(const float4*)&ql[8 * g + 4 * hh], D = *(const float4*)&qs[1][8 * g + 4 * hh];
     const float Lv[4] = {L.x, L.y, L.z, L.w}, Dv[4] = {D.x, D.y, D.z, D.w};
     float Rv[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (sizeof(T) == 4) {
@@ -1034,11 +1084,10 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
       ds[i] = p[i] * (ds[i] - Dv[e]);
     }
   }
-  if (!inner) {
+  if (some) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int q = i0 + at_pos(i, hh);
-      const bool ok = q >= K.row && q < K.end;
+      const bool ok = K.seen.sees(i0 + at_pos(i, hh));
       p[i] = ok ? p[i] : 0.f;
       ds[i] = ok ? ds[i] : 0.f;
     }
@@ -1054,15 +1103,16 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
   }
 }
 
-// Key tile, key head and share of its query heads of a block: the tiles with the most
-// queries (a long sequence's first) first.
+// Key tile, key head and share of its query heads of a block.
 struct KeyTile {
   int hk, k0, share, h0, nh;
-  __device__ inline KeyTile(const AttnArgs& a, int rows) {
-    const int id = blockIdx.x, x = id % (a.KV * a.hs), rep = a.H / a.KV;
+  template <int ROWS>
+  __device__ inline void init(const AttnArgs& a, const SeqTable& table, int (&keys)[260], int tid) {
+    const int rep = a.H / a.KV;
+    int x;
+    at_order<ROWS, false>(a, table, keys, a.KV * a.hs, tid, x, k0);
     hk = x % a.KV;
     share = x / a.KV;
-    k0 = id / (a.KV * a.hs) * rows;
     nh = rep / a.hs;
     h0 = hk * rep + share * nh;
   }
@@ -1078,7 +1128,7 @@ struct QueryStats {
     if constexpr (sizeof(T) == 4) R = a.stats[at + (int64_t)a.H * a.N];
   }
   __device__ inline void store(float (*qs)[32], int q) const {
-    qs[0][q] = L, qs[1][q] = D;
+    qs[0][q] = L, qs[1][q] = D, qs[3][q] = INFINITY;
     if constexpr (sizeof(T) == 4) qs[2][q] = R;
   }
 };
@@ -1117,19 +1167,20 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
   constexpr int VLDS = sizeof(T) == 2 ? AT_ROWS * I::ROWB : 16;
   AT_TWO_BUFFERS(2 * TILE);
   __shared__ __attribute__((aligned(1024))) char Vl[VLDS];
-  __shared__ __attribute__((aligned(16))) float qs[2][3][32];
+  __shared__ __attribute__((aligned(16))) float qs[2][4][32];
   __shared__ int ends[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
-  const KeyTile t(a, AT_ROWS);
+  KeyTile t;
+  t.init<AT_ROWS>(a, table, keys, tid);
   const int row0 = t.k0 + 32 * w, rc = min(row0 + r, a.N - 1);
   if constexpr (sizeof(T) == 2) {
     Loader<T, DP, AT_ROWS, 4> lv;
     lv.init(a.v_row, a.D, w, lane);
     lv.issue((const T*)a.v + t.hk * a.v_head, a.v_row, t.k0, a.N - 1, a.D, Vl, w);
   }
-  __syncthreads();
   Keys K;
   K.init(table, row0 + r);
   int blo, bhi;
@@ -1163,7 +1214,7 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
     at_exchange();
     if (n + 1 < total) issue(next);
     if (i0 < K.hi && i0 + 32 > K.lo)
-      at_dkv_block<T, DP>(Ql, Ql + TILE, qs[n & 1], i0, K.inner(i0, 32, row0), K, kf, value, a.c2, lane, dk, dv);
+      at_dkv_block<T, DP>(Ql, Ql + TILE, qs[n & 1], i0, K, kf, value, a.c2, lane, dk, dv);
     i0 += 32;
     if (i0 >= bhi) i0 = blo;
   };
@@ -1190,17 +1241,18 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   typedef Loader<T, DP, 32, 1> Ld;
   constexpr int MINE = 2 * TILE;
   AT_TWO_BUFFERS(4 * MINE);
-  __shared__ __attribute__((aligned(16))) float qs[4][3][32];
+  __shared__ __attribute__((aligned(16))) float qs[4][4][32];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
+  __shared__ __attribute__((aligned(16))) int keys[260];
   const SeqTable table(a, seq, tid);
-  const KeyTile t(a, AT_SPLIT);
+  KeyTile t;
+  t.init<AT_SPLIT>(a, table, keys, tid);
   const int rc = min(t.k0 + r, a.N - 1);
   Frag kf[NS], vf[NS];
   at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
   at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
   auto value = [&](int s) -> const Frag& { return vf[s]; };
-  __syncthreads();
   Keys K;
   K.init(table, t.k0 + r);
   Ld lq, lg;
@@ -1221,7 +1273,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
     if (lane < 32) st.store(qs[w], lane);
     at_landed<0>(false);
     if (NBUF == 2 && more) issue(n + 4, next);
-    at_dkv_block<T, DP>(Ql, Ql + TILE, qs[w], i0, K.inner(i0, 32, t.k0), K, kf, value, a.c2, lane, dk, dv);
+    at_dkv_block<T, DP>(Ql, Ql + TILE, qs[w], i0, K, kf, value, a.c2, lane, dk, dv);
     at_lds_free();
     if (NBUF == 1 && more) issue(n + 4, next);
   };
