@@ -154,10 +154,10 @@ struct Img {
   // Fragment of row R, elements 16 s + 8 hh .. + 8.
   static __device__ inline typename Op<T>::Frag rows(const char* img, int R, int s, int hh) {
     if constexpr (sizeof(T) == 2) {
-      return *(const bf16x8*)(img + off(R, 2 * s + hh));
+      return *(const bf16x8*)(img + (off(R, hh) ^ s << 5));
     } else {
-      const float4 a = *(const float4*)(img + off(R, 4 * s + 2 * hh));
-      const float4 b = *(const float4*)(img + off(R, 4 * s + 2 * hh + 1));
+      const float4 a = *(const float4*)(img + (off(R, 2 * hh) ^ s << 6));
+      const float4 b = *(const float4*)(img + (off(R, 2 * hh + 1) ^ s << 6));
       return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
     }
   }
@@ -166,10 +166,10 @@ struct Img {
   static __device__ inline typename Op<T>::Frag cols(const char* img, int R0, int kk, int cb, int lane) {
     if constexpr (sizeof(T) == 2) {
       const int G = lane >> 4, e = (lane >> 2) & 3, a = lane & 3;
-      const int c = 4 * cb + 2 * (G & 1) + (a >> 1);
-      const int R = R0 + 16 * kk + 4 * (G >> 1) + e;
-      const at_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_i16x4)(img + off(R, c) + 8 * (a & 1)));
-      const at_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_i16x4)(img + off(R + 8, c) + 8 * (a & 1)));
+      const int at = off(4 * (G >> 1) + e, 2 * (G & 1) + (a >> 1)) + 8 * (a & 1) ^ cb << 6;
+      const char* p = img + (R0 + 16 * kk) * ROWB;  // the swizzle is the same 16 rows on, and 8 rows on at ^ 32
+      const at_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_i16x4)(p + at));
+      const at_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_i16x4)(p + 8 * ROWB + (at ^ 32)));
       return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     } else {
       const int r = lane & 31, hh = lane >> 5, c = 8 * cb + (r >> 2);
@@ -206,9 +206,9 @@ struct Loader {
   // not know the descriptor's type: a body it parsed would leave the kernels without stubs.)
   __device__ inline void issue(const T* base, int64_t stride, int first, int hi, int D, char* img, int wave) const {
 #if defined(__HIP_DEVICE_COMPILE__)
-    const int64_t bytes = ((hi - first) * stride + D) * (int64_t)sizeof(T);
+    const int bytes = (min(hi - first, ROWS - 1) * (int)stride + D) * (int)sizeof(T);  // a row is 8 MiB at most
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + first * stride), (short)0,
-                                                        (int)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF), 0x00020000);
+                                                        bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void_t*)(img + (wave + NW * i) * 1024), 16, voff[i], 0, 0, 0);
@@ -246,6 +246,12 @@ __device__ inline void at_row(const T* row, int D, int hh, typename Op<T>::Frag 
 
 // Key (or query) position inside a 32-row block that accumulator register i holds.
 __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
+// The lane again, as a value that nothing was formed from yet: LDS addresses of a loop are
+// formed from it in each turn, where kept over the loop they take registers from the tiles.
+__device__ inline int at_fresh(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
 __device__ inline float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The offsets in LDS, every step-th of them where there are more than the table holds: one
@@ -1033,17 +1039,17 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
 // ---------------------------------------------------------------- backward: keys
 // A lane's key row, the queries that see it, and the queries that its wave meets.
 struct Keys {
-  int row, start, end;
-  bool in;
+  Span seen;   // from the row itself to the end of its sequence
   int lo, hi;  // queries the wave meets: [lo, hi)
-  Span seen;
+  __device__ inline int row() const { return seen.first; }
+  __device__ inline int end() const { return seen.first + seen.width; }
+  __device__ inline bool in() const { return seen.width > 0; }
   __device__ inline void init(const SeqTable& t, int r) {
-    row = r;
-    t.find(row, start, end);
-    in = start <= row;
-    lo = at_wave_min(in ? row : 0x7FFFFFFF);
-    hi = at_wave_max(in ? end : -1);
-    seen = {row, in ? end - row : 0};
+    int start, end;
+    t.find(r, start, end);
+    seen = {r, end - r};
+    lo = at_wave_min(in() ? r : 0x7FFFFFFF);
+    hi = at_wave_max(in() ? end : -1);
   }
 };
 
@@ -1056,6 +1062,7 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
                                     int lane, f32x16 (&dk)[DP / 32], f32x16 (&dv)[DP / 32]) {
   typedef Img<T, DP> I;
   typedef typename Op<T>::Frag Frag;
+  if constexpr (sizeof(T) == 2) lane = at_fresh(lane);  // (fp32 has room, and more addresses)
   const int r = lane & 31, hh = lane >> 5;
   f32x16 p = {}, ds = {};
 #pragma unroll
@@ -1137,19 +1144,19 @@ struct QueryStats {
 template <typename T, int DP>
 __device__ inline bool at_store_keys(const AttnArgs& a, const KeyTile& t, const Keys& K, const f32x16 (&dk)[DP / 32],
                                      const f32x16 (&dv)[DP / 32], int hh) {
-  if (K.row >= a.N) return false;
-  const int64_t at = ((int64_t)K.row * a.KV + t.hk) * a.D;
+  if (K.row() >= a.N) return false;
+  const int64_t at = ((int64_t)K.row() * a.KV + t.hk) * a.D;
   if (a.hs > 1) {
-    if (!K.in) return false;  // the sum over shares knows
+    if (!K.in()) return false;  // the sum over shares knows
     const int64_t plane = (int64_t)a.N * a.KV * a.D;
     float* pk = a.part + 2 * t.share * plane + at;
     const bool x = at_store_row<float, DP / 32>(pk, nullptr, dk, a.scale, true, a.D, hh);
     const bool y = at_store_row<float, DP / 32>(pk + plane, nullptr, dv, 1.f, true, a.D, hh);
     return x || y;
   }
-  if (!K.in && !a.fill) return false;
-  const bool x = at_store_row<T, DP / 32>((T*)a.dk + at, nullptr, dk, a.scale, K.in, a.D, hh);
-  const bool y = at_store_row<T, DP / 32>((T*)a.dv + at, nullptr, dv, 1.f, K.in, a.D, hh);
+  if (!K.in() && !a.fill) return false;
+  const bool x = at_store_row<T, DP / 32>((T*)a.dk + at, nullptr, dk, a.scale, K.in(), a.D, hh);
+  const bool y = at_store_row<T, DP / 32>((T*)a.dv + at, nullptr, dv, 1.f, K.in(), a.D, hh);
   return x || y;
 }
 
@@ -1227,7 +1234,7 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
   while (bad) {
     const int i = __builtin_ctzll(bad);
     bad &= bad - 1;
-    at_dkv_row<T>(at_args(), t.hk, t.share, row0 + i, __shfl(K.end, i, 64), lane);
+    at_dkv_row<T>(at_args(), t.hk, t.share, row0 + i, __shfl(K.end(), i, 64), lane);
   }
 }
 
@@ -1288,7 +1295,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   const Join<DP> join = {ldsA, ldsA + 2 * Join<DP>::SHARE};
   float odd = 0.f;
   const int rr = tid >> 3, row = t.k0 + rr;
-  const bool in = __shfl(K.start, rr, 64) <= row;
+  const bool in = __shfl(K.seen.width, rr, 64) > 0;
   const int64_t at = ((int64_t)row * a.KV + t.hk) * a.D, plane = (int64_t)a.N * a.KV * a.D;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -1310,7 +1317,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   }
   for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
     const int i = 8 * w + __builtin_ctz(bad);
-    at_dkv_row<T>(at_args(), t.hk, t.share, t.k0 + i, __shfl(K.end, i, 64), lane);
+    at_dkv_row<T>(at_args(), t.hk, t.share, t.k0 + i, __shfl(K.end(), i, 64), lane);
   }
 }
 
