@@ -911,7 +911,7 @@ __device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int 
 
 // dq, and D_i for the key side. Tiles and waves as the forward's.
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS, 2) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__(AT_THREADS, sizeof(T) == 4 && DP > 64 ? 1 : 2) void k_attn_dq(AttnArgs a) {
   constexpr int BK = FwdCfg<T, DP>::BK, TILE = FwdCfg<T, DP>::TILE, NC = DP / 32;
   AT_TWO_BUFFERS(2 * TILE);
   __shared__ int ends[2][4];
@@ -1386,13 +1386,22 @@ void at_form(int dtype, int D, F&& f) {
   else width(0.f);
 }
 
-// Blocks below which a launch leaves CUs without one of the two it holds.
-constexpr int64_t AT_FULL = 512;
+// Blocks of 128 rows below which the 32-row forms run: one a CU (bf16, 4096 tokens in four
+// sequences, 12 heads: D = 64 forward, dq, dk/dv 36, 44, 59 us against 34, 49, 83 split;
+// D = 128 47, 61, 90 against 57, 112, 129; 2048 tokens, 192 blocks, D = 64: 25, 30, 41 against
+// 17, 26, 35). For queries in fp32, whose products take eight times as long, the finer tiles
+// gain up to two a CU (D = 64: 4096 tokens, 12 heads forward, dq 141, 198 us against 115, 162;
+// 8192 tokens 240, 344 against 264, 370; the key side is even at 4096 tokens: 263 against
+// 233, D = 128 497 against 600).
+constexpr int64_t AT_FULL = 256;
 
-bool at_query_split(int64_t rows, int H) { return cdiv(rows, AT_ROWS) * H < AT_FULL; }
+bool at_query_split(int64_t rows, int H, int dtype) {
+  return cdiv(rows, AT_ROWS) * H < (dtype == PD_DTYPE_BF16 ? AT_FULL : 2 * AT_FULL);
+}
 
 // Shares of a group's heads and the tile of the key side: as few shares as fill the GPU
-// with 128-key tiles, else 32-key tiles whose waves share the queries.
+// eight times with 128-key tiles, else one head a share, else 32-key tiles whose waves share
+// the queries, two blocks a CU.
 struct KeyPlan {
   int hs;
   bool split;
@@ -1400,10 +1409,10 @@ struct KeyPlan {
 KeyPlan at_key_plan(int64_t rows, int H, int KV) {
   const int rep = H / KV;
   for (int hs = 1; hs <= rep; ++hs)
-    if (rep % hs == 0 && cdiv(rows, AT_ROWS) * KV * hs >= 4 * AT_FULL) return {hs, false};
+    if (rep % hs == 0 && cdiv(rows, AT_ROWS) * KV * hs >= 8 * AT_FULL) return {hs, false};
   if (cdiv(rows, AT_ROWS) * KV * rep >= AT_FULL) return {rep, false};
   for (int hs = 1; hs <= rep; ++hs)
-    if (rep % hs == 0 && cdiv(rows, AT_SPLIT) * KV * hs >= AT_FULL) return {hs, true};
+    if (rep % hs == 0 && cdiv(rows, AT_SPLIT) * KV * hs >= 2 * AT_FULL) return {hs, true};
   return {rep, true};
 }
 
@@ -1438,7 +1447,7 @@ int pd_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const 
   at_fill_args(a, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, rows, n_head, n_kv_head, head_dim, offsets, n_seq,
                scale, fill);
   a.out = out, a.rest = out_rest, a.stats = stats;
-  const bool split = at_query_split(rows, n_head);
+  const bool split = at_query_split(rows, n_head, dtype);
   const unsigned grid = (unsigned)(cdiv(rows, split ? AT_SPLIT : AT_ROWS) * n_head);
   at_form(dtype, head_dim, [&](auto t, auto dp) {
     typedef decltype(t) T;
@@ -1482,7 +1491,7 @@ int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const 
   a.hs = plan.hs;
   a.part = (float*)((char*)workspace + (size_t)cdiv(rows * n_head, 4) * 16);
   hipStream_t s = (hipStream_t)stream;
-  const bool split = at_query_split(rows, n_head);
+  const bool split = at_query_split(rows, n_head, dtype);
   const dim3 block(AT_THREADS), gq((unsigned)(cdiv(rows, split ? AT_SPLIT : AT_ROWS) * n_head)),
       gk((unsigned)(cdiv(rows, plan.split ? AT_SPLIT : AT_ROWS) * n_kv_head * plan.hs)),
       gs((unsigned)cdiv(2 * rows * n_kv_head * head_dim, 1024));
