@@ -455,3 +455,47 @@ def test_mixed_devices_are_refused(device):
         packed_attention(q, k, v, torch.tensor([0, 10], dtype=torch.int32))
     with pytest.raises(L.PDError, match="k is on cpu"):
         packed_attention(q, k.cpu(), v, _offsets(device, [10]))
+
+
+@pytest.mark.parametrize("dtype, H, KV, D", [(BF16, 32, 8, 64), (BF16, 32, 32, 128), (F32, 36, 36, 64)])
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+def test_hidden_rows_reach_nobody_in_large_grids(device, dtype, H, KV, D, poison):
+    """Waves of 128-row tiles that hold one sequence's end and the next one's start see
+    whole blocks in some lanes only: poison in the one sequence stays there."""
+    N, lengths, first = 2100, [517, 790, 3, 700], 2
+    q, k, v, g = _inputs(device, N, H, KV, D, dtype, seed=23)
+    off = _offsets(device, lengths, first)
+    clean = _grads(q, k, v, g, off)
+    val, tol = _definition(q, k, v, g, lengths, first)
+    _check(clean, val, tol)
+    seen = slice(first + 517, first + 517 + 790)
+    bad = [t.clone() for t in (q, k, v, g)]
+    for t in bad:
+        t[seen.start + 400] = poison
+        t[:first] = poison
+        t[first + sum(lengths):] = poison
+    others = torch.zeros(N, dtype=torch.bool, device=device)
+    others[first:first + sum(lengths)] = True
+    others[seen] = False
+    for x, y, e in zip(_grads(*bad, off), val, tol):
+        assert ((x.double() - y).abs() <= e)[others].all()
+
+
+@pytest.mark.parametrize("N, H, lengths, first", [(8300, 3, [1, 64, 700, 31] * 10, 5), (4100, 9, [129] * 31, 0)])
+def test_every_tile_is_taken_once(device, N, H, lengths, first):
+    """More tiles than the blocks put in order, and as many as they do, in 32-row forms."""
+    q, k, v, g = _inputs(device, N, H, 1, 64, BF16, seed=29)
+    got = _grads(q, k, v, g, _offsets(device, lengths, first))
+    _check(got, *_definition(q, k, v, g, lengths, first))
+
+
+def test_offsets_that_are_out_of_order_stay_inside_in_large_grids(device):
+    N = 2100
+    big = torch.full((N + 256, 32, 64), 3.0, dtype=BF16, device=device)
+    q, k, v, g = _inputs(device, N, 32, 32, 64, BF16)
+    for o in ([50, 20, 1999], [0, 5000, 7], [-9, 4, 2090], [2**31 - 1, -(2**31), 100], [1500, 100, 900, 0, 2100]):
+        out = big[128:128 + N]
+        ops.packed_attention_fwd(q, k, v, torch.tensor(o, dtype=torch.int32, device=device), out=out)
+        _grads(q, k, v, g, torch.tensor(o, dtype=torch.int32, device=device))
+        torch.cuda.synchronize()
+        assert (big[:128] == 3).all() and (big[128 + N:] == 3).all()
