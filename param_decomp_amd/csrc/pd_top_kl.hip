@@ -47,7 +47,7 @@ struct TopKLArgs {
   int idx64;
   int k;
   const float* lse;
-  float tau;
+  double tau;
   float c, c_lo;  // log2(e) / tau, rounded down, and the positive rest of it
   float itau;
   const float* weight;
@@ -104,11 +104,11 @@ __global__ __launch_bounds__(256) void k_top_kl_loss(TopKLArgs a) {
   if (r >= a.rows) return;
   const KLRow R = a.row[r];
   const T* row = (const T*)a.z + r * a.V;
-  const double itau = 1.0 / (double)a.tau;
+  const double itau = 1.0 / a.tau;
   auto entry = [&](int e, int64_t& v, double& t) -> bool {
     v = a.idx64 ? ((const int64_t*)a.idx)[r * a.k + e] : ((const int32_t*)a.idx)[r * a.k + e];
     t = (double)(a.top_dtype == PD_DTYPE_F32 ? ((const float*)a.top)[r * a.k + e]
-                                             : bf16_to_f32(((const bf16_t*)a.top)[r * a.k + e])) / (double)a.tau;
+                                             : bf16_to_f32(((const bf16_t*)a.top)[r * a.k + e])) / a.tau;
     return v >= 0 && v < a.V;
   };
   int64_t v;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(NT, 4) void k_top_kl(TopKLArgs a) {
     double sum_p = 0.0;
     if (a.lse) {  // in 64 bits: the rest is what they leave of 1
       if (has_top) {
-        const double lse = (double)lse_r, itau = 1.0 / (double)a.tau;
+        const double lse = (double)lse_r, itau = 1.0 / a.tau;
 #pragma unroll
         for (int j = 0; j < KT; ++j)
           if (own >> j & 1) {
@@ -508,7 +508,7 @@ extern "C" {
 size_t pd_top_kl_workspace_size(int64_t rows) { return rows > 0 ? (size_t)rows * sizeof(KLRow) : 0; }
 
 int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void* top, int top_dtype, const void* idx,
-              int idx_bits, int k, const float* clean_lse, float temperature, const float* row_weight, float* kl,
+              int idx_bits, int k, const float* clean_lse, double temperature, const float* row_weight, float* kl,
               void* grad, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != PD_DTYPE_F32 && dtype != PD_DTYPE_BF16) return fail(PD_EUNSUPPORTED, "pd_top_kl: logits are fp32 or bf16");
   if (top_dtype != PD_DTYPE_F32 && top_dtype != PD_DTYPE_BF16)
@@ -523,7 +523,7 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
   if (!z || !top || !idx || (!kl && !grad)) return fail(PD_EINVAL, "pd_top_kl: null pointer");
   if (kl && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < pd_top_kl_workspace_size(rows)))
     return fail(PD_EWORKSPACE, "pd_top_kl: workspace");
-  const double c = 1.4426950408889634074 / (double)temperature, itau = 1.0 / (double)temperature;
+  const double c = 1.4426950408889634074 / temperature, itau = 1.0 / temperature;
   float c_hi = (float)c;
   if ((double)c_hi >= c) c_hi = std::nextafter(c_hi, 0.f);
   const TopKLArgs a = {z, rows, (int)vocab, top, top_dtype, idx, idx_bits == 64, k, clean_lse, temperature, c_hi,

@@ -284,3 +284,12 @@ def test_mixed_devices_are_refused(device):
     z, top, idx, lse, w = _inputs(device, 2, 50, 4, F32)
     with pytest.raises(L.PDError, match="top_indices is on cpu"):
         ops.top_logits_kl(z, top, idx.cpu())
+
+
+def test_temperature_keeps_its_64_bits(device):
+    """0.7 in 32 bits is 2^-25.8 off: of a logit of 30000 that would be 7e-4 in an exponent."""
+    z, top, idx, _, w = _inputs(device, 40, 700, 8, F32, 0.7, seed=31)
+    z, top = z + 30000, top + 30000
+    clean = torch.logsumexp(top.double() / 0.7, -1) + 0.4
+    args = (z, top, idx, clean.float(), 0.7, w)
+    _check(_both(*args), *_definition(*args))
