@@ -731,7 +731,7 @@ int pd_layer_norm_bwd(const void* x, const void* d_y, int dtype, int64_t rows, i
  * kl fp32 [rows] (nullable); grad [rows, vocab] in `dtype` (nullable) = row_weight (fp32
  * [rows], NULL = 1) times d kl / d z; a row of weight 0 gets zeros whatever it holds.
  * vocab up to 2^19, k up to 1024. The workspace is needed with kl. */
-size_t pd_top_kl_workspace_size(int64_t rows);
+size_t pd_top_kl_workspace_size(int64_t rows, int k);
 int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void* top, int top_dtype, const void* idx,
               int idx_bits, int k, const float* clean_lse, double temperature, const float* row_weight, float* kl,
               void* grad, void* workspace, size_t workspace_bytes, void* stream);

@@ -132,7 +132,7 @@ _SIGNATURES = {
     "pd_layer_norm_fwd": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_p, _c_f32, _c_p, _c_p, _c_p]),
     "pd_layer_norm_bwd_workspace_size": (_c_sz, [_c_i64, _c_i64]),
     "pd_layer_norm_bwd": (_c_i32, [_c_p, _c_p, _c_i32, _c_i64, _c_i64] + [_c_p] * 6 + [_c_sz, _c_p]),
-    "pd_top_kl_workspace_size": (_c_sz, [_c_i64]),
+    "pd_top_kl_workspace_size": (_c_sz, [_c_i64, _c_i32]),
     "pd_top_kl": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_i32, _c_i32, _c_p, ctypes.c_double] + [_c_p] * 4 +
                   [_c_sz, _c_p]),
     "pd_faithfulness_workspace_size": (_c_sz, [_c_i64] * 4),

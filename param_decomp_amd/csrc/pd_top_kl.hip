@@ -27,6 +27,7 @@
 // hold the row. The gradient's rest is 64-bit too (what the listed leave of 1), its other
 // terms are 32-bit.
 #include <float.h>
+#include <type_traits>
 
 #include "pd_common.hpp"
 
@@ -35,6 +36,7 @@ namespace {
 
 constexpr double REST_MIN = 1.0 / (1 << 20);  // a rest below this is the rounding of its inputs: none
 constexpr int KL_MAX_K = 1024;
+constexpr int KL_LIST_NT = 256;  // forms of up to so many threads keep the listed logits for the loss
 constexpr int64_t KL_MAX_V = 1 << 19;  // 64 KiB of bits
 
 struct TopKLArgs {
@@ -54,6 +56,7 @@ struct TopKLArgs {
   float* kl;
   void* grad;
   struct KLRow* row;  // [rows] (NULL: no loss is wanted)
+  float* listed;      // [rows, k] the listed logits, for the loss (forms of few threads)
 };
 
 // 16 bytes of a row, at any element's boundary (the hardware takes them as one access).
@@ -96,14 +99,26 @@ struct KLRow {
   int listed, pad[3];
 };
 
-// kl of a row, a wave each.
-template <typename T>
+template <int G>
+__device__ inline double kl_group_sum(double v) {
+  for (int off = G / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// kl of a row, G lanes each. LIST: the listed logits come from the first kernel, in order; read
+// again from the rows they are a line of memory each (100000 x 1000, 32 listed, with the
+// gradient 202 us in place of 262). Where rows are long there are fewer of them, and keeping
+// the list costs the first kernel more (1500 x 32000 fp32, the loss alone: 50 us, 47 without).
+// With 16 lanes a wave takes the last step's logarithms for four rows at once; up to 4096
+// rows, where that would leave SIMDs without a wave, a row has a wave (2048 rows of 128
+// listed 9 us, 13 with 16 lanes; 8192 rows of 64 from the rows 23.4 us with 16, 24.7 with a
+// wave).
+template <typename T, int G, bool LIST>
 __global__ __launch_bounds__(256) void k_top_kl_loss(TopKLArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x % G;
+  const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (r >= a.rows) return;
   const KLRow R = a.row[r];
-  const T* row = (const T*)a.z + r * a.V;
   const double itau = 1.0 / a.tau;
   auto entry = [&](int e, int64_t& v, double& t) -> bool {
     v = a.idx64 ? ((const int64_t*)a.idx)[r * a.k + e] : ((const int32_t*)a.idx)[r * a.k + e];
@@ -117,24 +132,24 @@ __global__ __launch_bounds__(256) void k_top_kl_loss(TopKLArgs a) {
     norm = (double)a.lse[r];
   } else {  // log of the teacher's partition sum
     double mx = -INFINITY, s = 0.0;
-    for (int e = lane; e < a.k; e += 64)
+    for (int e = lane; e < a.k; e += G)
       if (entry(e, v, t)) mx = fmax(mx, t), valid += 1.0;
-    for (int off = 32; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor(mx, off, 64));
-    for (int e = lane; e < a.k; e += 64)
+    for (int off = G / 2; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor(mx, off, 64));
+    for (int e = lane; e < a.k; e += G)
       if (entry(e, v, t)) s += exp(t - mx);
-    norm = mx + log(wave_sum_d(s));
-    valid = wave_sum_d(valid);
+    norm = mx + log(kl_group_sum<G>(s));
+    valid = kl_group_sum<G>(valid);
   }
   double sum_p = 0.0, plogp = 0.0, pz = 0.0;
-  for (int e = lane; e < a.k; e += 64)
+  for (int e = lane; e < a.k; e += G)
     if (entry(e, v, t)) {
       const double l = t - norm, p = exp(l);
       sum_p += p;
-      if (p != 0.0) plogp += p * l, pz += p * (double)load_f<T>(row, v);
+      if (p != 0.0) plogp += p * l, pz += p * (double)(LIST ? a.listed[r * a.k + e] : load_f<T>((const T*)a.z + r * a.V, v));
     }
-  sum_p = wave_sum_d(sum_p);
-  plogp = wave_sum_d(plogp);
-  pz = wave_sum_d(pz);
+  sum_p = kl_group_sum<G>(sum_p);
+  plogp = kl_group_sum<G>(plogp);
+  pz = kl_group_sum<G>(pz);
   if (lane) return;
   const double M = fmax((double)R.mt, (double)R.mp);
   const double S = (double)R.st * exp(((double)R.mt - M) * itau) + (double)R.sp * exp(((double)R.mp - M) * itau);
@@ -152,7 +167,10 @@ __global__ __launch_bounds__(256) void k_top_kl_loss(TopKLArgs a) {
 
 // Entries of the list a thread takes: forms of few threads are used for short lists only.
 constexpr int kl_entries(int nt) { return nt >= 256 ? KL_MAX_K / nt : 4; }
-// REG: the row fits NT * U words and stays in registers between the two passes.
+// REG: the row fits NT * U words and stays in registers between the two passes. What bounds it
+// is a row's chain of passes (maximum, sum, gradient, with a reduction between each two) at
+// two rows a CU where rows are long: 8192 x 50277 bf16, 64 listed, the gradient 430 us,
+// 3.8 TB/s, the loss another 20; 1500 x 32000 fp32 93 us, 4.1 TB/s.
 template <typename T, int NT, int U, bool REG, bool GRAD>
 __global__ __launch_bounds__(NT, 4) void k_top_kl(TopKLArgs a) {
 #pragma clang fp contract(off)  // the same sums with and without the gradient
@@ -419,6 +437,12 @@ __global__ __launch_bounds__(NT, 4) void k_top_kl(TopKLArgs a) {
       repeated[par ^ 1] = 0;  // for the next row; this row's has been read
     }
 
+    if (NT <= KL_LIST_NT && a.row) {
+#pragma unroll
+      for (int j = 0; j < KT; ++j)
+        if (vi[j] >= 0) a.listed[r * a.k + at + j * NT] = zj[j];  // repeated entries too
+    }
+
     // ---- the gradient
     if constexpr (GRAD) {
       const float M = fmaxf(mt, mp), wt = scaled(mt - M), S = st * wt + sp * scaled(mp - M);
@@ -486,9 +510,23 @@ int top_kl_launch(const TopKLArgs& a, hipStream_t s) {
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024) != hipSuccess)
       return fail(PD_ELAUNCH, "pd_top_kl: shared memory");
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.rows < held ? a.rows : held)), dim3(nt), lds, s, a);
-    if (a.kl) hipLaunchKernelGGL(k_top_kl_loss<T>, dim3((unsigned)cdiv(a.rows, 4)), dim3(256), 0, s, a);
+    auto loss = [&](auto wave, auto list) {
+      constexpr int G = wave ? 64 : 16;
+      hipLaunchKernelGGL((k_top_kl_loss<T, G, list>), dim3((unsigned)cdiv(a.rows, 256 / G)), dim3(256), 0, s, a);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (a.kl) {
+      if (a.rows <= 4096) nt <= KL_LIST_NT ? loss(yes, yes) : loss(yes, no);
+      else nt <= KL_LIST_NT ? loss(no, yes) : loss(no, no);
+    }
     return check_launch("pd_top_kl");
   };
+  // The smallest form that holds the row (and, with one wave, its list): loss and gradient in
+  // the next two, and the streaming one: 100000 x 1000 bf16 291, 343, 895, 3628 us; 8192 x
+  // 16000 135, 193, 245, 343; 4096 x 50277 217, 319, streaming 295. The widest is even with the
+  // streaming one (2048 x 131000: 284 and 288) and reads a row once. 512 threads of 16 words
+  // with one block a CU, two, more: 289, 229, 231 us at 4096 x 50277.
   if (a.k <= 256 && words <= 64 * 2) return go(k_top_kl<T, 64, 2, true, GRAD>, 64, 256 * 16);
   if (a.k <= 256 && words <= 64 * 8) return go(k_top_kl<T, 64, 8, true, GRAD>, 64, 256 * 16);
   if (words <= 256 * 8) return go(k_top_kl<T, 256, 8, true, GRAD>, 256, 256 * 8);
@@ -505,7 +543,9 @@ using namespace pd;
 
 extern "C" {
 
-size_t pd_top_kl_workspace_size(int64_t rows) { return rows > 0 ? (size_t)rows * sizeof(KLRow) : 0; }
+size_t pd_top_kl_workspace_size(int64_t rows, int k) {
+  return rows > 0 && k > 0 ? (size_t)rows * (sizeof(KLRow) + (size_t)k * sizeof(float)) : 0;
+}
 
 int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void* top, int top_dtype, const void* idx,
               int idx_bits, int k, const float* clean_lse, double temperature, const float* row_weight, float* kl,
@@ -521,14 +561,14 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
     return fail(PD_EINVAL, "pd_top_kl: temperature must be positive and finite");
   if (!rows) return PD_OK;
   if (!z || !top || !idx || (!kl && !grad)) return fail(PD_EINVAL, "pd_top_kl: null pointer");
-  if (kl && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < pd_top_kl_workspace_size(rows)))
+  if (kl && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < pd_top_kl_workspace_size(rows, k)))
     return fail(PD_EWORKSPACE, "pd_top_kl: workspace");
   const double c = 1.4426950408889634074 / temperature, itau = 1.0 / temperature;
   float c_hi = (float)c;
   if ((double)c_hi >= c) c_hi = std::nextafter(c_hi, 0.f);
   const TopKLArgs a = {z, rows, (int)vocab, top, top_dtype, idx, idx_bits == 64, k, clean_lse, temperature, c_hi,
                        (float)(c - (double)c_hi), (float)itau, row_weight, kl,
-                       grad, kl ? (KLRow*)workspace : nullptr};
+                       grad, kl ? (KLRow*)workspace : nullptr, kl ? (float*)((KLRow*)workspace + rows) : nullptr};
   if (!std::isfinite(a.c) || !(a.c_lo > 0.f) || !std::isfinite(a.itau)) return fail(PD_EINVAL, "pd_top_kl: temperature is out of range");
   hipStream_t s = (hipStream_t)stream;
   if (dtype == PD_DTYPE_F32) return grad ? top_kl_launch<float, true>(a, s) : top_kl_launch<float, false>(a, s);

@@ -535,7 +535,7 @@ def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, tem
     kl = torch.empty(lead, dtype=torch.float32, device=device) if want_kl else None
     grad = torch.empty_like(z) if want_grad else None
     rows = math.prod(lead)
-    ws = L.workspace(L.load().pd_top_kl_workspace_size(rows), device) if want_kl else None
+    ws = L.workspace(L.load().pd_top_kl_workspace_size(rows, k), device) if want_kl else None
     if want_kl or want_grad:
         L.launch("pd_top_kl", device, L.ptr(z), L.dtype_code(z.dtype), rows, V, L.ptr(top_logits),
                  L.dtype_code(top_logits.dtype), L.ptr(top_indices), 8 * top_indices.element_size(), k,
