@@ -57,6 +57,6 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
         return packed_attention(q, k, v, offsets, scale=scale)[..., :D]
     q, k, v = _dense(q), _dense(k), _dense(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if ops.differentiated(q, k, v):
         return _PackedAttention.apply(q, k, v, offsets, scale)
     return ops.packed_attention_fwd(q, k, v, offsets, scale=scale)[0]

@@ -322,7 +322,7 @@ def top_logits_position_kl(masked_logits: torch.Tensor, top_logits: torch.Tensor
     masked = masked_logits.contiguous()
     top, indices = top_logits.detach().contiguous(), top_indices.contiguous()
     lse = None if clean_lse is None else clean_lse.detach().contiguous()
-    if torch.is_grad_enabled() and masked.requires_grad:
+    if ops.differentiated(masked):
         return _TopLogitsKL.apply(masked, top, indices, lse, float(temperature))
     return ops.top_logits_kl(masked, top, indices, clean_lse=lse, temperature=float(temperature))[0]
 

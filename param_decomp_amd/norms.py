@@ -32,7 +32,6 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x = x.contiguous()
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if ops.differentiated(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     return ops.layer_norm_fwd(x, weight, bias, eps=eps)[0]

@@ -10,6 +10,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from param_decomp_amd import _lib as L
 from param_decomp_amd.prng import Key
@@ -367,6 +368,15 @@ def source_ascend(opt: int, sources, grad, state_a=None, state_b=None, *, step_c
     return sources
 
 # ------------------------------------------------- around a language model's decomposed sites
+def differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these has to go through its autograd function: one of them needs a
+    gradient, or carries a forward-mode tangent (which the functions refuse; past them it
+    would be lost without a word)."""
+    given = [t for t in tensors if t is not None]
+    return ((torch.is_grad_enabled() and any(t.requires_grad for t in given)) or
+            any(forward_ad.unpack_dual(t).tangent is not None for t in given))
+
+
 def _one_device(name: str, first: torch.Tensor, labels: str, *others: torch.Tensor | None) -> torch.device:
     """The first tensor's device, which the others (named in `labels`) have to share."""
     device = first.device
