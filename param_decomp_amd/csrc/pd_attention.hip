@@ -38,7 +38,6 @@ constexpr int AT_THREADS = 256;  // 4 waves
 constexpr int AT_ROWS = 128;     // rows of a block whose waves own 32 each
 constexpr int AT_SPLIT = 32;     // rows of a block whose waves share them
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float AT_NONE = -1e30f;  // a row's reference score before its first key
 constexpr float AT_SLACK = 8.f;    // a row is rescaled once its maximum has grown past 2^this
 
 struct AttnArgs {
@@ -331,11 +330,12 @@ __device__ __attribute__((noinline)) void at_fwd_row(const AttnArgs* a, int h, i
   const T* q = (const T*)a->q + row * a->q_row + h * a->q_head;
   const T* k = (const T*)a->k + hk * a->k_head;
   const T* v = (const T*)a->v + hk * a->v_head;
-  float m = AT_NONE, l = 0.f, o0 = 0.f, o1 = 0.f;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 64) {
     const int j = j0 + lane;
     const float s = j <= row ? at_dot<T>(q, k + j * a->k_row, D) * a->c2 : -INFINITY;
-    const float mn = fmaxf(m, wave_max(s)), al = at_exp2(m - mn), p = j <= row ? at_exp2(s - mn) : 0.f;
+    const float mn = fmaxf(m, wave_max(s)), al = m == mn ? 1.f : at_exp2(m - mn);
+    const float p = s == -INFINITY ? 0.f : at_exp2(s - mn);  // (before the first finite score mn is -inf too)
     m = mn;
     l = l * al + wave_sum(p);
     o0 *= al, o1 *= al;
@@ -570,9 +570,10 @@ __device__ inline float at_halves_max(float v) {
 
 // ---------------------------------------------------------------- forward
 // One row block's online softmax over a tile of NB key blocks: scores sc (raw, masked ones
-// -inf) to weights in place, the running reference m (raw), the lane's own part of the sum l,
-// and the accumulators rescaled where a maximum has grown by more than the slack: weights
-// stay below 2^8 and a tile without growth costs no pass over the accumulators.
+// -inf) to weights in place, the running reference m (raw, -inf before the row's first finite
+// score: that one is taken whatever its size), the lane's own part of the sum l, and the
+// accumulators rescaled where a maximum has grown by more than the slack: weights stay below
+// 2^8 and a tile without growth costs no pass over the accumulators.
 template <int NB, int NC>
 __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float& m, float& l, f32x16 (&o)[NC],
                                            float c2) {
@@ -584,7 +585,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
     for (int i = 0; i < 16; ++i) x[i & 3] = fmaxf(x[i & 3], sc[b][i]);
   const float mt = hidden ? -INFINITY : at_halves_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   if (__any((mt - m) * c2 > AT_SLACK)) {
-    const float mn = fmaxf(m, mt), al = at_exp2((m - mn) * c2);
+    const float mn = fmaxf(m, mt), al = m == mn ? 1.f : at_exp2((m - mn) * c2);
     m = mn;
     l *= al;
 #pragma unroll
@@ -592,7 +593,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[c][i] *= al;
   }
-  const float mc = hidden ? -INFINITY : -m * c2;
+  const float mc = hidden || m == -INFINITY ? -INFINITY : -m * c2;  // -inf: weights 0
   float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   Loader<T, DP, BK, 4> lk, lv;
   lk.init(a.k_row, a.D, w, lane);
   lv.init(a.v_row, a.D, w, lane);
-  float m = AT_NONE, l = 0.f;
+  float m = -INFINITY, l = 0.f;
   f32x16 o[NC] = {};
   auto issue = [&](int j0, char* img) {
     lk.issue(kb, a.k_row, j0, bhi - 1, a.D, img, w);
@@ -784,7 +785,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   lv.init(a.v_row, a.D, 0, lane);
   char* Kl = ldsA + w * TILE;
   char* Vl = ldsB + w * TILE;
-  float m = AT_NONE, l = 0.f;
+  float m = -INFINITY, l = 0.f;
   f32x16 o[NC] = {};
   int j0 = R.lo < R.hi ? R.lo + 32 * w : R.hi;
   if (j0 < R.hi) {
@@ -818,6 +819,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   l += __shfl_xor(l, 32, 64);
   if (hh == 0) ml[0][w][r] = m, ml[1][w][r] = l;
   __syncthreads();
+  // (a row without a finite score has no reference: NaN, as its softmax is, or no sequence)
   const float M = fmaxf(fmaxf(ml[0][0][r], ml[0][1][r]), fmaxf(ml[0][2][r], ml[0][3][r]));
   float sum_l = 0.f;
 #pragma unroll
