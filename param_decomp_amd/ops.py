@@ -372,9 +372,11 @@ def differentiated(*tensors: torch.Tensor | None) -> bool:
     """Whether a call on these has to go through its autograd function: one of them needs a
     gradient, or carries a forward-mode tangent (which the functions refuse; past them it
     would be lost without a word)."""
-    given = [t for t in tensors if t is not None]
-    return ((torch.is_grad_enabled() and any(t.requires_grad for t in given)) or
-            any(forward_ad.unpack_dual(t).tangent is not None for t in given))
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None):
+            return True
+    return False
 
 
 def _one_device(name: str, first: torch.Tensor, labels: str, *others: torch.Tensor | None) -> torch.device:
