@@ -68,7 +68,7 @@ extern "C" {
 #define PD_BLOCK_FUSED_INPUT 1  /* BlockContraction "fused_input" */
 
 const char* pd_last_error(void);
-int pd_abi_version(void);
+int pd_abi_version(void); /* 2: pd_packed_attention's stats are [2, n_head, rows] with bf16 too */
 
 /* ---- mask draw: jax.random.uniform (pd/core/linear_plan.py:80-106 uniform_like) ---- */
 /* out[i] = uniform(key)[i], i < n, drawn in draw_dtype, stored in out_dtype. */
@@ -681,9 +681,10 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
  * infinities included, reaches no other row. Offsets outside [0, rows] or out of order
  * give wrong rows but no access outside the tensors.
  *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, fp32 statistics;
- * For the backward (nullable): stats, log2 of the rows' softmax sums, fp32 [n_head, rows]
- * (with fp32 tensors [2, n_head, rows]: then what rounding took off them), and with bf16
- * tensors out_rest [rows, n_head, head_dim] bf16, what rounding took off out.
+ * For the backward (nullable): stats fp32 [2, n_head, rows], a reference score q . k of each
+ * row and log2 of its softmax sum relative to that, and with bf16 tensors out_rest [rows,
+ * n_head, head_dim] bf16, what rounding took off out. Scores may have any size that fp32
+ * holds; weights depend on their differences alone.
  * The backward gives dq [rows, n_head, head_dim], dk and dv [rows, n_kv_head, head_dim]
  * (summed over the query heads that share a key head) from the forward's out, out_rest
  * (NULL with fp32) and stats and d_out [rows, n_head, head_dim]. out, d_out, dq, dk, dv are

@@ -12,6 +12,7 @@ import os
 
 import torch
 
+ABI_VERSION = 2  # of the C interface these signatures and buffer sizes are for
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libpd_mi355x.so")
 
 F32, BF16, U16 = 0, 1, 2
@@ -162,6 +163,8 @@ def load() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
+        if lib.pd_abi_version() != ABI_VERSION:
+            raise PDError(f"{LIB_PATH} has interface {lib.pd_abi_version()}, not {ABI_VERSION}: build it again")
         _lib = lib
     return _lib
 

@@ -3,7 +3,7 @@
 // The rows of q [N, H, D], k and v [N, KV, D] are tokens; sequence s is rows
 // [offsets[s], offsets[s+1]) and row i of it, for a query head h and its key head
 // h / (H / KV), with s_ij = scale q_i . k_j over start <= j <= i:
-//   L_i = log sum_j e^{s_ij}, p_ij = e^{s_ij - L_i}, o_i = sum_j p_ij v_j
+//   p_ij = e^{s_ij} / sum_j e^{s_ij}, o_i = sum_j p_ij v_j
 //   backward, D_i = do_i . o_i and dp_ij = do_i . v_j: ds_ij = scale p_ij (dp_ij - D_i),
 //   dq_i = sum_j ds_ij k_j, dk_j = sum_{h of the group} sum_i ds_ij q_i,
 //   dv_j = sum_{h of the group} sum_i p_ij do_i
@@ -23,6 +23,12 @@
 // read transposed from the row-major LDS image. P and dS are rounded to bf16 as operands
 // where the inputs are bf16 (as they would be if stored in the inputs' type) and stay fp32
 // otherwise; sums and statistics are fp32.
+//
+// A row keeps two statistics for the backward: a reference score m_i = q_i . k_j of one of its
+// keys and the log of its sum relative to that. p = 2^{c2 (q . k - m) - log}: the difference
+// of two scores is exact where they are close, whatever their size. (From the log of the sum
+// itself, one fp32 number, p was off by 2^(-24) of the scores' size: a row's only key got
+// weights of 0.96 to 1.04 at scores of 10^6 and 0 at 10^30.)
 #include <type_traits>
 
 #include "pd_gemm_dtl.hpp"
@@ -50,7 +56,7 @@ struct AttnArgs {
   int fill;         // rows of no sequence: 1 zeros, 0 left as they are
   void* out;        // [N, H, D]
   void* rest;       // bf16 [N, H, D]: what rounding took off out (NULL: not kept; fp32: none)
-  float* stats;     // [H, N]: L_i / ln 2; fp32: then [H, N] what rounding took off it
+  float* stats;     // [H, N] m_i, a score q . k of row i, then [H, N] log2 sum_j 2^{c2 (q_i . k_j - m_i)}
   const void* d_out;
   float* rowdot;  // [H, N]: D_i
   void *dq, *dk, *dv;
@@ -252,6 +258,12 @@ __device__ inline int at_fresh(int lane) {
   return lane;
 }
 __device__ inline float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// a b as a number of its own, joined with no addition: in exponents relative to a reference a b
+// its rounding is one factor for all of a row's weights, as long as every use has the same.
+__device__ inline float at_mul(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 
 // The offsets in LDS, every step-th of them where there are more than the table holds: one
 // round trip to memory for a block, where a search in memory takes one for each halving.
@@ -319,32 +331,81 @@ __device__ inline float at_dot(const T* a, const T* b, int D) {
   return s;
 }
 
+// The larger of a lane's value and its partner's in the wave's other half.
+__device__ inline float at_halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // ---------------------------------------------------------------- rows next to a NaN
 // A masked entry's weight is 0 in a tile's product, and 0 times a NaN or an infinity of a
 // row that the mask hides would be a NaN. So a wave that finds a NaN in a row's result forms
 // that row again here from the rows its mask allows alone: the same definition, one row per
-// wave. Rows with a NaN of their own get it again.
+// wave. Rows with a NaN of their own get it again. Rows of large scores come here too: their
+// weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
+
+// Products of the row y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
+// row `last`), by the tiles' instructions and in their order, so scores are the tiles' own
+// bits: register i is row j0 + at_pos(i, hh), the same in a half's 32 lanes.
 template <typename T>
-__device__ __attribute__((noinline)) void at_fwd_row(const AttnArgs* a, int h, int row, int start, int lane) {
-  const int D = a->D, hk = h / (a->H / a->KV);
+__device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, int D, int lane) {
+  const T* row = x + min(j0 + (lane & 31), last) * stride;
+  f32x16 s = {};
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 16) {
+    const int c = c0 + 8 * (lane >> 5);
+    const bool in = c < D;
+    s = Op<T>::mma(in ? Op<T>::load(row + c) : Op<T>::zero(), in ? Op<T>::load(y + c) : Op<T>::zero(), s);
+  }
+  return s;
+}
+// Adds w times each of the rows j0 .. min(j0 + 31, last) to channels lane and lane + 64; w as
+// at_products gives it.
+template <typename T>
+__device__ inline void at_add_rows(const T* x, int64_t stride, int j0, int last, const f32x16& w, int D, int lane,
+                                   float& o0, float& o1) {
+  const bool hh = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float other = __shfl_xor(w[i], 32, 64), ws[2] = {hh ? other : w[i], hh ? w[i] : other};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = j0 + at_pos(i, e);
+      if (j > last) continue;
+      const T* r = x + j * stride;
+      if (lane < D) o0 = fmaf(ws[e], at_f<T>(r[lane]), o0);
+      if (lane + 64 < D) o1 = fmaf(ws[e], at_f<T>(r[lane + 64]), o1);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void at_fwd_row(const AttnArgs* a, int h, int row, int start, int lane) {
+  const int D = a->D, hk = h / (a->H / a->KV), hh = lane >> 5;
   const T* q = (const T*)a->q + row * a->q_row + h * a->q_head;
   const T* k = (const T*)a->k + hk * a->k_head;
   const T* v = (const T*)a->v + hk * a->v_head;
+  // scores with the scale's sign, as at_query has them
+  const float sign = a->c2 > 0.f ? 1.f : a->c2 < 0.f ? -1.f : 0.f, c2 = a->c2 == 0.f ? 1.f : fabsf(a->c2);
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int j0 = start; j0 <= row; j0 += 64) {
-    const int j = j0 + lane;
-    const float s = j <= row ? at_dot<T>(q, k + j * a->k_row, D) * a->c2 : -INFINITY;
-    const float mn = fmaxf(m, wave_max(s)), al = m == mn ? 1.f : at_exp2(m - mn);
-    const float p = s == -INFINITY ? 0.f : at_exp2(s - mn);  // (before the first finite score mn is -inf too)
-    m = mn;
-    l = l * al + wave_sum(p);
-    o0 *= al, o1 *= al;
-    for (int i = 0; i < 64 && j0 + i <= row; ++i) {
-      const float w = __shfl(p, i, 64);
-      const T* vr = v + (j0 + i) * a->v_row;
-      if (lane < D) o0 = fmaf(w, at_f<T>(vr[lane]), o0);
-      if (lane + 64 < D) o1 = fmaf(w, at_f<T>(vr[lane + 64]), o1);
+  for (int j0 = start; j0 <= row; j0 += 32) {
+    f32x16 s = at_products<T>(k, a->k_row, j0, row, q, D, lane);
+    float mt = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = j0 + at_pos(i, hh) <= row ? s[i] * sign : -INFINITY;
+      mt = fmaxf(mt, s[i]);
     }
+    const float mn = fmaxf(m, at_halves_max(mt)), al = m == mn ? 1.f : at_exp2((m - mn) * c2);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // (before the first finite score mn is -inf too)
+      s[i] = s[i] == -INFINITY ? 0.f : at_exp2((s[i] - mn) * c2);
+      sum += s[i];
+    }
+    m = mn;
+    l = l * al + (sum + __shfl_xor(sum, 32, 64));
+    o0 *= al, o1 *= al;
+    at_add_rows<T>(v, a->v_row, j0, row, s, D, lane, o0, o1);
   }
   T* o = (T*)a->out + ((int64_t)row * a->H + h) * D;
   if (lane < D) store_f<T>(o, lane, o0 / l);
@@ -355,65 +416,61 @@ __device__ __attribute__((noinline)) void at_fwd_row(const AttnArgs* a, int h, i
     if (a->rest && lane + 64 < D) store_f<T>(rest, lane + 64, o1 / l - at_f<T>(o[lane + 64]));
   }
   if (a->stats && lane == 0) {
-    const float L = m + log2f(l);
-    a->stats[(int64_t)h * a->N + row] = L;
-    if (sizeof(T) == 4) a->stats[((int64_t)a->H + h) * a->N + row] = (m - L) + log2f(l);
+    a->stats[(int64_t)h * a->N + row] = m * sign;
+    a->stats[((int64_t)a->H + h) * a->N + row] = log2f(l);
   }
 }
 
 template <typename T>
-__device__ __attribute__((noinline)) void at_dq_row(const AttnArgs* a, int h, int row, int start, int lane) {
-  const int D = a->D, hk = h / (a->H / a->KV);
+__device__ __forceinline__ void at_dq_row(const AttnArgs* a, int h, int row, int start, int lane) {
+  const int D = a->D, hk = h / (a->H / a->KV), hh = lane >> 5;
   const T* q = (const T*)a->q + row * a->q_row + h * a->q_head;
   const T* g = (const T*)a->d_out + ((int64_t)row * a->H + h) * D;
   const T* k = (const T*)a->k + hk * a->k_head;
   const T* v = (const T*)a->v + hk * a->v_head;
-  const float L = a->stats[(int64_t)h * a->N + row];
+  const float m = a->stats[(int64_t)h * a->N + row], ll = a->stats[((int64_t)a->H + h) * a->N + row];
   float dot = at_dot<T>(g, (const T*)a->out + ((int64_t)row * a->H + h) * D, D);
   if (sizeof(T) == 2) dot += at_dot<T>(g, (const T*)a->rest + ((int64_t)row * a->H + h) * D, D);
   float o0 = 0.f, o1 = 0.f;
-  for (int j0 = start; j0 <= row; j0 += 64) {
-    const int j = j0 + lane;
-    float ds = 0.f;
-    if (j <= row)
-      ds = at_exp2(at_dot<T>(q, k + j * a->k_row, D) * a->c2 - L) * (at_dot<T>(g, v + j * a->v_row, D) - dot) * a->scale;
-    for (int i = 0; i < 64 && j0 + i <= row; ++i) {
-      const float w = __shfl(ds, i, 64);
-      const T* kr = k + (j0 + i) * a->k_row;
-      if (lane < D) o0 = fmaf(w, at_f<T>(kr[lane]), o0);
-      if (lane + 64 < D) o1 = fmaf(w, at_f<T>(kr[lane + 64]), o1);
-    }
+  for (int j0 = start; j0 <= row; j0 += 32) {
+    f32x16 ds = at_products<T>(k, a->k_row, j0, row, q, D, lane);
+    const f32x16 dp = at_products<T>(v, a->v_row, j0, row, g, D, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      ds[i] = j0 + at_pos(i, hh) <= row ? at_exp2(fmaf(ds[i] - m, a->c2, -ll)) * (dp[i] - dot) : 0.f;
+    at_add_rows<T>(k, a->k_row, j0, row, ds, D, lane, o0, o1);
   }
   T* o = (T*)a->dq + ((int64_t)row * a->H + h) * D;
-  if (lane < D) store_f<T>(o, lane, o0);
-  if (lane + 64 < D) store_f<T>(o, lane + 64, o1);
+  if (lane < D) store_f<T>(o, lane, o0 * a->scale);
+  if (lane + 64 < D) store_f<T>(o, lane + 64, o1 * a->scale);
 }
 
 template <typename T>
-__device__ __attribute__((noinline)) void at_dkv_row(const AttnArgs* a, int hk, int share, int row, int end,
+__device__ __forceinline__ void at_dkv_row(const AttnArgs* a, int hk, int share, int row, int end,
                                                          int lane) {
-  const int D = a->D, rep = a->H / a->KV, nh = rep / a->hs, h0 = hk * rep + share * nh;
+  const int D = a->D, rep = a->H / a->KV, nh = rep / a->hs, h0 = hk * rep + share * nh, hh = lane >> 5;
   const T* k = (const T*)a->k + row * a->k_row + hk * a->k_head;
   const T* v = (const T*)a->v + row * a->v_row + hk * a->v_head;
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int h = h0; h < h0 + nh; ++h)
-    for (int i0 = row; i0 < end; i0 += 64) {
-      const int i = i0 + lane;
-      float p = 0.f, ds = 0.f;
-      if (i < end) {
-        const T* q = (const T*)a->q + i * a->q_row + h * a->q_head;
-        const T* g = (const T*)a->d_out + ((int64_t)i * a->H + h) * D;
-        p = at_exp2(at_dot<T>(q, k, D) * a->c2 - a->stats[(int64_t)h * a->N + i]);
-        ds = p * (at_dot<T>(g, v, D) - a->rowdot[(int64_t)h * a->N + i]) * a->scale;
+  for (int h = h0; h < h0 + nh; ++h) {
+    const T* q = (const T*)a->q + h * a->q_head;
+    const T* g = (const T*)a->d_out + (int64_t)h * D;
+    const int64_t g_row = (int64_t)a->H * D, st = (int64_t)h * a->N, logs = (int64_t)a->H * a->N;
+    for (int i0 = row; i0 < end; i0 += 32) {
+      f32x16 p = at_products<T>(q, a->q_row, i0, end - 1, k, D, lane);
+      f32x16 ds = at_products<T>(g, g_row, i0, end - 1, v, D, lane);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = i0 + at_pos(i, hh);
+        const int64_t at = st + min(j, end - 1);
+        p[i] = j < end ? at_exp2(fmaf(p[i] - a->stats[at], a->c2, -a->stats[logs + at])) : 0.f;
+        ds[i] = j < end ? p[i] * (ds[i] - a->rowdot[at]) : 0.f;
       }
-      for (int t = 0; t < 64 && i0 + t < end; ++t) {
-        const float wp = __shfl(p, t, 64), ws = __shfl(ds, t, 64);
-        const T* q = (const T*)a->q + (i0 + t) * a->q_row + h * a->q_head;
-        const T* g = (const T*)a->d_out + ((int64_t)(i0 + t) * a->H + h) * D;
-        if (lane < D) k0 = fmaf(ws, at_f<T>(q[lane]), k0), v0 = fmaf(wp, at_f<T>(g[lane]), v0);
-        if (lane + 64 < D) k1 = fmaf(ws, at_f<T>(q[lane + 64]), k1), v1 = fmaf(wp, at_f<T>(g[lane + 64]), v1);
-      }
+      at_add_rows<T>(q, a->q_row, i0, end - 1, ds, D, lane, k0, k1);
+      at_add_rows<T>(g, g_row, i0, end - 1, p, D, lane, v0, v1);
     }
+  }
+  k0 *= a->scale, k1 *= a->scale;
   const int64_t at = ((int64_t)row * a->KV + hk) * D, plane = (int64_t)a->N * a->KV * D;
   if (a->hs > 1) {
     float* pk = a->part + 2 * share * plane + at;
@@ -489,7 +546,7 @@ struct Span {
   int first, width;
   __device__ inline bool sees(int j) const { return (unsigned)(j - first) < (unsigned)width; }
   // Whether any lane of the wave sees a part of [j, j + n). Where none does, a lane sees all
-  // of it, or it is `hidden` from it: one value, a row's infinite L or no maximum, hides it,
+  // of it, or it is `hidden` from it: one value, a row's infinite log or no maximum, hides it,
   // where a part takes a comparison an entry. A wave that holds a sequence's end and the next
   // one's start meets such blocks from the one's start on.
   __device__ inline bool some(int j, int n, bool& hidden) const {
@@ -554,18 +611,18 @@ __device__ inline bool at_store_row(T* orow, T* rest, const f32x16 (&o)[NC], flo
   return in && sum != 0.f;
 }
 
-// Row stats of one query: L and what rounding takes off it.
-template <typename T>
-__device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float mc, float l) {
-  const float ll = log2f(l), L = mc + ll;
-  a.stats[(int64_t)h * a.N + row] = L;
-  if constexpr (sizeof(T) == 4) a.stats[((int64_t)a.H + h) * a.N + row] = (mc - L) + ll;
-}
+// What rounding took off m c2 in the exponents of a row's weights. Beyond AT_FAR the weights
+// lose digits to it, and from 2^31 on all of them: such a row (scores of 5 10^7 and more) is
+// formed again from differences.
+constexpr float AT_FAR = 4.f;
+__device__ inline float at_rounded_off(float m, float c2) { return fmaf(m, c2, -at_mul(m, c2)); }
 
-// The larger of a lane's value and its partner's in the wave's other half.
-__device__ inline float at_halves_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+// Row stats of one query: the reference score (at_query may have turned its sign) and the log
+// of the sum.
+__device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float m, float l, float c2) {
+  const int64_t at = (int64_t)h * a.N + row;
+  a.stats[at] = a.c2 > 0.f ? m : a.c2 < 0.f ? -m : 0.f;
+  a.stats[(int64_t)a.H * a.N + at] = log2f(l) - at_rounded_off(m, c2);
 }
 
 // ---------------------------------------------------------------- forward
@@ -585,7 +642,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
     for (int i = 0; i < 16; ++i) x[i & 3] = fmaxf(x[i & 3], sc[b][i]);
   const float mt = hidden ? -INFINITY : at_halves_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
   if (__any((mt - m) * c2 > AT_SLACK)) {
-    const float mn = fmaxf(m, mt), al = m == mn ? 1.f : at_exp2((m - mn) * c2);
+    const float mn = fmaxf(m, mt), al = m == mn ? 1.f : at_exp2(at_mul(m, c2) - at_mul(mn, c2));
     m = mn;
     l *= al;
 #pragma unroll
@@ -593,7 +650,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[c][i] *= al;
   }
-  const float mc = hidden || m == -INFINITY ? -INFINITY : -m * c2;  // -inf: weights 0
+  const float mc = hidden || m == -INFINITY ? -INFINITY : -at_mul(m, c2);  // -inf: weights 0
   float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -703,7 +760,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   if (R.row < a.N && (R.in || a.fill)) {
     const int64_t at = ((int64_t)R.row * a.H + h) * a.D;
     odd = at_store_row<T, NC>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, o, 1.f / l, R.in, a.D, hh);
-    if (R.in && a.stats && hh == 0) at_store_stats<T>(a, h, R.row, m * c2, l);
+    if (R.in && a.stats && hh == 0) at_store_stats(a, h, R.row, m, l, c2);
+    odd |= R.in && fabsf(at_rounded_off(m, c2)) > AT_FAR;
   }
   // infinities count too: 0 times one is a NaN in another row's product
   unsigned long long bad = __ballot(odd);
@@ -823,11 +881,12 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   const float M = fmaxf(fmaxf(ml[0][0][r], ml[0][1][r]), fmaxf(ml[0][2][r], ml[0][3][r]));
   float sum_l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2((ml[0][i][r] - M) * c2);
+  for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2));
   const Join<DP> join = {ldsA, ldsB};
-  join.put(w, r, hh, o, at_exp2((m - M) * c2) / sum_l);
-  if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats<T>(a, h, R.row, M * c2, sum_l);
+  join.put(w, r, hh, o, at_exp2(at_mul(m, c2) - at_mul(M, c2)) / sum_l);
+  if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats(a, h, R.row, M, sum_l, c2);
   __syncthreads();
+  const unsigned long long far = __ballot(R.in && fabsf(at_rounded_off(M, c2)) > AT_FAR);
   const int rr = tid >> 3, row = q0 + rr;
   const int start = __shfl(R.start, rr, 64);
   const bool in = start <= row;
@@ -848,25 +907,24 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
                         v.z - bf16_to_f32(f32_to_bf16(v.z)), v.w - bf16_to_f32(f32_to_bf16(v.w)));
     }
   }
-  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
+  for (unsigned bad = at_join_odd(odd, in) | ((unsigned)far >> (8 * w) & 0xFF); bad; bad &= bad - 1) {
     const int i = 8 * w + __builtin_ctz(bad);
     at_fwd_row<T>(at_args(), h, q0 + i, __shfl(R.start, i, 64), lane);
   }
 }
 
 // ---------------------------------------------------------------- backward: queries
-// The row's operands: q and do fragments, L, and D = do . out from the stored out and what
+// The row's operands: q and do fragments, its statistics, and D = do . out from the stored out and what
 // rounding took off it (from the rounded out alone, D's error weighs on every key of a row
 // alike and was the largest of dq's), written for the key side.
 template <typename T, int DP>
 struct QueryRow {
   typename Op<T>::Frag q[DP / 16], g[DP / 16];
-  float L, Lr = 0.f, dot = 0.f;
+  float m, ll, dot = 0.f;
   __device__ inline void load(const AttnArgs& a, int h, int row, int hh) {
     const int rc = min(row, a.N - 1);
     const int64_t at = ((int64_t)rc * a.H + h) * a.D, st = (int64_t)h * a.N + rc;
-    L = a.stats[st];
-    if constexpr (sizeof(T) == 4) Lr = a.stats[(int64_t)a.H * a.N + st];
+    m = a.stats[st], ll = a.stats[(int64_t)a.H * a.N + st];
     at_row<T, DP>((const T*)a.d_out + at, a.D, hh, g);
     typename Op<T>::Frag o[DP / 16];
     at_row<T, DP>((const T*)a.out + at, a.D, hh, o);
@@ -879,10 +937,6 @@ struct QueryRow {
     }
     at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, q);
     dot += __shfl_xor(dot, 32, 64);
-  }
-  __device__ inline float p(float s, float c2, float L) const {
-    const float t = fmaf(s, c2, -L);
-    return at_exp2(sizeof(T) == 4 ? t - Lr : t);
   }
 };
 
@@ -900,9 +954,9 @@ __device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int 
   }
   bool hidden;
   const bool some = R.sees.some(j0, 32, hidden);
-  const float L = hidden ? INFINITY : Q.L;
+  const float ll = hidden ? INFINITY : Q.ll;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sc[i] = Q.p(sc[i], c2, L) * (dp[i] - Q.dot);
+  for (int i = 0; i < 16; ++i) sc[i] = at_exp2(fmaf(sc[i] - Q.m, c2, -ll)) * (dp[i] - Q.dot);
   if (some) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = R.sees.sees(j0 + at_pos(i, hh)) ? sc[i] : 0.f;
@@ -1062,9 +1116,9 @@ struct Keys {
   }
 };
 
-// One block of 32 queries (images at Ql, Gl; L, D, L's remainder and, for lanes that the
-// queries do not see, infinite L in qs): dv += p do, dk += ds / scale q. vf(s) gives
-// fragment s of the lane's value row.
+// One block of 32 queries (images at Ql, Gl; in qs their logs of sums, D, reference scores
+// and, for lanes that the queries do not see, infinite logs): dv += p do, dk += ds / scale q.
+// vf(s) gives fragment s of the lane's value row.
 template <typename T, int DP, typename VF>
 __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, const float (*qs)[32], int i0,
                                     const Keys& K, const typename Op<T>::Frag (&kf)[DP / 16], VF&& vf, float c2,
@@ -1084,19 +1138,13 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
   const float* ql = qs[hidden ? 3 : 0];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    const float4 L = *(const float4*)&ql[8 * g + 4 * hh], D = *(const float4*)&qs[1][8 * g + 4 * hh];
-    const float Lv[4] = {L.x, L.y, L.z, L.w}, Dv[4] = {D.x, D.y, D.z, D.w};
-    float Rv[4] = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (sizeof(T) == 4) {
-      const float4 Lr = *(const float4*)&qs[2][8 * g + 4 * hh];
-      Rv[0] = Lr.x, Rv[1] = Lr.y, Rv[2] = Lr.z, Rv[3] = Lr.w;
-    }
+    const int at = 8 * g + 4 * hh;
+    const float4 l = *(const float4*)&ql[at], D = *(const float4*)&qs[1][at], m = *(const float4*)&qs[2][at];
+    const float lv[4] = {l.x, l.y, l.z, l.w}, Dv[4] = {D.x, D.y, D.z, D.w}, mv[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 4 * g + e;
-      float t = fmaf(p[i], c2, -Lv[e]);
-      if constexpr (sizeof(T) == 4) t -= Rv[e];
-      p[i] = at_exp2(t);
+      p[i] = at_exp2(fmaf(p[i] - mv[e], c2, -lv[e]));
       ds[i] = p[i] * (ds[i] - Dv[e]);
     }
   }
@@ -1134,18 +1182,15 @@ struct KeyTile {
   }
 };
 
-// L, D (and L's remainder) of one query, for thread q of a block of 32.
-template <typename T>
+// Statistics and D of one query, for thread q of a block of 32.
 struct QueryStats {
-  float L, D, R;
+  float ll, D, m;
   __device__ inline void load(const AttnArgs& a, int h, int row) {
     const int64_t at = (int64_t)h * a.N + row;
-    L = a.stats[at], D = a.rowdot[at];
-    if constexpr (sizeof(T) == 4) R = a.stats[at + (int64_t)a.H * a.N];
+    m = a.stats[at], ll = a.stats[at + (int64_t)a.H * a.N], D = a.rowdot[at];
   }
   __device__ inline void store(float (*qs)[32], int q) const {
-    qs[0][q] = L, qs[1][q] = D, qs[3][q] = INFINITY;
-    if constexpr (sizeof(T) == 4) qs[2][q] = R;
+    qs[0][q] = ll, qs[1][q] = D, qs[2][q] = m, qs[3][q] = INFINITY;
   }
 };
 
@@ -1215,7 +1260,7 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
   lq.init(a.q_row, a.D, w, lane);
   lg.init((int64_t)a.H * a.D, a.D, w, lane);
   const int nq = blo < bhi ? (bhi - blo + 31) / 32 : 0, total = nq * t.nh;
-  QueryStats<T> st;
+  QueryStats st;
   int nh = t.h0, ni = blo;  // the next block to load
   auto issue = [&](char* img) {
     lq.issue((const T*)a.q + nh * a.q_head, a.q_row, ni, bhi - 1, a.D, img, w);
@@ -1277,7 +1322,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   lq.init(a.q_row, a.D, 0, lane);
   lg.init((int64_t)a.H * a.D, a.D, 0, lane);
   const int nq = K.lo < K.hi ? (K.hi - K.lo + 31) / 32 : 0, total = nq * t.nh;
-  QueryStats<T> st;
+  QueryStats st;
   auto issue = [&](int n, char* img) {
     const int h = t.h0 + n / nq, i = K.lo + n % nq * 32;
     lq.issue((const T*)a.q + h * a.q_head, a.q_row, i, K.hi - 1, a.D, img, 0);

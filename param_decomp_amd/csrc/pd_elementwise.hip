@@ -454,7 +454,7 @@ using namespace pd;
 extern "C" {
 
 const char* pd_last_error(void) { return g_last_error.c_str(); }
-int pd_abi_version(void) { return 1; }
+int pd_abi_version(void) { return 2; }
 
 int pd_uniform(uint32_t k0, uint32_t k1, int64_t n, int draw_dtype, int layout, void* out, int out_dtype,
                void* stream) {

@@ -425,7 +425,7 @@ def _attention_args(name: str, q, k, v, offsets, scale: float, fill: bool) -> li
 
 
 def _stats_shape(q: torch.Tensor) -> tuple:
-    return (2, q.shape[1], q.shape[0]) if q.dtype == torch.float32 else (q.shape[1], q.shape[0])
+    return (2, q.shape[1], q.shape[0])
 
 
 def _like_rows(name: str, label: str, t: torch.Tensor, q: torch.Tensor) -> torch.Tensor:
@@ -463,10 +463,10 @@ def packed_attention_bwd(q, k, v, offsets, out, saved, d_out, *, scale: float | 
     _like_rows(name, "out", out, q)
     _like_rows(name, "d_out", d_out, q)
     stats, rest = saved
-    if stats.dtype != torch.float32 or tuple(stats.shape) != _stats_shape(q):
-        raise L.PDError(f"{name}: saved stats are the forward's, float32 {_stats_shape(q)}")
     if (rest is None) != (q.dtype == torch.float32):
         raise L.PDError(f"{name}: the forward saves out_rest for bfloat16")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != _stats_shape(q):
+        raise L.PDError(f"{name}: saved stats are the forward's, float32 {_stats_shape(q)}")
     if rest is not None:
         _like_rows(name, "out_rest", rest, q)
     device = _one_device(name, q, "k v offsets out stats out_rest d_out", k, v, offsets, out, stats, rest, d_out)
