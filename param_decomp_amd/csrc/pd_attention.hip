@@ -249,6 +249,11 @@ __device__ inline void at_row(const T* row, int D, int hh, typename Op<T>::Frag 
   for (int s = 0; s < DP / 16; ++s) f[s] = 16 * s + 8 * hh < D ? Op<T>::load(row + 16 * s + 8 * hh) : Op<T>::zero();
 }
 
+// A sum of weights times a factor. Weights beside a large reference can leave fp32 (the row is
+// formed again where that one stays): a factor of 0 forgets them, where 0 times infinity would
+// make the row's sum a NaN. A NaN stays.
+__device__ inline float at_rescaled(float l, float f) { return f == 0.f && l == INFINITY ? 0.f : l * f; }
+
 // Key (or query) position inside a 32-row block that accumulator register i holds.
 __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
 // The lane again, as a value that nothing was formed from yet: LDS addresses of a loop are
@@ -341,8 +346,10 @@ __device__ inline float at_halves_max(float v) {
 // A masked entry's weight is 0 in a tile's product, and 0 times a NaN or an infinity of a
 // row that the mask hides would be a NaN. So a wave that finds a NaN in a row's result forms
 // that row again here from the rows its mask allows alone: the same definition, one row per
-// wave. Rows with a NaN of their own get it again. Rows of large scores come here too: their
-// weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
+// wave, which is slow. Rows whose NaN or infinity is their own keep the tile's result: what
+// the row's own statistics and the channels of the rows it sees tell costs a few loads, and a
+// batch that has diverged runs at about its normal speed. Rows of large scores come here too:
+// their weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
 
 // Products of the row y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
 // row `last`), by the tiles' instructions and in their order, so scores are the tiles' own
@@ -483,6 +490,130 @@ __device__ __forceinline__ void at_dkv_row(const AttnArgs* a, int hk, int share,
   T* dv = (T*)a->dv + at;
   if (lane < D) store_f<T>(dk, lane, k0), store_f<T>(dv, lane, v0);
   if (lane + 64 < D) store_f<T>(dk, lane + 64, k1), store_f<T>(dv, lane + 64, v1);
+}
+
+__device__ inline bool at_odd(float x) { return !(fabsf(x) < INFINITY); }
+
+// Whether the values of the channels lane and lane + 64 of a row are not finite.
+template <typename T>
+__device__ inline void at_odd_channels(const T* row, int D, int lane, bool& o0, bool& o1) {
+  o0 = lane < D && at_odd(at_f<T>(row[min(lane, D - 1)]));
+  o1 = lane + 64 < D && at_odd(at_f<T>(row[min(lane + 64, D - 1)]));
+}
+
+// Forms the wave's rows again that are marked in `far`, and those marked in `bad` whose NaN
+// or infinity in some channel is in no value row that they see. Behind the rows' stores.
+template <typename T>
+__device__ __forceinline__ void at_fwd_again(const AttnArgs* a, int h, int row0, unsigned bad, unsigned far, int start,
+                                             int lane) {
+  if (!(bad | far)) return;
+  __threadfence_block();
+  const int D = a->D;
+  const T* v = (const T*)a->v + (h / (a->H / a->KV)) * a->v_head;
+  const T* out = (const T*)a->out + ((int64_t)row0 * a->H + h) * D;
+  const int64_t o_row = (int64_t)a->H * D;
+  int from = -1, f0 = 0, f1 = 0;  // the first such value row of sequence `from`, by channel
+  for (unsigned left = bad | far; left; left &= left - 1) {
+    const int i = __builtin_ctz(left), row = row0 + i, first = __shfl(start, i, 64);
+    if (!(far >> i & 1)) {
+      bool o0, o1;
+      at_odd_channels<T>(out + i * o_row, D, lane, o0, o1);
+      if (first != from) {
+        from = first;
+        bool n0 = false, n1 = false;  // channels that a row of the sequence asks for
+        int last = row;
+        for (unsigned more = left & bad; more; more &= more - 1) {
+          const int e = __builtin_ctz(more);
+          if (__shfl(start, e, 64) != first) break;
+          bool p0, p1;
+          at_odd_channels<T>(out + e * o_row, D, lane, p0, p1);
+          n0 |= p0, n1 |= p1;
+          last = row0 + e;
+        }
+        f0 = n0 ? 0x7FFFFFFF : -1, f1 = n1 ? 0x7FFFFFFF : -1;
+        for (int j0 = first; j0 <= last && __any(max(f0, f1) == 0x7FFFFFFF); j0 += 8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            bool p0, p1;
+            at_odd_channels<T>(v + min(j0 + e, last) * a->v_row, D, lane, p0, p1);
+            if (p0) f0 = min(f0, min(j0 + e, last));
+            if (p1) f1 = min(f1, min(j0 + e, last));
+          }
+        }
+      }
+      if (!__any((o0 && f0 > row) || (o1 && f1 > row))) continue;
+    }
+    at_fwd_row<T>(a, h, row, first, lane);
+  }
+}
+
+// Forms the wave's key rows again that are marked in `bad`, but for those whose NaN or
+// infinity is their own: a query that sees the row has no weights (both gradients are NaN
+// then), or no finite D (dk is) and, for dv, a cotangent without a finite value in each of its
+// channels. `end`: of the lane's row's sequence.
+template <typename T>
+__device__ __forceinline__ void at_dkv_again(const AttnArgs* a, int hk, int share, int row0, unsigned bad, int end,
+                                             int lane) {
+  if (!bad) return;
+  __threadfence_block();
+  const int D = a->D, rep = a->H / a->KV, nh = rep / a->hs, h0 = hk * rep + share * nh;
+  const int64_t logs = (int64_t)a->H * a->N, plane = (int64_t)a->N * a->KV * D;
+  auto channels = [&](int row, bool dv, bool& o0, bool& o1) {
+    const int64_t at = ((int64_t)row * a->KV + hk) * D;
+    if (a->hs > 1) at_odd_channels<float>(a->part + (2 * share + dv) * plane + at, D, lane, o0, o1);
+    else at_odd_channels<T>((const T*)(dv ? a->dv : a->dk) + at, D, lane, o0, o1);
+  };
+  int to = -1, last_w = -1, last_d = -1, g0 = -1, g1 = -1;  // last such queries of the sequence that ends at `to`
+  bool scanned = false;
+  for (; bad; bad &= bad - 1) {
+    const int i = __builtin_ctz(bad), row = row0 + i, e = __shfl(end, i, 64);
+    if (e != to) {
+      to = e, last_w = last_d = g0 = g1 = -1, scanned = false;
+      for (int h = h0; h < h0 + nh; ++h)
+        for (int q0 = (e - 1) & ~63, w = -1, d = -1; q0 + 63 >= row && w < 0; q0 -= 64) {
+          const int q = q0 + lane;
+          const int64_t at = (int64_t)h * a->N + min(q, e - 1);
+          const bool in = q >= row && q < e;
+          const unsigned long long bw = __ballot(in && (at_odd(a->stats[at]) || at_odd(a->stats[logs + at])));
+          const unsigned long long bd = __ballot(in && at_odd(a->rowdot[at]));
+          if (bw) w = q0 + 63 - __builtin_clzll(bw);
+          if (bd && d < 0) d = q0 + 63 - __builtin_clzll(bd);
+          last_w = max(last_w, w), last_d = max(last_d, d);
+        }
+    }
+    if (last_w >= row) continue;
+    bool o0, o1;
+    if (last_d >= row) {
+      channels(row, true, o0, o1);
+      if (!__any(o0 || o1)) continue;
+      if (!scanned) {  // the last cotangents without a finite value, by channel, for the rows left
+        scanned = true;
+        bool n0 = o0, n1 = o1;
+        for (unsigned more = bad & (bad - 1); more; more &= more - 1) {
+          const int x = __builtin_ctz(more);
+          if (__shfl(end, x, 64) != e) break;
+          bool p0, p1;
+          channels(row0 + x, true, p0, p1);
+          n0 |= p0, n1 |= p1;
+        }
+        for (int h = h0; h < h0 + nh; ++h)
+          for (int q0 = last_d & ~63; q0 + 63 >= row && __any((n0 && g0 < 0) || (n1 && g1 < 0)); q0 -= 64) {
+            const int q = q0 + lane;
+            for (unsigned long long m = __ballot(q >= row && q < e && at_odd(a->rowdot[(int64_t)h * a->N + min(q, e - 1)])); m;) {
+              const int x = 63 - __builtin_clzll(m);
+              m ^= 1ull << x;
+              bool p0, p1;
+              at_odd_channels<T>((const T*)a->d_out + ((int64_t)(q0 + x) * a->H + h) * D, D, lane, p0, p1);
+              if (p0) g0 = max(g0, q0 + x);
+              if (p1) g1 = max(g1, q0 + x);
+              if (!__any((n0 && g0 < 0) || (n1 && g1 < 0))) break;
+            }
+          }
+      }
+      if (!__any((o0 && g0 < row) || (o1 && g1 < row))) continue;
+    }
+    at_dkv_row<T>(a, hk, share, row, e, lane);
+  }
 }
 
 // The kernel's own arguments, where they lie (a copy of them would live in scratch).
@@ -644,7 +775,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
   if (__any((mt - m) * c2 > AT_SLACK)) {
     const float mn = fmaxf(m, mt), al = m == mn ? 1.f : at_exp2(at_mul(m, c2) - at_mul(mn, c2));
     m = mn;
-    l *= al;
+    l = at_rescaled(l, al);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -659,7 +790,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
       sc[b][i] = at_exp2(fmaf(sc[b][i], c2, mc));
       y[i & 3] += sc[b][i];
     }
-  l += (y[0] + y[1]) + (y[2] + y[3]);
+  if (!hidden) l += (y[0] + y[1]) + (y[2] + y[3]);  // l holds what the row sees alone, NaN included
 }
 
 // Query fragments with the scale's sign: c2 is positive then. (Scale 0: zeros, c2 = 1.)
@@ -756,21 +887,18 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
     if (j0 + BK < bhi) tile(j0 + BK, ldsB, ldsA);
   }
   l += __shfl_xor(l, 32, 64);
-  bool odd = false;
+  bool odd = false, far = false;
   if (R.row < a.N && (R.in || a.fill)) {
     const int64_t at = ((int64_t)R.row * a.H + h) * a.D;
     odd = at_store_row<T, NC>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, o, 1.f / l, R.in, a.D, hh);
     if (R.in && a.stats && hh == 0) at_store_stats(a, h, R.row, m, l, c2);
-    odd |= R.in && fabsf(at_rounded_off(m, c2)) > AT_FAR;
+    // a NaN among the row's scores, or none that is finite: it is NaN in every channel
+    odd = odd && l == l && m != -INFINITY;
+    far = R.in && fabsf(at_rounded_off(m, c2)) > AT_FAR;
   }
   // infinities count too: 0 times one is a NaN in another row's product
-  unsigned long long bad = __ballot(odd);
-  bad = (bad | bad >> 32) & 0xFFFFFFFFull;
-  while (bad) {
-    const int i = __builtin_ctzll(bad);
-    bad &= bad - 1;
-    at_fwd_row<T>(at_args(), h, row0 + i, __shfl(R.start, i, 64), lane);
-  }
+  const unsigned long long bad = __ballot(odd), big = __ballot(far);
+  at_fwd_again<T>(at_args(), h, row0, (unsigned)(bad | bad >> 32), (unsigned)(big | big >> 32), R.start, lane);
 }
 
 // fp32 rows of four waves for a join, two waves in each of two LDS regions: value v of row r
@@ -881,12 +1009,13 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   const float M = fmaxf(fmaxf(ml[0][0][r], ml[0][1][r]), fmaxf(ml[0][2][r], ml[0][3][r]));
   float sum_l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2));
+  for (int i = 0; i < 4; ++i) sum_l += at_rescaled(ml[1][i][r], at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2)));
   const Join<DP> join = {ldsA, ldsB};
   join.put(w, r, hh, o, at_exp2(at_mul(m, c2) - at_mul(M, c2)) / sum_l);
   if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats(a, h, R.row, M, sum_l, c2);
   __syncthreads();
   const unsigned long long far = __ballot(R.in && fabsf(at_rounded_off(M, c2)) > AT_FAR);
+  const unsigned long long own = __ballot(sum_l != sum_l || M == -INFINITY);  // NaN in every channel
   const int rr = tid >> 3, row = q0 + rr;
   const int start = __shfl(R.start, rr, 64);
   const bool in = start <= row;
@@ -907,10 +1036,8 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
                         v.z - bf16_to_f32(f32_to_bf16(v.z)), v.w - bf16_to_f32(f32_to_bf16(v.w)));
     }
   }
-  for (unsigned bad = at_join_odd(odd, in) | ((unsigned)far >> (8 * w) & 0xFF); bad; bad &= bad - 1) {
-    const int i = 8 * w + __builtin_ctz(bad);
-    at_fwd_row<T>(at_args(), h, q0 + i, __shfl(R.start, i, 64), lane);
-  }
+  const unsigned rows = 0xFFu << (8 * w);
+  at_fwd_again<T>(at_args(), h, q0, at_join_odd(odd, in) << (8 * w) & ~(unsigned)own, (unsigned)far & rows, R.start, lane);
 }
 
 // ---------------------------------------------------------------- backward: queries
@@ -938,6 +1065,8 @@ struct QueryRow {
     at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, q);
     dot += __shfl_xor(dot, 32, 64);
   }
+  // The row has no weights or no finite D: no channel of its dq is finite.
+  __device__ inline bool odd() const { return at_odd(m) || at_odd(ll) || at_odd(dot); }
 };
 
 // ds / scale of one block (images of its 32 keys and values at row R0), and dq += ds k.
@@ -1018,7 +1147,7 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 4 && DP > 64 ? 1 : 2) void
   bool odd = false;
   if (R.row < a.N && (R.in || a.fill))
     odd = at_store_row<T, NC>((T*)a.dq + ((int64_t)R.row * a.H + h) * a.D, nullptr, dq, a.scale, R.in, a.D, hh);
-  unsigned long long bad = __ballot(odd);
+  unsigned long long bad = __ballot(odd && !Q.odd());
   bad = (bad | bad >> 32) & 0xFFFFFFFFull;
   while (bad) {
     const int i = __builtin_ctzll(bad);
@@ -1093,7 +1222,8 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dq_split(AttnArgs a) {
       if (ch < a.D) Op<T>::store4((T*)a.dq + ((int64_t)row * a.H + h) * a.D + ch, v.x, v.y, v.z, v.w);
     }
   }
-  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
+  const unsigned own = (unsigned)__ballot(Q.odd());
+  for (unsigned bad = at_join_odd(odd, in) & ~(own >> (8 * w)); bad; bad &= bad - 1) {
     const int i = 8 * w + __builtin_ctz(bad);
     at_dq_row<T>(at_args(), h, q0 + i, __shfl(R.start, i, 64), lane);
   }
@@ -1285,13 +1415,8 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
     block(n, ldsA, ldsB);
     if (n + 1 < total) block(n + 1, ldsB, ldsA);
   }
-  unsigned long long bad = __ballot(at_store_keys<T, DP>(a, t, K, dk, dv, hh));
-  bad = (bad | bad >> 32) & 0xFFFFFFFFull;
-  while (bad) {
-    const int i = __builtin_ctzll(bad);
-    bad &= bad - 1;
-    at_dkv_row<T>(at_args(), t.hk, t.share, row0 + i, __shfl(K.end(), i, 64), lane);
-  }
+  const unsigned long long bad = __ballot(at_store_keys<T, DP>(a, t, K, dk, dv, hh));
+  at_dkv_again<T>(at_args(), t.hk, t.share, row0, (unsigned)(bad | bad >> 32), K.end(), lane);
 }
 
 // The form for small grids: a block of 32 keys whose four waves take every fourth block of
@@ -1371,10 +1496,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
       }
     }
   }
-  for (unsigned bad = at_join_odd(odd, in); bad; bad &= bad - 1) {
-    const int i = 8 * w + __builtin_ctz(bad);
-    at_dkv_row<T>(at_args(), t.hk, t.share, t.k0 + i, __shfl(K.end(), i, 64), lane);
-  }
+  at_dkv_again<T>(at_args(), t.hk, t.share, t.k0, at_join_odd(odd, in) << (8 * w), K.end(), lane);
 }
 
 // dk and dv as the shares' sums in share order; rows of no sequence as `fill` says. One

@@ -79,13 +79,14 @@ def test_scores_of_any_size(device, dtype, sign, size, N, H, KV, D, lengths):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("H, KV", [(2, 2), (32, 32)])
-def test_low_scores_before_ordinary_ones(device, dtype, H, KV):
-    """The first rows see keys of scores near -1e38 alone; later ones ordinary keys too, in
+@pytest.mark.parametrize("size", [2.0**63, 2.0**63 * 219 / 128, 2.0**30 * 219 / 128])
+def test_low_scores_before_ordinary_ones(device, dtype, H, KV, size):
+    """The first rows see keys of scores of large negative size alone; later ones ordinary keys too, in
     the same tile and in later ones; -inf among them has no weight."""
     N, D = 2100, 64
     g = torch.Generator(device=device).manual_seed(3)
     q, k, v = (torch.randn(N, h, D, device=device, generator=g).to(dtype) for h in (H, KV, KV))
-    q[:, :, 0] = 2.0**63
+    q[:, :, 0] = min(size, 2.0**63)
     q[:, :, 1:] = q[:, :, 1:].round()  # scores that 32 bits hold exactly
     k[:, :, 1:] = k[:, :, 1:].round()
     k[:, :, 0] = 0.0
@@ -93,14 +94,16 @@ def test_low_scores_before_ordinary_ones(device, dtype, H, KV):
     low = {0: 31, 40: 100, 700: 200}  # as many keys of low scores first
     for a in starts:
         n = low[a]
-        k[a:a + n, :, 0] = -(2.0**63)
+        k[a:a + n, :, 0] = -size
         k[a:a + n, :, 1:] = 0.0
         k[a + 3, :, 0] = -math.inf
     off = torch.tensor(starts + [N], dtype=torch.int32, device=device)
     out = packed_attention(q, k, v, off)
     kk = k.clone()
-    kk[[a + 3 for a in starts], :, 0] = -(2.0**64)  # a score of no weight beside -2^126, in 64 bits
+    kk[[a + 3 for a in starts], :, 0] = -2.0 * size  # a score of no weight beside the others
     _check_out(out, q, kk, v, [40, 660, 1400], D**-0.5)
+    out = packed_attention(q, k, v, off, scale=0.3)
+    _check_out(out, q, kk, v, [40, 660, 1400], 0.3)
 
 
 def test_no_finite_score_is_no_number(device):
