@@ -249,11 +249,6 @@ __device__ inline void at_row(const T* row, int D, int hh, typename Op<T>::Frag 
   for (int s = 0; s < DP / 16; ++s) f[s] = 16 * s + 8 * hh < D ? Op<T>::load(row + 16 * s + 8 * hh) : Op<T>::zero();
 }
 
-// A sum of weights times a factor. Weights beside a large reference can leave fp32 (the row is
-// formed again where that one stays): a factor of 0 forgets them, where 0 times infinity would
-// make the row's sum a NaN. A NaN stays.
-__device__ inline float at_rescaled(float l, float f) { return f == 0.f && l == INFINITY ? 0.f : l * f; }
-
 // Key (or query) position inside a 32-row block that accumulator register i holds.
 __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
 // The lane again, as a value that nothing was formed from yet: LDS addresses of a loop are
@@ -346,9 +341,9 @@ __device__ inline float at_halves_max(float v) {
 // A masked entry's weight is 0 in a tile's product, and 0 times a NaN or an infinity of a
 // row that the mask hides would be a NaN. So a wave that finds a NaN in a row's result forms
 // that row again here from the rows its mask allows alone: the same definition, one row per
-// wave, which is slow. Rows whose NaN or infinity is their own keep the tile's result: what
-// the row's own statistics and the channels of the rows it sees tell costs a few loads, and a
-// batch that has diverged runs at about its normal speed. Rows of large scores come here too:
+// wave, which is slow. Rows whose NaN or infinity is their own keep the tile's result: their
+// statistics and the rows they see tell, mostly the first one looked at, and a batch that has
+// diverged runs at about its normal speed. Rows of large scores come here too:
 // their weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
 
 // Products of the row y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
@@ -501,28 +496,50 @@ __device__ inline void at_odd_channels(const T* row, int D, int lane, bool& o0, 
   o1 = lane + 64 < D && at_odd(at_f<T>(row[min(lane + 64, D - 1)]));
 }
 
-// Forms the wave's rows again that are marked in `far`, and those marked in `bad` whose NaN
-// or infinity in some channel is in no value row that they see. Behind the rows' stores.
+// Forms the wave's rows again that are marked in `far`, and those marked in `bad` whose NaN or
+// infinity is not their own: a NaN in the query, in a key or (by channel, and infinities too)
+// in a value that the row sees. `nan`: rows whose sum of weights is a NaN, which a key can have
+// caused. Behind the rows' stores.
 template <typename T>
-__device__ __forceinline__ void at_fwd_again(const AttnArgs* a, int h, int row0, unsigned bad, unsigned far, int start,
-                                             int lane) {
+__device__ __forceinline__ void at_fwd_again(const AttnArgs* a, int h, int row0, unsigned bad, unsigned nan, unsigned far,
+                                             int start, int lane) {
   if (!(bad | far)) return;
   __threadfence_block();
-  const int D = a->D;
-  const T* v = (const T*)a->v + (h / (a->H / a->KV)) * a->v_head;
+  const int D = a->D, hk = h / (a->H / a->KV);
+  const T* q = (const T*)a->q + h * a->q_head;
+  const T* k = (const T*)a->k + hk * a->k_head;
+  const T* v = (const T*)a->v + hk * a->v_head;
   const T* out = (const T*)a->out + ((int64_t)row0 * a->H + h) * D;
   const int64_t o_row = (int64_t)a->H * D;
-  int from = -1, f0 = 0, f1 = 0;  // the first such value row of sequence `from`, by channel
+  int k_from = -1, kf = 0;          // the first key row of sequence `k_from` with a NaN
+  int v_from = -1, f0 = 0, f1 = 0;  // the first value rows of `v_from` that are not finite, by channel
   for (unsigned left = bad | far; left; left &= left - 1) {
     const int i = __builtin_ctz(left), row = row0 + i, first = __shfl(start, i, 64);
-    if (!(far >> i & 1)) {
+    if (!(far >> i & 1) && nan >> i & 1) {
+      bool o0, o1;
+      at_odd_channels<T>(q + row * a->q_row, D, lane, o0, o1);
+      if (__any(o0 || o1)) continue;
+      if (first != k_from) {
+        k_from = first, kf = 0x7FFFFFFF;
+        const int last = min(row0 + 31, a->N - 1);
+        for (int j0 = first; j0 <= last && kf == 0x7FFFFFFF; j0 += 8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const T* r = k + min(j0 + e, last) * a->k_row;
+            const float x = at_f<T>(r[min(lane, D - 1)]), y = at_f<T>(r[min(lane + 64, D - 1)]);
+            if (__any(x != x || y != y)) kf = min(kf, min(j0 + e, last));
+          }
+        }
+      }
+      if (kf <= row) continue;
+    } else if (!(far >> i & 1)) {
       bool o0, o1;
       at_odd_channels<T>(out + i * o_row, D, lane, o0, o1);
-      if (first != from) {
-        from = first;
+      if (first != v_from) {
+        v_from = first;
         bool n0 = false, n1 = false;  // channels that a row of the sequence asks for
         int last = row;
-        for (unsigned more = left & bad; more; more &= more - 1) {
+        for (unsigned more = left & bad & ~nan; more; more &= more - 1) {
           const int e = __builtin_ctz(more);
           if (__shfl(start, e, 64) != first) break;
           bool p0, p1;
@@ -775,7 +792,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
   if (__any((mt - m) * c2 > AT_SLACK)) {
     const float mn = fmaxf(m, mt), al = m == mn ? 1.f : at_exp2(at_mul(m, c2) - at_mul(mn, c2));
     m = mn;
-    l = at_rescaled(l, al);
+    l *= al;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -790,7 +807,7 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
       sc[b][i] = at_exp2(fmaf(sc[b][i], c2, mc));
       y[i & 3] += sc[b][i];
     }
-  if (!hidden) l += (y[0] + y[1]) + (y[2] + y[3]);  // l holds what the row sees alone, NaN included
+  l += (y[0] + y[1]) + (y[2] + y[3]);
 }
 
 // Query fragments with the scale's sign: c2 is positive then. (Scale 0: zeros, c2 = 1.)
@@ -892,13 +909,13 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
     const int64_t at = ((int64_t)R.row * a.H + h) * a.D;
     odd = at_store_row<T, NC>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, o, 1.f / l, R.in, a.D, hh);
     if (R.in && a.stats && hh == 0) at_store_stats(a, h, R.row, m, l, c2);
-    // a NaN among the row's scores, or none that is finite: it is NaN in every channel
-    odd = odd && l == l && m != -INFINITY;
+    odd = odd && !(l == 0.f && m == -INFINITY);  // no finite score: NaN it is
     far = R.in && fabsf(at_rounded_off(m, c2)) > AT_FAR;
   }
   // infinities count too: 0 times one is a NaN in another row's product
-  const unsigned long long bad = __ballot(odd), big = __ballot(far);
-  at_fwd_again<T>(at_args(), h, row0, (unsigned)(bad | bad >> 32), (unsigned)(big | big >> 32), R.start, lane);
+  const unsigned long long bad = __ballot(odd);
+  at_fwd_again<T>(at_args(), h, row0, (unsigned)(bad | bad >> 32), (unsigned)__ballot(l != l), (unsigned)__ballot(far),
+                  R.start, lane);
 }
 
 // fp32 rows of four waves for a join, two waves in each of two LDS regions: value v of row r
@@ -1009,13 +1026,13 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   const float M = fmaxf(fmaxf(ml[0][0][r], ml[0][1][r]), fmaxf(ml[0][2][r], ml[0][3][r]));
   float sum_l = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum_l += at_rescaled(ml[1][i][r], at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2)));
+  for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2));
   const Join<DP> join = {ldsA, ldsB};
   join.put(w, r, hh, o, at_exp2(at_mul(m, c2) - at_mul(M, c2)) / sum_l);
   if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats(a, h, R.row, M, sum_l, c2);
   __syncthreads();
   const unsigned long long far = __ballot(R.in && fabsf(at_rounded_off(M, c2)) > AT_FAR);
-  const unsigned long long own = __ballot(sum_l != sum_l || M == -INFINITY);  // NaN in every channel
+  const unsigned long long nan = __ballot(sum_l != sum_l);
   const int rr = tid >> 3, row = q0 + rr;
   const int start = __shfl(R.start, rr, 64);
   const bool in = start <= row;
@@ -1037,7 +1054,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
     }
   }
   const unsigned rows = 0xFFu << (8 * w);
-  at_fwd_again<T>(at_args(), h, q0, at_join_odd(odd, in) << (8 * w) & ~(unsigned)own, (unsigned)far & rows, R.start, lane);
+  at_fwd_again<T>(at_args(), h, q0, at_join_odd(odd, in) << (8 * w), (unsigned)nan, (unsigned)far & rows, R.start, lane);
 }
 
 // ---------------------------------------------------------------- backward: queries
