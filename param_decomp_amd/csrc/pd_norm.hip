@@ -33,6 +33,13 @@ constexpr int LN_THREADS = 256 * 1024;
 constexpr int LN_GRAD_THREADS = 256 * 512;
 constexpr int LN_GRAD_ALL_D = 512;
 
+// Distances from the mean past 2^63 have squares past fp32: a row whose variance is infinite
+// takes them again times this (sums of x itself end at 3.4 10^38).
+constexpr float LN_WIDE = 0x1p-80f;
+__device__ inline float ln_wide_rstd(float sum, float d, float eps) {
+  return LN_WIDE / sqrtf(sum / d + eps * LN_WIDE * LN_WIDE);
+}
+
 struct LnStat {
   float base, delta, rstd;  // mean = base + delta
 };
@@ -109,6 +116,7 @@ __global__ __launch_bounds__(ln_threads(NT)) void k_ln_fwd(const T* __restrict__
                                                            float eps, T* __restrict__ y, LnStat* __restrict__ stats) {
   constexpr int VEC = 16 / sizeof(T), CH = E / VEC, RPB = ln_threads(NT) / NT, NW = NT <= 64 ? 1 : NT / 64;
   __shared__ float4 part[2][NW];
+  __shared__ float again[NW];
   const int tid = threadIdx.x % NT, wv = tid >> 6, lane = threadIdx.x & 63;
   int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / NT;
   const int64_t step = (int64_t)gridDim.x * RPB;
@@ -159,7 +167,22 @@ __global__ __launch_bounds__(ln_threads(NT)) void k_ln_fwd(const T* __restrict__
       }
       var = fmaxf(Q / (float)d, 0.f);
     }
-    const float rstd = 1.f / sqrtf(var + eps);
+    float rstd = 1.f / sqrtf(var + eps);
+    if (var == INFINITY) {  // the same for the row's threads
+      float t = tail ? ((vt - base) - delta) * LN_WIDE : 0.f, wide = t * t;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (VEC * (tid + (i / VEC) * NT) + VEC <= d) t = ((v[i] - base) - delta) * LN_WIDE, wide = fmaf(t, t, wide);
+      wide = ln_sum<NT>(wide);
+      if constexpr (NT > 64) {
+        if (lane == 0) again[wv] = wide;
+        __syncthreads();  // written anew behind a later row's barrier
+        wide = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) wide += again[i];
+      }
+      rstd = ln_wide_rstd(wide, (float)d, eps);
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int col = VEC * (tid + c * NT);
@@ -362,7 +385,16 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(const T* __restrict__ x, i
   }
   const float2 rq = block_sum2(res, q, red);
   const float delta = rq.x / (float)d;
-  const float rstd = 1.f / sqrtf(fmaxf(rq.y / (float)d - delta * delta, 0.f) + eps);
+  const float var = fmaxf(rq.y / (float)d - delta * delta, 0.f);
+  float rstd = 1.f / sqrtf(var + eps);
+  if (var == INFINITY) {
+    float wide = 0.f;
+    for (int64_t i = threadIdx.x; i < d; i += 1024) {
+      const float t = ((load_f<T>(row, i) - base) - delta) * LN_WIDE;
+      wide = fmaf(t, t, wide);
+    }
+    rstd = ln_wide_rstd(block_sum2(wide, 0.f, red).x, (float)d, eps);
+  }
   for (int64_t i = threadIdx.x; i < d; i += 1024)
     store_f<T>(y + (int64_t)blockIdx.x * d, i,
                fmaf(((load_f<T>(row, i) - base) - delta) * rstd, w ? w[i] : 1.f, b ? b[i] : 0.f));
