@@ -1552,7 +1552,7 @@ int at_check(const char* what, int dtype, int64_t rows, int H, int KV, int D, co
   if (D <= 0 || D % 8 || D > 128) return fail(PD_EUNSUPPORTED, w + ": head_dim must be a multiple of 8 up to 128");
   if (rows > (1 << 30) || n_seq > (1 << 30) || cdiv(rows, AT_SPLIT) * H > 0x7FFFFFFF)
     return fail(PD_EUNSUPPORTED, w + ": rows too many");
-  if (!std::isfinite(scale)) return fail(PD_EINVAL, w + ": scale must be finite");
+  if (!std::isfinite(scale * LOG2E)) return fail(PD_EINVAL, w + ": scale (times log2 e, as the kernels take it) must be finite");
   if (!rows) return PD_OK;
   if (!off) return fail(PD_EINVAL, w + ": null offsets");
   const int per = dtype == PD_DTYPE_F32 ? 4 : 8;
