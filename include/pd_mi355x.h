@@ -681,8 +681,8 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
  * infinities included, reaches no other row. Offsets outside [0, rows] or out of order
  * give wrong rows but no access outside the tensors.
  *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, fp32 statistics;
- * For the backward (nullable): stats fp32 [2, n_head, rows], a reference score q . k of each
- * row and log2 of its softmax sum relative to that, and with bf16 tensors out_rest [rows,
+ * For the backward (nullable): stats fp32 [2, n_head, rows], a reference score of each
+ * row (q . k with the scale's sign) and log2 of its softmax sum relative to that, and with bf16 tensors out_rest [rows,
  * n_head, head_dim] bf16, what rounding took off out. Scores may have any size that fp32
  * holds; weights depend on their differences alone.
  * The backward gives dq [rows, n_head, head_dim], dk and dv [rows, n_kv_head, head_dim]

@@ -52,11 +52,13 @@ struct AttnArgs {
   int N, H, KV, D;
   const int32_t* off;
   int S;
-  float scale, c2;  // c2 = scale log2 e
+  // scores enter as sign q . k and exponents take them times c2 = |scale| log2 e (scale 0: sign
+  // 0 and c2 1)
+  float scale, sign, c2;
   int fill;         // rows of no sequence: 1 zeros, 0 left as they are
   void* out;        // [N, H, D]
   void* rest;       // bf16 [N, H, D]: what rounding took off out (NULL: not kept; fp32: none)
-  float* stats;     // [H, N] m_i, a score q . k of row i, then [H, N] log2 sum_j 2^{c2 (q_i . k_j - m_i)}
+  float* stats;     // [H, N] m_i, a score sign q . k of row i, then [H, N] log2 sum_j 2^{c2 (sign q_i . k_j - m_i)}
   const void* d_out;
   float* rowdot;  // [H, N]: D_i
   void *dq, *dk, *dv;
@@ -249,6 +251,15 @@ __device__ inline void at_row(const T* row, int D, int hh, typename Op<T>::Frag 
   for (int s = 0; s < DP / 16; ++s) f[s] = 16 * s + 8 * hh < D ? Op<T>::load(row + 16 * s + 8 * hh) : Op<T>::zero();
 }
 
+// Gives a row's scores the scale's sign, forward and backward in the same operands (a product
+// of -q is not always the negative of q's to the bit), so that c2 is positive.
+template <typename T, int NS>
+__device__ inline void at_sign(const AttnArgs& a, typename Op<T>::Frag (&f)[NS]) {
+  if (a.sign == 1.f) return;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) f[s] = Op<T>::scaled(f[s], a.sign);
+}
+
 // Key (or query) position inside a 32-row block that accumulator register i holds.
 __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
 // The lane again, as a value that nothing was formed from yet: LDS addresses of a loop are
@@ -346,18 +357,21 @@ __device__ inline float at_halves_max(float v) {
 // diverged runs at about its normal speed. Rows of large scores come here too:
 // their weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
 
-// Products of the row y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
+// Products of sign y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
 // row `last`), by the tiles' instructions and in their order, so scores are the tiles' own
 // bits: register i is row j0 + at_pos(i, hh), the same in a half's 32 lanes.
 template <typename T>
-__device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, int D, int lane) {
+__device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, float sign, int D,
+                                     int lane) {
   const T* row = x + min(j0 + (lane & 31), last) * stride;
   f32x16 s = {};
 #pragma unroll 1
   for (int c0 = 0; c0 < D; c0 += 16) {
     const int c = c0 + 8 * (lane >> 5);
     const bool in = c < D;
-    s = Op<T>::mma(in ? Op<T>::load(row + c) : Op<T>::zero(), in ? Op<T>::load(y + c) : Op<T>::zero(), s);
+    typename Op<T>::Frag f = in ? Op<T>::load(y + c) : Op<T>::zero();
+    if (sign != 1.f) f = Op<T>::scaled(f, sign);
+    s = Op<T>::mma(in ? Op<T>::load(row + c) : Op<T>::zero(), f, s);
   }
   return s;
 }
@@ -387,21 +401,19 @@ __device__ __forceinline__ void at_fwd_row(const AttnArgs* a, int h, int row, in
   const T* q = (const T*)a->q + row * a->q_row + h * a->q_head;
   const T* k = (const T*)a->k + hk * a->k_head;
   const T* v = (const T*)a->v + hk * a->v_head;
-  // scores with the scale's sign, as at_query has them
-  const float sign = a->c2 > 0.f ? 1.f : a->c2 < 0.f ? -1.f : 0.f, c2 = a->c2 == 0.f ? 1.f : fabsf(a->c2);
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 32) {
-    f32x16 s = at_products<T>(k, a->k_row, j0, row, q, D, lane);
+    f32x16 s = at_products<T>(k, a->k_row, j0, row, q, a->sign, D, lane);
     float mt = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[i] = j0 + at_pos(i, hh) <= row ? s[i] * sign : -INFINITY;
+      s[i] = j0 + at_pos(i, hh) <= row ? s[i] : -INFINITY;
       mt = fmaxf(mt, s[i]);
     }
-    const float mn = fmaxf(m, at_halves_max(mt)), al = m == mn ? 1.f : at_exp2((m - mn) * c2);
+    const float mn = fmaxf(m, at_halves_max(mt)), al = m == mn ? 1.f : at_exp2((m - mn) * a->c2);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {  // (before the first finite score mn is -inf too)
-      s[i] = s[i] == -INFINITY ? 0.f : at_exp2((s[i] - mn) * c2);
+      s[i] = s[i] == -INFINITY ? 0.f : at_exp2((s[i] - mn) * a->c2);
       sum += s[i];
     }
     m = mn;
@@ -418,7 +430,7 @@ __device__ __forceinline__ void at_fwd_row(const AttnArgs* a, int h, int row, in
     if (a->rest && lane + 64 < D) store_f<T>(rest, lane + 64, o1 / l - at_f<T>(o[lane + 64]));
   }
   if (a->stats && lane == 0) {
-    a->stats[(int64_t)h * a->N + row] = m * sign;
+    a->stats[(int64_t)h * a->N + row] = m;
     a->stats[((int64_t)a->H + h) * a->N + row] = log2f(l);
   }
 }
@@ -435,8 +447,8 @@ __device__ __forceinline__ void at_dq_row(const AttnArgs* a, int h, int row, int
   if (sizeof(T) == 2) dot += at_dot<T>(g, (const T*)a->rest + ((int64_t)row * a->H + h) * D, D);
   float o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 32) {
-    f32x16 ds = at_products<T>(k, a->k_row, j0, row, q, D, lane);
-    const f32x16 dp = at_products<T>(v, a->v_row, j0, row, g, D, lane);
+    f32x16 ds = at_products<T>(k, a->k_row, j0, row, q, a->sign, D, lane);
+    const f32x16 dp = at_products<T>(v, a->v_row, j0, row, g, 1.f, D, lane);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       ds[i] = j0 + at_pos(i, hh) <= row ? at_exp2(fmaf(ds[i] - m, a->c2, -ll)) * (dp[i] - dot) : 0.f;
@@ -459,8 +471,8 @@ __device__ __forceinline__ void at_dkv_row(const AttnArgs* a, int hk, int share,
     const T* g = (const T*)a->d_out + (int64_t)h * D;
     const int64_t g_row = (int64_t)a->H * D, st = (int64_t)h * a->N, logs = (int64_t)a->H * a->N;
     for (int i0 = row; i0 < end; i0 += 32) {
-      f32x16 p = at_products<T>(q, a->q_row, i0, end - 1, k, D, lane);
-      f32x16 ds = at_products<T>(g, g_row, i0, end - 1, v, D, lane);
+      f32x16 p = at_products<T>(q, a->q_row, i0, end - 1, k, a->sign, D, lane);
+      f32x16 ds = at_products<T>(g, g_row, i0, end - 1, v, 1.f, D, lane);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = i0 + at_pos(i, hh);
@@ -765,12 +777,11 @@ __device__ inline bool at_store_row(T* orow, T* rest, const f32x16 (&o)[NC], flo
 constexpr float AT_FAR = 4.f;
 __device__ inline float at_rounded_off(float m, float c2) { return fmaf(m, c2, -at_mul(m, c2)); }
 
-// Row stats of one query: the reference score (at_query may have turned its sign) and the log
-// of the sum.
-__device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float m, float l, float c2) {
+// Row stats of one query: the reference score and the log of the sum.
+__device__ inline void at_store_stats(const AttnArgs& a, int h, int row, float m, float l) {
   const int64_t at = (int64_t)h * a.N + row;
-  a.stats[at] = a.c2 > 0.f ? m : a.c2 < 0.f ? -m : 0.f;
-  a.stats[(int64_t)a.H * a.N + at] = log2f(l) - at_rounded_off(m, c2);
+  a.stats[at] = m;
+  a.stats[(int64_t)a.H * a.N + at] = log2f(l) - at_rounded_off(m, a.c2);
 }
 
 // ---------------------------------------------------------------- forward
@@ -810,16 +821,6 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
   l += (y[0] + y[1]) + (y[2] + y[3]);
 }
 
-// Query fragments with the scale's sign: c2 is positive then. (Scale 0: zeros, c2 = 1.)
-template <typename T, int DP>
-__device__ inline float at_query(const AttnArgs& a, int h, int row, int hh, typename Op<T>::Frag (&f)[DP / 16]) {
-  at_row<T, DP>((const T*)a.q + (int64_t)min(row, a.N - 1) * a.q_row + h * a.q_head, a.D, hh, f);
-  if (a.c2 > 0.f) return a.c2;
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) f[s] = Op<T>::scaled(f[s], a.c2 < 0.f ? -1.f : 0.f);
-  return a.c2 < 0.f ? -a.c2 : 1.f;
-}
-
 // Two LDS buffers that loads and reads alternate between. They are two variables, and the
 // loops run two tiles a turn, so that the compiler can tell a load into one from a read of
 // the other: where it cannot, it waits for every load in flight before the read.
@@ -855,7 +856,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   Frag qf[NS];
-  const float c2 = at_query<T, DP>(a, h, row0 + r, hh, qf);
+  at_row<T, DP>((const T*)a.q + (int64_t)min(row0 + r, a.N - 1) * a.q_row + h * a.q_head, a.D, hh, qf);
+  at_sign<T>(a, qf);
+  const float c2 = a.c2;
   Rows R;
   R.init(table, row0 + r);
   int blo, bhi;
@@ -908,7 +911,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void k_attn_fwd(AttnArgs a) {
   if (R.row < a.N && (R.in || a.fill)) {
     const int64_t at = ((int64_t)R.row * a.H + h) * a.D;
     odd = at_store_row<T, NC>((T*)a.out + at, a.rest ? (T*)a.rest + at : nullptr, o, 1.f / l, R.in, a.D, hh);
-    if (R.in && a.stats && hh == 0) at_store_stats(a, h, R.row, m, l, c2);
+    if (R.in && a.stats && hh == 0) at_store_stats(a, h, R.row, m, l);
     odd = odd && !(l == 0.f && m == -INFINITY);  // no finite score: NaN it is
     far = R.in && fabsf(at_rounded_off(m, c2)) > AT_FAR;
   }
@@ -980,7 +983,9 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   const T* kb = (const T*)a.k + hk * a.k_head;
   const T* vb = (const T*)a.v + hk * a.v_head;
   Frag qf[NS];
-  const float c2 = at_query<T, DP>(a, h, q0 + r, hh, qf);
+  at_row<T, DP>((const T*)a.q + (int64_t)min(q0 + r, a.N - 1) * a.q_row + h * a.q_head, a.D, hh, qf);
+  at_sign<T>(a, qf);
+  const float c2 = a.c2;
   Rows R;
   R.init(table, q0 + r);
   Ld lk, lv;
@@ -1029,7 +1034,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
   for (int i = 0; i < 4; ++i) sum_l += ml[1][i][r] * at_exp2(at_mul(ml[0][i][r], c2) - at_mul(M, c2));
   const Join<DP> join = {ldsA, ldsB};
   join.put(w, r, hh, o, at_exp2(at_mul(m, c2) - at_mul(M, c2)) / sum_l);
-  if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats(a, h, R.row, M, sum_l, c2);
+  if (w == 0 && hh == 0 && R.in && a.stats) at_store_stats(a, h, R.row, M, sum_l);
   __syncthreads();
   const unsigned long long far = __ballot(R.in && fabsf(at_rounded_off(M, c2)) > AT_FAR);
   const unsigned long long nan = __ballot(sum_l != sum_l);
@@ -1080,6 +1085,7 @@ struct QueryRow {
       for (int s = 0; s < DP / 16; ++s) dot = Op<T>::dot(g[s], o[s], dot);
     }
     at_row<T, DP>((const T*)a.q + (int64_t)rc * a.q_row + h * a.q_head, a.D, hh, q);
+    at_sign<T>(a, q);
     dot += __shfl_xor(dot, 32, 64);
   }
   // The row has no weights or no finite D: no channel of its dq is finite.
@@ -1397,6 +1403,7 @@ __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv
   at_block_range(K.lo, K.hi, lane, w, ends, blo, bhi);
   Frag kf[NS], vf[sizeof(T) == 2 ? 1 : NS];
   at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
+  at_sign<T>(a, kf);
   if constexpr (sizeof(T) == 4)
     at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
   auto value = [&](int s) -> Frag {
@@ -1456,6 +1463,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   const int rc = min(t.k0 + r, a.N - 1);
   Frag kf[NS], vf[NS];
   at_row<T, DP>((const T*)a.k + (int64_t)rc * a.k_row + t.hk * a.k_head, a.D, hh, kf);
+  at_sign<T>(a, kf);
   at_row<T, DP>((const T*)a.v + (int64_t)rc * a.v_row + t.hk * a.v_head, a.D, hh, vf);
   auto value = [&](int s) -> const Frag& { return vf[s]; };
   Keys K;
@@ -1618,7 +1626,8 @@ void at_fill_args(AttnArgs& a, const void* q, int64_t q_row, int64_t q_head, con
   a.q = q, a.k = k, a.v = v;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
   a.N = (int)rows, a.H = H, a.KV = KV, a.D = D, a.off = off, a.S = (int)n_seq;
-  a.scale = scale, a.c2 = scale * LOG2E, a.fill = fill != 0, a.hs = 1;
+  a.scale = scale, a.sign = (float)((scale > 0.f) - (scale < 0.f)), a.c2 = scale == 0.f ? 1.f : std::fabs(scale * LOG2E);
+  a.fill = fill != 0, a.hs = 1;
 }
 
 }  // namespace

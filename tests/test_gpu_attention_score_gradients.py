@@ -124,7 +124,8 @@ def test_scores_around_an_offset(device, dtype, sign, size, N, H, KV, D, lengths
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("H, KV, N", [(2, 2, 60), (32, 32, 2100)])
-def test_one_key_rows_give_their_cotangent(device, dtype, H, KV, N):
+@pytest.mark.parametrize("scale", [0.125, -0.2])
+def test_one_key_rows_give_their_cotangent(device, dtype, H, KV, N, scale):
     """Sequences of one row with ordinary channels and scores of any size: out = v, dv = do and
     no other gradient (the products round, but there is nothing to compare a score with)."""
     gen = torch.Generator(device=device).manual_seed(5)
@@ -133,13 +134,13 @@ def test_one_key_rows_give_their_cotangent(device, dtype, H, KV, N):
     q, k = (q * sizes).to(dtype), (k * sizes).to(dtype)
     off = torch.arange(N + 1, dtype=torch.int32, device=device)
     leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
-    out = packed_attention(*leaves, off)
+    out = packed_attention(*leaves, off, scale=scale)
     dq, dk, dv = torch.autograd.grad(out, leaves, g)
     u = torch.finfo(dtype).eps / 2
     # weight, operand and result: two roundings of the type and the weight's own in 32 bits
     near = lambda x, y: ((x.double() - y.double()).abs() <= (2.1 * u + 64 * E) * y.double().abs()).all()  # noqa: E731
     assert near(out, v) and near(dv, g)
     # ds = p (do . v - do . out), each with the error of out, of a product sum and of p
-    size = (g.double().abs() * v.double().abs()).sum(-1, keepdim=True) * (2.1 * u + 200 * E) / 8
+    size = (g.double().abs() * v.double().abs()).sum(-1, keepdim=True) * (2.1 * u + 200 * E) * abs(scale)
     assert (dq.double().abs() <= 1.05 * size * k.double().abs() + 1e-30).all()
     assert (dk.double().abs() <= 1.05 * size * q.double().abs() + 1e-30).all()
