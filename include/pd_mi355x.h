@@ -680,7 +680,11 @@ int pd_faithfulness_bwd(int64_t n_mats, int64_t mats_per_site, int64_t d_in, int
  * left as they were (fill = 0); what they, other sequences and later rows hold, NaN and
  * infinities included, reaches no other row. Offsets outside [0, rows] or out of order
  * give wrong rows but no access outside the tensors.
- *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, fp32 statistics;
+ *   out [rows, n_head, head_dim] = softmax(scale q k^T) v, scores, statistics and sums fp32.
+ * With bf16 tensors the weights (and dS in the backward) enter their products rounded to
+ * bf16: half a step of each weight beside that of each result. A row whose softmax has no
+ * value (a NaN among its scores, none that is finite) is NaN. Rows beside a NaN that the
+ * mask hides in a block of 32 or 64 rows, and rows of scores past 5 10^7, take a slow path.
  * For the backward (nullable): stats fp32 [2, n_head, rows], a reference score of each
  * row (q . k with the scale's sign) and log2 of its softmax sum relative to that, and with bf16 tensors out_rest [rows,
  * n_head, head_dim] bf16, what rounding took off out. Scores may have any size that fp32
@@ -706,7 +710,8 @@ int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const 
  * weight and bias fp32 [d], NULL = 1 and 0.
  *   y = (x - mean) / sqrt(var + eps) weight + bias, mean and (biased) var over d;
  *   stats fp32 [rows, 3] (nullable): the mean as a base and its distance from it, and
- *   1 / sqrt(var + eps), for the backward.
+ *   1 / sqrt(var + eps), for the backward. Sums are fp32 (d times a row's largest entry below
+ *   3.4 10^38, or it is not finite; weight and bias gradients are fp32 sums over rows too).
  * The backward: d_x; d_weight = sum_rows d_y (x - mean) / sqrt(var + eps) and d_bias =
  * sum_rows d_y, fp32 [d], overwritten; each of the three may be NULL. workspace: needed
  * with d_weight or d_bias. Fixed-order sums: bit-identical from call to call. */
@@ -730,7 +735,9 @@ int pd_layer_norm_bwd(const void* x, const void* d_y, int dtype, int64_t rows, i
  *     exp(top / temperature - clean_lse), and the mass they leave (below 2^-20: none) is
  *     compared as one entry with the mass q gives all entries not listed.
  * kl fp32 [rows] (nullable); grad [rows, vocab] in `dtype` (nullable) = row_weight (fp32
- * [rows], NULL = 1) times d kl / d z; a row of weight 0 gets zeros whatever it holds.
+ * [rows], NULL = 1) times d kl / d z; a row of weight 0 gets zeros whatever it holds. A row's
+ * maxima and sums of exponentials are fp32: kl is off by up to a few 1e-7 whatever its size,
+ * so a kl far below 1e-5 keeps few digits and may come out just below 0.
  * vocab up to 2^19, k up to 1024. The workspace is needed with kl. */
 size_t pd_top_kl_workspace_size(int64_t rows, int k);
 int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void* top, int top_dtype, const void* idx,

@@ -48,7 +48,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     itself: q [rows, H, head_dim], k and v [rows, KV, head_dim], bf16 or fp32 (views of one
     projection's output are read as they are), H a multiple of KV, head_dim up to 128;
     offsets int32 [sequences + 1] on the same GPU. Returns [rows, H, head_dim], zeros in
-    rows of no sequence; differentiable in q, k and v. `scale`: head_dim^-0.5 by default."""
+    rows of no sequence; differentiable in q, k and v (not in forward mode, and once). Scores
+    and sums are fp32; bf16 operands meet weights rounded to bf16. `scale`: head_dim^-0.5 by
+    default."""
     D = q.shape[-1] if q.dim() else 0
     pad = (-D) % 8
     if pad and D <= 128:  # zero columns add nothing to the scores and are cut off the result

@@ -21,14 +21,18 @@
 // exchange between the wave's halves, and the accumulator's registers are, slice by slice,
 // the Y operand of the next product; its X partner (channels as rows, positions as k) is
 // read transposed from the row-major LDS image. P and dS are rounded to bf16 as operands
-// where the inputs are bf16 (as they would be if stored in the inputs' type) and stay fp32
-// otherwise; sums and statistics are fp32.
+// where the inputs are bf16 (as they would be if stored in the inputs' type: the products then
+// run at the bf16 rate, 7 times the fp32 one's) and stay fp32 otherwise; sums and statistics are
+// fp32. Against 64 bits a bf16 result is off by 2.0 10^-3 of its norm forward and 2.4 10^-3 with
+// its gradients, where rounding the results alone is 1.5 to 1.7 10^-3.
 //
 // A row keeps two statistics for the backward: a reference score m_i = q_i . k_j of one of its
 // keys and the log of its sum relative to that. p = 2^{c2 (q . k - m) - log}: the difference
 // of two scores is exact where they are close, whatever their size. (From the log of the sum
-// itself, one fp32 number, p was off by 2^(-24) of the scores' size: a row's only key got
-// weights of 0.96 to 1.04 at scores of 10^6 and 0 at 10^30.)
+// itself, one fp32 number, p is off by 2^-24 of the scores' size: a row's only key got weights
+// of 0.96 to 1.04 at scores of 10^6 and 0 at 10^30. The additional statistic costs the bf16 key
+// side 3 to 6%.)
+#include <algorithm>
 #include <type_traits>
 
 #include "pd_gemm_dtl.hpp"
@@ -52,13 +56,14 @@ struct AttnArgs {
   int N, H, KV, D;
   const int32_t* off;
   int S;
-  // scores enter as sign q . k and exponents take them times c2 = |scale| log2 e (scale 0: sign
-  // 0 and c2 1)
-  float scale, sign, c2;
+  // Scores take the scale's sign (flip: the sign bits of a word of q or k that change with it)
+  // and exponents take them times c2 = |scale| log2 e, or fp32's smallest number where that is 0.
+  float scale, c2;
+  uint32_t flip;
   int fill;         // rows of no sequence: 1 zeros, 0 left as they are
   void* out;        // [N, H, D]
   void* rest;       // bf16 [N, H, D]: what rounding took off out (NULL: not kept; fp32: none)
-  float* stats;     // [H, N] m_i, a score sign q . k of row i, then [H, N] log2 sum_j 2^{c2 (sign q_i . k_j - m_i)}
+  float* stats;     // [H, N] m_i, a score of row i, then [H, N] log2 sum_j 2^{c2 (score ij - m_i)}
   const void* d_out;
   float* rowdot;  // [H, N]: D_i
   void *dq, *dk, *dv;
@@ -83,13 +88,11 @@ struct Op<bf16_t> {
     return (Frag)(at_u32x4){pack_bf16x2(v[8 * kk], v[8 * kk + 1]), pack_bf16x2(v[8 * kk + 2], v[8 * kk + 3]),
                             pack_bf16x2(v[8 * kk + 4], v[8 * kk + 5]), pack_bf16x2(v[8 * kk + 6], v[8 * kk + 7])};
   }
-  static __device__ inline Frag scaled(const Frag& a, float f) {  // f = -1 or 0
-    const at_u32x4 x = (at_u32x4)a;
-    at_u32x4 y;
+  static __device__ inline void flip(Frag& a, uint32_t signs) {
+    at_u32x4 x = (at_u32x4)a;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      y[i] = pack_bf16x2(__uint_as_float(x[i] << 16) * f, __uint_as_float(x[i] & 0xFFFF0000u) * f);
-    return (Frag)y;
+    for (int i = 0; i < 4; ++i) x[i] ^= signs;
+    a = (Frag)x;
   }
   static __device__ inline float dot(const Frag& a, const Frag& b, float s) {
     const at_u32x4 x = (at_u32x4)a, y = (at_u32x4)b;
@@ -126,11 +129,9 @@ struct Op<float> {
     for (int i = 0; i < 8; ++i) f.v[i] = v[8 * kk + i];
     return f;
   }
-  static __device__ inline Frag scaled(const Frag& a, float f) {
-    Frag y;
+  static __device__ inline void flip(Frag& a, uint32_t signs) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y.v[i] = a.v[i] * f;
-    return y;
+    for (int i = 0; i < 8; ++i) a.v[i] = __uint_as_float(__float_as_uint(a.v[i]) ^ signs);
   }
   static __device__ inline float dot(const Frag& a, const Frag& b, float s) {
 #pragma unroll
@@ -255,9 +256,8 @@ __device__ inline void at_row(const T* row, int D, int hh, typename Op<T>::Frag 
 // of -q is not always the negative of q's to the bit), so that c2 is positive.
 template <typename T, int NS>
 __device__ inline void at_sign(const AttnArgs& a, typename Op<T>::Frag (&f)[NS]) {
-  if (a.sign == 1.f) return;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) f[s] = Op<T>::scaled(f[s], a.sign);
+  for (int s = 0; s < NS; ++s) Op<T>::flip(f[s], a.flip);
 }
 
 // Key (or query) position inside a 32-row block that accumulator register i holds.
@@ -357,11 +357,11 @@ __device__ inline float at_halves_max(float v) {
 // diverged runs at about its normal speed. Rows of large scores come here too:
 // their weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
 
-// Products of sign y with rows j0 .. j0 + 31 of an operand (those behind `last` read as
+// Products of y, its signs flipped by `signs`, with rows j0 .. j0 + 31 of an operand (those behind `last` read as
 // row `last`), by the tiles' instructions and in their order, so scores are the tiles' own
 // bits: register i is row j0 + at_pos(i, hh), the same in a half's 32 lanes.
 template <typename T>
-__device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, float sign, int D,
+__device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, uint32_t signs, int D,
                                      int lane) {
   const T* row = x + min(j0 + (lane & 31), last) * stride;
   f32x16 s = {};
@@ -370,7 +370,7 @@ __device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int las
     const int c = c0 + 8 * (lane >> 5);
     const bool in = c < D;
     typename Op<T>::Frag f = in ? Op<T>::load(y + c) : Op<T>::zero();
-    if (sign != 1.f) f = Op<T>::scaled(f, sign);
+    Op<T>::flip(f, signs);
     s = Op<T>::mma(in ? Op<T>::load(row + c) : Op<T>::zero(), f, s);
   }
   return s;
@@ -403,7 +403,7 @@ __device__ __forceinline__ void at_fwd_row(const AttnArgs* a, int h, int row, in
   const T* v = (const T*)a->v + hk * a->v_head;
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 32) {
-    f32x16 s = at_products<T>(k, a->k_row, j0, row, q, a->sign, D, lane);
+    f32x16 s = at_products<T>(k, a->k_row, j0, row, q, a->flip, D, lane);
     float mt = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -447,8 +447,8 @@ __device__ __forceinline__ void at_dq_row(const AttnArgs* a, int h, int row, int
   if (sizeof(T) == 2) dot += at_dot<T>(g, (const T*)a->rest + ((int64_t)row * a->H + h) * D, D);
   float o0 = 0.f, o1 = 0.f;
   for (int j0 = start; j0 <= row; j0 += 32) {
-    f32x16 ds = at_products<T>(k, a->k_row, j0, row, q, a->sign, D, lane);
-    const f32x16 dp = at_products<T>(v, a->v_row, j0, row, g, 1.f, D, lane);
+    f32x16 ds = at_products<T>(k, a->k_row, j0, row, q, a->flip, D, lane);
+    const f32x16 dp = at_products<T>(v, a->v_row, j0, row, g, 0, D, lane);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       ds[i] = j0 + at_pos(i, hh) <= row ? at_exp2(fmaf(ds[i] - m, a->c2, -ll)) * (dp[i] - dot) : 0.f;
@@ -471,8 +471,8 @@ __device__ __forceinline__ void at_dkv_row(const AttnArgs* a, int hk, int share,
     const T* g = (const T*)a->d_out + (int64_t)h * D;
     const int64_t g_row = (int64_t)a->H * D, st = (int64_t)h * a->N, logs = (int64_t)a->H * a->N;
     for (int i0 = row; i0 < end; i0 += 32) {
-      f32x16 p = at_products<T>(q, a->q_row, i0, end - 1, k, a->sign, D, lane);
-      f32x16 ds = at_products<T>(g, g_row, i0, end - 1, v, 1.f, D, lane);
+      f32x16 p = at_products<T>(q, a->q_row, i0, end - 1, k, a->flip, D, lane);
+      f32x16 ds = at_products<T>(g, g_row, i0, end - 1, v, 0, D, lane);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = i0 + at_pos(i, hh);
@@ -832,9 +832,10 @@ __device__ __forceinline__ void at_softmax(f32x16 (&sc)[NB], bool hidden, float&
 // through LDS BK rows at a time in two buffers: one barrier a tile, behind it the next
 // tile's loads go out and have this tile's products to land. The matrix cores and, in
 // between, a tile's exponentials bound long sequences (16384 tokens, 16/4 heads of 128:
-// 1008 us, 1090 TFLOP/s; 8192 tokens, 32/8 heads, the longest sequence 5003: 296 us), the
+// 1025 us, 1070 TFLOP/s; 8192 tokens, 32/8 heads, the longest sequence 5003: 290 us), the
 // longest tile's dependent chain of them short ones (0.85 us for 64 keys of D = 64 in a block
-// that is alone on its CU; 8192 tokens in ten sequences of up to 2048, 12 heads: 43 us).
+// that is alone on its CU; 8192 tokens in ten sequences of up to 2048, 12 heads: 44 us).
+// fp32 rows of more than 96 channels spill 36 registers at two waves a SIMD.
 template <typename T, int DP>
 struct FwdCfg {
   static constexpr int BK = Img<T, DP>::ROWB == 512 ? 32 : 64, TILE = BK * Img<T, DP>::ROWB;
@@ -1123,7 +1124,7 @@ __device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int 
 
 // dq, and D_i for the key side. Tiles, waves and bounds as the forward's (8192 tokens, 32/8
 // heads of 128: 385 us, 970 TFLOP/s over its three products; ten sequences, 12 heads of 64:
-// 55 us, the first 10 of them for the rows of q, do, out and its rest). fp32 rows of more than
+// 53 us, the first 10 of them for the rows of q, do, out and its rest). fp32 rows of more than
 // 64 channels take one wave a SIMD: with two, 100 values spilled (D = 128: 972 -> 620 us).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 4 && DP > 64 ? 1 : 2) void k_attn_dq(AttnArgs a) {
@@ -1281,9 +1282,13 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
   if constexpr (sizeof(T) == 2) lane = at_fresh(lane);  // (fp32 has room, and more addresses)
   const int r = lane & 31, hh = lane >> 5;
   f32x16 p = {}, ds = {};
-  float4 ref[4];  // the reference scores, read before the products (D = 64: 80 -> 73 us behind them)
+  // bf16: the reference scores, read before the products (8192 tokens in ten sequences, 12
+  // heads of 64: 73 us, 80 behind them); fp32 has no registers left for them there
+  float4 ref[4];
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) ref[g] = *(const float4*)&qs[2][8 * g + 4 * hh];
+    for (int g = 0; g < 4; ++g) ref[g] = *(const float4*)&qs[2][8 * g + 4 * hh];
+  }
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     p = Op<T>::mma(I::rows(Ql, r, s, hh), kf[s], p);
@@ -1295,7 +1300,8 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int at = 8 * g + 4 * hh;
-    const float4 l = *(const float4*)&ql[at], D = *(const float4*)&qs[1][at], m = ref[g];
+    const float4 l = *(const float4*)&ql[at], D = *(const float4*)&qs[1][at];
+    const float4 m = sizeof(T) == 2 ? ref[g] : *(const float4*)&qs[2][at];
     const float lv[4] = {l.x, l.y, l.z, l.w}, Dv[4] = {D.x, D.y, D.z, D.w}, mv[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -1376,8 +1382,8 @@ __device__ inline bool at_store_keys(const AttnArgs& a, const KeyTile& t, const 
 // order, so the result is the same on every run. The keys' fragments stay in registers and
 // the values' in LDS: with both in registers a wave takes more than 256 and a SIMD holds
 // one, with nothing beside it while it waits. LDS reads bound it beside the matrix cores: a
-// wave reads 40 KB for its 32 products of a block at D = 128 (8192 tokens, 32/8 heads: 513 us,
-// 970 TFLOP/s; ten sequences, 12 heads of 64: 72 us).
+// wave reads 40 KB for its 32 products of a block at D = 128 (8192 tokens, 32/8 heads: 540 us,
+// 920 TFLOP/s, with 15 spilled registers; ten sequences, 12 heads of 64: 74 us).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
   typedef Img<T, DP> I;
@@ -1625,11 +1631,12 @@ KeyPlan at_key_plan(int64_t rows, int H, int KV) {
 
 void at_fill_args(AttnArgs& a, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                   const void* v, int64_t v_row, int64_t v_head, int64_t rows, int H, int KV, int D, const int32_t* off,
-                  int64_t n_seq, float scale, int fill) {
+                  int64_t n_seq, float scale, int fill, int dtype) {
   a.q = q, a.k = k, a.v = v;
   a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
   a.N = (int)rows, a.H = H, a.KV = KV, a.D = D, a.off = off, a.S = (int)n_seq;
-  a.scale = scale, a.sign = (float)((scale > 0.f) - (scale < 0.f)), a.c2 = scale == 0.f ? 1.f : std::fabs(scale * LOG2E);
+  a.scale = scale, a.c2 = std::max(std::fabs(scale * LOG2E), 0x1p-149f);
+  a.flip = scale >= 0.f ? 0u : dtype == PD_DTYPE_BF16 ? 0x80008000u : 0x80000000u;
   a.fill = fill != 0, a.hs = 1;
 }
 
@@ -1653,7 +1660,7 @@ int pd_packed_attention_fwd(const void* q, int64_t q_row, int64_t q_head, const 
   if ((uintptr_t)out_rest & 15) return fail(PD_EUNSUPPORTED, "pd_packed_attention_fwd: tensors must be 16-byte aligned");
   AttnArgs a = {};
   at_fill_args(a, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, rows, n_head, n_kv_head, head_dim, offsets, n_seq,
-               scale, fill);
+               scale, fill, dtype);
   a.out = out, a.rest = out_rest, a.stats = stats;
   const bool split = at_query_split(rows, n_head, dtype);
   const unsigned grid = (unsigned)(cdiv(rows, split ? AT_SPLIT : AT_ROWS) * n_head);
@@ -1692,7 +1699,7 @@ int pd_packed_attention_bwd(const void* q, int64_t q_row, int64_t q_head, const 
     return fail(PD_EWORKSPACE, "pd_packed_attention_bwd: workspace");
   AttnArgs a = {};
   at_fill_args(a, q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, rows, n_head, n_kv_head, head_dim, offsets, n_seq,
-               scale, fill);
+               scale, fill, dtype);
   a.out = const_cast<void*>(out), a.rest = const_cast<void*>(out_rest), a.stats = const_cast<float*>(stats);
   a.d_out = d_out, a.dq = dq, a.dk = dk, a.dv = dv, a.rowdot = (float*)workspace;
   const KeyPlan plan = at_key_plan(rows, n_head, n_kv_head);

@@ -25,8 +25,8 @@ namespace pd {
 namespace {
 
 constexpr int LN_MAX_D = 16384;   // largest row held in registers
-// Most threads of a launch that walks over rows: forward 16384 x 4096 bf16 63 us with half as
-// many, 49, 48 with twice as many. Where each block leaves a row of partial gradients and rows
+// Most threads of a launch that walks over rows: forward 16384 x 4096 bf16 67 us with half as
+// many, 52, 53 with twice as many (60000 x 512 37, 25, 24). Where each block leaves a row of partial gradients and rows
 // are long, half of that (backward 93 us, 105 with all; 30000 x 1024 41, 50; but 60000 x 512
 // 43, 38).
 constexpr int LN_THREADS = 256 * 1024;
@@ -109,7 +109,7 @@ __device__ inline int ln_wave_count(int w, int d) {
 constexpr int ln_threads(int nt) { return nt <= 64 ? 256 : nt; }
 
 // Forward. Grid: row groups; a block holds RPB rows at a time (NT <= 64: rows share waves or
-// have one each, with no barrier). At the rate of a copy: 16384 x 4096 bf16 49 us, 5.5 TB/s.
+// have one each, with no barrier). At the rate of a copy: 16384 x 4096 bf16 52 us, 5.1 TB/s.
 template <typename T, int NT, int E>
 __global__ __launch_bounds__(ln_threads(NT)) void k_ln_fwd(const T* __restrict__ x, int64_t rows, int d,
                                                            const float* __restrict__ w, const float* __restrict__ b,
@@ -445,8 +445,9 @@ __global__ __launch_bounds__(256) void k_ln_dw_long(const T* __restrict__ x, con
 constexpr int LN_LONG_SLICES = 16;
 
 // Threads and elements a row is held in: the smallest of the built forms that covers d (a row
-// in twice the threads, half of them idle: forward, backward of 16384 x 4096 bf16 49, 93 ->
-// 84, 132 us; 100000 x 256 22, 33 -> 39, 45; one even case, the backward of 8192 x 8192).
+// in twice the threads, half of them idle: forward, backward of 16384 x 4096 bf16 52, 93 ->
+// 90, 134 us; 100000 x 256 22, 32 -> 38, 43; one even case, the backward of 8192 x 8192: 106,
+// 104). fp32 rows above 8192 spill 39 of the backward's registers and 7 of the forward's.
 // F is called with (NT, E) as integral constants.
 template <typename F>
 void ln_form(int64_t d, F&& f) {

@@ -24,8 +24,10 @@
 // The loss is a small difference of logarithms: a second kernel forms p, the logarithms and
 // the loss of a row in 64 bits from the row's maxima and sums (32-bit, their exponents with
 // log2(e) / tau in two parts). In the first kernel that arithmetic took the registers that
-// hold the row. The gradient's rest is 64-bit too (what the listed leave of 1), its other
-// terms are 32-bit.
+// hold the row. The 32-bit sums leave a loss off by up to a few 1e-7 whatever its size. The
+// gradient's rest is 64-bit too (what the listed leave of 1), its other terms are 32-bit: the
+// exponents of the entries not listed take log2(e) / tau in one part, off by 2^-23 of their
+// size, which is below a gradient's other roundings up to exponents of some tens.
 #include <float.h>
 #include <type_traits>
 
@@ -170,7 +172,10 @@ constexpr int kl_entries(int nt) { return nt >= 256 ? KL_MAX_K / nt : 4; }
 // REG: the row fits NT * U words and stays in registers between the two passes. What bounds it
 // is a row's chain of passes (maximum, sum, gradient, with a reduction between each two) at
 // two rows a CU where rows are long: 8192 x 50277 bf16, 64 listed, the gradient 430 us,
-// 3.8 TB/s, the loss another 20; 1500 x 32000 fp32 93 us, 4.1 TB/s.
+// 3.8 TB/s, the loss another 19; 1500 x 32000 fp32 93 us, 4.1 TB/s (calls one behind another).
+// At 128 registers a thread 16 words spill 27 of them with the gradient and 16 to 20 without
+// (20 to 22 and 12 to 16 in 1024 threads), 256 threads of 8 words 13 and 2, the streaming form
+// 5 to 10 with the gradient; the others none or 2.
 template <typename T, int NT, int U, bool REG, bool GRAD>
 __global__ __launch_bounds__(NT, 4) void k_top_kl(TopKLArgs a) {
 #pragma clang fp contract(off)  // the same sums with and without the gradient
@@ -526,7 +531,10 @@ int top_kl_launch(const TopKLArgs& a, hipStream_t s) {
   // the next two, and the streaming one: 100000 x 1000 bf16 291, 343, 895, 3628 us; 8192 x
   // 16000 135, 193, 245, 343; 4096 x 50277 217, 319, streaming 295. The widest is even with the
   // streaming one (2048 x 131000: 284 and 288) and reads a row once. 512 threads of 16 words
-  // with one block a CU, two, more: 289, 229, 231 us at 4096 x 50277.
+  // with one block a CU, two, more: 289, 229, 231 us at 4096 x 50277. The loss alone, in this
+  // form, the next one and the streaming one: 100000 x 1000 bf16 159, 225, 2878 us; 8192 x
+  // 16000 86, 141, 272; 8192 x 50277 245, 422, 393; 1500 x 32000 fp32 51, 66, 60; 2048 x 131072
+  // bf16 153, streaming 167.
   if (a.k <= 256 && words <= 64 * 2) return go(k_top_kl<T, 64, 2, true, GRAD>, 64, 256 * 16);
   if (a.k <= 256 && words <= 64 * 8) return go(k_top_kl<T, 64, 8, true, GRAD>, 64, 256 * 16);
   if (words <= 256 * 8) return go(k_top_kl<T, 256, 8, true, GRAD>, 256, 256 * 8);

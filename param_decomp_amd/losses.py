@@ -317,8 +317,9 @@ def top_logits_position_kl(masked_logits: torch.Tensor, top_logits: torch.Tensor
     `torch.logsumexp(clean_logits / temperature, -1)`) they are the clean model's own, and
     the mass of the entries not listed is compared as one: a lower bound of
     `categorical_kl_from_logits`'s KL that it meets at k = V. Returns fp32 [...];
-    differentiable in the masked logits. `ops.top_logits_kl` gives the loss and its weighted
-    gradient from one read of the logits."""
+    differentiable in the masked logits. Sums over the vocabulary are fp32: a loss is off by a
+    few 1e-7 at any size. `ops.top_logits_kl` gives the loss and its weighted gradient from one
+    read of the logits."""
     masked = masked_logits.contiguous()
     top, indices = top_logits.detach().contiguous(), top_indices.contiguous()
     lse = None if clean_lse is None else clean_lse.detach().contiguous()
