@@ -30,10 +30,10 @@
 // keys and the log of its sum relative to that. p = 2^{c2 (q . k - m) - log}: the difference
 // of two scores is exact where they are close, whatever their size. (From the log of the sum
 // itself, one fp32 number, p is off by 2^-24 of the scores' size: a row's only key got weights
-// of 0.96 to 1.04 at scores of 10^6 and 0 at 10^30. The additional statistic costs the bf16 key
-// side 3 to 6%.)
+// of 0.96 to 1.04 at scores of 10^6 and 0 at 10^30.)
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "pd_gemm_dtl.hpp"
 
@@ -260,6 +260,15 @@ __device__ inline void at_sign(const AttnArgs& a, typename Op<T>::Frag (&f)[NS])
   for (int s = 0; s < NS; ++s) Op<T>::flip(f[s], a.flip);
 }
 
+// Lane i's value of each row of 16 lanes, in all of them.
+template <int I>
+__device__ inline float at_of(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + I, 0xf, 0xf, true));  // row_newbcast
+}
+template <typename F, int... I>
+__device__ __forceinline__ void at_each(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
 // Key (or query) position inside a 32-row block that accumulator register i holds.
 __device__ inline int at_pos(int i, int hh) { return 8 * (i >> 2) + 4 * hh + (i & 3); }
 // The lane again, as a value that nothing was formed from yet: LDS addresses of a loop are
@@ -1124,7 +1133,7 @@ __device__ __forceinline__ void at_dq_block(const char* Kl, const char* Vl, int 
 
 // dq, and D_i for the key side. Tiles, waves and bounds as the forward's (8192 tokens, 32/8
 // heads of 128: 385 us, 970 TFLOP/s over its three products; ten sequences, 12 heads of 64:
-// 53 us, the first 10 of them for the rows of q, do, out and its rest). fp32 rows of more than
+// 51 us, the first 10 of them for the rows of q, do, out and its rest). fp32 rows of more than
 // 64 channels take one wave a SIMD: with two, 100 values spilled (D = 128: 972 -> 620 us).
 template <typename T, int DP>
 __global__ __launch_bounds__(AT_THREADS, sizeof(T) == 4 && DP > 64 ? 1 : 2) void k_attn_dq(AttnArgs a) {
@@ -1270,8 +1279,8 @@ struct Keys {
   }
 };
 
-// One block of 32 queries (images at Ql, Gl; in qs their logs of sums, D, reference scores
-// and, for lanes that the queries do not see, infinite logs): dv += p do, dk += ds / scale q.
+// One block of 32 queries (images at Ql, Gl; in qs their logs of sums, infinite ones for lanes
+// that the queries do not see, and pairs of references and D): dv += p do, dk += ds / scale q.
 // vf(s) gives fragment s of the lane's value row.
 template <typename T, int DP, typename VF>
 __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, const float (*qs)[32], int i0,
@@ -1282,13 +1291,11 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
   if constexpr (sizeof(T) == 2) lane = at_fresh(lane);  // (fp32 has room, and more addresses)
   const int r = lane & 31, hh = lane >> 5;
   f32x16 p = {}, ds = {};
-  // bf16: the reference scores, read before the products (8192 tokens in ten sequences, 12
-  // heads of 64: 73 us, 80 behind them); fp32 has no registers left for them there
-  float4 ref[4];
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int g = 0; g < 4; ++g) ref[g] = *(const float4*)&qs[2][8 * g + 4 * hh];
-  }
+  // lane 32 hh + i and 16 lanes on: the reference and D of the query in accumulator register i.
+  // One value a lane, handed to the others by the subtractions themselves: read from LDS as the
+  // logs are, four words a lane, they took a tenth of the reads that bound this product (8192
+  // tokens, 32/8 heads of 128: 565 -> 540 us).
+  const float2 mD = ((const float2*)qs[2])[lane & 47];
 #pragma unroll
   for (int s = 0; s < DP / 16; ++s) {
     p = Op<T>::mma(I::rows(Ql, r, s, hh), kf[s], p);
@@ -1296,20 +1303,17 @@ __device__ __forceinline__ void at_dkv_block(const char* Ql, const char* Gl, con
   }
   bool hidden;
   const bool some = K.seen.some(i0, 32, hidden);
-  const float* ql = qs[hidden ? 3 : 0];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int at = 8 * g + 4 * hh;
-    const float4 l = *(const float4*)&ql[at], D = *(const float4*)&qs[1][at];
-    const float4 m = sizeof(T) == 2 ? ref[g] : *(const float4*)&qs[2][at];
-    const float lv[4] = {l.x, l.y, l.z, l.w}, Dv[4] = {D.x, D.y, D.z, D.w}, mv[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 4 * g + e;
-      p[i] = at_exp2(fmaf(p[i] - mv[e], c2, -lv[e]));
-      ds[i] = p[i] * (ds[i] - Dv[e]);
-    }
-  }
+  const float* ql = qs[hidden ? 1 : 0];
+  at_each([&](auto group) {
+    constexpr int g = decltype(group)::value;
+    const float4 l = *(const float4*)&ql[8 * g + 4 * hh];
+    const float lv[4] = {l.x, l.y, l.z, l.w};
+    at_each([&](auto reg) {
+      constexpr int e = decltype(reg)::value, i = 4 * g + e;
+      p[i] = at_exp2(fmaf(p[i] - at_of<i>(mD.x), c2, -lv[e]));
+      ds[i] = p[i] * (ds[i] - at_of<i>(mD.y));
+    }, std::make_integer_sequence<int, 4>{});
+  }, std::make_integer_sequence<int, 4>{});
   if (some) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -1352,7 +1356,9 @@ struct QueryStats {
     m = a.stats[at], ll = a.stats[at + (int64_t)a.H * a.N], D = a.rowdot[at];
   }
   __device__ inline void store(float (*qs)[32], int q) const {
-    qs[0][q] = ll, qs[1][q] = D, qs[2][q] = m, qs[3][q] = INFINITY;
+    qs[0][q] = ll, qs[1][q] = INFINITY;
+    // at_pos(i, hh) = q at slot 32 hh + i: the pair of lane 32 hh + i
+    ((float2*)qs[2])[(q & 4) << 3 | (q >> 1 & 12) | (q & 3)] = make_float2(m, D);
   }
 };
 
@@ -1383,16 +1389,17 @@ __device__ inline bool at_store_keys(const AttnArgs& a, const KeyTile& t, const 
 // the values' in LDS: with both in registers a wave takes more than 256 and a SIMD holds
 // one, with nothing beside it while it waits. LDS reads bound it beside the matrix cores: a
 // wave reads 40 KB for its 32 products of a block at D = 128 (8192 tokens, 32/8 heads: 540 us,
-// 920 TFLOP/s, with 15 spilled registers; ten sequences, 12 heads of 64: 74 us).
+// 920 TFLOP/s; ten sequences, 12 heads of 64: 66 us). D = 64 keeps to three waves a SIMD: 66 us,
+// and 16 sequences of 512 29, where two took 68 and 36.
 template <typename T, int DP>
-__global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? 2 : 1) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__(AT_THREADS, sizeof(T) == 2 ? (DP == 64 ? 3 : 2) : 1) void k_attn_dkv(AttnArgs a) {
   typedef Img<T, DP> I;
   typedef typename Op<T>::Frag Frag;
   constexpr int TILE = 32 * I::ROWB, NS = DP / 16, NC = DP / 32;
   constexpr int VLDS = sizeof(T) == 2 ? AT_ROWS * I::ROWB : 16;
   AT_TWO_BUFFERS(2 * TILE);
   __shared__ __attribute__((aligned(1024))) char Vl[VLDS];
-  __shared__ __attribute__((aligned(16))) float qs[2][4][32];
+  __shared__ __attribute__((aligned(16))) float qs[2][5][32];
   __shared__ int ends[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
@@ -1462,7 +1469,7 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_dkv_split(AttnArgs a) {
   typedef Loader<T, DP, 32, 1> Ld;
   constexpr int MINE = 2 * TILE;
   AT_TWO_BUFFERS(4 * MINE);
-  __shared__ __attribute__((aligned(16))) float qs[4][4][32];
+  __shared__ __attribute__((aligned(16))) float qs[4][5][32];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, hh = lane >> 5;
   __shared__ int seq[SeqTable::SIZE];
   __shared__ __attribute__((aligned(16))) int keys[260];
