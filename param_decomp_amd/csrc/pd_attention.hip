@@ -375,31 +375,37 @@ __device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int las
   const T* row = x + min(j0 + (lane & 31), last) * stride;
   f32x16 s = {};
 #pragma unroll 1
-  for (int c0 = 0; c0 < D; c0 += 16) {
-    const int c = c0 + 8 * (lane >> 5);
-    const bool in = c < D;
-    typename Op<T>::Frag f = in ? Op<T>::load(y + c) : Op<T>::zero();
-    Op<T>::flip(f, signs);
-    s = Op<T>::mma(in ? Op<T>::load(row + c) : Op<T>::zero(), f, s);
+  for (int c0 = 0; c0 < D; c0 += 64) {  // four slices' loads before their products
+    typename Op<T>::Frag xs[4], ys[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + 16 * i + 8 * (lane >> 5);
+      xs[i] = Op<T>::load(row + min(c, D - 8)), ys[i] = Op<T>::load(y + min(c, D - 8));
+      if (c >= D) xs[i] = ys[i] = Op<T>::zero();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      Op<T>::flip(ys[i], signs);
+      s = Op<T>::mma(xs[i], ys[i], s);
+    }
   }
   return s;
 }
 // Adds w times each of the rows j0 .. min(j0 + 31, last) to channels lane and lane + 64; w as
-// at_products gives it.
+// at_products gives it, 0 behind `last` (that row is read there again: one that is seen).
 template <typename T>
 __device__ inline void at_add_rows(const T* x, int64_t stride, int j0, int last, const f32x16& w, int D, int lane,
                                    float& o0, float& o1) {
   const bool hh = lane >> 5;
+  const int c0 = min(lane, D - 1), c1 = min(lane + 64, D - 1);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float other = __shfl_xor(w[i], 32, 64), ws[2] = {hh ? other : w[i], hh ? w[i] : other};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int j = j0 + at_pos(i, e);
-      if (j > last) continue;
-      const T* r = x + j * stride;
-      if (lane < D) o0 = fmaf(ws[e], at_f<T>(r[lane]), o0);
-      if (lane + 64 < D) o1 = fmaf(ws[e], at_f<T>(r[lane + 64]), o1);
+      const T* r = x + min(j0 + at_pos(i, e), last) * stride;
+      o0 = fmaf(ws[e], at_f<T>(r[c0]), o0);
+      o1 = fmaf(ws[e], at_f<T>(r[c1]), o1);
     }
   }
 }
