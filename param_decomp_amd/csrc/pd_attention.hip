@@ -363,12 +363,12 @@ __device__ inline float at_halves_max(float v) {
 // that row again here from the rows its mask allows alone: the same definition, one row per
 // wave, which is slow. Rows whose NaN or infinity is their own keep the tile's result: their
 // statistics and the rows they see tell, mostly the first one looked at, and a batch that has
-// diverged runs at about its normal speed. Rows of large scores come here too:
-// their weights are formed from differences of scores, where a tile's take c2 s - round(c2 m).
+// diverged runs at about its normal speed. Rows of large scores come here too: their weights
+// are formed from differences of scores, where a tile's take c2 s - round(c2 m).
 
-// Products of y, its signs flipped by `signs`, with rows j0 .. j0 + 31 of an operand (those behind `last` read as
-// row `last`), by the tiles' instructions and in their order, so scores are the tiles' own
-// bits: register i is row j0 + at_pos(i, hh), the same in a half's 32 lanes.
+// Products of y, its signs flipped by `signs`, with rows j0 .. j0 + 31 of an operand (those
+// behind `last` read as row `last`), by the tiles' instructions and in their order, so scores
+// are the tiles' own bits: register i is row j0 + at_pos(i, hh), the same in a half's 32 lanes.
 template <typename T>
 __device__ inline f32x16 at_products(const T* x, int64_t stride, int j0, int last, const T* y, uint32_t signs, int D,
                                      int lane) {
@@ -431,18 +431,24 @@ __device__ __forceinline__ void at_fwd_row(const AttnArgs* a, int h, int row, in
       s[i] = s[i] == -INFINITY ? 0.f : at_exp2((s[i] - mn) * a->c2);
       sum += s[i];
     }
+    const float before = l * al;
     m = mn;
-    l = l * al + (sum + __shfl_xor(sum, 32, 64));
-    o0 *= al, o1 *= al;
+    l = before + (sum + __shfl_xor(sum, 32, 64));
+    // o is the result over the keys so far, so that values up to fp32's end add up to no more
+    const float inv = l == 0.f ? 0.f : 1.f / l, kept = before * inv;
+    o0 *= kept, o1 *= kept;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= inv;
     at_add_rows<T>(v, a->v_row, j0, row, s, D, lane, o0, o1);
   }
+  if (l == 0.f) o0 = o1 = NAN;  // no finite score
   T* o = (T*)a->out + ((int64_t)row * a->H + h) * D;
-  if (lane < D) store_f<T>(o, lane, o0 / l);
-  if (lane + 64 < D) store_f<T>(o, lane + 64, o1 / l);
+  if (lane < D) store_f<T>(o, lane, o0);
+  if (lane + 64 < D) store_f<T>(o, lane + 64, o1);
   if constexpr (sizeof(T) == 2) {
     T* rest = (T*)a->rest + ((int64_t)row * a->H + h) * D;
-    if (a->rest && lane < D) store_f<T>(rest, lane, o0 / l - at_f<T>(o[lane]));
-    if (a->rest && lane + 64 < D) store_f<T>(rest, lane + 64, o1 / l - at_f<T>(o[lane + 64]));
+    if (a->rest && lane < D) store_f<T>(rest, lane, o0 - at_f<T>(o[lane]));
+    if (a->rest && lane + 64 < D) store_f<T>(rest, lane + 64, o1 - at_f<T>(o[lane + 64]));
   }
   if (a->stats && lane == 0) {
     a->stats[(int64_t)h * a->N + row] = m;
@@ -1079,9 +1085,9 @@ __global__ __launch_bounds__(AT_THREADS, 1) void k_attn_fwd_split(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------- backward: queries
-// The row's operands: q and do fragments, its statistics, and D = do . out from the stored out and what
-// rounding took off it (from the rounded out alone, D's error weighs on every key of a row
-// alike and was the largest of dq's), written for the key side.
+// The row's operands: q and do fragments, its statistics, and D = do . out from the stored out
+// and what rounding took off it (from the rounded out alone, D's error weighs on every key of
+// a row alike and was the largest of dq's), written for the key side.
 template <typename T, int DP>
 struct QueryRow {
   typename Op<T>::Frag q[DP / 16], g[DP / 16];

@@ -116,3 +116,15 @@ def test_no_finite_score_is_no_number(device):
     stats = ops.packed_attention_fwd(q, k, v, torch.tensor([0, 40], dtype=torch.int32, device=device),
                                      want_saved=True)[1][0]
     assert not torch.isfinite(stats[..., :3]).all() and torch.isfinite(stats[..., 3:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("N, H, KV, D, lengths", GRIDS)
+def test_values_at_the_end_of_fp32(device, dtype, N, H, KV, D, lengths):
+    """A mean of values stays among them, where their sum or a product with a weight past 1
+    would be infinite."""
+    g = torch.Generator(device=device).manual_seed(9)
+    q, k, v = (torch.randn(N, h, D, device=device, generator=g).round().to(dtype) for h in (H, KV, KV))
+    v = (v.float().clamp(-1, 1) * 2.0**127).to(dtype)
+    off = torch.tensor([0] + torch.tensor(lengths).cumsum(0).tolist(), dtype=torch.int32, device=device)
+    _check_out(packed_attention(q, k, v, off, scale=0.125), q, k, v, lengths, 0.125)
