@@ -744,6 +744,96 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
               int idx_bits, int k, const float* clean_lse, double temperature, const float* row_weight, float* kl,
               void* grad, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- cross entropy over a vocabulary whose logits are never kept ---------------------------
+ * z = act head^T with act [N, d] and head [V, d] in dtype (bf16 with d a multiple of 8, or fp32):
+ *   loss [N] fp32 = logsumexp(z_i) - z_i[target_i], 0 where the target is ignore_index or lies
+ *   outside [0, V): such positions do not count, and nothing that they hold reaches a result.
+ * targets int32 or int64 [N] (target_bits). stats fp32 [N, 2] (nullable), for the backward: a row's
+ * largest logit and its sum of e^(z - that). Products of bf16 operands accumulate in fp32 and
+ * logits are not rounded.
+ * The backward gives d_act [N, d] and d_head [V, d] (in dtype, each nullable) of sum g_i loss_i, g
+ * fp32 [N]: G = g (softmax(z) - 1_target), d_act = G head, d_head = G^T act, going over the vocabulary
+ * in pieces of G of at most 512 MiB. With bf16 G enters both products rounded to bf16. Positions of
+ * g = 0 do not count either. Bit-identical from call to call. N up to 2^21, bf16 tensors below 2 GiB. */
+size_t pd_streamed_ce_fwd_workspace_size(int dtype, int64_t N, int64_t d, int64_t V);
+int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                       const void* targets, int target_bits, int64_t ignore_index, float* loss, float* stats,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t pd_streamed_ce_bwd_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact);
+int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                       const void* targets, int target_bits, int64_t ignore_index, const float* stats, const float* g,
+                       void* d_act, void* d_head, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- AdamW over many tensors ------------------------------------------------------------
+ * One step of AdamW (Loshchilov & Hutter, 2019) on n_tensors fp32 tensors of sizes[i] values,
+ * dense and in place; the arrays are host memory, read during the call. With t = *step + 1,
+ *   m += (1 - beta1) (g - m), v += (1 - beta2) (g^2 - v), g = gradient * *grad_scale
+ *   p -= lr (weight_decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)).
+ * grads[i] is fp32 or bf16 (grad_dtypes[i]); NULL leaves tensor i and its states as they are.
+ * m_scale[i] and v_scale[i] NULL (or the arrays NULL): m[i] and v[i] are fp32. Else they are e4m3
+ * codes (OCP, no infinities) of m and of sqrt(v), with fp32 scales [ceil(sizes[i] / 256)] that 256
+ * consecutive values share (largest finite magnitude / 448); codes are rounded stochastically: up
+ * with the probability of the fraction in 16 bits of threefry2x32(fold_in((k0, k1), t), pair)
+ * for values 2 pair and 2 pair + 1 (a word each, its low half for m, its high half for
+ * sqrt(v)), counted through all tensors, each padded to a multiple of 256. A root above zero
+ * never becomes zero; values that are not finite become NaN codes.
+ * copies[i] (nullable, the array too): bf16 [sizes[i]], receives p. step int32 [1] in device
+ * memory is advanced by one behind the last tensor, and ticket uint32 [1] (device) is zero
+ * between calls, so a captured call goes on counting when it is replayed. lr_dev and grad_scale
+ * (nullable): fp32 [1] in device memory, read when the call runs; lr_dev replaces lr. Calls on
+ * the same tensors, step or ticket must be ordered by the caller. */
+int pd_adamw_step(int n_tensors, const int64_t* sizes, void* const* p, const void* const* grads,
+                  const int32_t* grad_dtypes, void* const* m, void* const* v, void* const* m_scale,
+                  void* const* v_scale, void* const* copies, int32_t* step, uint32_t* ticket, double lr,
+                  const float* lr_dev, const float* grad_scale, double beta1, double beta2, double eps,
+                  double weight_decay, uint32_t k0, uint32_t k1, void* stream);
+
+/* ---- routing by scores ------------------------------------------------------------------
+ * pd_router_topk's choice with scores of other kinds. logits [T, E] in `dtype` (bf16 or fp32),
+ * E up to 1024. s = softmax(logits), or with `sigmoid` 1 / (1 + e^-logits); key = s + bias (fp32
+ * [E], nullable: it has a part in the choice alone). Of n_groups (up to 64) runs of E / n_groups
+ * experts the top_groups best stay, by the sum of the two best keys; top_idx int32 [T, k] are
+ * the k best keys of those (k up to 64), best first. Equal keys go to the lower index; keys are
+ * compared in 64 bits (without bias and groups the logits themselves are). weights fp32 [T, k]
+ * = scale s[top_idx], with `renormalize` over their sum. A logit of -inf masks its expert: it
+ * is chosen behind all others and has weight 0 (all weights are 0 where nothing else is
+ * left); a NaN is chosen first and shows in the weights. The backward gives d_logits
+ * [T, E] in `dtype` from d_weights fp32 [T, k] and the forward's top_idx; the choice itself has no
+ * gradient. */
+int pd_route_scores_fwd(const void* logits, int dtype, int64_t T, int E, int k, int sigmoid, const float* bias,
+                        int n_groups, int top_groups, int renormalize, float scale, float* weights, int32_t* top_idx,
+                        void* stream);
+int pd_route_scores_bwd(const void* logits, int dtype, int64_t T, int E, int k, int sigmoid, int renormalize,
+                        float scale, const int32_t* top_idx, const float* d_weights, void* d_logits, void* stream);
+
+/* ---- norms around a residual branch -------------------------------------------------------
+ * x and stream_out [rows, d] in x_dtype, branch and y [rows, d] in branch_dtype: both bf16, both
+ * fp32, or an fp32 stream with a bf16 branch; d up to 16384. With rms(u) = u / sqrt(mean(u^2) + eps):
+ *   n = post_norm ? rms(branch) post : branch
+ *   stream_out = x + scale gate n,  y = rms(stream_out) pre
+ * post = post_weight + weight_offset (fp32 [d], NULL: 1), pre likewise: an offset of 1 for weights
+ * kept around zero. gate [gate_rows, d] (fp32 or bf16, nullable): row r takes gate row
+ * r / (rows / gate_rows), so 1 row is a gate of channels, one for each of equally long
+ * sequences or each row their own. y norms the stream as it is stored. branch NULL: y = rms(x)
+ * pre, and stream_out is not written (the backward takes x in its place). stats fp32 [rows, 2]
+ * (nullable), for the backward: 1 / sqrt(mean + eps) of branch and stream.
+ * The backward, from d_stream (x_dtype) and d_y (branch_dtype; either NULL: zero): d_x, d_branch,
+ * d_post and d_pre fp32 [d], d_gate [gate_rows, d] in gate_dtype, each nullable and overwritten.
+ * workspace: gate_rows 0 without a gate, want_weights for d_post or d_pre. Fixed-order fp32 sums:
+ * bit-identical from call to call. */
+int pd_residual_norm_fwd(const void* x, int x_dtype, const void* branch, int branch_dtype, int64_t rows, int64_t d,
+                         int post_norm, const float* post_weight, const void* gate, int gate_dtype,
+                         int64_t gate_rows, float scale, const float* pre_weight, float weight_offset, float eps,
+                         void* stream_out, void* y, float* stats, void* stream);
+size_t pd_residual_norm_bwd_workspace_size(int64_t rows, int64_t d, int64_t gate_rows, int want_weights,
+                                           int want_gate);
+int pd_residual_norm_bwd(const void* stream_out, int x_dtype, const void* branch, int branch_dtype, int64_t rows,
+                         int64_t d, int post_norm, const float* post_weight, const void* gate, int gate_dtype,
+                         int64_t gate_rows, float scale, const float* pre_weight, float weight_offset,
+                         const float* stats, const void* d_stream, const void* d_y, void* d_x, void* d_branch,
+                         float* d_post, void* d_gate, float* d_pre, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

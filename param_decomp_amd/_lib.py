@@ -136,6 +136,19 @@ _SIGNATURES = {
     "pd_top_kl_workspace_size": (_c_sz, [_c_i64, _c_i32]),
     "pd_top_kl": (_c_i32, [_c_p, _c_i32, _c_i64, _c_i64, _c_p, _c_i32, _c_p, _c_i32, _c_i32, _c_p, ctypes.c_double] + [_c_p] * 4 +
                   [_c_sz, _c_p]),
+    "pd_streamed_ce_fwd_workspace_size": (_c_sz, [_c_i32] + [_c_i64] * 3),
+    "pd_streamed_ce_fwd": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p] * 3 + [_c_sz, _c_p]),
+    "pd_streamed_ce_bwd_workspace_size": (_c_sz, [_c_i32] + [_c_i64] * 3 + [_c_i32]),
+    "pd_streamed_ce_bwd": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p] * 5 + [_c_sz, _c_p]),
+    "pd_route_scores_fwd": (_c_i32, [_c_p, _c_i32, _c_i64] + [_c_i32] * 3 + [_c_p] + [_c_i32] * 3 + [_c_f32] + [_c_p] * 3),
+    "pd_route_scores_bwd": (_c_i32, [_c_p, _c_i32, _c_i64] + [_c_i32] * 4 + [_c_f32] + [_c_p] * 4),
+    "pd_residual_norm_fwd": (_c_i32, [_c_p, _c_i32] * 2 + [_c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i64, _c_f32, _c_p,
+                                      _c_f32, _c_f32] + [_c_p] * 4),
+    "pd_residual_norm_bwd_workspace_size": (_c_sz, [_c_i64] * 3 + [_c_i32] * 2),
+    "pd_residual_norm_bwd": (_c_i32, [_c_p, _c_i32] * 2 + [_c_i64, _c_i64, _c_i32, _c_p, _c_p, _c_i32, _c_i64, _c_f32, _c_p,
+                                      _c_f32] + [_c_p] * 9 + [_c_sz, _c_p]),
+    "pd_adamw_step": (_c_i32, [_c_i32] + [_c_p] * 11 + [ctypes.c_double] + [_c_p] * 2 + [ctypes.c_double] * 4 +
+                      [_c_u32, _c_u32, _c_p]),
     "pd_faithfulness_workspace_size": (_c_sz, [_c_i64] * 4),
     "pd_faithfulness_fwd": (_c_i32, [_c_i64] * 5 + [_c_p, _c_i32] + [_c_p] * 3 + [_c_f32] + [_c_p] * 4 +
                             [_c_sz, _c_p]),

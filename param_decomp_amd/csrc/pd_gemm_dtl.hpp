@@ -68,7 +68,8 @@ typedef __attribute__((__vector_size__(8 * sizeof(short)))) short bf16x8;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-enum GemmMode { MODE_DENSE = 0, MODE_GROUPED = 1, MODE_GROUPED_K = 2, MODE_BATCHED = 3, MODE_SPLITK = 4 };
+enum GemmMode { MODE_DENSE = 0, MODE_GROUPED = 1, MODE_GROUPED_K = 2, MODE_BATCHED = 3, MODE_SPLITK = 4,
+                MODE_COUNTED = 5, MODE_COUNTED_K = 6 };
 
 struct GemmArgs {
   int64_t M, N, K;
@@ -129,6 +130,18 @@ __device__ inline void dense_tile(int& my, int& nx) {
   const int within = L - g * GROUP * gx;
   my = first + within % gm;
   nx = within / gm;
+}
+
+// dense_tile over gy rows of tiles of which only the device knows how many there are: false for
+// blocks past the last.
+__device__ inline bool counted_tile(int64_t gy, int& my, int& nx) {
+  const int64_t gx = gridDim.x, total = gx * gy, lin = (int64_t)blockIdx.y * gx + blockIdx.x;
+  if (lin >= total) return false;
+  const int64_t L = xcd_contiguous(lin, total), g = L / (8 * gx), first = g * 8;
+  const int64_t gm = gy - first < 8 ? gy - first : 8, within = L - g * 8 * gx;
+  my = (int)(first + within % gm);
+  nx = (int)(within / gm);
+  return true;
 }
 
 // One block's output tile: rows [m0, M) of the block's problem (M is an absolute bound),
@@ -234,6 +247,28 @@ __device__ inline bool map_tile(const GemmArgs& p, int lane, TileJob& t) {
     t.kbeg = (int64_t)blockIdx.z * p.strideA;
     t.kend = t.kbeg + p.strideA < p.K ? t.kbeg + p.strideA : p.K;
     t.C = (TC*)p.C + (int64_t)blockIdx.z * p.strideC;
+  } else if (MODE == MODE_COUNTED) {
+    // the first offsets[0] of M rows (NULL: all), over the contraction slice blockIdx.z as
+    // MODE_SPLITK takes it
+    int my, nx;
+    if (p.offsets) {
+      const int64_t rows = p.offsets[0];
+      if (rows < t.M) t.M = rows;
+    }
+    if (!counted_tile((t.M + BM - 1) / BM, my, nx)) return false;
+    t.m0 = (int64_t)my * BM;
+    t.n0 = (int64_t)nx * BN;
+    t.kbeg = (int64_t)blockIdx.z * p.strideA;
+    t.kend = t.kbeg + p.strideA < p.K ? t.kbeg + p.strideA : p.K;
+    t.C = (TC*)p.C + (int64_t)blockIdx.z * p.strideC;
+  } else if (MODE == MODE_COUNTED_K) {
+    // a dense tile over the first offsets[0] of K
+    int my, nx;
+    dense_tile(my, nx);
+    t.m0 = (int64_t)my * BM;
+    t.n0 = (int64_t)nx * BN;
+    const int64_t k = p.offsets[0];
+    if (k < t.kend) t.kend = k;
   } else if (MODE == MODE_BATCHED) {
     // blockIdx.z = batch; each operand advances by its own stride (0 = shared)
     const int64_t z = blockIdx.z;

@@ -554,3 +554,196 @@ def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, tem
                  L.ptr(clean_lse), temperature, L.ptr(row_weight), L.ptr(kl), L.ptr(grad), L.ptr(ws),
                  ws.numel() if want_kl else 0)
     return kl, grad
+
+
+def route_scores_fwd(logits, k: int, *, sigmoid: bool = False, bias=None, n_groups: int = 1, top_groups: int = 1,
+                     renormalize: bool = True, scale: float = 1.0):
+    """(weights fp32 [T, k], top_idx int32 [T, k]) of logits [T, E], see `routed.experts.route_scores`."""
+    name = "route_scores_fwd"
+    T, E = _route_checks(name, logits, k, scale)
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise L.PDError(f"{name}: bias is float32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+    if not 1 <= n_groups <= 64 or E % n_groups or not 1 <= top_groups <= n_groups or k > E // n_groups * top_groups:
+        raise L.PDError(f"{name}: {top_groups} of {n_groups} equal groups (64 at most) of {E} experts have to hold {k}")
+    device = _one_device(name, logits, "bias", bias)
+    w = torch.empty((T, k), dtype=torch.float32, device=device)
+    idx = torch.empty((T, k), dtype=torch.int32, device=device)
+    L.launch("pd_route_scores_fwd", device, L.ptr(logits), L.dtype_code(logits.dtype), T, E, k, int(sigmoid), L.ptr(bias),
+             n_groups, top_groups, int(renormalize), scale, L.ptr(w), L.ptr(idx))
+    return w, idx
+
+
+def route_scores_bwd(logits, top_idx, d_weights, *, sigmoid: bool = False, renormalize: bool = True, scale: float = 1.0):
+    """d_logits from the forward's logits and choice."""
+    name = "route_scores_bwd"
+    k = top_idx.shape[-1] if top_idx.dim() else 0
+    T, E = _route_checks(name, logits, k, scale)
+    if top_idx.dtype != torch.int32 or d_weights.dtype != torch.float32 or tuple(top_idx.shape) != (T, k) or \
+            d_weights.shape != top_idx.shape:
+        raise L.PDError(f"{name}: top_idx int32 and d_weights float32 are [{T}, k], got {top_idx.dtype} "
+                        f"{tuple(top_idx.shape)}, {d_weights.dtype} {tuple(d_weights.shape)}")
+    device = _one_device(name, logits, "top_idx d_weights", top_idx, d_weights)
+    d = torch.empty_like(logits)
+    L.launch("pd_route_scores_bwd", device, L.ptr(logits), L.dtype_code(logits.dtype), T, E, k, int(sigmoid),
+             int(renormalize), scale, L.ptr(top_idx), L.ptr(d_weights), L.ptr(d))
+    return d
+
+
+def _route_checks(name: str, logits, k: int, scale: float) -> tuple[int, int]:
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise L.PDError(f"{name}: logits are float32 or bfloat16 [T, E], got {logits.dtype} {tuple(logits.shape)}")
+    T, E = logits.shape
+    if not 1 <= E <= 1024 or not 1 <= k <= min(E, 64):
+        raise L.PDError(f"{name}: up to 1024 experts and 64 of them chosen, got {k} of {E}")
+    if not math.isfinite(scale):
+        raise L.PDError(f"{name}: scale must be finite, got {scale}")
+    return T, E
+
+
+def _residual_checks(name: str, x, branch, y_dtype, post_norm, post_weight, gate, pre_weight, scale):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
+        raise L.PDError(f"{name}: rows of 1 to 16384 columns, got {tuple(x.shape)}")
+    d = x.shape[-1]
+    if (x.dtype, y_dtype) not in ((torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
+                                  (torch.float32, torch.bfloat16)):
+        raise L.PDError(f"{name}: stream and branch are bfloat16, float32, or a float32 stream with a bfloat16 branch, "
+                        f"got {x.dtype}, {y_dtype}")
+    if branch is not None and branch.shape != x.shape:
+        raise L.PDError(f"{name}: branch is {tuple(branch.shape)}, not {tuple(x.shape)}")
+    for label, t in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (d,)):
+            raise L.PDError(f"{name}: {label} is float32 [{d}], got {t.dtype} {tuple(t.shape)}")
+    if branch is None and (gate is not None or post_weight is not None):
+        raise L.PDError(f"{name}: a gate or post_weight without a branch")
+    if post_weight is not None and not post_norm:
+        raise L.PDError(f"{name}: post_weight without the branch's norm")
+    rows = math.prod(x.shape[:-1])
+    gate_rows = 0
+    if gate is not None:
+        gate_rows = math.prod(gate.shape[:-1]) if gate.dim() else 0
+        if gate.dtype not in (torch.float32, torch.bfloat16) or gate.dim() < 1 or gate.shape[-1] != d or \
+                gate_rows < 1 and rows or gate_rows and rows % gate_rows:
+            raise L.PDError(f"{name}: gate is float32 or bfloat16 [..., {d}] whose rows divide the {rows} rows, got "
+                            f"{gate.dtype} {tuple(gate.shape)}")
+    if not math.isfinite(scale):
+        raise L.PDError(f"{name}: scale must be finite, got {scale}")
+    return rows, d, gate_rows
+
+
+def residual_norm_fwd(x, branch=None, *, post_norm: bool = True, post_weight=None, gate=None, pre_weight=None,
+                      scale: float = 1.0, weight_offset: float = 0.0, eps: float = 1e-6, y_dtype=None,
+                      want_stats: bool = False):
+    """(stream, y, stats), see `norms.residual_norm`; stats fp32 [rows, 2] for the backward, None
+    unless wanted. Without a branch stream is x itself and y its norm."""
+    name = "residual_norm_fwd"
+    y_dtype = branch.dtype if branch is not None else y_dtype or x.dtype
+    post_norm = post_norm and branch is not None
+    rows, d, gate_rows = _residual_checks(name, x, branch, y_dtype, post_norm, post_weight, gate, pre_weight, scale)
+    device = _one_device(name, x, "branch post_weight gate pre_weight", branch, post_weight, gate, pre_weight)
+    h = x if branch is None else torch.empty_like(x)
+    y = torch.empty(x.shape, dtype=y_dtype, device=device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=device) if want_stats else None
+    L.launch("pd_residual_norm_fwd", device, L.ptr(x), L.dtype_code(x.dtype), L.ptr(branch), L.dtype_code(y_dtype), rows, d,
+             int(post_norm), L.ptr(post_weight), L.ptr(gate), L.dtype_code(gate.dtype) if gate is not None else 0, gate_rows,
+             scale, L.ptr(pre_weight), weight_offset, eps, None if branch is None else L.ptr(h), L.ptr(y), L.ptr(stats))
+    return h, y, stats
+
+
+def residual_norm_bwd(stream, branch, stats, d_stream, d_y, *, post_norm: bool = True, post_weight=None, gate=None,
+                      pre_weight=None, scale: float = 1.0, weight_offset: float = 0.0, y_dtype=None, want_dx: bool = True,
+                      want_dbranch: bool = True, want_dpost: bool = True, want_dgate: bool = True, want_dpre: bool = True):
+    """(dx, dbranch, dpost, dgate, dpre) from the forward's stream, branch and stats; None for those
+    not wanted. d_stream or d_y None: zero."""
+    name = "residual_norm_bwd"
+    x = stream
+    y_dtype = branch.dtype if branch is not None else y_dtype or x.dtype
+    post_norm = post_norm and branch is not None
+    rows, d, gate_rows = _residual_checks(name, x, branch, y_dtype, post_norm, post_weight, gate, pre_weight, scale)
+    for label, t, dt in (("d_stream", d_stream, x.dtype), ("d_y", d_y, y_dtype)):
+        if t is not None and (t.shape != x.shape or t.dtype != dt):
+            raise L.PDError(f"{name}: {label} is {tuple(t.shape)} {t.dtype}, not {tuple(x.shape)} {dt}")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 2):
+        raise L.PDError(f"{name}: stats is the forward's, float32 [rows, 2]")
+    device = _one_device(name, x, "branch stats d_stream d_y post_weight gate pre_weight", branch, stats, d_stream, d_y,
+                         post_weight, gate, pre_weight)
+    dx = torch.empty_like(x) if want_dx else None
+    db = torch.empty_like(branch) if want_dbranch and branch is not None else None
+    # sums over no rows are zero; the entry point writes those of the weights itself
+    dg = (torch.zeros_like if not rows else torch.empty_like)(gate) if want_dgate and gate is not None else None
+    dpost = torch.empty(d, dtype=torch.float32, device=device) if want_dpost and post_norm else None
+    dpre = torch.empty(d, dtype=torch.float32, device=device) if want_dpre else None
+    params = dpost is not None or dpre is not None
+    nbytes = L.load().pd_residual_norm_bwd_workspace_size(rows, d, gate_rows, int(params), int(dg is not None))
+    ws = L.workspace(nbytes, device) if nbytes else None
+    L.launch("pd_residual_norm_bwd", device, L.ptr(x), L.dtype_code(x.dtype), L.ptr(branch), L.dtype_code(y_dtype), rows, d,
+             int(post_norm), L.ptr(post_weight), L.ptr(gate), L.dtype_code(gate.dtype) if gate is not None else 0, gate_rows,
+             scale, L.ptr(pre_weight), weight_offset, L.ptr(stats), L.ptr(d_stream), L.ptr(d_y), L.ptr(dx), L.ptr(db),
+             L.ptr(dpost), L.ptr(dg), L.ptr(dpre), L.ptr(ws), ws.numel() if nbytes else 0)
+    return dx, db, dpost, dg, dpre
+
+
+def _ce_checks(name: str, act, head, targets):
+    if act.dim() != 2 or head.dim() != 2 or act.shape[1] != head.shape[1] or targets.shape != act.shape[:1]:
+        raise L.PDError(f"{name}: act [N, d], head [V, d] and targets [N], got {tuple(act.shape)}, {tuple(head.shape)}, "
+                        f"{tuple(targets.shape)}")
+    if act.dtype not in (torch.float32, torch.bfloat16) or head.dtype != act.dtype:
+        raise L.PDError(f"{name}: act and head share one dtype, float32 or bfloat16, got {act.dtype}, {head.dtype}")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise L.PDError(f"{name}: targets are int32 or int64, got {targets.dtype}")
+    if head.shape[0] < 1 or head.shape[1] < 1 or (act.dtype == torch.bfloat16 and head.shape[1] % 8):
+        raise L.PDError(f"{name}: V >= 1 and d >= 1 (bfloat16: a multiple of 8), got head {tuple(head.shape)}")
+    device = _one_device(name, act, "head targets", head, targets)
+    N, d = act.shape
+    return device, [L.dtype_code(act.dtype), N, d, head.shape[0]]
+
+
+def _ce_args(act, head, targets, ignore_index: int) -> list:
+    return [L.ptr(act), L.ptr(head), L.ptr(targets), 8 * targets.element_size(), int(ignore_index)]
+
+
+def streamed_cross_entropy_fwd(act, head, targets, *, ignore_index: int = -100, want_stats: bool = False):
+    """(loss fp32 [N], stats) of act [N, d] @ head[V, d]^T against targets [N]; stats fp32 [N, 2] for the
+    backward, None unless wanted (see `losses.streamed_position_cross_entropy`)."""
+    name = "streamed_cross_entropy_fwd"
+    device, sizes = _ce_checks(name, act, head, targets)
+    loss = torch.empty(act.shape[0], dtype=torch.float32, device=device)
+    stats = torch.empty((act.shape[0], 2), dtype=torch.float32, device=device) if want_stats else None
+    ws = L.workspace(L.load().pd_streamed_ce_fwd_workspace_size(*sizes), device)
+    L.launch("pd_streamed_ce_fwd", device, *sizes, *_ce_args(act, head, targets, ignore_index), L.ptr(loss), L.ptr(stats),
+             L.ptr(ws), ws.numel())
+    return loss, stats
+
+
+def streamed_cross_entropy_bwd(act, head, targets, stats, g, *, ignore_index: int = -100, want_dact: bool = True,
+                               want_dhead: bool = True):
+    """(d_act, d_head) of sum g_i loss_i from the forward's stats, g fp32 [N]; None for those not wanted."""
+    name = "streamed_cross_entropy_bwd"
+    device, sizes = _ce_checks(name, act, head, targets)
+    N = act.shape[0]
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (N, 2) or g.dtype != torch.float32 or tuple(g.shape) != (N,):
+        raise L.PDError(f"{name}: stats float32 [{N}, 2] and g float32 [{N}], got {stats.dtype} {tuple(stats.shape)}, "
+                        f"{g.dtype} {tuple(g.shape)}")
+    _one_device(name, act, "stats g", stats, g)
+    if not N:
+        return torch.empty_like(act) if want_dact else None, torch.zeros_like(head) if want_dhead else None
+    da = torch.empty_like(act) if want_dact else None
+    dh = torch.empty_like(head) if want_dhead else None
+    if want_dact or want_dhead:
+        ws = L.workspace(L.load().pd_streamed_ce_bwd_workspace_size(*sizes, int(want_dact)), device)
+        L.launch("pd_streamed_ce_bwd", device, *sizes, *_ce_args(act, head, targets, ignore_index), L.ptr(stats), L.ptr(g),
+                 L.ptr(da), L.ptr(dh), L.ptr(ws), ws.numel())
+    return da, dh
+
+
+def streamed_cross_entropy(act, head, targets, *, ignore_index: int = -100, row_weight=None, want_dact: bool = False,
+                           want_dhead: bool = False):
+    """(loss, d_act, d_head): per-position cross entropy (see `losses.streamed_position_cross_entropy`) and
+    row_weight (fp32 [N]; None: 1) times its gradients; None for those not wanted."""
+    want = want_dact or want_dhead
+    if row_weight is None and want:
+        row_weight = torch.ones(act.shape[:1], dtype=torch.float32, device=act.device)
+    loss, stats = streamed_cross_entropy_fwd(act, head, targets, ignore_index=ignore_index, want_stats=want)
+    if not want:
+        return loss, None, None
+    return (loss, *streamed_cross_entropy_bwd(act, head, targets, stats, row_weight, ignore_index=ignore_index,
+                                              want_dact=want_dact, want_dhead=want_dhead))

@@ -15,7 +15,9 @@ from dataclasses import dataclass
 from typing import Literal
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from param_decomp_amd import _lib as L
 from param_decomp_amd import ops
 
 GroupedMatmulBackend = Literal["hip"]
@@ -152,3 +154,42 @@ def route_tokens(logits: torch.Tensor, k: int):
     renormalized mixing weights (`pd/targets/qwen36_moe.py:473-514`). Returns
     (probs [T,E], top_idx [T,k] int32, weights [T,k] fp32)."""
     return ops.router_topk(logits.float().contiguous(), k)
+
+
+class _RouteScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, k, opts, groups):
+        w, idx = ops.route_scores_fwd(logits, k, bias=bias, **opts, **groups)
+        ctx.save_for_backward(logits, idx)
+        ctx.opts = opts
+        ctx.mark_non_differentiable(idx)
+        return w, idx
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        logits, idx = ctx.saved_tensors
+        return ops.route_scores_bwd(logits, idx, g.contiguous(), **ctx.opts), None, None, None, None
+
+
+def route_scores(logits: torch.Tensor, k: int, *, scoring: Literal["softmax", "sigmoid"] = "softmax",
+                 bias: torch.Tensor | None = None, n_groups: int = 1, top_groups: int | None = None,
+                 renormalize: bool = True, scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """`route_tokens` for routers that score otherwise: (weights fp32 [T, k], top_idx int32 [T, k])
+    of logits [T, E] (bf16 or fp32, E up to 1024, k up to 64), for `routed_jobs` and `combine_jobs`.
+
+    Scores are the softmax of a row or the sigmoid of each logit. `bias` fp32 [E] is added for the
+    choice alone (a balance that is kept beside training), `n_groups` runs of experts are cut to the
+    `top_groups` whose two best keys sum highest (None: all), and the k best keys of those are
+    chosen, best first, equal ones by the lower index. weights = scale * scores of the chosen, over
+    their sum with `renormalize`. A logit of -inf masks its expert. Keys are compared in 64 bits;
+    differentiable in the logits through the weights, once; the choice and `bias` have no gradient."""
+    if scoring not in ("softmax", "sigmoid"):
+        raise L.PDError(f"route_scores: scoring is softmax or sigmoid, got {scoring!r}")
+    logits = logits.contiguous()
+    bias = None if bias is None else bias.detach().contiguous()
+    opts = dict(sigmoid=scoring == "sigmoid", renormalize=bool(renormalize), scale=float(scale))
+    groups = dict(n_groups=int(n_groups), top_groups=int(n_groups if top_groups is None else top_groups))
+    if ops.differentiated(logits):
+        return _RouteScores.apply(logits, bias, int(k), opts, groups)
+    return ops.route_scores_fwd(logits, int(k), bias=bias, **opts, **groups)
