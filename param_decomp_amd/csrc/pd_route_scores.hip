@@ -78,8 +78,14 @@ __device__ inline uint32_t rt_fold(uint32_t v, F&& f) {
   v = f(v, rt_dpp<0x4E>(v));   // 2, 3, 0, 1
   v = f(v, rt_dpp<0x141>(v));  // the other quad of 8 lanes
   if constexpr (NT > 8) v = f(v, rt_dpp<0x140>(v));  // the other 8 of 16
-  if constexpr (NT > 16) v = f(v, (uint32_t)__shfl_xor((int)v, 16, 64));
-  if constexpr (NT > 32) v = f(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+  if constexpr (NT > 16) {  // each 16 lanes beside the next 16, then each 32
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(p[0], p[1]);
+  }
+  if constexpr (NT > 32) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = f(p[0], p[1]);
+  }
   return v;
 }
 template <int NT>
@@ -192,10 +198,13 @@ __device__ inline uint64_t rt_groups(const RtArgs& a, const D (&key)[J], D* lds,
   return ((uint64_t)hi << 32) | lo;
 }
 
-// The choice from 64-bit scores: idx into sel.
+// The choice from 64-bit scores of the row's logits xs (in LDS): indices into won[r].y.
 template <int NT, int J>
-__device__ __noinline__ void rt_choose_wide(const RtArgs& a, const float (&x)[J], int lane, double* lds, int32_t* sel) {
+__device__ __noinline__ void rt_choose_wide(const RtArgs& a, const float* xs, int lane, double* lds, uint2* won) {
   double key[J];
+  float x[J];
+#pragma unroll
+  for (int j = 0; j < J; ++j) x[j] = xs[lane * J + j];
   const bool raw = !a.bias && a.groups == 1;
   if (!raw && !a.sigmoid) {
     float m = -INFINITY;
@@ -241,39 +250,132 @@ __device__ __noinline__ void rt_choose_wide(const RtArgs& a, const float (&x)[J]
       if (o != 0x7FFFFFFF && (at == 0x7FFFFFFF || v > best || (v == best && o < at))) best = v, at = o;
     }
     if (at / J == lane) gone |= 1u << (at % J);
-    if (lane == 0) sel[r] = at;
+    if (lane == 0) won[r].y = (uint32_t)at;
   }
 }
 
+// The order of n candidates won[i] (words and their lanes' first experts) by 64-bit scores: the k
+// best of them into won[r].y. Each lane ranks its candidates against all.
+template <int NT, int J>
+__device__ __noinline__ void rt_rank_wide(const RtArgs& a, const float* xs, int lane, int n, double* lds, uint2* won) {
+  double m = 0.0, total = 1.0;
+  const bool raw = !a.bias && a.groups == 1;
+  if (a.bias && !a.sigmoid) {
+    float top = -INFINITY;
+    for (int j = 0; j < J; ++j) top = fmaxf(top, xs[lane * J + j]);
+    m = (double)rt_max<NT>(top);
+    total = 0.0;
+    for (int j = 0; j < J; ++j) total += exp((double)xs[lane * J + j] - m);
+    total = rt_add_d<NT>(total);
+  }
+  int32_t* order = (int32_t*)(lds + RT_MAX_K);
+  for (int i = lane; i < n; i += NT) {
+    const int e = (int)(won[i].y + (J - 1 - (won[i].x & (J - 1))));
+    const double v = (double)xs[e];
+    // without a bias the logits are in the scores' order
+    double key = raw || !a.bias ? v : a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - m) / total;
+    if (a.bias) key += (double)a.bias[e];
+    lds[i] = key;
+    won[i].y = (uint32_t)e;
+  }
+  rt_wave_sync();
+  for (int i = lane; i < n; i += NT) {
+    const double mine = lds[i];
+    const uint32_t e = won[i].y;
+    int rank = 0;
+    for (int o = 0; o < n; ++o) {
+      const double other = lds[o];
+      rank += other > mine || (other == mine && won[o].y < e);
+    }
+    order[rank] = (int32_t)e;
+  }
+  rt_wave_sync();
+  for (int r = lane; r < a.k; r += NT) won[r].y = (uint32_t)order[r];
+}
+
+__device__ inline void rt_swap(uint32_t& a, uint32_t& b) {  // the larger first
+  const uint32_t hi = a > b ? a : b, lo = a > b ? b : a;
+  a = hi, b = lo;
+}
+// A lane's words in falling order (Batcher's odd-even merge network).
+template <int J>
+__device__ inline void rt_sort(uint32_t (&v)[J]) {
+#pragma unroll
+  for (int p = 1; p < J; p *= 2)
+#pragma unroll
+    for (int k = p; k > 0; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < J; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < J && (i + j) / (2 * p) == (i + j + k) / (2 * p)) rt_swap(v[i + j], v[i + j + k]);
+}
+
+// Whether the lane's group stays, where each lane's experts are of one group and a group has a
+// power of two of lanes: the two best keys are merged over its lanes.
+template <int NT, int J>
+__device__ inline bool rt_lane_group(const RtArgs& a, const float (&key)[J], float* lds, int lane, float& low, float& high) {
+  const int lanes = a.E / a.groups / J, mine = lane / lanes;
+  float b1 = key[0], b2 = -INFINITY;
+#pragma unroll
+  for (int j = 1; j < J; ++j) {
+    b2 = fmaxf(b2, fminf(b1, key[j]));
+    b1 = fmaxf(b1, key[j]);
+  }
+  for (int off = 1; off < lanes; off *= 2) {
+    const float o1 = __shfl_xor(b1, off, 64), o2 = __shfl_xor(b2, off, 64);
+    b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+    b1 = fmaxf(b1, o1);
+  }
+  const float score = b2 > -INFINITY ? b1 + b2 : b1;
+  const bool in = mine < a.groups;
+  if (in) lds[mine] = score;
+  rt_wave_sync();
+  int rank = 0;
+  for (int o = 0; o < a.groups; ++o) {
+    const float other = lds[o];
+    rank += other > score || (other == score && o < mine);
+  }
+  rt_wave_sync();
+  const bool stays = in && rank < a.top_groups;
+  low = -rt_max<NT>(stays ? -score : -INFINITY);
+  high = rt_max<NT>(in && !stays ? score : -INFINITY);
+  return stays;
+}
+
 template <typename T, int NT, int J>
-__global__ __launch_bounds__(256) void k_rt_fwd(RtArgs a) {
-  constexpr int TEAMS = 256 / NT, SEL = RT_MAX_K + 1;
+__global__ __launch_bounds__(256, J > 8 ? 4 : 8) void k_rt_fwd(RtArgs a) {
+  constexpr int TEAMS = 256 / NT, SPAN = NT * J < RT_MAX_GROUPS ? RT_MAX_GROUPS : NT * J;
   constexpr uint32_t LOW = J - 1;
-  __shared__ double wide[TEAMS][NT * J < RT_MAX_GROUPS ? RT_MAX_GROUPS : NT * J];
-  __shared__ int32_t sels[TEAMS][SEL];
-  __shared__ uint32_t tops[TEAMS][SEL];
+  constexpr bool WHOLE = sizeof(T) == 2;  // whether a word without bias and groups holds the index
+  __shared__ float rows[TEAMS][SPAN];
+  __shared__ double wides[4][SPAN + RT_MAX_K / 2];        // one a wave: its teams take the second look in turn
+  __shared__ uint2 wons[TEAMS][RT_MAX_K];  // words chosen and their lanes' first expert
   const int lane = threadIdx.x % NT, team = threadIdx.x / NT;
   const int64_t row = (int64_t)blockIdx.x * TEAMS + team;
   if (row >= a.T) return;  // whole teams; nothing below waits for the block
   const T* xr = (const T*)a.x + row * a.E;
-  int32_t* sel = sels[team];
-  uint32_t* top = tops[team];
   const int e0 = lane * J;
+  float* xs = rows[team];
+  uint2* won = wons[team];
   float x[J];
   rt_load<T, J>(xr, e0, a.E, x);
   const bool raw = !a.bias && a.groups == 1;
   bool again = false;
   uint32_t key[J];
-  float smax = 1.f, m = -INFINITY, total = 1.f;
+  float smax = 1.f, m = -INFINITY, total = 0.f;
   if (!a.sigmoid) {
 #pragma unroll
     for (int j = 0; j < J; ++j) m = fmaxf(m, x[j]);
     m = rt_max<NT>(m);
+#pragma unroll
+    for (int j = 0; j < J; ++j) total += __expf(x[j] - m);
+    total = rt_add<NT>(total);
   }
   if (raw) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if constexpr (sizeof(T) == 2) {
+      if constexpr (WHOLE) {
         const uint32_t u = x[j] != x[j] ? 0xFFFF0000u : rt_order(x[j]) & 0xFFFF0000u;
         key[j] = u | (uint32_t)(0xFFFF - (e0 + j));
       } else {
@@ -287,13 +389,9 @@ __global__ __launch_bounds__(256) void k_rt_fwd(RtArgs a) {
 #pragma unroll
       for (int j = 0; j < J; ++j) s[j] = __builtin_amdgcn_rcpf(1.f + __expf(-x[j]));
     } else {
-      float t = 0.f;
+      smax = 1.f / total;
 #pragma unroll
-      for (int j = 0; j < J; ++j) t += s[j] = __expf(x[j] - m);
-      t = rt_add<NT>(t);
-      smax = 1.f / t;
-#pragma unroll
-      for (int j = 0; j < J; ++j) s[j] *= smax;
+      for (int j = 0; j < J; ++j) s[j] = __expf(x[j] - m) * smax;
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -301,99 +399,166 @@ __global__ __launch_bounds__(256) void k_rt_fwd(RtArgs a) {
       again |= !(fabsf(s[j]) < INFINITY);
       if (x[j] == -INFINITY) s[j] = -INFINITY;
     }
-    uint64_t stay = ~0ull;
+    const int size = a.E / a.groups;
+    uint32_t stay = ~0u;  // bits of the lane's experts
     if (a.groups > 1) {
       float low, high;
-      stay = rt_groups<NT, J, float>(a, s, (float*)wide[team], lane, low, high);
+      const int lanes = size / J;
+      if (size % J == 0 && (lanes & (lanes - 1)) == 0) {
+        stay = rt_lane_group<NT, J>(a, s, xs, lane, low, high) ? ~0u : 0u;
+      } else {
+        const uint64_t groups = rt_groups<NT, J, float>(a, s, xs, lane, low, high);
+        stay = 0u;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (e0 + j < a.E) stay |= (uint32_t)((groups >> ((e0 + j) / size)) & 1) << j;
+      }
       again |= high > -INFINITY && !(low - high > 3e-6f * smax + 5e-7f * fmaxf(fabsf(low), fabsf(high)));
     }
-    const int size = a.E / a.groups;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       key[j] = s[j] == -INFINITY ? LOW + 1u : rt_order(s[j]);
-      key[j] = (key[j] & ~LOW) | (LOW - j);
-      if (a.groups > 1 && e0 + j < a.E && !((stay >> ((e0 + j) / size)) & 1)) key[j] = 0u;
+      key[j] = (stay >> j) & 1 ? (key[j] & ~LOW) | (LOW - j) : 0u;
     }
   }
 #pragma unroll
   for (int j = 0; j < J; ++j)
     if (e0 + j >= a.E) key[j] = 0u;
-  uint32_t won = 0;
-  for (int r = 0; r <= a.k; ++r) {
-    uint32_t best = key[0];
+  rt_sort<J>(key);
+  uint32_t wins = 0;
+  for (int r = 0; r < a.k; ++r) {
+    const uint32_t M = rt_max_u<NT>(key[0]);
+    if (key[0] == M) {
+      won[r] = make_uint2(M, (uint32_t)e0);
+      ++wins;
 #pragma unroll
-    for (int j = 1; j < J; ++j) best = key[j] > best ? key[j] : best;
-    const uint32_t M = rt_max_u<NT>(best);
-    if (lane == 0) top[r] = M;
-    if (best == M && r < a.k) {
-      ++won;
-      int at = e0;
-#pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (key[j] == M) key[j] = 0u, at = e0 + j;
-      sel[r] = at;
+      for (int j = 0; j + 1 < J; ++j) key[j] = key[j + 1];
+      key[J - 1] = 0u;
     }
   }
+  uint32_t rest = rt_max_u<NT>(key[0]);
+#pragma unroll
+  for (int j = 0; j < J; ++j) xs[e0 + j] = x[j];  // the row's logits beside the choice
   rt_wave_sync();
-  if (!(raw && sizeof(T) == 2)) {
-    again |= rt_add_u<NT>(won) != (uint32_t)a.k;
-    for (int r = lane; r < a.k; r += NT) {
-      const uint32_t hi = top[r], lo = top[r + 1];
-      if (raw) {
-        again |= (hi & ~LOW) == (lo & ~LOW);
-      } else if (lo) {
-        const float f = rt_unorder(hi & ~LOW), g = rt_unorder(lo & ~LOW);
-        again |= !(f - g > 1.5e-6f * smax + (J * 1.2e-7f + 5e-7f) * fmaxf(fabsf(f), fabsf(g)));
+  bool ranked = false;  // whether won[r].y is the choice itself
+  if (!(raw && WHOLE)) {
+    // whether 64 bits may order two words the other way round
+    auto close = [&](uint32_t hi, uint32_t lo) {
+      if (raw) return (hi & ~LOW) == (lo & ~LOW);
+      const float f = rt_unorder(hi & ~LOW), g = rt_unorder(lo & ~LOW);
+      return lo != 0u && !(f - g > 1.5e-6f * smax + (J * 1.2e-7f + 5e-7f) * fmaxf(fabsf(f), fabsf(g)));
+    };
+    // the rest that may belong to the k best joins them
+    int n = a.k;
+    const uint32_t last = won[a.k - 1].x;
+    while (rest && close(last, rest)) {
+      if (n == RT_MAX_K) {
+        again = true;
+        break;
+      }
+      if (key[0] == rest) {
+        won[n] = make_uint2(rest, (uint32_t)e0);
+        ++wins;
+#pragma unroll
+        for (int j = 0; j + 1 < J; ++j) key[j] = key[j + 1];
+        key[J - 1] = 0u;
+      }
+      ++n;
+      rest = rt_max_u<NT>(key[0]);
+    }
+    rt_wave_sync();
+    bool look = n > a.k;
+    for (int r = lane; r + 1 < a.k; r += NT) look |= close(won[r].x, won[r + 1].x);
+    again |= rt_add_u<NT>(wins) != (uint32_t)n;
+    const uint32_t flags = rt_fold<NT>((again ? 2u : 0u) | (look ? 1u : 0u), [](uint32_t p, uint32_t q) { return p | q; });
+    ranked = flags != 0u;
+    if (__ballot(ranked)) {
+      for (int t = 0; t < 64 / NT; ++t) {
+        if (ranked && team % (64 / NT) == t) {
+          if (flags & 2u) rt_choose_wide<NT, J>(a, xs, lane, wides[threadIdx.x >> 6], won);
+          else rt_rank_wide<NT, J>(a, xs, lane, n, wides[threadIdx.x >> 6], won);
+        }
+        rt_wave_sync();
       }
     }
-    if (rt_add_u<NT>(again ? 1u : 0u)) {
-      rt_wave_sync();
-      rt_choose_wide<NT, J>(a, x, lane, wide[team], sel);
-      rt_wave_sync();
-    }
   }
-  // weights of the chosen, NT at a time
-  if (!a.sigmoid && !a.renorm) {
-    float t = 0.f;
-#pragma unroll
-    for (int j = 0; j < J; ++j) t += expf(x[j] - m);
-    total = rt_add<NT>(t);
-  }
-  float lmax = -INFINITY, sum = 0.f;
+  auto chosen = [&](int r) {
+    const uint2 w = won[r];
+    return ranked ? (int)w.y : raw && WHOLE ? (int)(0xFFFFu - (w.x & 0xFFFFu)) : (int)(w.y + (LOW - (w.x & LOW)));
+  };
+  float* wout = a.w + row * a.k;
+  int32_t* iout = a.idx + row * a.k;
   uint32_t live = 0;  // whether one is not masked
-  if (!a.renorm) {
+  if (a.sigmoid) {
+    float sum = 0.f;
+    for (int r = lane; r < a.k; r += NT) {
+      const int e = chosen(r);
+      const float s = 1.f / (1.f + expf(-xs[e]));
+      won[r] = make_uint2(__float_as_uint(s), (uint32_t)e);
+      sum += s;
+    }
+    float by = a.scale;
+    if (a.renorm) {
+      sum = rt_add<NT>(sum);
+      if (sum < 0x1p-60f) {  // the same for the team: scores that may have left fp32, by their logarithms
+        float lmax = -INFINITY, total = 0.f;
+        for (int r = lane; r < a.k; r += NT) {
+          const float v = xs[won[r].y], l = fminf(v, 0.f) - log1pf(expf(-fabsf(v)));
+          won[r].x = __float_as_uint(l);
+          live |= v != -INFINITY;
+          lmax = fmaxf(lmax, l);
+        }
+        lmax = rt_max<NT>(lmax);
+        for (int r = lane; r < a.k; r += NT) {
+          const float e = expf(__uint_as_float(won[r].x) - lmax);
+          won[r].x = __float_as_uint(e);
+          total += e;
+        }
+        total = rt_add<NT>(total);
+        if (!rt_fold<NT>(live, [](uint32_t p, uint32_t q) { return p | q; })) {  // all are masked
+          for (int r = lane; r < a.k; r += NT) won[r].x = 0u;
+          total = 1.f;
+        }
+        sum = total;
+      }
+      by /= sum;
+    }
+    for (int r = lane; r < a.k; r += NT) {
+      wout[r] = __uint_as_float(won[r].x) * by;
+      iout[r] = (int32_t)won[r].y;
+    }
+    return;
+  }
+  if (a.renorm) {  // over the chosen: from the largest of them on
+    m = -INFINITY;
+    for (int r = lane; r < a.k; r += NT) {
+      const int e = chosen(r);
+      const float v = xs[e];
+      won[r] = make_uint2(__float_as_uint(v), (uint32_t)e);
+      live |= v != -INFINITY;
+      m = fmaxf(m, v);
+    }
+    m = rt_max<NT>(m);
+    total = 0.f;
+    for (int r = lane; r < a.k; r += NT) {
+      const float e = expf(__uint_as_float(won[r].x) - m);
+      won[r].x = __float_as_uint(e);
+      total += e;
+    }
+    total = rt_add<NT>(total);
+  } else {
 #pragma unroll
     for (int j = 0; j < J; ++j) live |= x[j] != -INFINITY;
-  } else {
     for (int r = lane; r < a.k; r += NT) {
-      const float v = load_f<T>(xr, sel[r]);
-      live |= v != -INFINITY;
-      const float l = a.sigmoid ? fminf(v, 0.f) - log1pf(expf(-fabsf(v))) : v;
-      lmax = fmaxf(lmax, l);
+      const int e = chosen(r);
+      won[r] = make_uint2(__float_as_uint(expf(xs[e] - m)), (uint32_t)e);
     }
-    lmax = rt_max<NT>(lmax);
-    for (int r = lane; r < a.k; r += NT) {
-      const float v = load_f<T>(xr, sel[r]);
-      const float l = a.sigmoid ? fminf(v, 0.f) - log1pf(expf(-fabsf(v))) : v;
-      sum += expf(l - lmax);
-    }
-    sum = rt_add<NT>(sum);
   }
-  const bool none = !rt_fold<NT>(live, [](uint32_t p, uint32_t q) { return p | q; });
+  const bool none = !rt_fold<NT>(live, [](uint32_t p, uint32_t q) { return p | q; });  // all are masked
+  const float by = a.scale / total;
   for (int r = lane; r < a.k; r += NT) {
-    const int e = sel[r];
-    const float v = load_f<T>(xr, e);
-    float w;
-    if (a.renorm) {
-      const float l = a.sigmoid ? fminf(v, 0.f) - log1pf(expf(-fabsf(v))) : v;
-      w = none ? 0.f : expf(l - lmax) / sum;
-    } else if (a.sigmoid) {
-      w = 1.f / (1.f + expf(-v));
-    } else {
-      w = none ? 0.f : expf(v - m) / total;
-    }
-    a.w[row * a.k + r] = w * a.scale;
-    a.idx[row * a.k + r] = e;
+    wout[r] = none ? 0.f : __uint_as_float(won[r].x) * by;
+    iout[r] = (int32_t)won[r].y;
   }
 }
 

@@ -25,7 +25,11 @@
 namespace pd {
 namespace {
 
-constexpr size_t CE_PIECE = (size_t)512 << 20;
+constexpr size_t CE_PIECE = (size_t)1024 << 20;
+// The one-call form keeps a chunk of positions' softmax (16 bits) below this, the end of a product's
+// operands.
+constexpr size_t CE_KEPT = ((size_t)1 << 31) - ((size_t)1 << 22);
+constexpr int CE_SPAN = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct CETargets {
@@ -40,7 +44,7 @@ struct CETargets {
 };
 
 // rows[0 .. count) = the positions that count, in order; pos[i] = position i's place among them or
-// -1. With `loss` those that do not get loss 0 and statistics (0, 1). One block.
+// -1. With `loss` those that do not get loss 0 and, with `stats`, statistics (0, 1). One block.
 __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* __restrict__ g, int64_t N,
                                                      int32_t* __restrict__ rows, int32_t* __restrict__ pos,
                                                      int32_t* __restrict__ count, float* __restrict__ loss,
@@ -67,7 +71,7 @@ __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* _
       if (pos) pos[i] = on ? at : -1;
       if (loss && !on) {
         loss[i] = 0.f;
-        stats[i] = make_float2(0.f, 1.f);
+        if (stats) stats[i] = make_float2(0.f, 1.f);
       }
     }
   }
@@ -93,18 +97,20 @@ __global__ __launch_bounds__(256) void k_ce_gather_f32(const float* __restrict__
     dst[i] = i / d < held ? src[(int64_t)rows[i / d] * d + i % d] : 0.f;
 }
 
-// d_act[i] = the sum over `slabs` of the row of position i, zeros where it does not count.
+// d_act[i] = the sum over `slabs` of the row of position i, of the positions whose place is in
+// [first, first + R); zeros where it does not count.
 template <typename T>
 __global__ __launch_bounds__(256) void k_ce_scatter(const float* __restrict__ part, int slabs, int64_t stride,
                                                     int64_t N, int64_t d, const int32_t* __restrict__ pos,
+                                                    int64_t first, int64_t R,
                                                     T* __restrict__ d_act) {
-  const int64_t q = d / 4;  // bf16: d is a multiple of 8
-  const bool vec = d % 4 == 0;
-  const int64_t total = vec ? N * q : N * d;
+  const bool vec = d % 4 == 0;  // bf16: d is a multiple of 8
+  const int64_t q = vec ? d / 4 : d, total = N * q;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = vec ? i / q : i / d, at = pos[r];
+    const int64_t r = i / q, c = (i - r * q) * (vec ? 4 : 1);
+    const int64_t at = pos[r] < 0 ? -1 : pos[r] - first;
+    if (at < 0 ? pos[r] >= 0 : at >= R) continue;  // another chunk's
     if (vec) {
-      const int64_t c = i % q * 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (at >= 0)
         for (int k = 0; k < slabs; ++k) {
@@ -114,7 +120,6 @@ __global__ __launch_bounds__(256) void k_ce_scatter(const float* __restrict__ pa
       if constexpr (sizeof(T) == 2) *(uint2*)(d_act + r * d + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
       else *(float4*)(d_act + r * d + c) = s;
     } else {
-      const int64_t c = i % d;
       float s = 0.f;
       if (at >= 0)
         for (int k = 0; k < slabs; ++k) s += part[k * stride + at * d + c];
@@ -153,43 +158,54 @@ struct EpiCEStats {
   template <bool FULL>
   __device__ static void run_t(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
                                f32x16 (&z)[CFG::TM][CFG::TN], char* smem) {
-    const int lane = tid & 63, rl = lane & 31;
+    const int lane = tid & 63;
     float2* red = (float2*)smem;  // [WN][BM]
     lds_write_barrier();          // the k loop's stage buffers are free
 #pragma unroll
     for (int i = 0; i < CFG::TM; ++i) {
-      const int64_t row = t.m0 + wm * CFG::WTM + i * 32 + rl;
-      int want = -1;  // the target's place in this lane's columns
-      if (row < t.M) want = a.t.at(a.rows ? a.rows[row] : row);
-      if (want >= 0) want -= (int)t.n0 + wn * CFG::WTN + 4 * (lane >> 5);
-      float m = -INFINITY, s = 0.f;
+      const int rl = wm * CFG::WTM + i * 32 + (lane & 31);
+      float m, s;
+      row_stats<FULL>(p, a, t, t.m0 + rl, t.n0 + wn * CFG::WTN + 4 * (lane >> 5), z[i], m, s);
+      if (lane < 32) red[wn * CFG::BM + rl] = make_float2(m, s);
+    }
+    lds_write_barrier();
+    store(a, t, tid, red);
+  }
+  // A row's maximum and sum over the wave's columns (`first`: the lane's first one); z becomes
+  // e^{z - m}, and the target's logit is kept.
+  template <bool FULL>
+  __device__ static void row_stats(const GemmArgs& p, const Args& a, const TileJob& t, int64_t row, int64_t first,
+                                   f32x16 (&z)[CFG::TN], float& m, float& s) {
+    int want = -1;  // the target's place in this lane's columns
+    if (row < t.M) want = a.t.at(a.rows ? a.rows[row] : row);
+    if (want >= 0) want -= (int)first;
+    m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int j = 0; j < CFG::TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int c = j * 32 + 8 * (v >> 2) + (v & 3);
+        if (FULL || first + c < p.N) {
+          m = fmaxf(m, z[j][v]);
+          if (want == c) a.target[row] = z[j][v];
+        }
+      }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    if (m > -INFINITY) {  // columns there are, and numbers in them
 #pragma unroll
       for (int j = 0; j < CFG::TN; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           const int c = j * 32 + 8 * (v >> 2) + (v & 3);
-          const float x = z[i][j][v];
-          if (FULL || t.n0 + wn * CFG::WTN + 4 * (lane >> 5) + c < p.N) {
-            m = fmaxf(m, x);
-            if (want == c) a.target[row] = x;
-          }
+          z[j][v] = ce_exp(z[j][v] - m);
+          if (FULL || first + c < p.N) s += z[j][v];
         }
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      if (m > -INFINITY) {  // columns there are, and numbers in them
-#pragma unroll
-        for (int j = 0; j < CFG::TN; ++j)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const int c = j * 32 + 8 * (v >> 2) + (v & 3);
-            if (FULL || t.n0 + wn * CFG::WTN + 4 * (lane >> 5) + c < p.N) s += ce_exp(z[i][j][v] - m);
-          }
-      } else if (t.n0 + wn * CFG::WTN < p.N) {
-        s = NAN;  // NaN or -inf throughout: no softmax
-      }
-      s += __shfl_xor(s, 32, 64);
-      if (lane < 32) red[wn * CFG::BM + wm * CFG::WTM + i * 32 + rl] = make_float2(m, s);
+    } else if (FULL || (first & ~(int64_t)7) < p.N) {
+      s = NAN;  // NaN or -inf throughout: no softmax
     }
-    lds_write_barrier();
+    s += __shfl_xor(s, 32, 64);
+  }
+  __device__ static void store(const Args& a, const TileJob& t, int tid, const float2* red) {
     for (int r = tid; r < CFG::BM; r += CFG::NT) {
       if (t.m0 + r >= t.M) continue;
       float2 o = red[r];
@@ -260,11 +276,71 @@ struct EpiCEGrad {
   }
 };
 
+// Epilogue of the one-call form: a row's maximum m and sum over each wave's CE_SPAN columns, and
+// 2^15 e^{z - m} in fp16: 11 bits down to 2^-29 of that maximum, 2^-39 at least. (One maximum for the
+// tile would have all its accumulators wait for the others': 66 of them spilled.)
+template <class CFG>
+struct EpiCEKeep {
+  static constexpr int RSB = CFG::BN * 2 + 16, IMAGE = CFG::BM * RSB;
+  static constexpr int LDS_BYTES = IMAGE + CFG::WN * CFG::BM * 8;
+  struct Args {
+    typename EpiCEStats<CFG>::Args st;
+    uint16_t* E;
+    int64_t ld;
+  };
+  template <class, typename>
+  __device__ static void run(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
+                             f32x16 (&z)[CFG::TM][CFG::TN], char* smem) {
+    if (t.n0 + CFG::BN <= p.N) run_t<true>(p, a, t, wm, wn, tid, z, smem);
+    else run_t<false>(p, a, t, wm, wn, tid, z, smem);
+  }
+  template <bool FULL>
+  __device__ static void run_t(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
+                               f32x16 (&z)[CFG::TM][CFG::TN], char* smem) {
+    const int lane = tid & 63;
+    const int64_t first = t.n0 + wn * CFG::WTN + 4 * (lane >> 5);  // the lane's first column
+    float2* red = (float2*)(smem + IMAGE);                         // [BM][WN]
+    lds_write_barrier();  // the k loop's stage buffers are free
+#pragma unroll
+    for (int i = 0; i < CFG::TM; ++i) {
+      const int rl = wm * CFG::WTM + i * 32 + (lane & 31);
+      float m, s;
+      EpiCEStats<CFG>::template row_stats<FULL>(p, a.st, t, t.m0 + rl, first, z[i], m, s);
+      if (lane < 32) red[rl * CFG::WN + wn] = make_float2(m, s);
+#pragma unroll
+      for (int j = 0; j < CFG::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = j * 32 + 8 * q;
+          uint16_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = FULL || first + c + e < p.N ? __builtin_bit_cast(uint16_t, (_Float16)(z[i][j][4 * q + e] * 32768.f)) : 0;
+          *(uint2*)(smem + rl * RSB + (wn * CFG::WTN + c + 4 * (lane >> 5)) * 2) =
+              make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+        }
+    }
+    lds_write_barrier();
+    static_assert(CFG::WTN == CE_SPAN, "a wave's columns");
+    const int64_t sub = t.n0 / CE_SPAN;
+    for (int i = tid; i < CFG::BM * CFG::WN; i += CFG::NT) {
+      const int r = i / CFG::WN, w = i % CFG::WN;
+      if (t.m0 + r < t.M && sub + w < a.st.n_tiles) a.st.part[(t.m0 + r) * a.st.n_tiles + sub + w] = red[i];
+    }
+    constexpr int CPR = CFG::BN / 8, RPP = CFG::NT / CPR;
+    const int cc = tid % CPR;
+    const int64_t col = t.n0 + cc * 8;
+    for (int r = tid / CPR; r < CFG::BM; r += RPP)
+      if (t.m0 + r < t.M && col < p.N) *(uint4*)(a.E + (t.m0 + r) * a.ld + col) = *(const uint4*)(smem + r * RSB + cc * 16);
+  }
+};
+
 // loss and statistics of the positions that count: one wave a row, the tiles' partials in a fixed order.
 __global__ __launch_bounds__(256) void k_ce_merge(const float2* __restrict__ part, const float* __restrict__ target,
                                                   int64_t N, int64_t n_tiles, const int32_t* __restrict__ rows,
                                                   const int32_t* __restrict__ count, CETargets t,
-                                                  float* __restrict__ loss, float2* __restrict__ stats) {
+                                                  float* __restrict__ loss, float2* __restrict__ stats,
+                                                  float2* __restrict__ row_stats) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (count ? (int64_t)*count : N)) return;
@@ -277,6 +353,63 @@ __global__ __launch_bounds__(256) void k_ce_merge(const float2* __restrict__ par
     const bool on = t.at(r) >= 0;
     loss[r] = on ? (o.x - target[row]) + logf(o.y) : 0.f;
     if (stats) stats[r] = on ? o : make_float2(0.f, 1.f);
+    if (row_stats) row_stats[row] = o;
+  }
+}
+
+// counts[c] = how many of count rows are in chunk c of R.
+__global__ void k_ce_counts(const int32_t* __restrict__ count, int64_t R, int chunks, int32_t* __restrict__ counts) {
+  for (int c = threadIdx.x; c < chunks; c += 64) {
+    const int64_t left = (int64_t)*count - c * R;
+    counts[c] = (int32_t)(left < 0 ? 0 : (left < R ? left : R));
+  }
+}
+// G = g (softmax - 1_t) in bf16 over what EpiCEKeep kept, in place: the values of each CE_SPAN
+// columns times e^{their m - m} g / s. A position of weight zero gets zeros whatever it holds. Blocks: a row, 8192
+// columns of it.
+__global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int64_t ld, const float2* __restrict__ part,
+                                                  int64_t n_tiles, const float2* __restrict__ st,
+                                                  const float* __restrict__ target, const int32_t* __restrict__ rows,
+                                                  const int32_t* __restrict__ count, CETargets t, const float* __restrict__ g) {
+  const int64_t row = blockIdx.x;
+  if (row >= *count) return;
+  const int64_t r = rows[row], want = t.at(r);
+  const float2 o = st[row];
+  const float gr = g[r], by = gr / o.y * 0x1p-15f;
+  // p - 1 at the target from the sum of the others: p may be near 1
+  const float hit = -gr * ((o.y - ce_exp(target[row] - o.x)) / o.y);
+  uint16_t* e = E + row * ld;
+  const int64_t c0 = (int64_t)blockIdx.y * 8192 + threadIdx.x * 8;
+  uint4 w[4];
+  float f[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t c = c0 + k * 2048;
+    if (c >= ld) continue;
+    w[k] = *(const uint4*)(e + c);
+    f[k] = ce_exp(part[row * n_tiles + c / CE_SPAN].x - o.x) * by;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t c = c0 + k * 2048;
+    if (c >= ld) continue;
+    const uint32_t in[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+    uint32_t out[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float lo = (float)__builtin_bit_cast(_Float16, (uint16_t)in[q]) * f[k];
+      float hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(in[q] >> 16)) * f[k];
+      if (c + 2 * q == want) lo = hit;
+      if (c + 2 * q + 1 == want) hi = hit;
+      out[q] = gr == 0.f ? 0u : pack_bf16x2(lo, hi);
+    }
+    *(uint4*)(e + c) = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+__global__ __launch_bounds__(256) void k_ce_round(const float4* __restrict__ src, int64_t n, uint2* __restrict__ dst) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const float4 v = src[i];
+    dst[i] = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   }
 }
 
@@ -385,6 +518,25 @@ struct CEBwdPlan {
   float* part;  // [splits][N][d]
   size_t total;
 };
+// Tiles and slices of the contraction of d_act = G head (N x d over cw columns a piece): its few tiles
+// fill the chip only in slices, each of which leaves an fp32 slab to write and read. The rounds are
+// those of all positions and, with a quarter of the weight, of three quarters of them, since how many
+// count is not known here. us of 1 / 4 / 5 / 7 / 8 slices of 256x256 tiles: 8192 x 768 over 50277 columns 1466 /
+// 772 / 610 / 682 / 616 (128x128: 824 in 1, 724 in 4); 3072 of 4096 x 4096 over 131072 3921 / 3045 /
+// 3168 / 3446 / 3085, all 4096 3901 / 4009 / 4041 / 4089 / 4135.
+void ce_dact_form(int64_t N, int64_t d, int64_t cw, int64_t V, bool& big, int& splits) {
+  double best = 1e30;
+  for (int b = 0; b < 2; ++b)
+    for (int sp = 1; sp <= 64 && (sp == 1 || cw / sp >= 1024); ++sp) {
+      const int64_t t = b ? 256 : 128, round = b ? 256 : 512;
+      auto rounds = [&](int64_t rows) { return (double)tiles_up(tiles_up(rows, t) * tiles_up(d, t) * sp, round); };
+      const double per_round = 2.0 * t * t * round * ((double)V / sp) / (b ? 1.2e15 : 1.0e15);
+      const double slabs = (double)sp * N * d * 4 * 2 * cdiv(V, cw) / 4e12;
+      const double time = (0.75 * rounds(N) + 0.25 * rounds(cdiv(3 * N, 4))) * per_round + slabs;
+      if (time < best) best = time, big = b, splits = sp;
+    }
+}
+
 CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, char* base) {
   CEBwdPlan P{};
   size_t off = 0;
@@ -392,7 +544,6 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   const size_t esz = dtype == PD_DTYPE_BF16 ? 2 : 4;
   P.cw = std::min<int64_t>((V + 7) & ~(int64_t)7, std::max<int64_t>(256, (int64_t)(CE_PIECE / ((size_t)N * esz)) & ~(int64_t)255));
   P.big = ce_big(N, P.cw);
-  P.big_act = big_tiles(N, d, P.cw);
   P.big_head = big_tiles(P.cw, d, N);
   P.count = (int32_t*)take(4);
   P.rows = (int32_t*)take((size_t)N * 4);
@@ -402,19 +553,53 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   P.splits = 1;
   if (dact) {
     if (dtype == PD_DTYPE_BF16) {
-      // the fewest slices of the contraction (each at least 1024 deep) that fill whole rounds to 90%
-      const int64_t t = P.big_act ? 256 : 128, round = P.big_act ? 256 : 512;
-      const int64_t tiles = tiles_up(N, t) * tiles_up(d, t);
-      double best = 0.0;
-      for (int sp = 1; sp <= 8 && (sp == 1 || P.cw / sp >= 1024); ++sp) {
-        const double eff = (double)(tiles * sp) / (double)(tiles_up(tiles * sp, round) * round);
-        if (eff > best + 1e-9) best = eff, P.splits = sp;
-        if (eff >= 0.9) break;
-      }
+      ce_dact_form(N, d, P.cw, V, P.big_act, P.splits);
     }
     P.part = (float*)take((size_t)P.splits * N * d * 4);
   }
   P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
+  P.total = off;
+  return P;
+}
+
+struct CEOnePlan {
+  int64_t R, ld, n_tiles;  // positions of a chunk, E's row, partials of a row
+  int chunks, splits;
+  bool big, big_act, big_head;
+  int64_t slice;
+  int32_t *rows, *pos, *count, *counts;
+  bf16_t *act, *E;
+  float2 *part, *stats;
+  float *target, *slabs, *head;
+  size_t total;
+};
+CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, char* base) {
+  CEOnePlan P{};
+  size_t off = 0;
+  auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
+  P.ld = (V + 7) & ~(int64_t)7;
+  P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * 2)) - 128) & ~(int64_t)255);
+  if (P.R <= 0) P.R = N;
+  P.chunks = (int)cdiv(N, P.R);
+  P.big = ce_big(P.R, V);
+  P.n_tiles = tiles_up(V, CE_SPAN);
+  P.big_head = big_tiles(V, d, P.R);
+  P.count = (int32_t*)take(4);
+  P.counts = (int32_t*)take((size_t)P.chunks * 4);
+  P.rows = (int32_t*)take((size_t)N * 4);
+  P.pos = (int32_t*)take((size_t)N * 4);
+  P.act = (bf16_t*)take((size_t)N * d * 2);
+  P.E = (bf16_t*)take((size_t)P.R * P.ld * 2);
+  P.part = (float2*)take((size_t)P.R * P.n_tiles * 8);
+  P.stats = (float2*)take((size_t)P.R * 8);
+  P.target = (float*)take((size_t)P.R * 4);
+  P.splits = 1;
+  if (dact) {
+    ce_dact_form(P.R, d, V, V, P.big_act, P.splits);
+    P.slabs = (float*)take((size_t)P.splits * P.R * d * 4);
+  }
+  P.slice = tiles_up(tiles_up(V, P.splits), 64) * 64;
+  if (dhead && P.chunks > 1) P.head = (float*)take((size_t)V * d * 4);
   P.total = off;
   return P;
 }
@@ -486,7 +671,7 @@ int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
       ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t},
                                                                                    1, d % 64 != 0, s);
     hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, P.rows,
-                       P.count, t, loss, (float2*)stats);
+                       P.count, t, loss, (float2*)stats, nullptr);
     return check_launch(what);
   }
   for (int64_t c = 0; c < V; c += P.cw) {
@@ -497,7 +682,7 @@ int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
     hipLaunchKernelGGL(k_ce_piece_stats, dim3((unsigned)N), dim3(256), 0, s, P.z, w, P.cw, c, t, P.part, P.target);
   }
   hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, (int64_t)1, nullptr,
-                     nullptr, t, loss, (float2*)stats);
+                     nullptr, t, loss, (float2*)stats, nullptr);
   return check_launch(what);
 }
 
@@ -546,7 +731,7 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
     }
     if (d_act)
       hipLaunchKernelGGL(k_ce_scatter<bf16_t>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 4, 256), 8192)), dim3(256), 0, s,
-                         P.part, P.splits, N * d, N, d, P.pos, (bf16_t*)d_act);
+                         P.part, P.splits, N * d, N, d, P.pos, (int64_t)0, N, (bf16_t*)d_act);
     return check_launch(what);
   }
   float *act_c = (float*)P.act, *G = (float*)P.G;
@@ -567,7 +752,79 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
   }
   if (d_act)
     hipLaunchKernelGGL(k_ce_scatter<float>, dim3((unsigned)std::min<int64_t>(cdiv(N * d, 256), 8192)), dim3(256), 0, s, P.part,
-                       1, N * d, N, d, P.pos, (float*)d_act);
+                       1, N * d, N, d, P.pos, (int64_t)0, N, (float*)d_act);
+  return check_launch(what);
+}
+
+size_t pd_streamed_ce_train_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
+  if (N <= 0 || d <= 0 || V <= 0) return 0;
+  if (dtype == PD_DTYPE_BF16) return ce_one_plan(N, d, V, want_dact, want_dhead, nullptr).total;
+  return up256((size_t)N * 8) + std::max(ce_fwd_plan(dtype, N, d, V, nullptr).total,
+                                         ce_bwd_plan(dtype, N, d, V, want_dact, nullptr).total);
+}
+
+int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                         const void* targets, int target_bits, int64_t ignore_index, const float* g, float* loss,
+                         void* d_act, void* d_head, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "pd_streamed_ce_train";
+  if (int rc = ce_check(what, dtype, N, d, V, act, head, targets, target_bits)) return rc;
+  if (!N || !g || !loss || (!d_act && !d_head)) return fail(PD_EINVAL, std::string(what) + ": positions, g, loss and a gradient required");
+  const size_t need = pd_streamed_ce_train_workspace_size(dtype, N, d, V, d_act != nullptr, d_head != nullptr);
+  if (!workspace || workspace_bytes < need) return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype != PD_DTYPE_BF16) {
+    float* stats = (float*)workspace;
+    char* ws = (char*)workspace + up256((size_t)N * 8);
+    const size_t left = workspace_bytes - up256((size_t)N * 8);
+    if (int rc = pd_streamed_ce_fwd(dtype, N, d, V, act, head, targets, target_bits, ignore_index, loss, stats, ws, left, stream))
+      return rc;
+    return pd_streamed_ce_bwd(dtype, N, d, V, act, head, targets, target_bits, ignore_index, stats, g, d_act, d_head, ws, left,
+                              stream);
+  }
+  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, (char*)workspace);
+  if (!dtl_fits_mn(P.R, P.ld)) return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
+  const CETargets t{targets, target_bits, ignore_index, V};
+  const bf16_t* hd = (const bf16_t*)head;
+  hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, P.pos, P.count, loss, nullptr);
+  hipLaunchKernelGGL(k_ce_gather<false>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 8, 256), 4096)), dim3(256), 0, s,
+                     (const uint4*)act, N, d / 8, P.rows, P.count, (uint4*)P.act);
+  hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
+  for (int c = 0; c < P.chunks; ++c) {
+    const int64_t R = P.R;
+    const int32_t *rows = P.rows + c * R, *count = P.counts + c;
+    const int64_t M = std::min(R, N - c * R);
+    const bf16_t* a_c = P.act + c * R * d;
+    const bool edge = d % 64 != 0;
+    const GemmArgs a{M, V, d, a_c, d, hd, d, nullptr, 0, 1.f, 0.f, count, 0, 0, 0, cdiv(d, 64) * 64, nullptr, nullptr, nullptr};
+    if (P.big)
+      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEKeep<CfgBig>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
+    else
+      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
+    hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
+                       loss, nullptr, P.stats);
+    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(P.ld, 8192)), dim3(256), 0, s, P.E, P.ld, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g);
+    if (d_act) {
+      GemmArgs b{M, d, V, P.E, P.ld, hd, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
+      if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+      hipLaunchKernelGGL(k_ce_scatter<bf16_t>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 4, 256), 8192)), dim3(256), 0, s,
+                         P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (bf16_t*)d_act);
+    }
+    if (d_head) {
+      GemmArgs b{V, d, M, P.E, P.ld, a_c, d, P.chunks > 1 ? (void*)P.head : d_head, d, 1.f, c ? 1.f : 0.f, count, 0, 0, 0, 0,
+                 nullptr, nullptr, nullptr};
+      if (P.chunks > 1) {
+        if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+        else ce_launch<CfgSmall, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+      } else {
+        if (P.big_head) ce_launch<CfgBig, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+        else ce_launch<CfgSmall, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+      }
+    }
+  }
+  if (d_head && P.chunks > 1)
+    hipLaunchKernelGGL(k_ce_round, dim3((unsigned)std::min<int64_t>(cdiv(V * d / 4, 256), 16384)), dim3(256), 0, s,
+                       (const float4*)P.head, V * d / 4, (uint2*)d_head);
   return check_launch(what);
 }
 

@@ -739,11 +739,22 @@ def streamed_cross_entropy(act, head, targets, *, ignore_index: int = -100, row_
                            want_dhead: bool = False):
     """(loss, d_act, d_head): per-position cross entropy (see `losses.streamed_position_cross_entropy`) and
     row_weight (fp32 [N]; None: 1) times its gradients; None for those not wanted."""
-    want = want_dact or want_dhead
-    if row_weight is None and want:
-        row_weight = torch.ones(act.shape[:1], dtype=torch.float32, device=act.device)
-    loss, stats = streamed_cross_entropy_fwd(act, head, targets, ignore_index=ignore_index, want_stats=want)
-    if not want:
-        return loss, None, None
-    return (loss, *streamed_cross_entropy_bwd(act, head, targets, stats, row_weight, ignore_index=ignore_index,
-                                              want_dact=want_dact, want_dhead=want_dhead))
+    name = "streamed_cross_entropy"
+    N = act.shape[0] if act.dim() else 0
+    if row_weight is not None and (row_weight.dtype != torch.float32 or tuple(row_weight.shape) != (N,)):
+        raise L.PDError(f"{name}: row_weight is float32 [{N}], got {row_weight.dtype} {tuple(row_weight.shape)}")
+    if not (want_dact or want_dhead):
+        return streamed_cross_entropy_fwd(act, head, targets, ignore_index=ignore_index)[0], None, None
+    device, sizes = _ce_checks(name, act, head, targets)
+    if row_weight is None:
+        row_weight = torch.ones(N, dtype=torch.float32, device=device)
+    _one_device(name, act, "row_weight", row_weight)
+    loss = torch.empty(N, dtype=torch.float32, device=device)
+    if not N:
+        return loss, torch.empty_like(act) if want_dact else None, torch.zeros_like(head) if want_dhead else None
+    da = torch.empty_like(act) if want_dact else None
+    dh = torch.empty_like(head) if want_dhead else None
+    ws = L.workspace(L.load().pd_streamed_ce_train_workspace_size(*sizes, int(want_dact), int(want_dhead)), device)
+    L.launch("pd_streamed_ce_train", device, *sizes, *_ce_args(act, head, targets, ignore_index), L.ptr(row_weight),
+             L.ptr(loss), L.ptr(da), L.ptr(dh), L.ptr(ws), ws.numel())
+    return loss, da, dh
