@@ -122,9 +122,9 @@ __device__ inline void rt_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Words in the order of floats; 0 is below all.
+// Words in the order of floats (both zeros the same); 0 is below all.
 __device__ inline uint32_t rt_order(float f) {
-  const uint32_t u = __float_as_uint(f);
+  const uint32_t u = __float_as_uint(f + 0.f);
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 __device__ inline float rt_unorder(uint32_t u) {
@@ -529,7 +529,9 @@ __global__ __launch_bounds__(256, J > 8 ? 4 : 8) void k_rt_fwd(RtArgs a) {
     }
     return;
   }
+  float by = a.scale;
   if (a.renorm) {  // over the chosen: from the largest of them on
+    if (total != total) by = NAN;  // a row that holds a NaN has no softmax, whatever is chosen of it
     m = -INFINITY;
     for (int r = lane; r < a.k; r += NT) {
       const int e = chosen(r);
@@ -555,7 +557,7 @@ __global__ __launch_bounds__(256, J > 8 ? 4 : 8) void k_rt_fwd(RtArgs a) {
     }
   }
   const bool none = !rt_fold<NT>(live, [](uint32_t p, uint32_t q) { return p | q; });  // all are masked
-  const float by = a.scale / total;
+  by /= total;
   for (int r = lane; r < a.k; r += NT) {
     wout[r] = none ? 0.f : __uint_as_float(won[r].x) * by;
     iout[r] = (int32_t)won[r].y;

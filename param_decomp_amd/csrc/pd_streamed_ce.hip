@@ -365,12 +365,13 @@ __global__ void k_ce_counts(const int32_t* __restrict__ count, int64_t R, int ch
   }
 }
 // G = g (softmax - 1_t) in bf16 over what EpiCEKeep kept, in place: the values of each CE_SPAN
-// columns times e^{their m - m} g / s. A position of weight zero gets zeros whatever it holds. Blocks: a row, 8192
-// columns of it.
+// columns times e^{their m - m} g / s. A position of weight zero gets zeros whatever it holds, and so
+// does its row of the activations: d_head's product has 0 times it. Blocks: a row, 8192 columns of it.
 __global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int64_t ld, const float2* __restrict__ part,
                                                   int64_t n_tiles, const float2* __restrict__ st,
                                                   const float* __restrict__ target, const int32_t* __restrict__ rows,
-                                                  const int32_t* __restrict__ count, CETargets t, const float* __restrict__ g) {
+                                                  const int32_t* __restrict__ count, CETargets t, const float* __restrict__ g,
+                                                  uint4* __restrict__ act, int64_t words) {
   const int64_t row = blockIdx.x;
   if (row >= *count) return;
   const int64_t r = rows[row], want = t.at(r);
@@ -378,6 +379,8 @@ __global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int6
   const float gr = g[r], by = gr / o.y * 0x1p-15f;
   // p - 1 at the target from the sum of the others: p may be near 1
   const float hit = -gr * ((o.y - ce_exp(target[row] - o.x)) / o.y);
+  if (gr == 0.f && blockIdx.y == 0)
+    for (int64_t c = threadIdx.x; c < words; c += 256) act[row * words + c] = make_uint4(0u, 0u, 0u, 0u);
   uint16_t* e = E + row * ld;
   const int64_t c0 = (int64_t)blockIdx.y * 8192 + threadIdx.x * 8;
   uint4 w[4];
@@ -802,7 +805,7 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
       ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
     hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
                        loss, nullptr, P.stats);
-    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(P.ld, 8192)), dim3(256), 0, s, P.E, P.ld, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g);
+    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(P.ld, 8192)), dim3(256), 0, s, P.E, P.ld, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)(P.act + c * R * d), d / 8);
     if (d_act) {
       GemmArgs b{M, d, V, P.E, P.ld, hd, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
       if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);

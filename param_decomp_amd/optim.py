@@ -50,16 +50,15 @@ class AdamW:
         device = self.params[0].device
         if device.type != "cuda":
             raise L.PDError("pd kernels take GPU tensors")
-        seen = set()
         for i, p in enumerate(self.params):
             _plain(name, f"parameter {i}", p, p.numel(), (torch.float32,), device)
-            if p.numel() and p.data_ptr() in seen:
-                raise L.PDError(f"{name}: parameter {i} is there twice")
-            seen.add(p.data_ptr())
+        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise L.PDError(f"{name}: two parameters share memory")
         self.device, self.lr, self.betas, self.eps, self.weight_decay = device, lr, betas, eps, weight_decay
         self.key = (int(key[0]), int(key[1]))
         sizes = [p.numel() for p in self.params]
-        small = [state_bits == 32 or n < min_8bit_size for n in sizes]
+        small = [state_bits == 32 or n < min_8bit_size for n in sizes]  # states of 32 bits
         self.state = self._zeros(sizes, small) if state is None else state
         self._check_state(sizes, small)
         if copies is not None:
@@ -71,17 +70,27 @@ class AdamW:
                     _plain(name, f"copy {i}", c, n, (torch.bfloat16,), device)
         self.copies = copies
         self._ticket = torch.zeros(1, dtype=torch.int32, device=device)
-        n = len(sizes)
-        ptrs = lambda ts: (ctypes.c_void_p * n)(*[None if t is None else t.data_ptr() for t in ts])  # noqa: E731
-        st = self.state
-        self._n, self._sizes, self._p = n, (ctypes.c_int64 * n)(*sizes), ptrs(self.params)
-        self._shapes = [p.shape for p in self.params]
-        self._m, self._v = ptrs(st["m"]), ptrs(st["v"])
-        scales = state_bits == 8
-        self._ms, self._vs = (ptrs(st["m_scale"]), ptrs(st["v_scale"])) if scales else (None, None)
-        self._c = ptrs(copies) if copies is not None else None
-        self._written = self.params + [c for c in copies or () if c is not None]
-        self._state_bits = state_bits
+        self._sizes, self._shapes = sizes, [p.shape for p in self.params]
+        self._c_sizes = L.host_array(ctypes.c_int64, sizes)
+        n, st = len(sizes), self.state
+        none = [None] * n
+        # the tensors of each argument, in the entry point's order
+        self._held = [list(ts) for ts in (self.params, st["m"], st["v"], st.get("m_scale") or none, st.get("v_scale") or none,
+                                          copies or none)]
+        self._written = self._held[0] + [c for c in self._held[5] if c is not None]
+        self._at: list[int] | None = None
+
+    def _pointers(self) -> None:
+        """The arrays of addresses, formed again where a tensor's memory has been exchanged (`p.data = ...`)."""
+        at = [0 if t is None else t.data_ptr() for ts in self._held for t in ts]
+        if at == self._at:
+            return
+        n = len(self._sizes)
+        for i, (p, size) in enumerate(zip(self.params, self._sizes)):
+            _plain("AdamW", f"parameter {i}", p, size, (torch.float32,), self.device)
+        arrays = [L.host_array(ctypes.c_void_p, [a or None for a in at[k * n:(k + 1) * n]]) for k in range(6)]
+        self._p, self._m, self._v, self._ms, self._vs, self._c = arrays
+        self._at = at
 
     def _zeros(self, sizes, small) -> dict:
         dev = self.device
@@ -116,7 +125,7 @@ class AdamW:
         parameter whose gradient is None stays as it is. `lr`: this step's, a number or an fp32
         tensor of one value on the GPU, and `grad_scale` such a tensor that gradients are
         multiplied with: both are read when the step runs, also in a replayed graph."""
-        name, n = "AdamW.step", self._n
+        name, n = "AdamW.step", len(self._sizes)
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != n:
             raise L.PDError(f"{name}: {len(grads)} gradients for {n} parameters")
@@ -137,7 +146,8 @@ class AdamW:
         lr = self.lr if lr is None else lr
         lr_dev = self._scalar("lr", lr) if isinstance(lr, torch.Tensor) else None
         scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
-        L.launch("pd_adamw_step", self.device, n, self._sizes, self._p, (ctypes.c_void_p * n)(*ptrs),
+        self._pointers()
+        L.launch("pd_adamw_step", self.device, n, self._c_sizes, self._p, (ctypes.c_void_p * n)(*ptrs),
                  (ctypes.c_int32 * n)(*types), self._m, self._v, self._ms, self._vs, self._c,
                  self.state["step"].data_ptr(), self._ticket.data_ptr(), 0.0 if lr_dev else float(lr), lr_dev, scale,
                  self.betas[0], self.betas[1], self.eps, self.weight_decay, self.key[0], self.key[1])
@@ -153,12 +163,14 @@ class AdamW:
 
     def load_state_dict(self, state: dict) -> None:
         """Copies `state`, of an optimizer over parameters of the same sizes and bits, into this one's."""
+        pairs = []
         for name, mine in self.state.items():
             theirs = state.get(name)
-            for a, b in zip(*((x if isinstance(x, (list, tuple)) else [x]) for x in (mine, theirs)), strict=True):
-                if (a is None) != (b is None) or (a is not None and (a.dtype != b.dtype or a.shape != b.shape)):
-                    raise L.PDError(f"AdamW.load_state_dict: {name} is of other sizes or bits")
-        for name, mine in self.state.items():
-            for a, b in zip(*((x if isinstance(x, (list, tuple)) else [x]) for x in (mine, state[name]))):
-                if a is not None:
-                    a.copy_(b)
+            mine, theirs = ([x] if x is None or isinstance(x, torch.Tensor) else list(x) for x in (mine, theirs))
+            if len(mine) != len(theirs) or any((a is None) != (b is None) or
+                                               (a is not None and (a.dtype != b.dtype or a.shape != b.shape))
+                                               for a, b in zip(mine, theirs)):
+                raise L.PDError(f"AdamW.load_state_dict: {name} is of other sizes or bits")
+            pairs += [(a, b) for a, b in zip(mine, theirs) if a is not None]
+        for a, b in pairs:
+            a.copy_(b)

@@ -1,0 +1,229 @@
+"""The streamed cross entropy against the formula in 64 bits.
+
+Tolerances: a logit is a sum of d products in fp32, off by at most (d + 1) 2^-24 sum |act head| =: e. The
+loss is a difference of two of them and of a logarithm: 2 e and 16 2^-24 of what is added (it, the largest
+logit's distance, 1). G's entries are off by (2 e + 16 2^-24) p g and, in bf16, by half a step (2^-8 of
+them; the one-call form rounds to 2^-12 of them before, in fp16 relative to the largest of 64 neighbours:
+2^15 p / p_max has steps of 2^-24 at least, which is 2^-39 of p_max <= 1, so 2^-40 g more); what is summed from them likewise times the other
+operand, with n 2^-24 of the sum of magnitudes for n terms, and half a step of the result."""
+
+import pytest
+import torch
+
+from param_decomp_amd import _lib as L
+from param_decomp_amd import losses, ops
+
+pytestmark = pytest.mark.gpu
+
+F64, BF16, F32 = torch.float64, torch.bfloat16, torch.float32
+U = 2.0**-24
+HALF = {BF16: 2.0**-8, F32: U}
+
+
+def _inputs(device, N, d, V, dtype, seed=0, skip=0.0, scale=1.0, bits=64):
+    g = torch.Generator(device=device).manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, device=device, generator=g)  # noqa: E731
+    act, head = rnd(N, d).to(dtype), (rnd(V, d) * (2 * scale / d**0.5)).to(dtype)
+    t = torch.randint(V, (N,), device=device, generator=g)
+    off = torch.rand(N, device=device, generator=g) < skip
+    t = torch.where(off, torch.tensor([-100, -1, V, V + 7], device=device)[torch.arange(N, device=device) % 4], t)
+    w = torch.randn(N, device=device, generator=g)
+    return act, head, t.to(torch.int32 if bits == 32 else torch.int64), w
+
+
+def _expected(act, head, t, w):
+    """(loss, d_act, d_head) and their bounds, in 64 bits."""
+    dt, (N, d), V = act.dtype, act.shape, head.shape[0]
+    a, h, w = act.double(), head.double(), w.double()
+    on = (t >= 0) & (t < V)
+    a = torch.where(on[:, None], a, torch.zeros_like(a))
+    w = torch.where(on, w, torch.zeros_like(w))
+    z, e = a @ h.T, (d + 1) * U * (a.abs() @ h.abs().T)
+    at = t.long().clamp(0, V - 1)[:, None]
+    lp = torch.log_softmax(z, -1)
+    loss = torch.where(on, -lp.gather(1, at)[:, 0], torch.zeros(N, dtype=F64, device=z.device))
+    spread = z.amax(-1) - z.gather(1, at)[:, 0]
+    bl = 2 * e.amax(-1) + 16 * U * (1 + loss.abs() + spread.abs())
+    p = lp.exp()
+    G = (p.scatter_add(1, at, -torch.ones_like(p[:, :1]))) * w[:, None]
+    bG = (2 * e.amax(-1, keepdim=True) + 16 * U) * p * w.abs()[:, None] + 16 * U * G.abs()
+    bG = bG + (HALF[dt] + (2.0**-12 if dt == BF16 else 0)) * (G.abs() + bG)
+    if dt == BF16:
+        bG = bG + 2.0**-40 * w.abs()[:, None]
+    da, dh = G @ h, G.T @ a
+    ba = bG @ h.abs() + (V + 64) * U * (G.abs() @ h.abs())
+    bh = bG.T @ a.abs() + (N + 64) * U * (G.abs().T @ a.abs())
+    return (loss, da, dh), (bl, ba + HALF[dt] * (da.abs() + ba) + 1e-40, bh + HALF[dt] * (dh.abs() + bh) + 1e-40)
+
+
+def _check(got, want, bounds):
+    for n, a, b, c in zip(("loss", "d_act", "d_head"), got, want, bounds):
+        err = (a.double() - b).abs()
+        assert (err <= c).all(), (n, float((err - c).max()), float((err / c.clamp(min=1e-300)).max()))
+
+
+def _both_forms(act, head, t, w, ignore=-100):
+    one = ops.streamed_cross_entropy(act, head, t, ignore_index=ignore, row_weight=w, want_dact=True, want_dhead=True)
+    loss, stats = ops.streamed_cross_entropy_fwd(act, head, t, ignore_index=ignore, want_stats=True)
+    return one, (loss, *ops.streamed_cross_entropy_bwd(act, head, t, stats, w, ignore_index=ignore))
+
+
+SHAPES = [(1, 8, 1), (1, 64, 7), (2, 16, 129), (33, 72, 1000), (127, 64, 64), (128, 128, 65), (129, 200, 257), (300, 136, 3001),
+          (513, 64, 777), (1000, 520, 4099)]
+
+
+@pytest.mark.parametrize("N, d, V", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("skip", [0.0, 0.4])
+def test_loss_and_gradients(device, N, d, V, dtype, skip):
+    act, head, t, w = _inputs(device, N, d, V, dtype, N + V, skip, bits=32 if V % 2 else 64)
+    want, bounds = _expected(act, head, t, w)
+    for got in _both_forms(act, head, t, w):
+        assert got[1].dtype == got[2].dtype == dtype and got[0].dtype == F32
+        _check(got, want, bounds)
+
+
+@pytest.mark.parametrize("d", [1, 33, 100, 1000])
+def test_odd_widths_through_autograd(device, d):
+    for dtype in (BF16, F32):
+        act, head, t, w = _inputs(device, 70, d, 333, dtype, d, 0.2)
+        act, head = act.requires_grad_(), head.requires_grad_()
+        loss = losses.streamed_position_cross_entropy(act.view(7, 10, d), head, t.view(7, 10))
+        assert loss.shape == (7, 10)
+        got = (loss.view(-1), *torch.autograd.grad(loss, (act, head), w.view(7, 10)))
+        _check(got, *_expected(act.detach(), head.detach(), t, w))
+
+
+def test_mean_and_one_gradient_alone(device):
+    act, head, t, _ = _inputs(device, 200, 64, 500, F32, 3, 0.3)
+    on = (t >= 0) & (t < 500)
+    want, bounds = _expected(act, head, t, on.float() / on.sum())
+    a = act.clone().requires_grad_()
+    loss = losses.streamed_cross_entropy(a, head, t)
+    assert abs(float(loss) - float(want[0].sum() / on.sum())) <= float(bounds[0].mean()) * 200 / int(on.sum()) + 200 * U * float(loss)
+    (da,) = torch.autograd.grad(loss, a)
+    # the weight 1 / count is rounded
+    assert ((da.double() - want[1]).abs() <= bounds[1] + 4 * U * want[1].abs()).all()
+    h = head.clone().requires_grad_()
+    (dh,) = torch.autograd.grad(losses.streamed_cross_entropy(act, h, t), h)
+    assert ((dh.double() - want[2]).abs() <= bounds[2] + 4 * U * want[2].abs()).all()
+    assert float(losses.streamed_cross_entropy(act, head, torch.full_like(t, -100))) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_positions_that_do_not_count_reach_nothing(device, dtype):
+    act, head, t, w = _inputs(device, 300, 64, 400, dtype, 4, 0.3)
+    w[5::9] = 0  # counts in the loss, has no gradient
+    skip = (t < 0) | (t >= 400)
+    clean = _both_forms(act, head, t, w)
+    act[skip] = float("nan")
+    got = _both_forms(act, head, t, w)
+    for a, b in zip(clean, got):
+        assert (b[0][skip] == 0).all() and (b[1][skip] == 0).all()
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+    zero = (w == 0) & ~skip
+    act[zero] = float("inf")
+    for a, b in zip(clean, _both_forms(act, head, t, w)):
+        assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2]) and (b[1][zero] == 0).all()
+        assert not torch.isfinite(b[0][zero]).any() and torch.equal(a[0][~zero], b[0][~zero])
+
+
+def test_a_nan_that_counts_shows(device):
+    for dtype in (BF16, F32):
+        act, head, t, w = _inputs(device, 140, 64, 300, dtype, 5)
+        w = w.abs() + 0.1
+        clean = _both_forms(act, head, t, w)
+        act[17, 3] = float("nan")
+        for a, b in zip(clean, _both_forms(act, head, t, w)):
+            bad = torch.zeros(140, dtype=torch.bool, device=device)
+            bad[17] = True
+            assert torch.equal(torch.isnan(b[0]), bad) and torch.isnan(b[1][17]).all()
+            assert torch.equal(a[0][~bad], b[0][~bad]) and torch.equal(a[1][~bad], b[1][~bad])
+            assert torch.isnan(b[2]).all()
+
+
+def test_none_counts(device):
+    for dtype, N in ((BF16, 3), (BF16, 500), (F32, 5)):
+        act, head, t, w = _inputs(device, N, 32, 100, dtype, 6)
+        for loss, da, dh in _both_forms(act, head, torch.full_like(t, 7), w, ignore=7):
+            assert not loss.any() and not da.any() and not dh.any()
+        loss, da, dh = ops.streamed_cross_entropy(act[:0], head, t[:0], want_dact=True, want_dhead=True)
+        assert loss.numel() == 0 and da.shape == (0, 32) and not dh.any()
+        a = act[:0].clone().requires_grad_()
+        h = head.clone().requires_grad_()
+        da, dh = torch.autograd.grad(losses.streamed_position_cross_entropy(a, h, t[:0]).sum(), (a, h))
+        assert da.shape == (0, 32) and not dh.any()
+
+
+@pytest.mark.parametrize("scale", [1e-3, 10.0, 60.0])
+def test_small_and_large_logits(device, scale):
+    """From logits that are all but equal to rows of one probability: what is 1 less a probability keeps its digits."""
+    for dtype in (BF16, F32):
+        act, head, t, w = _inputs(device, 260, 64, 600, dtype, 7, 0.0, scale)
+        t[::2] = (act[::2].double() @ head.double().T).argmax(-1)
+        want, bounds = _expected(act, head, t, w)
+        for got in _both_forms(act, head, t, w):
+            _check(got, want, bounds)
+
+
+def test_pieces_of_the_vocabulary_and_chunks_of_positions(device):
+    """More than 1 GiB of G in the backward, and more than 2 GiB of softmax in the one-call form."""
+    act, head, t, w = _inputs(device, 8200, 16, 140000, BF16, 8, 0.02)
+    one, two = _both_forms(act, head, t, w)
+    want, bounds = None, None
+    dh, bh = torch.zeros(140000, 16, dtype=F64, device=device), torch.zeros(140000, 16, dtype=F64, device=device)
+    for r in range(0, 8200, 820):
+        s = slice(r, r + 820)
+        want, bounds = _expected(act[s], head, t[s], w[s])
+        for got in (one, two):
+            _check((got[0][s], got[1][s]), want[:2], bounds[:2])
+        # the rest of the sum's roundings is that of 8200 terms in place of 820
+        dh += want[2]
+        bh += bounds[2] * 11
+    for got in (one, two):
+        _check((got[0][:0], got[1][:0], got[2]), (dh[:0, 0], dh[:0], dh), (bh[:0, 0], bh[:0], bh))
+
+
+def test_twice_the_same_and_on_other_streams(device):
+    act, head, t, w = _inputs(device, 400, 128, 1500, BF16, 9, 0.1)
+    first = _both_forms(act, head, t, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = _both_forms(act, head, t, w)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, again):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+def test_gradients_are_the_losses_differences(device):
+    """Directional differences of the loss in fp32, where the loss is off by about 1e-6."""
+    act, head, t, w = _inputs(device, 50, 24, 90, F32, 10, 0.2)
+    w = w.abs()
+    _, da, dh = ops.streamed_cross_entropy(act, head, t, row_weight=w, want_dact=True, want_dhead=True)
+    g = torch.Generator(device=device).manual_seed(1)
+    for x, d in ((act, da), (head, dh)):
+        v = torch.randn(x.shape, device=device, generator=g)
+        h = 1e-3
+        f = lambda s: float((ops.streamed_cross_entropy(*((x + s * v, head) if x is act else (act, x + s * v)), t)[0].double()  # noqa: E731
+                             * w.double()).sum())
+        diff, want = (f(h) - f(-h)) / (2 * h), float((d.double() * v.double()).sum())
+        dz = v.double() @ head.double().T if x is act else act.double() @ v.double().T
+        # h^2 / 6 times a third derivative (a third central moment of dz), and the losses' own bounds and the
+        # moved operand's rounding over h
+        third = h * h / 6 * float((w.double() * (2 * dz.abs().amax(-1))**3).sum())
+        noise = float((w.double() * (_expected(act, head, t, w)[1][0] + 2 * U * (act.double().abs() @ head.double().abs().T).amax(-1))).sum())
+        assert abs(diff - want) <= third + noise / h + 1e-4 * abs(want)
+
+
+def test_refusals(device):
+    act, head, t, w = _inputs(device, 4, 16, 9, BF16)
+    for bad in ((act.cpu(), head, t), (act, head.cpu(), t), (act, head, t.cpu()), (act.t(), head, t)):
+        with pytest.raises(L.PDError):
+            ops.streamed_cross_entropy_fwd(*bad)
+    with pytest.raises(L.PDError, match="row_weight"):
+        ops.streamed_cross_entropy(act, head, t, row_weight=w.double(), want_dact=True)
+    with pytest.raises(L.PDError, match="stats"):
+        ops.streamed_cross_entropy_bwd(act, head, t, w, w)
