@@ -174,6 +174,42 @@ __device__ inline float rn_rstd(const float (&u)[CH][8], float d, float eps, flo
   return RN_WIDE / sqrtf(s[0] / d + eps * RN_WIDE * RN_WIDE);
 }
 
+// The same in 64 bits: squares of bf16 values are exact in fp32, a thread's eight or sixteen of them are added
+// there and the threads' sums in 64 bits; the root is fp32's with a Newton step.
+template <int NT, int CH>
+__device__ inline double rn_rstd_d(const float (&u)[CH][8], int d, float eps, double* part, float (*part_f)[1], int tid) {
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(u[c][e], u[c][e], s);
+  double t = (double)s;
+#pragma unroll
+  for (int off = (NT < 64 ? NT : 64) / 2; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+  if constexpr (NT > 64) {
+    if ((tid & 63) == 0) part[tid >> 6] = t;
+    __syncthreads();
+    t = 0.0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) t += part[i];
+  }
+  // the same way for the team's threads
+  if (!(t < INFINITY)) {
+    if constexpr (NT > 64) __syncthreads();
+    return (double)rn_rstd<NT, CH>(u, (float)d, eps, part_f, tid);
+  }
+  const double ms = t / (double)d + (double)eps;
+  if (!(ms > 1e-30 && ms < 1e30)) return 1.0 / sqrt(ms);
+  const double r = (double)(1.f / sqrtf((float)ms));
+  return r * (1.5 - 0.5 * ms * r * r);
+}
+// To bf16 by way of fp32, as a cast does: the compiler may take the two conversions as one.
+__device__ inline float rn_bf16(double v) {
+  float f = (float)v;
+  asm volatile("" : "+v"(f));
+  return bf16_to_f32(f32_to_bf16(f));
+}
+
 struct RnFwd {
   const void *x, *b;  // b NULL: h = x, not written
   const float *post, *pre;
@@ -201,6 +237,7 @@ template <typename TX, typename TB, int NT, int CH>
 __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
   constexpr int NW = NT > 64 ? NT / 64 : 1, TEAMS = rn_threads(NT) / NT;
   __shared__ float part[4][2 * NW][1];
+  __shared__ double part_d[2][NW];
   const int tid = threadIdx.x % NT, d = a.d;
   const int64_t run = (int64_t)blockIdx.x * TEAMS + threadIdx.x / NT;
   if (run >= a.runs.runs) return;  // whole teams; with NT > 64 none
@@ -208,7 +245,13 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
   a.runs.rows(run, lo, hi);
   const TX* x = (const TX*)a.x;
   const TB* b = (const TB*)a.b;
-  float pre[CH][8], post[CH][8], gate[CH][8];
+  // A bf16 stream is formed in 64 bits and rounded from there: y and the gradients go on from what
+  // is stored, and a neighbour of the right bf16 would move them by far more than their own roundings (in
+  // fp32 99 of 3.6 10^6 values were one).
+  constexpr bool ONCE = sizeof(TX) == 2;
+  typedef std::conditional_t<ONCE, double, float> TF;
+  float pre[CH][8], post[CH][8];
+  TF factor[CH][8];  // scale gate post
   rn_param<CH>(a.pre, a.weight_offset, tid, NT, d, pre);
   rn_param<CH>(a.post, a.weight_offset, tid, NT, d, post);
   const int64_t per = a.gate.kind == 2 ? 1 : a.runs.per_group;
@@ -228,26 +271,34 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
     if (r + 1 < hi) load(r + 1, xn, bn);
     if (left == 0) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) rn_gate(a.gate, r / per, d, 8 * (tid + c * NT), a.scale, gate[c]);
+      for (int c = 0; c < CH; ++c) {
+        float g[8];
+        rn_gate(a.gate, r / per, d, 8 * (tid + c * NT), 1.f, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) factor[c][e] = (TF)a.scale * (TF)g[e] * (TF)post[c][e];
+      }
       left = per - r % per;
     }
     --left;
-    float u[CH][8], rb = 1.f;
+    float u[CH][8];
+    TF rb = (TF)1;
     if (b) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[c][e] = bc[c][e];
-      if (a.post_norm) rb = rn_rstd<NT, CH>(u, (float)d, a.eps, part[2 * it], tid);
+      if (a.post_norm) {
+        if constexpr (ONCE) rb = rn_rstd_d<NT, CH>(u, d, a.eps, part_d[it], part[2 * it], tid);
+        else rb = rn_rstd<NT, CH>(u, (float)d, a.eps, part[2 * it], tid);
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[c][e] = fmaf(gate[c][e], u[c][e] * rb * post[c][e], xc[c][e]);
-        rn_store<TX>((TX*)a.h + r * d, 8 * (tid + c * NT), d, u[c]);
-        if constexpr (sizeof(TX) == 2) {  // the stream as it is stored is what is normed
-#pragma unroll
-          for (int e = 0; e < 8; ++e) u[c][e] = bf16_to_f32(f32_to_bf16(u[c][e]));
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (ONCE) u[c][e] = rn_bf16(fma(factor[c][e] * rb, (double)u[c][e], (double)xc[c][e]));
+          else u[c][e] = fmaf(factor[c][e], u[c][e] * rb, xc[c][e]);
         }
+        rn_store<TX>((TX*)a.h + r * d, 8 * (tid + c * NT), d, u[c]);
       }
     } else {
 #pragma unroll
@@ -262,7 +313,7 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
       for (int e = 0; e < 8; ++e) u[c][e] = u[c][e] * rh * pre[c][e];
       rn_store<TB>((TB*)a.y + r * d, 8 * (tid + c * NT), d, u[c]);
     }
-    if (a.stats && tid == 0) *(float2*)(a.stats + 2 * r) = make_float2(rb, rh);
+    if (a.stats && tid == 0) *(float2*)(a.stats + 2 * r) = make_float2((float)rb, rh);
 #pragma unroll
     for (int c = 0; c < CH; ++c) xc[c] = xn[c], bc[c] = bn[c];
   }
@@ -397,8 +448,9 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
   }
 }
 
-// Sums of n partial rows of `cols` values in a fixed order, 16 columns by 64 slices of the rows a
-// block: a job for the parameters (columns dpost | dpre) and one for each group of the gate.
+// Sums of n partial rows of `cols` values in a fixed order: a block's 16 waves take a slice of the rows
+// each, 64 columns. A job for the parameters (columns dpost | dpre) and one for each group of the gate. (16 columns
+// by 64 slices a block, the gates' few partials among them: 16 us at d = 4096 with 16 gates.)
 struct RnSums {
   const float* par;
   int64_t par_n;
@@ -410,29 +462,27 @@ struct RnSums {
   int64_t d;
 };
 __global__ __launch_bounds__(1024) void k_rn_sums(RnSums a) {
-  __shared__ float red[16][17];
-  const int c = threadIdx.x & 15, sl = threadIdx.x >> 4, wv = threadIdx.x >> 6;
+  __shared__ float red[16][64];
+  const int c = threadIdx.x & 63, sl = threadIdx.x >> 6;
   const bool gates = a.gate && (int64_t)blockIdx.y >= (a.par ? 1 : 0);
   const int64_t group = (int64_t)blockIdx.y - (a.par ? 1 : 0);
   const int64_t cols = gates ? a.d : 2 * a.d, n = gates ? a.gate_n : a.par_n;
-  if ((int64_t)blockIdx.x * 16 >= cols) return;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
-  const int64_t per = (n + 63) / 64, lo = sl * per < n ? sl * per : n;
+  if ((int64_t)blockIdx.x * 64 >= cols) return;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  const int64_t per = (n + 15) / 16, lo = sl * per < n ? sl * per : n;
   const int64_t hi = col < cols ? (lo + per < n ? lo + per : n) : lo;
   const float* p = (gates ? a.gate + group * n * cols : a.par) + col;
   float s = 0.f;
-  for (int64_t i = lo; i < hi; i += 8) {
-    float v[8];
+  for (int64_t i = lo; i < hi; i += 16) {
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = i + j < hi ? p[(i + j) * cols] : 0.f;
+    for (int j = 0; j < 16; ++j) v[j] = i + j < hi ? p[(i + j) * cols] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += v[j];
+    for (int j = 0; j < 16; ++j) s += v[j];
   }
-  s += __shfl_xor(s, 16, 64);
-  s += __shfl_xor(s, 32, 64);
-  if ((threadIdx.x & 63) < 16) red[wv][c] = s;
+  red[sl][c] = s;
   __syncthreads();
-  if (threadIdx.x >= 16 || col >= cols) return;
+  if (sl || col >= cols) return;
   s = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s += red[i][c];
@@ -591,7 +641,7 @@ int pd_residual_norm_bwd(const void* stream_out, int x_dtype, const void* branch
   if (!rows) {  // sums over no rows
     if (params) {
       const RnSums z{(const float*)(d_post ? d_post : d_pre), 0, d_post, d_pre, nullptr, 0, nullptr, 0, d};
-      hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)cdiv(2 * d, 16)), dim3(1024), 0, s, z);
+      hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)cdiv(2 * d, 64)), dim3(1024), 0, s, z);
     }
     return check_launch(what);
   }
@@ -614,7 +664,7 @@ int pd_residual_norm_bwd(const void* stream_out, int x_dtype, const void* branch
   });
   if (params || P.gate_part) {
     const RnSums z{a.dpar, P.slots, d_post, d_pre, a.dgate_part, P.runs.slices, d_gate, gate_dtype == PD_DTYPE_BF16, d};
-    hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)cdiv(params ? 2 * d : d, 16),
+    hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)cdiv(params ? 2 * d : d, 64),
                                        (unsigned)((params ? 1 : 0) + (P.gate_part ? P.runs.groups : 0))),
                        dim3(1024), 0, s, z);
   }
