@@ -24,6 +24,7 @@ namespace pd {
 namespace {
 
 constexpr int ADAMW_TENSORS = 48;  // in one launch: 3.9 KB of its 4 KB of arguments
+constexpr int64_t ADAMW_BLOCKS = (1 << 24) - 1;  // of a launch: 2^32 threads less one
 constexpr int QB = 256;            // values that share a scale
 constexpr float FP8_TOP = 448.f;
 
@@ -322,7 +323,7 @@ extern "C" int pd_adamw_step(int n_tensors, const int64_t* sizes, void* const* p
     return fail(PD_EINVAL, std::string(what) + ": lr and weight_decay must be finite");
   int64_t total = 0, base = 0;
   for (int i = 0; i < n_tensors; ++i) {
-    if (sizes[i] < 0 || sizes[i] > (int64_t)1 << 40) return fail(PD_EINVAL, std::string(what) + ": size of a tensor");
+    if (sizes[i] < 0 || sizes[i] > (int64_t)1 << 37) return fail(PD_EINVAL, std::string(what) + ": size of a tensor");
     if (!sizes[i] || !grads[i]) continue;
     const void *ms = m_scale ? m_scale[i] : nullptr, *vs = v_scale ? v_scale[i] : nullptr;
     if (!p[i] || !m[i] || !v[i] || !ms != !vs) return fail(PD_EINVAL, std::string(what) + ": null pointer");
@@ -362,7 +363,7 @@ extern "C" int pd_adamw_step(int n_tensors, const int64_t* sizes, void* const* p
     base += cdiv(n, QB) * QB;
     if (!n || !grads[i]) continue;
     const int64_t need = cdiv(n, chunk);
-    if (a.n_tensors == ADAMW_TENSORS || blocks + need > 0x7FFFFFFF) launch(false);
+    if (a.n_tensors == ADAMW_TENSORS || (a.n_tensors && blocks + need > ADAMW_BLOCKS)) launch(false);
     AdamWTensor& t = a.t[a.n_tensors++];
     t.p = (float*)p[i], t.g = grads[i], t.m = m[i], t.v = v[i];
     t.m_scale = m_scale ? (float*)m_scale[i] : nullptr, t.v_scale = v_scale ? (float*)v_scale[i] : nullptr;

@@ -688,8 +688,8 @@ int rt_check(const char* what, int dtype, int64_t T, int E, int k, float scale) 
   if (dtype != PD_DTYPE_F32 && dtype != PD_DTYPE_BF16)
     return fail(PD_EUNSUPPORTED, std::string(what) + ": logits are fp32 or bf16");
   if (T < 0 || E < 1 || k < 1 || k > E) return fail(PD_EINVAL, std::string(what) + ": T >= 0 and 1 <= k <= E");
-  if (E > RT_MAX_E || k > RT_MAX_K || T > ((int64_t)1 << 31))
-    return fail(PD_EUNSUPPORTED, std::string(what) + ": up to 1024 experts, 64 of them chosen, and 2^31 rows");
+  if (E > RT_MAX_E || k > RT_MAX_K || T >= ((int64_t)1 << 26))
+    return fail(PD_EUNSUPPORTED, std::string(what) + ": up to 1024 experts, 64 of them chosen, and 2^26 rows");
   if (!std::isfinite(scale)) return fail(PD_EINVAL, std::string(what) + ": scale must be finite");
   return PD_OK;
 }

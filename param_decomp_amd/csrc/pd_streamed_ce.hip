@@ -16,7 +16,9 @@
 // what they hold reaches nothing. How many count only the device knows: grids cover all positions
 // and the products read the count (MODE_COUNTED).
 //
-// fp32 runs pieces of logits through pd_gemm and passes over them.
+// fp32 operands go through the same bf16 products as three bf16 parts each (8 + 8 + 8 bits, exact): the six
+// products of parts that reach 2^-24 of the whole are one contraction six times as long. 1003 x 1000 over
+// 32003 with gradients: XX us; fp32 products on the matrix cores are a sixteenth of bf16's rate.
 #include <algorithm>
 #include <cmath>
 
@@ -148,6 +150,7 @@ struct EpiCEStats {
     float* target;           // [M]
     const int32_t* rows;     // NULL: row r is position r
     CETargets t;
+    int64_t first = 0;       // the piece's first column of the vocabulary (whole tiles)
   };
   template <class, typename>
   __device__ static void run(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
@@ -178,7 +181,7 @@ struct EpiCEStats {
                                    f32x16 (&z)[CFG::TN], float& m, float& s) {
     int want = -1;  // the target's place in this lane's columns
     if (row < t.M) want = a.t.at(a.rows ? a.rows[row] : row);
-    if (want >= 0) want -= (int)first;
+    want = want < 0 ? -1 : want - (int)(a.first + first);
     m = -INFINITY, s = 0.f;
 #pragma unroll
     for (int j = 0; j < CFG::TN; ++j)
@@ -211,7 +214,7 @@ struct EpiCEStats {
       float2 o = red[r];
 #pragma unroll
       for (int w = 1; w < CFG::WN; ++w) ce_merge(o, red[w * CFG::BM + r]);
-      a.part[(t.m0 + r) * a.n_tiles + t.n0 / CFG::BN] = o;
+      a.part[(t.m0 + r) * a.n_tiles + (a.first + t.n0) / CFG::BN] = o;
     }
   }
 };
@@ -416,58 +419,74 @@ __global__ __launch_bounds__(256) void k_ce_round(const float4* __restrict__ src
   }
 }
 
-// ---------------------------------------------------------------- fp32: pieces of logits in memory
-// Row r's maximum and sum over the piece's w columns, added to those of the pieces before.
-__global__ __launch_bounds__(256) void k_ce_piece_stats(const float* __restrict__ z, int64_t w, int64_t ld,
-                                                        int64_t first, CETargets t, float2* __restrict__ run,
-                                                        float* __restrict__ target) {
-  __shared__ float red[4];
-  __shared__ float2 both[4];
-  const int64_t r = blockIdx.x;
-  const float* row = z + r * ld;
-  float m = -INFINITY, s = 0.f;
-  for (int64_t v = threadIdx.x; v < w; v += 256) m = fmaxf(m, row[v]);
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  for (int64_t v = threadIdx.x; v < w; v += 256) s += m > -INFINITY ? expf(row[v] - m) : NAN;
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) both[threadIdx.x >> 6] = make_float2(m, s);
-  __syncthreads();
-  if (threadIdx.x) return;
-  float2 o = make_float2(m, (both[0].y + both[1].y) + (both[2].y + both[3].y));
-  if (first) {
-    float2 old = run[r];
-    ce_merge(old, o);
-    o = old;
+// ---------------------------------------------------------------- fp32 as parts of bf16
+// The products of parts a_i b_j, i + j <= 4, and which part of each operand a segment of the contraction holds.
+constexpr int CE_PARTS = 6;
+__device__ constexpr int CE_PART_A[CE_PARTS] = {0, 0, 0, 1, 1, 2}, CE_PART_B[CE_PARTS] = {0, 1, 2, 0, 1, 0};
+
+// x = p[0] + p[1] + p[2]; what is not finite is all in the first.
+__device__ inline void ce_parts(float x, bf16_t (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    p[i] = f32_to_bf16(x);
+    const float f = bf16_to_f32(p[i]);
+    x = fabsf(f) < INFINITY ? x - f : 0.f;
   }
-  run[r] = o;
-  const int64_t want = (int64_t)t.at(r) - first;
-  if (want >= 0 && want < w) target[r] = row[want];
 }
-// z -> G in place for the rows that count, zeros for the others.
-__global__ __launch_bounds__(256) void k_ce_piece_grad(float* __restrict__ z, int64_t w, int64_t ld, int64_t first,
-                                                       CETargets t, const float2* __restrict__ stats,
+// rows x cols of src (row pitch ld) as segments of the contraction: SIDE 0 the parts of a product's left operand, 1
+// of its right one. `along` side by side in a row of CE_PARTS * wide (columns from cols to wide are zeros), `below`
+// one below the other, CE_PARTS * rows_below rows of `wide` (rows from `rows` on zeros); either may be NULL.
+template <int SIDE>
+__global__ __launch_bounds__(256) void k_ce_parts(const float* __restrict__ src, int64_t rows, int64_t cols, int64_t ld,
+                                                  int64_t wide, int64_t rows_below, bf16_t* __restrict__ along,
+                                                  bf16_t* __restrict__ below) {
+  const int64_t total = rows_below * wide;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / wide, c = i - r * wide;
+    bf16_t p[3] = {0, 0, 0};
+    if (r < rows && c < cols) ce_parts(src[r * ld + c], p);
+#pragma unroll
+    for (int s = 0; s < CE_PARTS; ++s) {
+      const bf16_t v = p[SIDE ? CE_PART_B[s] : CE_PART_A[s]];
+      if (along && r < rows) along[(r * CE_PARTS + s) * wide + c] = v;
+      if (below) below[(s * rows_below + r) * wide + c] = v;
+    }
+  }
+}
+// The parts of G = g (softmax - 1_t), from the logits z [N][w] (pitch wide) of the rows that count; zeros for the others.
+__global__ __launch_bounds__(256) void k_ce_parts_grad(const float* __restrict__ z, int64_t N, int64_t w, int64_t wide,
+                                                       int64_t first, CETargets t, const float2* __restrict__ stats,
                                                        const float* __restrict__ g, const int32_t* __restrict__ rows,
-                                                       const int32_t* __restrict__ count) {
+                                                       const int32_t* __restrict__ count, bf16_t* __restrict__ along,
+                                                       bf16_t* __restrict__ below) {
   const int64_t r = blockIdx.x;
-  float* row = z + r * ld;
   const bool on = r < *count;
-  const int64_t i = on ? rows[r] : 0;
+  const int64_t i = on ? rows[r] : 0, want = on ? (int64_t)t.at(i) - first : -1;
   const float2 st = on ? stats[i] : make_float2(0.f, 1.f);
   const float gi = on ? g[i] : 0.f, gs = gi / st.y;
-  const int64_t want = (int64_t)t.at(i) - first;
-  for (int64_t v = threadIdx.x; v < w; v += 256) {
-    float x = on ? expf(row[v] - st.x) * gs : 0.f;
-    if (v == want) x -= gi;
-    row[v] = x;
+  for (int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x; c < wide; c += (int64_t)gridDim.y * 256) {
+    float x = 0.f;
+    if (on && c < w) {
+      const float e = expf(z[r * wide + c] - st.x);
+      x = c == want ? -gi * ((st.y - e) / st.y) : e * gs;
+    }
+    bf16_t p[3];
+    ce_parts(x, p);
+#pragma unroll
+    for (int s = 0; s < CE_PARTS; ++s) {
+      along[(r * CE_PARTS + s) * wide + c] = p[CE_PART_A[s]];
+      below[(s * N + r) * wide + c] = p[CE_PART_A[s]];
+    }
   }
 }
 
 // ---------------------------------------------------------------- plans and launches
 typedef CfgDtl CfgSmall;
 typedef CfgDtlBig CfgBig;
+
+// Rows of the head that one product takes: its operands end at 2 GiB (whole tiles, and the rows that a last stage of
+// an operand stored along the other axis may reach).
+int64_t ce_head_rows(int64_t d) { return (0x7FFFFFFF / (2 * d) - 128) & ~(int64_t)255; }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -480,8 +499,7 @@ struct CEFwdPlan {
   int32_t *rows, *count;
   float* target;
   float2 *part;
-  bf16_t* act;
-  float* z;
+  bf16_t *act, *head;  // fp32: parts side by side, of a piece of cw rows of the head
   size_t total;
 };
 bool ce_big(int64_t N, int64_t V) { return big_rounds(tiles_up(N, 256) * tiles_up(V, 256), tiles_up(N, 128) * tiles_up(V, 128), SHARED_ROUND); }
@@ -491,20 +509,21 @@ CEFwdPlan ce_fwd_plan(int dtype, int64_t N, int64_t d, int64_t V, char* base) {
   size_t off = 0;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
   P.target = (float*)take((size_t)N * 4);
+  P.big = ce_big(N, V);
+  P.n_tiles = tiles_up(V, P.big ? 256 : 128);
+  P.part = (float2*)take((size_t)N * P.n_tiles * 8);
   if (dtype == PD_DTYPE_BF16) {
     P.compact = N > CE_COMPACT;
-    P.big = ce_big(N, V);
-    P.n_tiles = tiles_up(V, P.big ? 256 : 128);
-    P.part = (float2*)take((size_t)N * P.n_tiles * 8);
     if (P.compact) {
       P.count = (int32_t*)take(4);
       P.rows = (int32_t*)take((size_t)N * 4);
       P.act = (bf16_t*)take((size_t)N * d * 2);
     }
   } else {
-    P.cw = std::min<int64_t>(V, std::max<int64_t>(64, (int64_t)(CE_PIECE / ((size_t)N * 4)) & ~(int64_t)63));
-    P.part = (float2*)take((size_t)N * 8);
-    P.z = (float*)take((size_t)N * P.cw * 4);
+    const size_t row = (size_t)CE_PARTS * tiles_up(d, 8) * 8 * 2;
+    P.cw = std::min<int64_t>(V, std::max<int64_t>(256, (int64_t)(CE_PIECE / row) & ~(int64_t)255));
+    P.act = (bf16_t*)take((size_t)N * row);
+    P.head = (bf16_t*)take((size_t)P.cw * row);
   }
   P.total = off;
   return P;
@@ -519,6 +538,9 @@ struct CEBwdPlan {
   void* act;
   void* G;
   float* part;  // [splits][N][d]
+  // fp32: a part's columns, and parts side by side and one below the other
+  int64_t wide;
+  bf16_t *act_along, *act_below, *head_along, *head_below, *G_along, *G_below;
   size_t total;
 };
 // Tiles and slices of the contraction of d_act = G head (N x d over cw columns a piece): its few tiles
@@ -544,23 +566,39 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   CEBwdPlan P{};
   size_t off = 0;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
-  const size_t esz = dtype == PD_DTYPE_BF16 ? 2 : 4;
-  P.cw = std::min<int64_t>((V + 7) & ~(int64_t)7, std::max<int64_t>(256, (int64_t)(CE_PIECE / ((size_t)N * esz)) & ~(int64_t)255));
-  P.big = ce_big(N, P.cw);
-  P.big_head = big_tiles(P.cw, d, N);
   P.count = (int32_t*)take(4);
   P.rows = (int32_t*)take((size_t)N * 4);
   P.pos = (int32_t*)take((size_t)N * 4);
-  P.act = take((size_t)N * d * esz);
-  P.G = take((size_t)N * P.cw * esz);
-  P.splits = 1;
-  if (dact) {
-    if (dtype == PD_DTYPE_BF16) {
-      ce_dact_form(N, d, P.cw, V, P.big_act, P.splits);
-    }
-    P.part = (float*)take((size_t)P.splits * N * d * 4);
+  const int64_t V8 = (V + 7) & ~(int64_t)7;
+  auto piece = [&](size_t total, size_t bytes) {  // columns of so many bytes
+    return std::min<int64_t>(V8, std::max<int64_t>(256, (int64_t)(total / bytes) & ~(int64_t)255));
+  };
+  if (dtype == PD_DTYPE_BF16) {
+    P.cw = std::min(piece(CE_PIECE, (size_t)N * 2), ce_head_rows(d));
+    P.act = take((size_t)N * d * 2);
+    P.G = take((size_t)N * P.cw * 2);
+    P.splits = 1;
+    if (dact) ce_dact_form(N, d, P.cw, V, P.big_act, P.splits);
+    P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
+  } else {
+    // a column's logits, both forms of its G and of its row of the head
+    P.wide = tiles_up(d, 8) * 8;
+    P.cw = piece(2 * CE_PIECE, (size_t)N * (4 + 2 * CE_PARTS * 2) + (size_t)P.wide * 2 * CE_PARTS * 2);
+    P.act = take((size_t)N * d * 4);
+    P.G = take((size_t)N * P.cw * 4);
+    P.act_along = (bf16_t*)take((size_t)N * P.wide * CE_PARTS * 2);
+    P.act_below = (bf16_t*)take((size_t)N * P.wide * CE_PARTS * 2);
+    P.head_along = (bf16_t*)take((size_t)P.cw * P.wide * CE_PARTS * 2);
+    P.head_below = (bf16_t*)take((size_t)P.cw * P.wide * CE_PARTS * 2);
+    P.G_along = (bf16_t*)take((size_t)N * P.cw * CE_PARTS * 2);
+    P.G_below = (bf16_t*)take((size_t)N * P.cw * CE_PARTS * 2);
+    P.splits = 1;
+    if (dact) ce_dact_form(N, d, P.cw * CE_PARTS, V * CE_PARTS, P.big_act, P.splits);
+    P.slice = tiles_up(tiles_up(P.cw * CE_PARTS, P.splits), 64) * 64;
   }
-  P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
+  P.big = ce_big(N, P.cw);
+  P.big_head = big_tiles(P.cw, d, dtype == PD_DTYPE_BF16 ? N : CE_PARTS * N);
+  if (dact) P.part = (float*)take((size_t)P.splits * N * d * 4);
   P.total = off;
   return P;
 }
@@ -576,6 +614,11 @@ struct CEOnePlan {
   float *target, *slabs, *head;
   size_t total;
 };
+// bf16 with a head that one product takes and a softmax whose shortest chunk is below CE_KEPT; else the
+// two calls, one after the other.
+bool ce_one_form(int dtype, int64_t d, int64_t V) {
+  return dtype == PD_DTYPE_BF16 && V <= ce_head_rows(d) && (size_t)(256 + 128) * ((V + 7) & ~(int64_t)7) * 2 < CE_KEPT;
+}
 CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, char* base) {
   CEOnePlan P{};
   size_t off = 0;
@@ -614,6 +657,13 @@ void ce_launch(const GemmArgs& a, const typename EPI::Args& ea, int slices, bool
   else hipLaunchKernelGGL((k_gemm_dtl<CFG, TC, MODE, false, EPI, AMN, BMN>), grid, dim3(CFG::NT), 0, s, a, ea);
 }
 
+template <int SIDE>
+void ce_split(const float* src, int64_t rows, int64_t cols, int64_t ld, int64_t wide, int64_t rows_below, bf16_t* along,
+              bf16_t* below, hipStream_t s) {
+  hipLaunchKernelGGL(k_ce_parts<SIDE>, dim3((unsigned)std::min<int64_t>(cdiv(rows_below * wide, 256), 8192)), dim3(256), 0, s, src,
+                     rows, cols, ld, wide, rows_below, along, below);
+}
+
 int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
              const void* targets, int bits) {
   if (dtype != PD_DTYPE_F32 && dtype != PD_DTYPE_BF16)
@@ -624,9 +674,12 @@ int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const
   if (dtype == PD_DTYPE_BF16) {
     if (d % 8) return fail(PD_EUNSUPPORTED, std::string(what) + ": bf16 needs d to be a multiple of 8");
     if (N && (((uintptr_t)act | (uintptr_t)head) & 15)) return fail(PD_EINVAL, std::string(what) + ": 16-byte aligned tensors");
-    if (!dtl_fits(N, d, V, d) || !dtl_fits_mn(V, d) || !dtl_fits_mn(N, d))
-      return fail(PD_EUNSUPPORTED, std::string(what) + ": operands of 2 GiB or more");
+    if (!dtl_fits_mn(N, d) || d > 1 << 20)
+      return fail(PD_EUNSUPPORTED, std::string(what) + ": activations of 2 GiB or more");
   }
+  const int64_t wide = CE_PARTS * (((d + 7) & ~(int64_t)7) + 8);
+  if (dtype == PD_DTYPE_F32 && (!dtl_fits(N, wide, N, CE_PARTS * 256) || !dtl_fits_mn(CE_PARTS * N, wide / CE_PARTS)))
+    return fail(PD_EUNSUPPORTED, std::string(what) + ": fp32 takes N d up to 1.7 10^8 and N up to 690000");
   if (tiles_up(N, 128) > 65535 || tiles_up(V, 128) > 65535 || N > (int64_t)1 << 21)
     return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
   return PD_OK;
@@ -667,25 +720,33 @@ int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
       a.A = P.act;
       a.offsets = P.count;
     }
-    if (P.big)
-      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t}, 1,
-                                                                               d % 64 != 0, s);
-    else
-      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t},
-                                                                                   1, d % 64 != 0, s);
+    for (int64_t c = 0, most = ce_head_rows(d); c < V; c += most) {
+      a.N = std::min(most, V - c);
+      a.B = (const bf16_t*)head + c * d;
+      if (P.big)
+        ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1,
+                                                                                 d % 64 != 0, s);
+      else
+        ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(
+            a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1, d % 64 != 0, s);
+    }
     hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, P.rows,
                        P.count, t, loss, (float2*)stats, nullptr);
     return check_launch(what);
   }
+  const int64_t wide = tiles_up(d, 8) * 8, K = CE_PARTS * wide;
+  ce_split<0>((const float*)act, N, d, d, wide, N, P.act, nullptr, s);
   for (int64_t c = 0; c < V; c += P.cw) {
     const int64_t w = std::min(P.cw, V - c);
-    if (int rc = pd_gemm(PD_DTYPE_F32, N, w, d, act, d, 0, (const float*)head + c * d, d, 1, P.z, P.cw, PD_DTYPE_F32, 1.f,
-                         0.f, stream))
-      return rc;
-    hipLaunchKernelGGL(k_ce_piece_stats, dim3((unsigned)N), dim3(256), 0, s, P.z, w, P.cw, c, t, P.part, P.target);
+    ce_split<1>((const float*)head + c * d, w, d, d, wide, w, P.head, nullptr, s);
+    const GemmArgs a{N, w, K, P.act, K, P.head, K, nullptr, 0, 1.f, 0.f, nullptr, 0, 0, 0, cdiv(K, 64) * 64, nullptr, nullptr, nullptr};
+    if (P.big)
+      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, nullptr, t, c}, 1, K % 64 != 0, s);
+    else
+      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(a, {P.part, P.n_tiles, P.target, nullptr, t, c}, 1, K % 64 != 0, s);
   }
-  hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, (int64_t)1, nullptr,
-                     nullptr, t, loss, (float2*)stats, nullptr);
+  hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, nullptr, nullptr, t,
+                     loss, (float2*)stats, nullptr);
   return check_launch(what);
 }
 
@@ -737,31 +798,44 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
                          P.part, P.splits, N * d, N, d, P.pos, (int64_t)0, N, (bf16_t*)d_act);
     return check_launch(what);
   }
-  float *act_c = (float*)P.act, *G = (float*)P.G;
+  float *act_c = (float*)P.act, *z = (float*)P.G;
+  const int64_t K = CE_PARTS * P.wide;
   hipLaunchKernelGGL(k_ce_gather_f32, dim3((unsigned)std::min<int64_t>(cdiv(N * d, 256), 4096)), dim3(256), 0, s,
                      (const float*)act, N, d, P.rows, P.count, act_c);
+  ce_split<0>(act_c, N, d, d, P.wide, N, P.act_along, nullptr, s);
+  ce_split<1>(act_c, N, d, d, P.wide, N, nullptr, P.act_below, s);
   for (int64_t c = 0; c < V; c += P.cw) {
-    const int64_t w = std::min(P.cw, V - c);
-    const float* h = (const float*)head + c * d;
-    int rc = pd_gemm(PD_DTYPE_F32, N, w, d, act_c, d, 0, h, d, 1, G, P.cw, PD_DTYPE_F32, 1.f, 0.f, stream);
-    if (rc) return rc;
-    hipLaunchKernelGGL(k_ce_piece_grad, dim3((unsigned)N), dim3(256), 0, s, G, w, P.cw, c, t, (const float2*)stats, g, P.rows,
-                       P.count);
-    if (d_act && (rc = pd_gemm(PD_DTYPE_F32, N, d, w, G, P.cw, 0, h, d, 0, P.part, d, PD_DTYPE_F32, 1.f, c ? 1.f : 0.f, stream)))
-      return rc;
-    if (d_head && (rc = pd_gemm(PD_DTYPE_F32, w, d, N, G, P.cw, 1, act_c, d, 0, (float*)d_head + c * d, d, PD_DTYPE_F32, 1.f,
-                                0.f, stream)))
-      return rc;
+    const int64_t w = std::min(P.cw, V - c), w8 = (w + 7) & ~(int64_t)7;
+    ce_split<1>((const float*)head + c * d, w, d, d, P.wide, w8, P.head_along, P.head_below, s);
+    const GemmArgs a{N, w, K, P.act_along, K, P.head_along, K, z, w8, 1.f, 0.f, nullptr, 0, 0, 0, cdiv(K, 64) * 64, nullptr, nullptr, nullptr};
+    if (P.big) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, false>(a, {}, 1, K % 64 != 0, s);
+    else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, false>(a, {}, 1, K % 64 != 0, s);
+    hipLaunchKernelGGL(k_ce_parts_grad, dim3((unsigned)N, (unsigned)std::min<int64_t>(cdiv(w8, 1024), 64)), dim3(256), 0, s, z, N, w,
+                       w8, c, t, (const float2*)stats, g, P.rows, P.count, P.G_along, P.G_below);
+    if (d_act) {
+      const int64_t kw = CE_PARTS * w8;
+      const GemmArgs b{N, d, kw, P.G_along, kw, P.head_below, P.wide, P.part, d, 1.f, c ? 1.f : 0.f, nullptr, 0, 0, N * d, P.slice,
+                       nullptr, nullptr, nullptr};
+      if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, kw % 64 != 0, s);
+      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, kw % 64 != 0, s);
+    }
+    if (d_head) {
+      const int64_t kn = CE_PARTS * N;
+      const GemmArgs b{w, d, kn, P.G_below, w8, P.act_below, P.wide, (float*)d_head + c * d, d, 1.f, 0.f, nullptr, 0, 0, 0,
+                       cdiv(kn, 64) * 64, nullptr, nullptr, nullptr};
+      if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, true, true>(b, {}, 1, kn % 64 != 0, s);
+      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, true, true>(b, {}, 1, kn % 64 != 0, s);
+    }
   }
   if (d_act)
     hipLaunchKernelGGL(k_ce_scatter<float>, dim3((unsigned)std::min<int64_t>(cdiv(N * d, 256), 8192)), dim3(256), 0, s, P.part,
-                       1, N * d, N, d, P.pos, (int64_t)0, N, (float*)d_act);
+                       P.splits, N * d, N, d, P.pos, (int64_t)0, N, (float*)d_act);
   return check_launch(what);
 }
 
 size_t pd_streamed_ce_train_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
   if (N <= 0 || d <= 0 || V <= 0) return 0;
-  if (dtype == PD_DTYPE_BF16) return ce_one_plan(N, d, V, want_dact, want_dhead, nullptr).total;
+  if (ce_one_form(dtype, d, V)) return ce_one_plan(N, d, V, want_dact, want_dhead, nullptr).total;
   return up256((size_t)N * 8) + std::max(ce_fwd_plan(dtype, N, d, V, nullptr).total,
                                          ce_bwd_plan(dtype, N, d, V, want_dact, nullptr).total);
 }
@@ -775,7 +849,7 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
   const size_t need = pd_streamed_ce_train_workspace_size(dtype, N, d, V, d_act != nullptr, d_head != nullptr);
   if (!workspace || workspace_bytes < need) return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
   hipStream_t s = (hipStream_t)stream;
-  if (dtype != PD_DTYPE_BF16) {
+  if (!ce_one_form(dtype, d, V)) {
     float* stats = (float*)workspace;
     char* ws = (char*)workspace + up256((size_t)N * 8);
     const size_t left = workspace_bytes - up256((size_t)N * 8);

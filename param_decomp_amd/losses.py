@@ -352,6 +352,12 @@ class _StreamedCE(torch.autograd.Function):
                                                 want_dact=want[0], want_dhead=want[1]), None, None)
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Dense and from a 16-byte boundary on, as the products take it."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, *,
                                     ignore_index: int = -100) -> torch.Tensor:
     """Per-position cross entropy of the logits `act @ head^T` against `targets`, without keeping the
@@ -367,7 +373,7 @@ def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targe
         act, head = torch.nn.functional.pad(act, (0, pad)), torch.nn.functional.pad(head, (0, pad))
     if targets.shape != lead:
         raise L.PDError(f"streamed_position_cross_entropy: targets are {tuple(lead)}, got {tuple(targets.shape)}")
-    a, h, t = act.reshape(-1, d + pad).contiguous(), head.contiguous(), targets.reshape(-1).contiguous()
+    a, h, t = _aligned(act.reshape(-1, d + pad)), _aligned(head), targets.reshape(-1).contiguous()
     if ops.differentiated(a, h):
         loss = _StreamedCE.apply(a, h, t, int(ignore_index))
     else:

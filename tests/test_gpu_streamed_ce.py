@@ -1,11 +1,14 @@
 """The streamed cross entropy against the formula in 64 bits.
 
-Tolerances: a logit is a sum of d products in fp32, off by at most (d + 1) 2^-24 sum |act head| =: e. The
+Tolerances: a logit is a sum of n = d products in fp32, off by at most (n + 1) 2^-24 sum |act head| =: e. An fp32
+product is the sum of six of bf16 parts, what is left out below 2^-24 of it: n counts them, and 1 more each. The
 loss is a difference of two of them and of a logarithm: 2 e and 16 2^-24 of what is added (it, the largest
 logit's distance, 1). G's entries are off by (2 e + 16 2^-24) p g and, in bf16, by half a step (2^-8 of
 them; the one-call form rounds to 2^-12 of them before, in fp16 relative to the largest of 64 neighbours:
 2^15 p / p_max has steps of 2^-24 at least, which is 2^-39 of p_max <= 1, so 2^-40 g more); what is summed from them likewise times the other
-operand, with n 2^-24 of the sum of magnitudes for n terms, and half a step of the result."""
+operand, with n 2^-24 of the sum of magnitudes for n terms, and half a step of the result. The matrix cores take and give
+no denormal numbers: each part of an entry, product and sum may be off by 2^-126 besides (the entries of G go down
+to 10^-36 where logits are large, and their third parts to 10^-41)."""
 
 import pytest
 import torch
@@ -17,6 +20,7 @@ pytestmark = pytest.mark.gpu
 
 F64, BF16, F32 = torch.float64, torch.bfloat16, torch.float32
 U = 2.0**-24
+TINY = 2.0**-126
 HALF = {BF16: 2.0**-8, F32: U}
 
 
@@ -38,7 +42,8 @@ def _expected(act, head, t, w):
     on = (t >= 0) & (t < V)
     a = torch.where(on[:, None], a, torch.zeros_like(a))
     w = torch.where(on, w, torch.zeros_like(w))
-    z, e = a @ h.T, (d + 1) * U * (a.abs() @ h.abs().T)
+    many = 1 if dt == BF16 else 7  # products and roundings for each
+    z, e = a @ h.T, (many * d + 1) * U * (a.abs() @ h.abs().T)
     at = t.long().clamp(0, V - 1)[:, None]
     lp = torch.log_softmax(z, -1)
     loss = torch.where(on, -lp.gather(1, at)[:, 0], torch.zeros(N, dtype=F64, device=z.device))
@@ -50,10 +55,11 @@ def _expected(act, head, t, w):
     bG = bG + (HALF[dt] + (2.0**-12 if dt == BF16 else 0)) * (G.abs() + bG)
     if dt == BF16:
         bG = bG + 2.0**-40 * w.abs()[:, None]
+    bG = bG + 3 * TINY
     da, dh = G @ h, G.T @ a
-    ba = bG @ h.abs() + (V + 64) * U * (G.abs() @ h.abs())
-    bh = bG.T @ a.abs() + (N + 64) * U * (G.abs().T @ a.abs())
-    return (loss, da, dh), (bl, ba + HALF[dt] * (da.abs() + ba) + 1e-40, bh + HALF[dt] * (dh.abs() + bh) + 1e-40)
+    ba = bG @ h.abs() + (many * V + 64) * U * (G.abs() @ h.abs())
+    bh = bG.T @ a.abs() + (many * N + 64) * U * (G.abs().T @ a.abs())
+    return (loss, da, dh), (bl, ba + HALF[dt] * (da.abs() + ba) + 2 * many * V * TINY, bh + HALF[dt] * (dh.abs() + bh) + 2 * many * N * TINY)
 
 
 def _check(got, want, bounds):
@@ -183,6 +189,46 @@ def test_pieces_of_the_vocabulary_and_chunks_of_positions(device):
         bh += bounds[2] * 11
     for got in (one, two):
         _check((got[0][:0], got[1][:0], got[2]), (dh[:0, 0], dh[:0], dh), (bh[:0, 0], bh[:0], bh))
+
+
+def test_a_head_of_more_than_2_gib(device):
+    act, head, t, w = _inputs(device, 5, 4096, 263000, BF16, 13)
+    t[3] = 262999
+    got = _both_forms(act, head, t, w)
+    z = torch.cat([act.double() @ head[c:c + 65536].double().T for c in range(0, 263000, 65536)], -1)
+    e = 4097 * U * torch.cat([act.double().abs() @ head[c:c + 65536].double().abs().T for c in range(0, 263000, 65536)], -1).amax(-1)
+    loss = torch.logsumexp(z, -1) - z.gather(1, t[:, None])[:, 0]
+    G = torch.softmax(z, -1).scatter_add(1, t[:, None], -torch.ones(5, 1, dtype=F64, device=device)) * w.double()[:, None]
+    bG = (2 * e[:, None] + 16 * U + 2.0**-8 + 2.0**-12) * 2 * G.abs() + 2.0**-40 * w.abs()[:, None]
+    da, ba = torch.zeros(5, 4096, dtype=F64, device=device), torch.zeros(5, 4096, dtype=F64, device=device)
+    for c in range(0, 263000, 65536):
+        h = head[c:c + 65536].double()
+        da += G[:, c:c + 65536] @ h
+        ba += (bG + 264000 * U * G.abs())[:, c:c + 65536] @ h.abs()
+        dh, bh = G[:, c:c + 65536].T @ act.double(), (bG + 70 * U * G.abs())[:, c:c + 65536].T @ act.double().abs()
+        for g in got:
+            assert ((g[2][c:c + 65536].double() - dh).abs() <= bh + 2.0**-8 * (dh.abs() + bh) + 1e-36).all()
+    for g in got:
+        assert ((g[0].double() - loss).abs() <= 2 * e + 16 * U * (1 + loss.abs() + 20)).all()
+        assert ((g[1].double() - da).abs() <= ba + 2.0**-8 * (da.abs() + ba)).all()
+
+
+def test_unaligned_views(device):
+    act, head, t, w = _inputs(device, 20, 64, 300, BF16, 14)
+    flat = torch.empty(20 * 64 + 3, dtype=BF16, device=device)
+    flat[3:] = act.view(-1)
+    a = losses.streamed_position_cross_entropy(act, head, t)
+    assert torch.equal(a, losses.streamed_position_cross_entropy(flat[3:].view(20, 64), head, t))
+    with pytest.raises(L.PDError, match="aligned"):
+        ops.streamed_cross_entropy_fwd(flat[3:].view(20, 64), head, t)
+
+
+def test_pieces_of_fp32(device):
+    """More than 2 GiB of logits, of parts of G and of the head's in the backward (28 bytes a logit)."""
+    act, head, t, w = _inputs(device, 1100, 24, 80000, F32, 12, 0.1)
+    want, bounds = _expected(act, head, t, w)
+    for got in _both_forms(act, head, t, w):
+        _check(got, want, bounds)
 
 
 def test_twice_the_same_and_on_other_streams(device):

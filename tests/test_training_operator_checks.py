@@ -65,7 +65,8 @@ def test_cross_entropy_entry_points_refuse():
         return lib.pd_streamed_ce_fwd(c["dtype"], c["N"], c["d"], c["V"], b, b, b, c["bits"], -100, b, None, b, ws, None)
 
     for kw, rc in ((dict(dtype=5), 3), (dict(d=12), 3), (dict(V=0), 1), (dict(N=-1), 1), (dict(bits=16), 1),
-                   (dict(N=(1 << 21) + 1), 3), (dict(V=1 << 24), 3), (dict(ws=16), 4)):
+                   (dict(N=(1 << 21) + 1), 3), (dict(V=1 << 24), 3), (dict(N=1 << 20, d=1024), 3),
+                   (dict(dtype=L.F32, N=1 << 20, d=8), 3), (dict(ws=16), 4)):
         assert fwd(**kw) == rc, kw
     assert fwd(N=0) == 0
     size = lib.pd_streamed_ce_train_workspace_size
@@ -106,7 +107,7 @@ def test_route_scores_entry_points_refuse():
     f = L.load().pd_route_scores_fwd
     args = lambda **k: [b, k.get("dt", 0), k.get("T", 4), k.get("E", 8), k.get("k", 2), 0, None, k.get("g", 1),  # noqa: E731
                         k.get("top", 1), 1, k.get("scale", 1.0), k.get("w", b), b, None]
-    for kw, rc in ((dict(dt=2), 3), (dict(T=-1), 1), (dict(k=9), 1), (dict(E=2000), 3), (dict(E=100, k=65), 3),
+    for kw, rc in ((dict(dt=2), 3), (dict(T=-1), 1), (dict(T=1 << 26), 3), (dict(k=9), 1), (dict(E=2000), 3), (dict(E=100, k=65), 3),
                    (dict(g=3), 1), (dict(g=8, top=1), 1), (dict(scale=float("nan")), 1), (dict(w=None), 1)):
         assert f(*args(**kw)) == rc, kw
     assert f(*args(T=0)) == 0
