@@ -370,7 +370,7 @@ __global__ void k_ce_counts(const int32_t* __restrict__ count, int64_t R, int ch
 // G = g (softmax - 1_t) in bf16 over what EpiCEKeep kept, in place: the values of each CE_SPAN
 // columns times e^{their m - m} g / s. A position of weight zero gets zeros whatever it holds, and so
 // does its row of the activations: d_head's product has 0 times it. Blocks: a row, 8192 columns of it.
-__global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int64_t ld, const float2* __restrict__ part,
+__global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int64_t ld, int64_t cols, const float2* __restrict__ part,
                                                   int64_t n_tiles, const float2* __restrict__ st,
                                                   const float* __restrict__ target, const int32_t* __restrict__ rows,
                                                   const int32_t* __restrict__ count, CETargets t, const float* __restrict__ g,
@@ -391,14 +391,14 @@ __global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int6
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t c = c0 + k * 2048;
-    if (c >= ld) continue;
+    if (c >= cols) continue;
     w[k] = *(const uint4*)(e + c);
     f[k] = ce_exp(part[row * n_tiles + c / CE_SPAN].x - o.x) * by;
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t c = c0 + k * 2048;
-    if (c >= ld) continue;
+    if (c >= cols) continue;
     const uint32_t in[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
     uint32_t out[4];
 #pragma unroll
@@ -488,6 +488,10 @@ typedef CfgDtlBig CfgBig;
 // an operand stored along the other axis may reach).
 int64_t ce_head_rows(int64_t d) { return (0x7FFFFFFF / (2 * d) - 128) & ~(int64_t)255; }
 
+// Row pitch of G: whole 128-byte lines, an odd number of them (rows a power of two apart are in the same
+// memory channels).
+int64_t ce_pitch(int64_t cols) { return (tiles_up(cols, 64) | 1) * 64; }
+
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // Positions from which the forward leaves out those that do not count: one row of tiles saves nothing.
@@ -531,7 +535,7 @@ CEFwdPlan ce_fwd_plan(int dtype, int64_t N, int64_t d, int64_t V, char* base) {
 
 struct CEBwdPlan {
   bool big, big_act, big_head;
-  int64_t cw;  // columns of a piece
+  int64_t cw, ld;  // columns of a piece, G's row pitch
   int splits;
   int64_t slice;
   int32_t *rows, *pos, *count;
@@ -576,7 +580,8 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   if (dtype == PD_DTYPE_BF16) {
     P.cw = std::min(piece(CE_PIECE, (size_t)N * 2), ce_head_rows(d));
     P.act = take((size_t)N * d * 2);
-    P.G = take((size_t)N * P.cw * 2);
+    P.ld = ce_pitch(P.cw);
+    P.G = take((size_t)N * P.ld * 2);
     P.splits = 1;
     if (dact) ce_dact_form(N, d, P.cw, V, P.big_act, P.splits);
     P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
@@ -617,13 +622,13 @@ struct CEOnePlan {
 // bf16 with a head that one product takes and a softmax whose shortest chunk is below CE_KEPT; else the
 // two calls, one after the other.
 bool ce_one_form(int dtype, int64_t d, int64_t V) {
-  return dtype == PD_DTYPE_BF16 && V <= ce_head_rows(d) && (size_t)(256 + 128) * ((V + 7) & ~(int64_t)7) * 2 < CE_KEPT;
+  return dtype == PD_DTYPE_BF16 && V <= ce_head_rows(d) && (size_t)(256 + 128) * ce_pitch(V) * 2 < CE_KEPT;
 }
 CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, char* base) {
   CEOnePlan P{};
   size_t off = 0;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
-  P.ld = (V + 7) & ~(int64_t)7;
+  P.ld = ce_pitch(V);
   P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * 2)) - 128) & ~(int64_t)255);
   if (P.R <= 0) P.R = N;
   P.chunks = (int)cdiv(N, P.R);
@@ -778,17 +783,17 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
       GemmArgs a{N, w, d, act_c, d, h, d, nullptr, 0, 1.f, 0.f, P.count, 0, 0, 0, cdiv(d, 64) * 64, nullptr, nullptr, nullptr};
       if (P.big)
         ce_launch<CfgBig, float, MODE_COUNTED, EpiCEGrad<CfgBig>, false, false>(
-            a, {(const float2*)stats, g, P.rows, t, c, G, P.cw}, 1, d % 64 != 0, s);
+            a, {(const float2*)stats, g, P.rows, t, c, G, P.ld}, 1, d % 64 != 0, s);
       else
         ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEGrad<CfgSmall>, false, false>(
-            a, {(const float2*)stats, g, P.rows, t, c, G, P.cw}, 1, d % 64 != 0, s);
+            a, {(const float2*)stats, g, P.rows, t, c, G, P.ld}, 1, d % 64 != 0, s);
       if (d_act) {  // slabs [splits][N][d] += G [count, w] head [w, d], a slice of w each
-        GemmArgs b{N, d, w, G, P.cw, h, d, P.part, d, 1.f, c ? 1.f : 0.f, P.count, 0, 0, N * d, P.slice, nullptr, nullptr, nullptr};
+        GemmArgs b{N, d, w, G, P.ld, h, d, P.part, d, 1.f, c ? 1.f : 0.f, P.count, 0, 0, N * d, P.slice, nullptr, nullptr, nullptr};
         if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, w % 64 != 0, s);
         else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, w % 64 != 0, s);
       }
       if (d_head) {  // [w, d] = G^T act over the positions that count
-        GemmArgs b{w, d, N, G, P.cw, act_c, d, (bf16_t*)d_head + c * d, d, 1.f, 0.f, P.count, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+        GemmArgs b{w, d, N, G, P.ld, act_c, d, (bf16_t*)d_head + c * d, d, 1.f, 0.f, P.count, 0, 0, 0, 0, nullptr, nullptr, nullptr};
         if (P.big_head) ce_launch<CfgBig, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
         else ce_launch<CfgSmall, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
       }
@@ -879,7 +884,7 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
       ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
     hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
                        loss, nullptr, P.stats);
-    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(P.ld, 8192)), dim3(256), 0, s, P.E, P.ld, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)(P.act + c * R * d), d / 8);
+    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(V, 8192)), dim3(256), 0, s, P.E, P.ld, (V + 7) & ~(int64_t)7, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)(P.act + c * R * d), d / 8);
     if (d_act) {
       GemmArgs b{M, d, V, P.E, P.ld, hd, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
       if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
