@@ -754,8 +754,8 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
  * The backward gives d_act [N, d] and d_head [V, d] (in dtype, each nullable) of sum g_i loss_i, g
  * fp32 [N]: G = g (softmax(z) - 1_target), d_act = G head, d_head = G^T act, going over the vocabulary
  * in pieces of G of at most 1 GiB. With bf16 G enters both products rounded to bf16. Positions of
- * g = 0 do not count either. Bit-identical from call to call. N up to 2^21, bf16 activations below 2 GiB; fp32, whose
- * products are those of three bf16 parts of each operand: N d up to 1.7 10^8, N up to 690000. */
+ * g = 0 do not count either. Bit-identical from call to call. N up to 2^21, bf16 activations below 2 GiB.
+ * fp32 operands enter the products as three bf16 parts each, with fp32 sums. */
 size_t pd_streamed_ce_fwd_workspace_size(int dtype, int64_t N, int64_t d, int64_t V);
 int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
                        const void* targets, int target_bits, int64_t ignore_index, float* loss, float* stats,

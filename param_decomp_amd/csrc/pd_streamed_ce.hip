@@ -16,9 +16,9 @@
 // what they hold reaches nothing. How many count only the device knows: grids cover all positions
 // and the products read the count (MODE_COUNTED).
 //
-// fp32 operands go through the same bf16 products as three bf16 parts each (8 + 8 + 8 bits, exact): the six
-// products of parts that reach 2^-24 of the whole are one contraction six times as long. 1003 x 1000 over
-// 32003 with gradients: XX us; fp32 products on the matrix cores are a sixteenth of bf16's rate.
+// fp32: the matrix cores take bf16 at sixteen times fp32's rate, so each operand enters as three bf16 parts
+// (8 + 8 + 8 bits: exact) and a product as the six products of parts that reach 2^-24 of it, with fp32 sums. The
+// parts are formed between a tile's loads and LDS (k_gemm_parts).
 #include <algorithm>
 #include <cmath>
 
@@ -80,23 +80,22 @@ __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* _
   if (threadIdx.x == 0) *count = base;
 }
 
-// dst[r] = src[rows[r]] for r < count (words of 16 bytes, n a row); ZERO: zeros for the rest.
-template <bool ZERO>
-__global__ __launch_bounds__(256) void k_ce_gather(const uint4* __restrict__ src, int64_t N, int64_t n,
-                                                   const int32_t* __restrict__ rows, const int32_t* __restrict__ count,
-                                                   uint4* __restrict__ dst) {
-  const int64_t held = *count, total = (ZERO ? N : held) * n;
+// dst[r] = src[rows[r]] for r < count, n words of T a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_ce_gather(const T* __restrict__ src, int64_t n, const int32_t* __restrict__ rows,
+                                                   const int32_t* __restrict__ count, T* __restrict__ dst) {
+  const int64_t total = *count * n;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / n;
-    dst[i] = r < held ? src[(int64_t)rows[r] * n + i % n] : make_uint4(0u, 0u, 0u, 0u);
+    dst[i] = src[(int64_t)rows[r] * n + (i - r * n)];
   }
 }
-__global__ __launch_bounds__(256) void k_ce_gather_f32(const float* __restrict__ src, int64_t N, int64_t d,
-                                                       const int32_t* __restrict__ rows,
-                                                       const int32_t* __restrict__ count, float* __restrict__ dst) {
-  const int64_t held = *count;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * d; i += (int64_t)gridDim.x * 256)
-    dst[i] = i / d < held ? src[(int64_t)rows[i / d] * d + i % d] : 0.f;
+void ce_gather(bool half, const void* src, int64_t N, int64_t d, const int32_t* rows, const int32_t* count, void* dst,
+               hipStream_t s) {
+  const int64_t n = half ? d / 8 : d;
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv(N * n, 256), 4096));
+  if (half) hipLaunchKernelGGL(k_ce_gather<uint4>, grid, dim3(256), 0, s, (const uint4*)src, n, rows, count, (uint4*)dst);
+  else hipLaunchKernelGGL(k_ce_gather<float>, grid, dim3(256), 0, s, (const float*)src, n, rows, count, (float*)dst);
 }
 
 // d_act[i] = the sum over `slabs` of the row of position i, of the positions whose place is in
@@ -420,64 +419,177 @@ __global__ __launch_bounds__(256) void k_ce_round(const float4* __restrict__ src
 }
 
 // ---------------------------------------------------------------- fp32 as parts of bf16
-// The products of parts a_i b_j, i + j <= 4, and which part of each operand a segment of the contraction holds.
-constexpr int CE_PARTS = 6;
-__device__ constexpr int CE_PART_A[CE_PARTS] = {0, 0, 0, 1, 1, 2}, CE_PART_B[CE_PARTS] = {0, 1, 2, 0, 1, 0};
+// EpiCEGrad with G in fp32, straight from the registers.
+template <class CFG>
+struct EpiCEGradF {
+  static constexpr int LDS_BYTES = 0;
+  struct Args {
+    const float2* stats;
+    const float* g;
+    const int32_t* rows;
+    CETargets t;
+    int64_t first;
+    float* G;
+    int64_t ldg;  // a multiple of 4
+  };
+  template <class, typename>
+  __device__ static void run(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
+                             f32x16 (&z)[CFG::TM][CFG::TN], char*) {
+    const int lane = tid & 63;
+#pragma unroll
+    for (int i = 0; i < CFG::TM; ++i) {
+      const int64_t row = t.m0 + wm * CFG::WTM + i * 32 + (lane & 31);
+      if (row >= t.M) continue;
+      const int64_t r = a.rows[row];
+      const float2 st = a.stats[r];
+      const float g = a.g[r], gs = g / st.y;
+      const int64_t first = t.n0 + wn * CFG::WTN + 4 * (lane >> 5);
+      const int want = a.t.at(r) - (int)(a.first + first);
+#pragma unroll
+      for (int j = 0; j < CFG::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = j * 32 + 8 * q;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = expf(z[i][j][4 * q + e] - st.x);
+            v[e] = want == c + e ? -g * ((st.y - x) / st.y) : x * gs;
+          }
+          float* dst = a.G + row * a.ldg + first + c;
+          if (first + c + 3 < p.N) {
+            *(float4*)dst = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (first + c + e < p.N) dst[e] = v[e];
+          }
+        }
+    }
+  }
+};
 
-// x = p[0] + p[1] + p[2]; what is not finite is all in the first.
-__device__ inline void ce_parts(float x, bf16_t (&p)[3]) {
-#pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    p[i] = f32_to_bf16(x);
-    const float f = bf16_to_f32(p[i]);
-    x = fabsf(f) < INFINITY ? x - f : 0.f;
+struct __attribute__((packed, aligned(4))) CEWord {  // at any element's boundary
+  float v[4];
+};
+typedef float ce_f8 __attribute__((ext_vector_type(8)));
+// 8 floats from p on; EDGE: those from `left` on are zeros (none is read).
+template <bool EDGE>
+__device__ inline ce_f8 ce_load8(const float* __restrict__ p, int64_t left) {
+  ce_f8 v;
+  if (!EDGE || left >= 8) {
+    const CEWord a = *(const CEWord*)p, b = *(const CEWord*)(p + 4);
+    v = ce_f8{a.v[0], a.v[1], a.v[2], a.v[3], b.v[0], b.v[1], b.v[2], b.v[3]};
+  } else {
+    v = (ce_f8)0.f;
+    if (left > 0) v[0] = p[0];
+    if (left > 1) v[1] = p[1];
+    if (left > 2) v[2] = p[2];
+    if (left > 3) v[3] = p[3];
+    if (left > 4) v[4] = p[4];
+    if (left > 5) v[5] = p[5];
+    if (left > 6) v[6] = p[6];
   }
+  return v;
 }
-// rows x cols of src (row pitch ld) as segments of the contraction: SIDE 0 the parts of a product's left operand, 1
-// of its right one. `along` side by side in a row of CE_PARTS * wide (columns from cols to wide are zeros), `below`
-// one below the other, CE_PARTS * rows_below rows of `wide` (rows from `rows` on zeros); either may be NULL.
-template <int SIDE>
-__global__ __launch_bounds__(256) void k_ce_parts(const float* __restrict__ src, int64_t rows, int64_t cols, int64_t ld,
-                                                  int64_t wide, int64_t rows_below, bf16_t* __restrict__ along,
-                                                  bf16_t* __restrict__ below) {
-  const int64_t total = rows_below * wide;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / wide, c = i - r * wide;
-    bf16_t p[3] = {0, 0, 0};
-    if (r < rows && c < cols) ce_parts(src[r * ld + c], p);
-#pragma unroll
-    for (int s = 0; s < CE_PARTS; ++s) {
-      const bf16_t v = p[SIDE ? CE_PART_B[s] : CE_PART_A[s]];
-      if (along && r < rows) along[(r * CE_PARTS + s) * wide + c] = v;
-      if (below) below[(s * rows_below + r) * wide + c] = v;
-    }
-  }
+// Word u of a thread's share of an operand's stage: 8 values of a tile of R rows from `first` on (below `end`) and
+// 64 k from k0 on (below kend). K-major: row i / 8, chunk i % 8 of its k; MN-major: k-row i / (R / 8), chunk i % (R / 8).
+template <bool MN, int R, int NT, bool EDGE>
+__device__ inline ce_f8 ce_word(const float* __restrict__ base, int64_t ld, int64_t first, int64_t end, int64_t k0,
+                                int64_t kend, int u, int tid) {
+  const int i = tid + u * NT;
+  const int64_t x = first + (MN ? i % (R / 8) * 8 : i / 8), k = k0 + (MN ? i / (R / 8) : i % 8 * 8);
+  const int64_t left = EDGE && (x >= end || k >= kend) ? 0 : MN ? end - x : kend - k;
+  return ce_load8<EDGE>(base + (EDGE && left <= 0 ? 0 : MN ? k * ld + x : x * ld + k), left);
 }
-// The parts of G = g (softmax - 1_t), from the logits z [N][w] (pitch wide) of the rows that count; zeros for the others.
-__global__ __launch_bounds__(256) void k_ce_parts_grad(const float* __restrict__ z, int64_t N, int64_t w, int64_t wide,
-                                                       int64_t first, CETargets t, const float2* __restrict__ stats,
-                                                       const float* __restrict__ g, const int32_t* __restrict__ rows,
-                                                       const int32_t* __restrict__ count, bf16_t* __restrict__ along,
-                                                       bf16_t* __restrict__ below) {
-  const int64_t r = blockIdx.x;
-  const bool on = r < *count;
-  const int64_t i = on ? rows[r] : 0, want = on ? (int64_t)t.at(i) - first : -1;
-  const float2 st = on ? stats[i] : make_float2(0.f, 1.f);
-  const float gi = on ? g[i] : 0.f, gs = gi / st.y;
-  for (int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x; c < wide; c += (int64_t)gridDim.y * 256) {
-    float x = 0.f;
-    if (on && c < w) {
-      const float e = expf(z[r * wide + c] - st.x);
-      x = c == want ? -gi * ((st.y - e) / st.y) : e * gs;
-    }
-    bf16_t p[3];
-    ce_parts(x, p);
+template <bool MN, int R, int NT>
+__device__ inline char* ce_place(char* region, int u, int tid) {
+  const int i = tid + u * NT, row = MN ? i / (R / 8) : i / 8, c = MN ? i % (R / 8) : i % 8;
+  return region + (MN ? row * 2 * R + ((c ^ (4 * (row & 3))) << 4) : row * 128 + ((c ^ dtl_swz(row)) << 4));
+}
+// The three parts of 8 values, to the same place of each plane.
+__device__ inline void ce_parts8(char* at, int plane, ce_f8 v) {
+  uint32_t p[3][4];
 #pragma unroll
-    for (int s = 0; s < CE_PARTS; ++s) {
-      along[(r * CE_PARTS + s) * wide + c] = p[CE_PART_A[s]];
-      below[(s * N + r) * wide + c] = p[CE_PART_A[s]];
+  for (int k = 0; k < 4; ++k) {
+    float a = v[2 * k], b = v[2 * k + 1];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      p[i][k] = pack_bf16x2(a, b);
+      a -= __uint_as_float(p[i][k] << 16);
+      b -= __uint_as_float(p[i][k] & 0xFFFF0000u);
     }
   }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) *(uint4*)(at + i * plane) = make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]);
+}
+
+// C = op(A) op(B) as k_gemm_dtl gives it (the same tiles, LDS layout and epilogues), of fp32 operands (p.A and p.B
+// point to floats, lda and ldb count them) at any alignment. A stage of 64 k is loaded into registers while the
+// one before is multiplied, and goes to LDS as three planes of parts. Bound by what lies between the stages' two barriers: forming
+// and writing the parts (6 vector instructions a value) beside the fragments' reads.
+template <class CFG, int MODE, class EPI, bool AMN, bool BMN>
+__global__ __launch_bounds__(CFG::NT) void k_gemm_parts(GemmArgs p, typename EPI::Args ea) {
+  constexpr int BM = CFG::BM, BN = CFG::BN, TM = CFG::TM, TN = CFG::TN, PLANE = CFG::STAGE_BYTES;
+  constexpr int AW = BM * 8 / CFG::NT, BW = BN * 8 / CFG::NT;  // 8-value words of a thread
+  static_assert(BM * 8 % CFG::NT == 0 && BN * 8 % CFG::NT == 0, "whole words");
+  constexpr int LDS = 3 * PLANE > EPI::LDS_BYTES ? 3 * PLANE : EPI::LDS_BYTES;
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  const int wm = wave / CFG::WN, wn = wave % CFG::WN;
+  TileJob t;
+  if (!map_tile<BM, BN, MODE, float>(p, lane, t)) return;
+  const float *A = (const float*)p.A, *B = (const float*)p.B;
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+  ce_f8 wa[AW], wb[BW];
+  const bool whole = t.m0 + BM <= t.M && t.n0 + BN <= p.N;
+  auto load = [&](int64_t k0) {
+    if (whole && k0 + 64 <= t.kend) {
+#pragma unroll
+      for (int u = 0; u < AW; ++u) wa[u] = ce_word<AMN, BM, CFG::NT, false>(A, p.lda, t.m0, t.M, k0, t.kend, u, tid);
+#pragma unroll
+      for (int u = 0; u < BW; ++u) wb[u] = ce_word<BMN, BN, CFG::NT, false>(B, p.ldb, t.n0, p.N, k0, t.kend, u, tid);
+    } else {
+#pragma unroll
+      for (int u = 0; u < AW; ++u) wa[u] = ce_word<AMN, BM, CFG::NT, true>(A, p.lda, t.m0, t.M, k0, t.kend, u, tid);
+#pragma unroll
+      for (int u = 0; u < BW; ++u) wb[u] = ce_word<BMN, BN, CFG::NT, true>(B, p.ldb, t.n0, p.N, k0, t.kend, u, tid);
+    }
+  };
+  auto store = [&]() {
+#pragma unroll
+    for (int u = 0; u < AW; ++u) ce_parts8(ce_place<AMN, BM, CFG::NT>(smem, u, tid), PLANE, wa[u]);
+#pragma unroll
+    for (int u = 0; u < BW; ++u) ce_parts8(ce_place<BMN, BN, CFG::NT>(smem + BM * CFG::ROWB, u, tid), PLANE, wb[u]);
+  };
+  const FragOffs<CFG, AMN, BMN> fo(wm, wn, lane);
+  if (t.kbeg < t.kend) load(t.kbeg);
+  for (int64_t k0 = t.kbeg; k0 < t.kend; k0 += 64) {
+    __syncthreads();  // the last stage's fragments have been read
+    store();
+    __syncthreads();
+    if (k0 + 64 < t.kend) load(k0 + 64);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      Frags<CFG> f[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) read_frags<CFG>(smem + i * PLANE, fo, lane, kk, f[i]);
+      // the small ones first
+      dtl_mfma<CFG>(f[2].a, f[0].b, acc);
+      dtl_mfma<CFG>(f[0].a, f[2].b, acc);
+      dtl_mfma<CFG>(f[1].a, f[1].b, acc);
+      dtl_mfma<CFG>(f[1].a, f[0].b, acc);
+      dtl_mfma<CFG>(f[0].a, f[1].b, acc);
+      dtl_mfma<CFG>(f[0].a, f[0].b, acc);
+    }
+  }
+  EPI::template run<CFG, float>(p, ea, t, wm, wn, tid, acc, smem);
 }
 
 // ---------------------------------------------------------------- plans and launches
@@ -499,11 +611,11 @@ constexpr int64_t CE_COMPACT = 128;
 
 struct CEFwdPlan {
   bool compact, big;
-  int64_t n_tiles, cw;
+  int64_t n_tiles;
   int32_t *rows, *count;
   float* target;
   float2 *part;
-  bf16_t *act, *head;  // fp32: parts side by side, of a piece of cw rows of the head
+  void* act;
   size_t total;
 };
 bool ce_big(int64_t N, int64_t V) { return big_rounds(tiles_up(N, 256) * tiles_up(V, 256), tiles_up(N, 128) * tiles_up(V, 128), SHARED_ROUND); }
@@ -513,21 +625,14 @@ CEFwdPlan ce_fwd_plan(int dtype, int64_t N, int64_t d, int64_t V, char* base) {
   size_t off = 0;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
   P.target = (float*)take((size_t)N * 4);
-  P.big = ce_big(N, V);
+  P.big = dtype == PD_DTYPE_BF16 && ce_big(N, V);
   P.n_tiles = tiles_up(V, P.big ? 256 : 128);
   P.part = (float2*)take((size_t)N * P.n_tiles * 8);
-  if (dtype == PD_DTYPE_BF16) {
-    P.compact = N > CE_COMPACT;
-    if (P.compact) {
-      P.count = (int32_t*)take(4);
-      P.rows = (int32_t*)take((size_t)N * 4);
-      P.act = (bf16_t*)take((size_t)N * d * 2);
-    }
-  } else {
-    const size_t row = (size_t)CE_PARTS * tiles_up(d, 8) * 8 * 2;
-    P.cw = std::min<int64_t>(V, std::max<int64_t>(256, (int64_t)(CE_PIECE / row) & ~(int64_t)255));
-    P.act = (bf16_t*)take((size_t)N * row);
-    P.head = (bf16_t*)take((size_t)P.cw * row);
+  P.compact = N > CE_COMPACT;
+  if (P.compact) {
+    P.count = (int32_t*)take(4);
+    P.rows = (int32_t*)take((size_t)N * 4);
+    P.act = take((size_t)N * d * (dtype == PD_DTYPE_BF16 ? 2 : 4));
   }
   P.total = off;
   return P;
@@ -542,9 +647,6 @@ struct CEBwdPlan {
   void* act;
   void* G;
   float* part;  // [splits][N][d]
-  // fp32: a part's columns, and parts side by side and one below the other
-  int64_t wide;
-  bf16_t *act_along, *act_below, *head_along, *head_below, *G_along, *G_below;
   size_t total;
 };
 // Tiles and slices of the contraction of d_act = G head (N x d over cw columns a piece): its few tiles
@@ -553,13 +655,14 @@ struct CEBwdPlan {
 // count is not known here. us of 1 / 4 / 5 / 7 / 8 slices of 256x256 tiles: 8192 x 768 over 50277 columns 1466 /
 // 772 / 610 / 682 / 616 (128x128: 824 in 1, 724 in 4); 3072 of 4096 x 4096 over 131072 3921 / 3045 /
 // 3168 / 3446 / 3085, all 4096 3901 / 4009 / 4041 / 4089 / 4135.
-void ce_dact_form(int64_t N, int64_t d, int64_t cw, int64_t V, bool& big, int& splits) {
+void ce_dact_form(int64_t N, int64_t d, int64_t cw, int64_t V, bool half, bool& big, int& splits) {
   double best = 1e30;
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < (half ? 2 : 1); ++b)
     for (int sp = 1; sp <= 64 && (sp == 1 || cw / sp >= 1024); ++sp) {
-      const int64_t t = b ? 256 : 128, round = b ? 256 : 512;
-      auto rounds = [&](int64_t rows) { return (double)tiles_up(tiles_up(rows, t) * tiles_up(d, t) * sp, round); };
-      const double per_round = 2.0 * t * t * round * ((double)V / sp) / (b ? 1.2e15 : 1.0e15);
+      // 256x256 or two 128x128 a CU; fp32 one of 256x128 or 128x128
+      const int64_t tm = half ? (b ? 256 : 128) : (N > 128 ? 256 : 128), tn = b ? 256 : 128, round = b || !half ? 256 : 512;
+      auto rounds = [&](int64_t rows) { return (double)tiles_up(tiles_up(rows, tm) * tiles_up(d, tn) * sp, round); };
+      const double per_round = 2.0 * tm * tn * round * ((double)V / sp) / (b ? 1.2e15 : half ? 1.0e15 : 1.7e14);
       const double slabs = (double)sp * N * d * 4 * 2 * cdiv(V, cw) / 4e12;
       const double time = (0.75 * rounds(N) + 0.25 * rounds(cdiv(3 * N, 4))) * per_round + slabs;
       if (time < best) best = time, big = b, splits = sp;
@@ -574,35 +677,18 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   P.rows = (int32_t*)take((size_t)N * 4);
   P.pos = (int32_t*)take((size_t)N * 4);
   const int64_t V8 = (V + 7) & ~(int64_t)7;
-  auto piece = [&](size_t total, size_t bytes) {  // columns of so many bytes
-    return std::min<int64_t>(V8, std::max<int64_t>(256, (int64_t)(total / bytes) & ~(int64_t)255));
-  };
-  if (dtype == PD_DTYPE_BF16) {
-    P.cw = std::min(piece(CE_PIECE, (size_t)N * 2), ce_head_rows(d));
-    P.act = take((size_t)N * d * 2);
-    P.ld = ce_pitch(P.cw);
-    P.G = take((size_t)N * P.ld * 2);
-    P.splits = 1;
-    if (dact) ce_dact_form(N, d, P.cw, V, P.big_act, P.splits);
-    P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
-  } else {
-    // a column's logits, both forms of its G and of its row of the head
-    P.wide = tiles_up(d, 8) * 8;
-    P.cw = piece(2 * CE_PIECE, (size_t)N * (4 + 2 * CE_PARTS * 2) + (size_t)P.wide * 2 * CE_PARTS * 2);
-    P.act = take((size_t)N * d * 4);
-    P.G = take((size_t)N * P.cw * 4);
-    P.act_along = (bf16_t*)take((size_t)N * P.wide * CE_PARTS * 2);
-    P.act_below = (bf16_t*)take((size_t)N * P.wide * CE_PARTS * 2);
-    P.head_along = (bf16_t*)take((size_t)P.cw * P.wide * CE_PARTS * 2);
-    P.head_below = (bf16_t*)take((size_t)P.cw * P.wide * CE_PARTS * 2);
-    P.G_along = (bf16_t*)take((size_t)N * P.cw * CE_PARTS * 2);
-    P.G_below = (bf16_t*)take((size_t)N * P.cw * CE_PARTS * 2);
-    P.splits = 1;
-    if (dact) ce_dact_form(N, d, P.cw * CE_PARTS, V * CE_PARTS, P.big_act, P.splits);
-    P.slice = tiles_up(tiles_up(P.cw * CE_PARTS, P.splits), 64) * 64;
-  }
-  P.big = ce_big(N, P.cw);
-  P.big_head = big_tiles(P.cw, d, dtype == PD_DTYPE_BF16 ? N : CE_PARTS * N);
+  const bool half = dtype == PD_DTYPE_BF16;
+  const size_t esz = half ? 2 : 4;
+  P.cw = std::min<int64_t>(V8, std::max<int64_t>(256, (int64_t)(CE_PIECE / ((size_t)N * esz)) & ~(int64_t)255));
+  if (half) P.cw = std::min(P.cw, ce_head_rows(d));
+  P.ld = ce_pitch(P.cw);
+  P.act = take((size_t)N * d * esz);
+  P.G = take((size_t)N * P.ld * esz);
+  P.splits = 1;
+  if (dact) ce_dact_form(N, d, P.cw, V, half, P.big_act, P.splits);
+  P.slice = tiles_up(tiles_up(P.cw, P.splits), 64) * 64;
+  P.big = half && ce_big(N, P.cw);
+  P.big_head = half && big_tiles(P.cw, d, N);
   if (dact) P.part = (float*)take((size_t)P.splits * N * d * 4);
   P.total = off;
   return P;
@@ -646,7 +732,7 @@ CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, ch
   P.target = (float*)take((size_t)P.R * 4);
   P.splits = 1;
   if (dact) {
-    ce_dact_form(P.R, d, V, V, P.big_act, P.splits);
+    ce_dact_form(P.R, d, V, V, true, P.big_act, P.splits);
     P.slabs = (float*)take((size_t)P.splits * P.R * d * 4);
   }
   P.slice = tiles_up(tiles_up(V, P.splits), 64) * 64;
@@ -662,12 +748,22 @@ void ce_launch(const GemmArgs& a, const typename EPI::Args& ea, int slices, bool
   else hipLaunchKernelGGL((k_gemm_dtl<CFG, TC, MODE, false, EPI, AMN, BMN>), grid, dim3(CFG::NT), 0, s, a, ea);
 }
 
-template <int SIDE>
-void ce_split(const float* src, int64_t rows, int64_t cols, int64_t ld, int64_t wide, int64_t rows_below, bf16_t* along,
-              bf16_t* below, hipStream_t s) {
-  hipLaunchKernelGGL(k_ce_parts<SIDE>, dim3((unsigned)std::min<int64_t>(cdiv(rows_below * wide, 256), 8192)), dim3(256), 0, s, src,
-                     rows, cols, ld, wide, rows_below, along, below);
+// 256 x 128 tiles from the second row of 128 x 128 ones on: 12 fragments read for 24 MFMAs of a wave in place of 9
+// for 12. 1003 x 1000 over 32003: the four products 512, 459, 452, 416 -> 392, 393, 375, 367 us, 170 TFLOP/s of the
+// product itself (fp32 MFMAs end at 157).
+typedef DtlCfg<256, 128, 4, 2, false> CfgParts;
+template <class CFG, int MODE, class EPI, bool AMN, bool BMN>
+void ce_launch_parts(const GemmArgs& a, const typename EPI::Args& ea, int slices, hipStream_t s) {
+  const dim3 grid((unsigned)tiles_up(a.N, CFG::BN), (unsigned)tiles_up(a.M, CFG::BM), (unsigned)slices);
+  hipLaunchKernelGGL((k_gemm_parts<CFG, MODE, EPI, AMN, BMN>), grid, dim3(CFG::NT), 0, s, a, ea);
 }
+template <int MODE, template <class> class EPI, bool AMN, bool BMN, class... Args>
+void ce_launch_f32(const GemmArgs& a, int slices, hipStream_t s, Args... args) {
+  if (a.M > 128) ce_launch_parts<CfgParts, MODE, EPI<CfgParts>, AMN, BMN>(a, {args...}, slices, s);
+  else ce_launch_parts<CfgSmall, MODE, EPI<CfgSmall>, AMN, BMN>(a, {args...}, slices, s);
+}
+template <class>
+using EpiCEStore = EpiStore;
 
 int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
              const void* targets, int bits) {
@@ -682,9 +778,6 @@ int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const
     if (!dtl_fits_mn(N, d) || d > 1 << 20)
       return fail(PD_EUNSUPPORTED, std::string(what) + ": activations of 2 GiB or more");
   }
-  const int64_t wide = CE_PARTS * (((d + 7) & ~(int64_t)7) + 8);
-  if (dtype == PD_DTYPE_F32 && (!dtl_fits(N, wide, N, CE_PARTS * 256) || !dtl_fits_mn(CE_PARTS * N, wide / CE_PARTS)))
-    return fail(PD_EUNSUPPORTED, std::string(what) + ": fp32 takes N d up to 1.7 10^8 and N up to 690000");
   if (tiles_up(N, 128) > 65535 || tiles_up(V, 128) > 65535 || N > (int64_t)1 << 21)
     return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
   return PD_OK;
@@ -713,44 +806,27 @@ int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
   if (!workspace || workspace_bytes < P.total) return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
   hipStream_t s = (hipStream_t)stream;
   const CETargets t{targets, target_bits, ignore_index, V};
-  if (dtype == PD_DTYPE_BF16) {
-    GemmArgs a{N, V, d, (const bf16_t*)act, d, (const bf16_t*)head, d, nullptr, 0, 1.f, 0.f, nullptr, 0, 0, 0, d,
-               nullptr, nullptr, nullptr};
-    a.strideA = cdiv(d, 64) * 64;  // one slice
-    if (P.compact) {
-      hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, nullptr, P.count, loss,
-                         (float2*)stats);
-      hipLaunchKernelGGL(k_ce_gather<false>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 8, 256), 4096)), dim3(256), 0, s,
-                         (const uint4*)act, N, d / 8, P.rows, P.count, (uint4*)P.act);
-      a.A = P.act;
-      a.offsets = P.count;
-    }
-    for (int64_t c = 0, most = ce_head_rows(d); c < V; c += most) {
-      a.N = std::min(most, V - c);
-      a.B = (const bf16_t*)head + c * d;
-      if (P.big)
-        ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1,
-                                                                                 d % 64 != 0, s);
-      else
-        ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(
-            a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1, d % 64 != 0, s);
-    }
-    hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, P.rows,
-                       P.count, t, loss, (float2*)stats, nullptr);
-    return check_launch(what);
+  const bool half = dtype == PD_DTYPE_BF16;
+  GemmArgs a{N, V, d, (const bf16_t*)act, d, (const bf16_t*)head, d, nullptr, 0, 1.f, 0.f, nullptr, 0, 0, 0, cdiv(d, 64) * 64,
+             nullptr, nullptr, nullptr};
+  if (P.compact) {
+    hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, nullptr, P.count, loss, (float2*)stats);
+    ce_gather(half, act, N, d, P.rows, P.count, P.act, s);
+    a.A = (const bf16_t*)P.act;
+    a.offsets = P.count;
   }
-  const int64_t wide = tiles_up(d, 8) * 8, K = CE_PARTS * wide;
-  ce_split<0>((const float*)act, N, d, d, wide, N, P.act, nullptr, s);
-  for (int64_t c = 0; c < V; c += P.cw) {
-    const int64_t w = std::min(P.cw, V - c);
-    ce_split<1>((const float*)head + c * d, w, d, d, wide, w, P.head, nullptr, s);
-    const GemmArgs a{N, w, K, P.act, K, P.head, K, nullptr, 0, 1.f, 0.f, nullptr, 0, 0, 0, cdiv(K, 64) * 64, nullptr, nullptr, nullptr};
+  if (!half) ce_launch_f32<MODE_COUNTED, EpiCEStats, false, false>(a, 1, s, P.part, P.n_tiles, P.target, (const int32_t*)P.rows, t);
+  for (int64_t c = 0, most = ce_head_rows(d); half && c < V; c += most) {
+    a.N = std::min(most, V - c);
+    a.B = (const bf16_t*)head + c * d;
     if (P.big)
-      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, nullptr, t, c}, 1, K % 64 != 0, s);
+      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEStats<CfgBig>, false, false>(a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1,
+                                                                               d % 64 != 0, s);
     else
-      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(a, {P.part, P.n_tiles, P.target, nullptr, t, c}, 1, K % 64 != 0, s);
+      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEStats<CfgSmall>, false, false>(
+          a, {P.part, P.n_tiles, P.target, P.rows, t, c}, 1, d % 64 != 0, s);
   }
-  hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, nullptr, nullptr, t,
+  hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(N, 4)), dim3(256), 0, s, P.part, P.target, N, P.n_tiles, P.rows, P.count, t,
                      loss, (float2*)stats, nullptr);
   return check_launch(what);
 }
@@ -775,8 +851,7 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
   hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, g, N, P.rows, P.pos, P.count, nullptr, nullptr);
   if (dtype == PD_DTYPE_BF16) {
     bf16_t *act_c = (bf16_t*)P.act, *G = (bf16_t*)P.G;
-    hipLaunchKernelGGL(k_ce_gather<false>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 8, 256), 4096)), dim3(256), 0, s,
-                       (const uint4*)act, N, d / 8, P.rows, P.count, (uint4*)act_c);
+    ce_gather(true, act, N, d, P.rows, P.count, act_c, s);
     for (int64_t c = 0; c < V; c += P.cw) {
       const int64_t w = std::min(P.cw, V - c);
       const bf16_t* h = (const bf16_t*)head + c * d;
@@ -803,33 +878,21 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
                          P.part, P.splits, N * d, N, d, P.pos, (int64_t)0, N, (bf16_t*)d_act);
     return check_launch(what);
   }
-  float *act_c = (float*)P.act, *z = (float*)P.G;
-  const int64_t K = CE_PARTS * P.wide;
-  hipLaunchKernelGGL(k_ce_gather_f32, dim3((unsigned)std::min<int64_t>(cdiv(N * d, 256), 4096)), dim3(256), 0, s,
-                     (const float*)act, N, d, P.rows, P.count, act_c);
-  ce_split<0>(act_c, N, d, d, P.wide, N, P.act_along, nullptr, s);
-  ce_split<1>(act_c, N, d, d, P.wide, N, nullptr, P.act_below, s);
+  float *act_c = (float*)P.act, *G = (float*)P.G;
+  ce_gather(false, act, N, d, P.rows, P.count, act_c, s);
+  auto as = [](const float* p) { return (const bf16_t*)p; };  // as k_gemm_parts takes its operands
   for (int64_t c = 0; c < V; c += P.cw) {
-    const int64_t w = std::min(P.cw, V - c), w8 = (w + 7) & ~(int64_t)7;
-    ce_split<1>((const float*)head + c * d, w, d, d, P.wide, w8, P.head_along, P.head_below, s);
-    const GemmArgs a{N, w, K, P.act_along, K, P.head_along, K, z, w8, 1.f, 0.f, nullptr, 0, 0, 0, cdiv(K, 64) * 64, nullptr, nullptr, nullptr};
-    if (P.big) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, false>(a, {}, 1, K % 64 != 0, s);
-    else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, false>(a, {}, 1, K % 64 != 0, s);
-    hipLaunchKernelGGL(k_ce_parts_grad, dim3((unsigned)N, (unsigned)std::min<int64_t>(cdiv(w8, 1024), 64)), dim3(256), 0, s, z, N, w,
-                       w8, c, t, (const float2*)stats, g, P.rows, P.count, P.G_along, P.G_below);
+    const int64_t w = std::min(P.cw, V - c);
+    const float* h = (const float*)head + c * d;
+    const GemmArgs a{N, w, d, as(act_c), d, as(h), d, nullptr, 0, 1.f, 0.f, P.count, 0, 0, 0, cdiv(d, 64) * 64, nullptr, nullptr, nullptr};
+    ce_launch_f32<MODE_COUNTED, EpiCEGradF, false, false>(a, 1, s, (const float2*)stats, g, (const int32_t*)P.rows, t, c, G, P.ld);
     if (d_act) {
-      const int64_t kw = CE_PARTS * w8;
-      const GemmArgs b{N, d, kw, P.G_along, kw, P.head_below, P.wide, P.part, d, 1.f, c ? 1.f : 0.f, nullptr, 0, 0, N * d, P.slice,
-                       nullptr, nullptr, nullptr};
-      if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, kw % 64 != 0, s);
-      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, kw % 64 != 0, s);
+      const GemmArgs b{N, d, w, as(G), P.ld, as(h), d, P.part, d, 1.f, c ? 1.f : 0.f, P.count, 0, 0, N * d, P.slice, nullptr, nullptr, nullptr};
+      ce_launch_f32<MODE_COUNTED, EpiCEStore, false, true>(b, P.splits, s);
     }
     if (d_head) {
-      const int64_t kn = CE_PARTS * N;
-      const GemmArgs b{w, d, kn, P.G_below, w8, P.act_below, P.wide, (float*)d_head + c * d, d, 1.f, 0.f, nullptr, 0, 0, 0,
-                       cdiv(kn, 64) * 64, nullptr, nullptr, nullptr};
-      if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, true, true>(b, {}, 1, kn % 64 != 0, s);
-      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, true, true>(b, {}, 1, kn % 64 != 0, s);
+      const GemmArgs b{w, d, N, as(G), P.ld, as(act_c), d, (float*)d_head + c * d, d, 1.f, 0.f, P.count, 0, 0, 0, 0, nullptr, nullptr, nullptr};
+      ce_launch_f32<MODE_COUNTED_K, EpiCEStore, true, true>(b, 1, s);
     }
   }
   if (d_act)
@@ -868,8 +931,7 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
   const CETargets t{targets, target_bits, ignore_index, V};
   const bf16_t* hd = (const bf16_t*)head;
   hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, P.pos, P.count, loss, nullptr);
-  hipLaunchKernelGGL(k_ce_gather<false>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 8, 256), 4096)), dim3(256), 0, s,
-                     (const uint4*)act, N, d / 8, P.rows, P.count, (uint4*)P.act);
+  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
   hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
   for (int c = 0; c < P.chunks; ++c) {
     const int64_t R = P.R;

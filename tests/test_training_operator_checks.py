@@ -66,7 +66,7 @@ def test_cross_entropy_entry_points_refuse():
 
     for kw, rc in ((dict(dtype=5), 3), (dict(d=12), 3), (dict(V=0), 1), (dict(N=-1), 1), (dict(bits=16), 1),
                    (dict(N=(1 << 21) + 1), 3), (dict(V=1 << 24), 3), (dict(N=1 << 20, d=1024), 3),
-                   (dict(dtype=L.F32, N=1 << 20, d=8), 3), (dict(ws=16), 4)):
+                   (dict(ws=16), 4)):
         assert fwd(**kw) == rc, kw
     assert fwd(N=0) == 0
     size = lib.pd_streamed_ce_train_workspace_size
