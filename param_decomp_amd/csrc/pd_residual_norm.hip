@@ -16,6 +16,10 @@
 // row's sums. Runs end where a gate's group of rows ends or hold whole groups, so the gate of a
 // group and its gradient stay in registers; gradients of shared parameters are written as one
 // partial row a run (or wave) and added in a fixed order by a second kernel.
+//
+// Measured at 6 10^7 values, both streams and branch (bf16 and bf16; fp32 and fp32), a gate a sequence: forward
+// 106-110 us and 199-224 us from 64 to 4096 columns (4.4-4.8 TB/s; 768 in bf16 123 us, a quarter of its lanes idle and the sums
+// in 64 bits shown), backward with all gradients 156-164 us and 300-325 us (4.4-4.8 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -43,7 +47,8 @@ struct RnWord {
     else return __uint_as_float(v[e]);
   }
 };
-// Columns from d on are zero. `row` NULL: all are.
+// Columns from d on are zero. `row` NULL: all are. The last columns of a row are a branch of their own: as the other
+// side of the first one, lanes past the row would enter it, and the wait before its writes ends the loads ahead.
 template <typename T>
 __device__ inline RnWord<T> rn_load(const T* __restrict__ row, int col, int d) {
   RnWord<T> w;
@@ -60,7 +65,8 @@ __device__ inline RnWord<T> rn_load(const T* __restrict__ row, int col, int d) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w.v[i] = p.v[i], w.v[4 + i] = q.v[i];
     }
-  } else if (col < d) {
+  }
+  if (col < d && col + 8 > d) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (col + e < d) {
@@ -249,6 +255,7 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
   // is stored, and a neighbour of the right bf16 would move them by far more than their own roundings (in
   // fp32 99 of 3.6 10^6 values were one).
   constexpr bool ONCE = sizeof(TX) == 2;
+  constexpr bool AHEAD = NT < 1024;  // the next row's loads before this row's sums, where registers are left for it
   typedef std::conditional_t<ONCE, double, float> TF;
   float pre[CH][8], post[CH][8];
   TF factor[CH][8];  // scale gate post
@@ -268,7 +275,9 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
   };
   if (lo < hi) load(lo, xc, bc);
   for (int64_t r = lo, it = 0; r < hi; ++r, it ^= 1) {
-    if (r + 1 < hi) load(r + 1, xn, bn);
+    if constexpr (AHEAD) {
+      if (r + 1 < hi) load(r + 1, xn, bn);
+    } else if (r > lo) load(r, xc, bc);
     if (left == 0) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -314,8 +323,10 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_fwd(RnFwd a) {
       rn_store<TB>((TB*)a.y + r * d, 8 * (tid + c * NT), d, u[c]);
     }
     if (a.stats && tid == 0) *(float2*)(a.stats + 2 * r) = make_float2((float)rb, rh);
+    if constexpr (AHEAD) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) xc[c] = xn[c], bc[c] = bn[c];
+      for (int c = 0; c < CH; ++c) xc[c] = xn[c], bc[c] = bn[c];
+    }
   }
 }
 
@@ -330,11 +341,13 @@ struct RnBwd {
   float* dpar;       // [slots][2][d]: partial dpost and dpre (NULL: neither is wanted)
   void* dgate;       // gate's type, where a run holds whole groups of it (or it has a row for each)
   float* dgate_part; // [runs][d] otherwise
+  float* means;      // [rows]: mean(a hh) for k_rn_cols
   int d;
   RnRuns runs;
 };
 
-template <typename TX, typename TB, int NT, int CH>
+// SUMS: the gradients of gate and weights with it (else k_rn_cols's).
+template <typename TX, typename TB, int NT, int CH, bool SUMS>
 __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
   constexpr int NW = NT > 64 ? NT / 64 : 1, TEAMS = rn_threads(NT) / NT;
   __shared__ float part[2][NW][3];
@@ -372,7 +385,9 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
   };
   if (lo < hi) load(lo, hc, gc, bc, yc, st);
   for (int64_t r = lo, it = 0; r < hi; ++r, it ^= 1) {
-    if (r + 1 < hi) load(r + 1, hn, gn, bn, yn, stn);
+    if constexpr (SUMS) {
+      if (r + 1 < hi) load(r + 1, hn, gn, bn, yn, stn);
+    } else if (r > lo) load(r, hc, gc, bc, yc, st);
     if (left == 0) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) rn_gate(a.gate, r / per, d, 8 * (tid + c * NT), a.scale, gate[c]);
@@ -389,7 +404,7 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
         s[0] = fmaf(ga, hh, s[0]);
         s[1] = fmaf(cb, fmaf(rh, ga, gc[c][e]), s[1]);
         s[2] = fmaf(cb, rh * hh, s[2]);
-        dpre[c][e] = fmaf(yc[c][e], hh, dpre[c][e]);
+        if constexpr (SUMS) dpre[c][e] = fmaf(yc[c][e], hh, dpre[c][e]);
       }
     rn_sum<NT, 3>(s, part[it], tid);
     const float m1 = s[0] * invd, m2 = a.post_norm ? (s[1] - m1 * s[2]) * invd : 0.f;
@@ -402,13 +417,15 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
         const float hh = hc[c][e] * rh, bh = bc[c][e] * rb;
         dx[e] = fmaf(rh, fmaf(-hh, m1, yc[c][e] * pre[c][e]), gc[c][e]);
         const float dn = gate[c][e] * dx[e];
-        dpost[c][e] = fmaf(dn, bh, dpost[c][e]);
-        dg[e] = a.scale * dx[e] * (bh * post[c][e]);
+        if constexpr (SUMS) {
+          dpost[c][e] = fmaf(dn, bh, dpost[c][e]);
+          dg[e] = a.scale * dx[e] * (bh * post[c][e]);
+        }
         db[e] = rb * fmaf(-bh, m2, dn * post[c][e]);
       }
       if (a.dx) rn_store<TX>((TX*)a.dx + r * d, col, d, dx);
       if (a.db) rn_store<TB>((TB*)a.db + r * d, col, d, db);
-      if (want_gate) {
+      if (SUMS && want_gate) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) dgate[c][e] += dg[e];
         if (left == 0 && !a.dgate_part) {
@@ -419,10 +436,14 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
         }
       }
     }
+    if (!SUMS && a.means && tid == 0) a.means[r] = m1;
+    if constexpr (SUMS) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) hc[c] = hn[c], gc[c] = gn[c], bc[c] = bn[c], yc[c] = yn[c];
-    st = stn;
+      for (int c = 0; c < CH; ++c) hc[c] = hn[c], gc[c] = gn[c], bc[c] = bn[c], yc[c] = yn[c];
+      st = stn;
+    }
   }
+  if constexpr (!SUMS) return;
   if (a.dgate_part && run < a.runs.runs) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) rn_store<float>(a.dgate_part + run * d, 8 * (tid + c * NT), d, dgate[c]);
@@ -446,6 +467,57 @@ __global__ __launch_bounds__(rn_threads(NT)) void k_rn_bwd(RnBwd a) {
       rn_store<float>(a.dpar + slot * 2 * d + d, 8 * (tid + c * NT), d, dpre[c]);
     }
   }
+}
+
+// The gradients of gate and weights of rows wider than k_rn_bwd has registers for beside its own: a block takes
+// 2048 columns of a run and forms dx again from the row's mean. It reads the row's four inputs a second time; with the
+// sums held by k_rn_bwd, in scratch then, both took 399 us at 8192 columns and 1177 us at 16384 (6 10^7 values in
+// bf16), apart 278 and 542 us.
+template <typename TX, typename TB>
+__global__ __launch_bounds__(256) void k_rn_cols(RnBwd a) {
+  const int d = a.d, col = 8 * ((int)blockIdx.x * 256 + (int)threadIdx.x);
+  if (col >= d) return;
+  const int64_t run = blockIdx.y;
+  int64_t lo, hi;
+  a.runs.rows(run, lo, hi);
+  const TX *h = (const TX*)a.h, *dh = (const TX*)a.dh;
+  const TB *b = (const TB*)a.b, *dy = (const TB*)a.dy;
+  const RnWord<float> pw = rn_load<float>(a.pre, col, d), qw = rn_load<float>(a.post, col, d);
+  float gate[8], dpre[8], dpost[8], dgate[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) dpre[e] = dpost[e] = dgate[e] = 0.f;
+  const int64_t per = a.gate.kind == 2 ? 1 : a.runs.per_group;
+  const bool want_gate = a.dgate || a.dgate_part;
+  int64_t left = 0;
+  for (int64_t r = lo; r < hi; ++r) {
+    const RnWord<TX> hw = rn_load<TX>(h + r * d, col, d), gw = rn_load<TX>(dh ? dh + r * d : nullptr, col, d);
+    const RnWord<TB> bw = rn_load<TB>(b ? b + r * d : nullptr, col, d), yw = rn_load<TB>(dy ? dy + r * d : nullptr, col, d);
+    const float2 st = *(const float2*)(a.stats + 2 * r);
+    const float m1 = a.means[r], rb = a.post_norm ? st.x : 1.f, rh = st.y;
+    if (left == 0) {
+      rn_gate(a.gate, r / per, d, col, a.scale, gate);
+      left = per - r % per;
+    }
+    --left;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float pre = a.pre ? pw[e] + a.weight_offset : 1.f, post = a.post ? qw[e] + a.weight_offset : 1.f;
+      const float hh = hw[e] * rh, bh = bw[e] * rb, dx = fmaf(rh, fmaf(-hh, m1, yw[e] * pre), gw[e]);
+      dpre[e] = fmaf(yw[e], hh, dpre[e]);
+      dpost[e] = fmaf(gate[e] * dx, bh, dpost[e]);
+      dgate[e] = fmaf(a.scale * dx, bh * post, dgate[e]);
+    }
+    if (want_gate && left == 0 && !a.dgate_part) {
+      if (a.gate.bf16) rn_store<bf16_t>((bf16_t*)a.dgate + r / per * d, col, d, dgate);
+      else rn_store<float>((float*)a.dgate + r / per * d, col, d, dgate);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dgate[e] = 0.f;
+    }
+  }
+  if (a.dgate_part) rn_store<float>(a.dgate_part + run * d, col, d, dgate);
+  if (!a.dpar) return;
+  rn_store<float>(a.dpar + run * 2 * d, col, d, dpost);
+  rn_store<float>(a.dpar + run * 2 * d + d, col, d, dpre);
 }
 
 // Sums of n partial rows of `cols` values in a fixed order: a block's 16 waves take a slice of the rows
@@ -513,14 +585,11 @@ void rn_form(int64_t d, F&& f) {
 }
 
 constexpr int64_t RN_THREADS = 256 * 1024;
+constexpr int64_t RN_SUMS_D = 4096;  // widest rows whose sums k_rn_bwd holds
+constexpr int64_t RN_COL_RUNS = 256;
 
-// The runs of a launch of at most `threads` threads (or a block a CU).
-RnRuns rn_runs(int64_t rows, int64_t groups, int64_t d, int64_t threads) {
-  int64_t teams = 1;
-  rn_form(d, [&](auto nt, auto) {
-    constexpr int NT = decltype(nt)::value;
-    teams = std::max<int64_t>(threads / NT, 256);
-  });
+// Runs for so many teams.
+RnRuns rn_team_runs(int64_t rows, int64_t groups, int64_t teams) {
   RnRuns r;
   r.groups = groups, r.per_group = rows / groups;
   if (teams >= groups) {
@@ -534,6 +603,15 @@ RnRuns rn_runs(int64_t rows, int64_t groups, int64_t d, int64_t threads) {
     r.runs = cdiv(groups, r.run_groups);
   }
   return r;
+}
+// The runs of a launch of at most `threads` threads (or a block a CU).
+RnRuns rn_runs(int64_t rows, int64_t groups, int64_t d, int64_t threads) {
+  int64_t teams = 1;
+  rn_form(d, [&](auto nt, auto) {
+    constexpr int NT = decltype(nt)::value;
+    teams = std::max<int64_t>(threads / NT, 256);
+  });
+  return rn_team_runs(rows, groups, teams);
 }
 
 template <typename F>
@@ -567,23 +645,29 @@ RnGate rn_make_gate(const void* gate, int dtype, int64_t groups, int64_t rows) {
 int64_t rn_groups(const RnGate& g) { return g.kind == 1 ? g.groups : 1; }
 
 struct RnPlan {
-  RnRuns runs;
+  RnRuns runs, col_runs;
   int64_t slots;
-  bool gate_part;
-  size_t par_bytes, total;
+  bool cols, gate_part;
+  size_t par_bytes, gate_bytes, total;
 };
 RnPlan rn_plan(int64_t rows, int64_t d, int64_t groups, bool params, bool dgate, bool full_gate) {
   RnPlan P;
-  P.runs = rn_runs(rows, full_gate ? 1 : groups, d, RN_THREADS / 2);
+  if (full_gate) groups = 1;
+  P.cols = d > RN_SUMS_D && (params || dgate);
+  P.runs = rn_runs(rows, groups, d, RN_THREADS / 2);
+  P.col_runs = rn_team_runs(rows, groups, RN_COL_RUNS);
   int64_t blocks = 0;
   rn_form(d, [&](auto nt, auto) {
     constexpr int NT = decltype(nt)::value;
     blocks = cdiv(P.runs.runs, rn_threads(NT) / NT);
     P.slots = NT <= 64 ? blocks * 4 : blocks;
   });
-  P.gate_part = dgate && !full_gate && P.runs.slices > 1;
+  const RnRuns& sums = P.cols ? P.col_runs : P.runs;
+  if (P.cols) P.slots = sums.runs;
+  P.gate_part = dgate && !full_gate && sums.slices > 1;
   P.par_bytes = params ? ((size_t)P.slots * 2 * d * 4 + 255) & ~(size_t)255 : 0;
-  P.total = P.par_bytes + (P.gate_part ? (size_t)P.runs.runs * d * 4 : 0);
+  P.gate_bytes = P.gate_part ? ((size_t)sums.runs * d * 4 + 255) & ~(size_t)255 : 0;
+  P.total = P.par_bytes + P.gate_bytes + (P.cols ? (size_t)rows * 4 : 0);
   return P;
 }
 
@@ -647,23 +731,28 @@ int pd_residual_norm_bwd(const void* stream_out, int x_dtype, const void* branch
   }
   RnBwd a{stream_out, branch, d_stream, d_y, post_weight, pre_weight, post_norm, weight_offset, scale,
           rn_make_gate(branch ? gate : nullptr, gate_dtype, gate_rows, rows), stats, d_x, d_branch, nullptr, d_gate, nullptr,
-          (int)d, {}};
+          nullptr, (int)d, {}};
   const RnPlan P = rn_plan(rows, d, rn_groups(a.gate), params, d_gate != nullptr, a.gate.kind == 2);
   if (P.total && (!workspace || workspace_bytes < P.total)) return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
   a.runs = P.runs;
   if (params) a.dpar = (float*)workspace;
   if (P.gate_part) a.dgate_part = (float*)((char*)workspace + P.par_bytes), a.dgate = nullptr;
+  if (P.cols) a.means = (float*)((char*)workspace + P.par_bytes + P.gate_bytes);
   rn_types(x_dtype, branch_dtype, [&](auto tx, auto tb) {
     typedef std::remove_pointer_t<decltype(tx)> TX;
     typedef std::remove_pointer_t<decltype(tb)> TB;
     rn_form(d, [&](auto nt, auto ch) {
       constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value;
-      hipLaunchKernelGGL((k_rn_bwd<TX, TB, NT, CH>), dim3((unsigned)cdiv(a.runs.runs, rn_threads(NT) / NT)),
-                         dim3(rn_threads(NT)), 0, s, a);
+      hipLaunchKernelGGL((k_rn_bwd<TX, TB, NT, CH, (NT * CH * 8 <= RN_SUMS_D)>),
+                         dim3((unsigned)cdiv(a.runs.runs, rn_threads(NT) / NT)), dim3(rn_threads(NT)), 0, s, a);
     });
+    if (P.cols) {
+      a.runs = P.col_runs;
+      hipLaunchKernelGGL((k_rn_cols<TX, TB>), dim3((unsigned)cdiv(d, 2048), (unsigned)P.col_runs.runs), dim3(256), 0, s, a);
+    }
   });
   if (params || P.gate_part) {
-    const RnSums z{a.dpar, P.slots, d_post, d_pre, a.dgate_part, P.runs.slices, d_gate, gate_dtype == PD_DTYPE_BF16, d};
+    const RnSums z{a.dpar, P.slots, d_post, d_pre, a.dgate_part, (P.cols ? P.col_runs : P.runs).slices, d_gate, gate_dtype == PD_DTYPE_BF16, d};
     hipLaunchKernelGGL(k_rn_sums, dim3((unsigned)cdiv(params ? 2 * d : d, 64),
                                        (unsigned)((params ? 1 : 0) + (P.gate_part ? P.runs.groups : 0))),
                        dim3(1024), 0, s, z);
