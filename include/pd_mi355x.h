@@ -755,7 +755,7 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
  * fp32 [N]: G = g (softmax(z) - 1_target), d_act = G head, d_head = G^T act, going over the vocabulary
  * in pieces of G of at most 1 GiB. With bf16 G enters both products rounded to bf16. Positions of
  * g = 0 do not count either. Bit-identical from call to call. N up to 2^21, bf16 activations below 2 GiB.
- * fp32 operands enter the products as three bf16 parts each, with fp32 sums. */
+ * fp32 operands enter the products as three bf16 parts each, with fp32 sums (an infinity among them: NaN). */
 size_t pd_streamed_ce_fwd_workspace_size(int dtype, int64_t N, int64_t d, int64_t V);
 int pd_streamed_ce_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
                        const void* targets, int target_bits, int64_t ignore_index, float* loss, float* stats,
@@ -777,7 +777,7 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
  * One step of AdamW (Loshchilov & Hutter, 2019) on n_tensors fp32 tensors of sizes[i] values,
  * dense and in place; the arrays are host memory, read during the call. With t = *step + 1,
  *   m += (1 - beta1) (g - m), v += (1 - beta2) (g^2 - v), g = gradient * *grad_scale
- *   p -= lr (weight_decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)).
+ *   p -= lr (weight_decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)), eps at least 2^-126.
  * grads[i] is fp32 or bf16 (grad_dtypes[i]); NULL leaves tensor i and its states as they are.
  * m_scale[i] and v_scale[i] NULL (or the arrays NULL): m[i] and v[i] are fp32. Else they are e4m3
  * codes (OCP, no infinities) of m and of sqrt(v), with fp32 scales [ceil(sizes[i] / 256)] that 256

@@ -317,8 +317,9 @@ extern "C" int pd_adamw_step(int n_tensors, const int64_t* sizes, void* const* p
     return fail(PD_EINVAL, std::string(what) + ": null argument");
   if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
     return fail(PD_EINVAL, std::string(what) + ": betas must be in [0, 1)");
-  if (!(eps > 0.0) || !std::isfinite(eps) || !(float(eps) > 0.f))
-    return fail(PD_EINVAL, std::string(what) + ": eps must be positive and finite");
+  // below the smallest normal number its reciprocal is infinite, and a value without gradient would become NaN
+  if (!std::isfinite((float)eps) || !((float)eps >= 0x1p-126f))
+    return fail(PD_EINVAL, std::string(what) + ": eps must be at least 2^-126 and finite");
   if (!std::isfinite(lr) || !std::isfinite(weight_decay))
     return fail(PD_EINVAL, std::string(what) + ": lr and weight_decay must be finite");
   int64_t total = 0, base = 0;

@@ -653,7 +653,7 @@ struct CEBwdPlan {
 // fill the chip only in slices, each of which leaves an fp32 slab to write and read. The rounds are
 // those of all positions and, with a quarter of the weight, of three quarters of them, since how many
 // count is not known here. us of 1 / 4 / 5 / 7 / 8 slices of 256x256 tiles: 8192 x 768 over 50277 columns 1466 /
-// 772 / 610 / 682 / 616 (128x128: 824 in 1, 724 in 4); 3072 of 4096 x 4096 over 131072 3921 / 3045 /
+// 772 / 610 / 682 / 616 (128x128: 824 in 1, 724 in 4); three quarters of 4096 x 4096 over 131072 3921 / 3045 /
 // 3168 / 3446 / 3085, all 4096 3901 / 4009 / 4041 / 4089 / 4135.
 void ce_dact_form(int64_t N, int64_t d, int64_t cw, int64_t V, bool half, bool& big, int& splits) {
   double best = 1e30;

@@ -52,9 +52,6 @@ class AdamW:
             raise L.PDError("pd kernels take GPU tensors")
         for i, p in enumerate(self.params):
             _plain(name, f"parameter {i}", p, p.numel(), (torch.float32,), device)
-        spans = sorted((p.data_ptr(), p.data_ptr() + 4 * p.numel()) for p in self.params if p.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise L.PDError(f"{name}: two parameters share memory")
         self.device, self.lr, self.betas, self.eps, self.weight_decay = device, lr, betas, eps, weight_decay
         self.key = (int(key[0]), int(key[1]))
         sizes = [p.numel() for p in self.params]
@@ -77,6 +74,10 @@ class AdamW:
         # the tensors of each argument, in the entry point's order
         self._held = [list(ts) for ts in (self.params, st["m"], st["v"], st.get("m_scale") or none, st.get("v_scale") or none,
                                           copies or none)]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for ts in (*self._held, [st["step"]]) for t in ts if t is not None and t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise L.PDError(f"{name}: two of the parameters, states and copies share memory")
         self._written = self._held[0] + [c for c in self._held[5] if c is not None]
         self._at: list[int] | None = None
 

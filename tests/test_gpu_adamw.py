@@ -246,6 +246,11 @@ def test_refusals(device):
         AdamW(p, state={**opt.state, "m": opt.state["m"][:1]})
     with pytest.raises(L.PDError):
         AdamW(p, state_bits=8, state=opt.state)
+    half = torch.zeros(64, dtype=torch.bfloat16, device=device)
+    for kw in (dict(copies=[half, half[:8]]), dict(state={**opt.state, "v": opt.state["m"]}),
+               dict(state={**opt.state, "m": [p[0], opt.state["m"][1]]})):
+        with pytest.raises(L.PDError, match="share memory"):
+            AdamW(p, **kw)
     for bad in (g[:1], [g[0][:5], g[1]], [g[0].double(), g[1]], [g[0].cpu(), g[1]]):
         with pytest.raises(L.PDError):
             opt.step(bad)

@@ -165,7 +165,7 @@ def test_adamw_entry_point_refuses():
 
     null = (ctypes.c_void_p * 1)(None)
     for kw in (dict(n=-1), dict(p=None), dict(count=None), dict(ticket=None), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)),
-               dict(eps=0.0), dict(eps=1e-60), dict(lr=float("nan")), dict(wd=float("inf")), dict(p=null), dict(m=null),
+               dict(eps=0.0), dict(eps=1e-60), dict(eps=1e-40), dict(eps=1e39), dict(lr=float("nan")), dict(wd=float("inf")), dict(p=null), dict(m=null),
                dict(ms=one), dict(sizes=(ctypes.c_int64 * 1)(-1))):
         assert step(**kw) == 1, kw
     assert step(types=(ctypes.c_int32 * 1)(2)) == 3
