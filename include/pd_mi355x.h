@@ -773,6 +773,19 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
                          const void* targets, int target_bits, int64_t ignore_index, const float* g, float* loss,
                          void* d_act, void* d_head, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The same in two calls, for weights g that come after the loss, as autograd's do: the first leaves the softmax in
+ * `kept` (pd_streamed_ce_kept_size bytes; 0: bf16 alone, less than 2 GiB of it and of the head, else the pair above), which the
+ * second reads and leaves as it is. The workspace is that of want_dact and want_dhead; the first call's of 0 and 0. */
+size_t pd_streamed_ce_kept_size(int dtype, int64_t N, int64_t d, int64_t V);
+size_t pd_streamed_ce_kept_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead);
+int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                            const void* targets, int target_bits, int64_t ignore_index, float* loss, void* kept,
+                            size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int pd_streamed_ce_kept_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                            const void* targets, int target_bits, int64_t ignore_index, const void* kept,
+                            size_t kept_bytes, const float* g, void* d_act, void* d_head, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- AdamW over many tensors ------------------------------------------------------------
  * One step of AdamW (Loshchilov & Hutter, 2019) on n_tensors fp32 tensors of sizes[i] values,
  * dense and in place; the arrays are host memory, read during the call. With t = *step + 1,

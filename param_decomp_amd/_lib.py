@@ -141,6 +141,12 @@ _SIGNATURES = {
     "pd_streamed_ce_bwd_workspace_size": (_c_sz, [_c_i32] + [_c_i64] * 3 + [_c_i32]),
     "pd_streamed_ce_bwd": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p] * 5 + [_c_sz, _c_p]),
     "pd_streamed_ce_train_workspace_size": (_c_sz, [_c_i32] + [_c_i64] * 3 + [_c_i32] * 2),
+    "pd_streamed_ce_kept_size": (_c_sz, [_c_i32] + [_c_i64] * 3),
+    "pd_streamed_ce_kept_workspace_size": (_c_sz, [_c_i32] + [_c_i64] * 3 + [_c_i32] * 2),
+    "pd_streamed_ce_kept_fwd": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p] * 2 +
+                                [_c_sz, _c_p, _c_sz, _c_p]),
+    "pd_streamed_ce_kept_bwd": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p, _c_sz] + [_c_p] * 4 +
+                                [_c_sz, _c_p]),
     "pd_streamed_ce_train": (_c_i32, [_c_i32] + [_c_i64] * 3 + [_c_p] * 3 + [_c_i32, _c_i64] + [_c_p] * 5 + [_c_sz, _c_p]),
     "pd_route_scores_fwd": (_c_i32, [_c_p, _c_i32, _c_i64] + [_c_i32] * 3 + [_c_p] + [_c_i32] * 3 + [_c_f32] + [_c_p] * 3),
     "pd_route_scores_bwd": (_c_i32, [_c_p, _c_i32, _c_i64] + [_c_i32] * 4 + [_c_f32] + [_c_p] * 4),

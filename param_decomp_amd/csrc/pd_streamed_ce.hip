@@ -11,6 +11,11 @@
 // The softmax is formed from the row's maximum and sum, kept apart: the log of the sum alone would
 // round a probability near one to 1e-6.
 //
+// Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep), 6 N d V in all: in one call
+// for weights known beforehand, or from the loss to its gradients (pd_streamed_ce_kept_*). bf16, loss and both gradients:
+// 8192 x 768 over 50277 2874 us with the logits formed again, 2663 kept (product and epilogue 820, apply 360, d_act 683,
+// d_head 719); three quarters of 4096 x 4096 over 131072 11.7 and 9.0 ms (2735, 300, 2990, 2940: 1.12 PFLOP/s).
+//
 // Positions whose target lies outside the vocabulary do not count (nor, backward, those of weight
 // zero): their rows are left out of a dense copy of the activations, so they cost no products and
 // what they hold reaches nothing. How many count only the device knows: grids cover all positions
@@ -366,10 +371,10 @@ __global__ void k_ce_counts(const int32_t* __restrict__ count, int64_t R, int ch
     counts[c] = (int32_t)(left < 0 ? 0 : (left < R ? left : R));
   }
 }
-// G = g (softmax - 1_t) in bf16 over what EpiCEKeep kept, in place: the values of each CE_SPAN
+// G = g (softmax - 1_t) in bf16 from what EpiCEKeep kept (E; G may be its memory): the values of each CE_SPAN
 // columns times e^{their m - m} g / s. A position of weight zero gets zeros whatever it holds, and so
 // does its row of the activations: d_head's product has 0 times it. Blocks: a row, 8192 columns of it.
-__global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int64_t ld, int64_t cols, const float2* __restrict__ part,
+__global__ __launch_bounds__(256) void k_ce_apply(const uint16_t* E, uint16_t* G, int64_t ld, int64_t cols, const float2* __restrict__ part,
                                                   int64_t n_tiles, const float2* __restrict__ st,
                                                   const float* __restrict__ target, const int32_t* __restrict__ rows,
                                                   const int32_t* __restrict__ count, CETargets t, const float* __restrict__ g,
@@ -383,7 +388,7 @@ __global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int6
   const float hit = -gr * ((o.y - ce_exp(target[row] - o.x)) / o.y);
   if (gr == 0.f && blockIdx.y == 0)
     for (int64_t c = threadIdx.x; c < words; c += 256) act[row * words + c] = make_uint4(0u, 0u, 0u, 0u);
-  uint16_t* e = E + row * ld;
+  const uint16_t* e = E + row * ld;
   const int64_t c0 = (int64_t)blockIdx.y * 8192 + threadIdx.x * 8;
   uint4 w[4];
   float f[4];
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(256) void k_ce_apply(uint16_t* __restrict__ E, int6
       if (c + 2 * q + 1 == want) hi = hit;
       out[q] = gr == 0.f ? 0u : pack_bf16x2(lo, hi);
     }
-    *(uint4*)(e + c) = make_uint4(out[0], out[1], out[2], out[3]);
+    *(uint4*)(G + row * ld + c) = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 __global__ __launch_bounds__(256) void k_ce_round(const float4* __restrict__ src, int64_t n, uint2* __restrict__ dst) {
@@ -694,25 +699,27 @@ CEBwdPlan ce_bwd_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, cha
   return P;
 }
 
+// The form that keeps the softmax: what the gradients take from the loss (`kept`), and the memory of either.
 struct CEOnePlan {
   int64_t R, ld, n_tiles;  // positions of a chunk, E's row, partials of a row
   int chunks, splits;
   bool big, big_act, big_head;
   int64_t slice;
   int32_t *rows, *pos, *count, *counts;
-  bf16_t *act, *E;
+  bf16_t *act, *E, *G;
   float2 *part, *stats;
   float *target, *slabs, *head;
-  size_t total;
+  size_t kept, work;
 };
 // bf16 with a head that one product takes and a softmax whose shortest chunk is below CE_KEPT; else the
 // two calls, one after the other.
 bool ce_one_form(int dtype, int64_t d, int64_t V) {
   return dtype == PD_DTYPE_BF16 && V <= ce_head_rows(d) && (size_t)(256 + 128) * ce_pitch(V) * 2 < CE_KEPT;
 }
-CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, char* base) {
+CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, bool apart, char* kept, char* work) {
   CEOnePlan P{};
   size_t off = 0;
+  char* base = kept;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
   P.ld = ce_pitch(V);
   P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * 2)) - 128) & ~(int64_t)255);
@@ -725,11 +732,14 @@ CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, ch
   P.counts = (int32_t*)take((size_t)P.chunks * 4);
   P.rows = (int32_t*)take((size_t)N * 4);
   P.pos = (int32_t*)take((size_t)N * 4);
-  P.act = (bf16_t*)take((size_t)N * d * 2);
   P.E = (bf16_t*)take((size_t)P.R * P.ld * 2);
   P.part = (float2*)take((size_t)P.R * P.n_tiles * 8);
   P.stats = (float2*)take((size_t)P.R * 8);
   P.target = (float*)take((size_t)P.R * 4);
+  P.kept = off;
+  base = work, off = 0;
+  P.act = (bf16_t*)take((size_t)N * d * 2);
+  P.G = apart && (dact || dhead) ? (bf16_t*)take((size_t)P.R * P.ld * 2) : P.E;
   P.splits = 1;
   if (dact) {
     ce_dact_form(P.R, d, V, V, true, P.big_act, P.splits);
@@ -737,7 +747,7 @@ CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, ch
   }
   P.slice = tiles_up(tiles_up(V, P.splits), 64) * 64;
   if (dhead && P.chunks > 1) P.head = (float*)take((size_t)V * d * 4);
-  P.total = off;
+  P.work = off;
   return P;
 }
 
@@ -781,6 +791,51 @@ int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const
   if (tiles_up(N, 128) > 65535 || tiles_up(V, 128) > 65535 || N > (int64_t)1 << 21)
     return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
   return PD_OK;
+}
+
+// The logits of chunk c: softmax kept, loss and statistics.
+void ce_one_loss(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const bf16_t* head, const CETargets& t,
+                 float* loss, hipStream_t s) {
+  const int64_t R = P.R, M = std::min(R, N - c * R);
+  const int32_t *rows = P.rows + c * R, *count = P.counts + c;
+  const bool edge = d % 64 != 0;
+  const GemmArgs a{M, V, d, P.act + c * R * d, d, head, d, nullptr, 0, 1.f, 0.f, count, 0, 0, 0, cdiv(d, 64) * 64,
+                   nullptr, nullptr, nullptr};
+  if (P.big)
+    ce_launch<CfgBig, float, MODE_COUNTED, EpiCEKeep<CfgBig>, false, false>(
+        a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
+  else
+    ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(
+        a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
+  hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
+                     loss, nullptr, P.stats);
+}
+// Its gradients.
+void ce_one_grads(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const bf16_t* head, const CETargets& t,
+                  const float* g, void* d_act, void* d_head, hipStream_t s) {
+  const int64_t R = P.R, M = std::min(R, N - c * R);
+  const int32_t *rows = P.rows + c * R, *count = P.counts + c;
+  bf16_t* a_c = P.act + c * R * d;
+  hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(V, 8192)), dim3(256), 0, s, P.E, P.G, P.ld,
+                     (V + 7) & ~(int64_t)7, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)a_c, d / 8);
+  if (d_act) {
+    const GemmArgs b{M, d, V, P.G, P.ld, head, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
+    if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+    else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+    hipLaunchKernelGGL(k_ce_scatter<bf16_t>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 4, 256), 8192)), dim3(256), 0, s,
+                       P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (bf16_t*)d_act);
+  }
+  if (d_head) {
+    const GemmArgs b{V, d, M, P.G, P.ld, a_c, d, P.chunks > 1 ? (void*)P.head : d_head, d, 1.f, c ? 1.f : 0.f, count, 0, 0, 0, 0,
+                     nullptr, nullptr, nullptr};
+    if (P.chunks > 1) {
+      if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+      else ce_launch<CfgSmall, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+    } else {
+      if (P.big_head) ce_launch<CfgBig, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+      else ce_launch<CfgSmall, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
+    }
+  }
 }
 
 }  // namespace
@@ -903,7 +958,10 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
 
 size_t pd_streamed_ce_train_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
   if (N <= 0 || d <= 0 || V <= 0) return 0;
-  if (ce_one_form(dtype, d, V)) return ce_one_plan(N, d, V, want_dact, want_dhead, nullptr).total;
+  if (ce_one_form(dtype, d, V)) {
+    const CEOnePlan P = ce_one_plan(N, d, V, want_dact, want_dhead, false, nullptr, nullptr);
+    return P.kept + P.work;
+  }
   return up256((size_t)N * 8) + std::max(ce_fwd_plan(dtype, N, d, V, nullptr).total,
                                          ce_bwd_plan(dtype, N, d, V, want_dact, nullptr).total);
 }
@@ -926,7 +984,8 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
     return pd_streamed_ce_bwd(dtype, N, d, V, act, head, targets, target_bits, ignore_index, stats, g, d_act, d_head, ws, left,
                               stream);
   }
-  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, (char*)workspace);
+  const size_t kept = ce_one_plan(N, d, V, false, false, false, nullptr, nullptr).kept;
+  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, false, (char*)workspace, (char*)workspace + kept);
   if (!dtl_fits_mn(P.R, P.ld)) return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
   const CETargets t{targets, target_bits, ignore_index, V};
   const bf16_t* hd = (const bf16_t*)head;
@@ -934,41 +993,64 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
   ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
   hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
   for (int c = 0; c < P.chunks; ++c) {
-    const int64_t R = P.R;
-    const int32_t *rows = P.rows + c * R, *count = P.counts + c;
-    const int64_t M = std::min(R, N - c * R);
-    const bf16_t* a_c = P.act + c * R * d;
-    const bool edge = d % 64 != 0;
-    const GemmArgs a{M, V, d, a_c, d, hd, d, nullptr, 0, 1.f, 0.f, count, 0, 0, 0, cdiv(d, 64) * 64, nullptr, nullptr, nullptr};
-    if (P.big)
-      ce_launch<CfgBig, float, MODE_COUNTED, EpiCEKeep<CfgBig>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
-    else
-      ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
-    hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
-                       loss, nullptr, P.stats);
-    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(V, 8192)), dim3(256), 0, s, P.E, P.ld, (V + 7) & ~(int64_t)7, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)(P.act + c * R * d), d / 8);
-    if (d_act) {
-      GemmArgs b{M, d, V, P.E, P.ld, hd, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
-      if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
-      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
-      hipLaunchKernelGGL(k_ce_scatter<bf16_t>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 4, 256), 8192)), dim3(256), 0, s,
-                         P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (bf16_t*)d_act);
-    }
-    if (d_head) {
-      GemmArgs b{V, d, M, P.E, P.ld, a_c, d, P.chunks > 1 ? (void*)P.head : d_head, d, 1.f, c ? 1.f : 0.f, count, 0, 0, 0, 0,
-                 nullptr, nullptr, nullptr};
-      if (P.chunks > 1) {
-        if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
-        else ce_launch<CfgSmall, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
-      } else {
-        if (P.big_head) ce_launch<CfgBig, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
-        else ce_launch<CfgSmall, bf16_t, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
-      }
-    }
+    ce_one_loss(P, c, N, d, V, hd, t, loss, s);
+    ce_one_grads(P, c, N, d, V, hd, t, g, d_act, d_head, s);
   }
   if (d_head && P.chunks > 1)
     hipLaunchKernelGGL(k_ce_round, dim3((unsigned)std::min<int64_t>(cdiv(V * d / 4, 256), 16384)), dim3(256), 0, s,
                        (const float4*)P.head, V * d / 4, (uint2*)d_head);
+  return check_launch(what);
+}
+
+size_t pd_streamed_ce_kept_size(int dtype, int64_t N, int64_t d, int64_t V) {
+  if (N <= 0 || d <= 0 || V <= 0 || !ce_one_form(dtype, d, V)) return 0;
+  const CEOnePlan P = ce_one_plan(N, d, V, false, false, true, nullptr, nullptr);
+  return P.chunks == 1 && dtl_fits_mn(P.R, P.ld) ? P.kept : 0;
+}
+
+size_t pd_streamed_ce_kept_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
+  if (!pd_streamed_ce_kept_size(dtype, N, d, V)) return 0;
+  return ce_one_plan(N, d, V, want_dact, want_dhead, true, nullptr, nullptr).work;
+}
+
+int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                            const void* targets, int target_bits, int64_t ignore_index, float* loss, void* kept,
+                            size_t kept_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "pd_streamed_ce_kept_fwd";
+  if (int rc = ce_check(what, dtype, N, d, V, act, head, targets, target_bits)) return rc;
+  if (!N || !loss) return fail(PD_EINVAL, std::string(what) + ": positions and loss required");
+  const size_t need = pd_streamed_ce_kept_size(dtype, N, d, V);
+  if (!need) return fail(PD_EUNSUPPORTED, std::string(what) + ": nothing is kept at this size");
+  const CEOnePlan P = ce_one_plan(N, d, V, false, false, true, (char*)kept, (char*)workspace);
+  if (!kept || kept_bytes < need || !workspace || workspace_bytes < P.work)
+    return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
+  hipStream_t s = (hipStream_t)stream;
+  const CETargets t{targets, target_bits, ignore_index, V};
+  hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, P.pos, P.count, loss, nullptr);
+  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
+  hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
+  ce_one_loss(P, 0, N, d, V, (const bf16_t*)head, t, loss, s);
+  return check_launch(what);
+}
+
+int pd_streamed_ce_kept_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
+                            const void* targets, int target_bits, int64_t ignore_index, const void* kept,
+                            size_t kept_bytes, const float* g, void* d_act, void* d_head, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const char* what = "pd_streamed_ce_kept_bwd";
+  if (int rc = ce_check(what, dtype, N, d, V, act, head, targets, target_bits)) return rc;
+  if (!d_act && !d_head) return PD_OK;
+  if (!N || !g) return fail(PD_EINVAL, std::string(what) + ": positions and g required");
+  const size_t need = pd_streamed_ce_kept_size(dtype, N, d, V);
+  if (!need) return fail(PD_EUNSUPPORTED, std::string(what) + ": nothing is kept at this size");
+  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, true, (char*)const_cast<void*>(kept),
+                                  (char*)workspace);
+  if (!kept || kept_bytes < need || !workspace || workspace_bytes < P.work)
+    return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
+  hipStream_t s = (hipStream_t)stream;
+  const CETargets t{targets, target_bits, ignore_index, V};
+  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
+  ce_one_grads(P, 0, N, d, V, (const bf16_t*)head, t, g, d_act, d_head, s);
   return check_launch(what);
 }
 

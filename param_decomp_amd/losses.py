@@ -337,19 +337,25 @@ def top_logits_kl(masked_logits, top_logits, top_indices, *, clean_lse=None, tem
 
 class _StreamedCE(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, act, head, targets, ignore_index):
-        loss, stats = ops.streamed_cross_entropy_fwd(act, head, targets, ignore_index=ignore_index, want_stats=True)
-        ctx.save_for_backward(act, head, targets, stats)
+    def forward(ctx, act, head, targets, ignore_index, keep):
+        kept = None
+        if keep:
+            loss, kept = ops.streamed_cross_entropy_kept_fwd(act, head, targets, ignore_index=ignore_index)
+        ctx.bwd = ops.streamed_cross_entropy_kept_bwd
+        if kept is None:
+            loss, kept = ops.streamed_cross_entropy_fwd(act, head, targets, ignore_index=ignore_index, want_stats=True)
+            ctx.bwd = ops.streamed_cross_entropy_bwd
+        ctx.save_for_backward(act, head, targets, kept)
         ctx.ignore_index = ignore_index
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        act, head, targets, stats = ctx.saved_tensors
+        act, head, targets, kept = ctx.saved_tensors
         want = ctx.needs_input_grad
-        return (*ops.streamed_cross_entropy_bwd(act, head, targets, stats, g.contiguous(), ignore_index=ctx.ignore_index,
-                                                want_dact=want[0], want_dhead=want[1]), None, None)
+        return (*ctx.bwd(act, head, targets, kept, g.contiguous(), ignore_index=ctx.ignore_index, want_dact=want[0],
+                         want_dhead=want[1]), None, None, None)
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -359,13 +365,16 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, *,
-                                    ignore_index: int = -100) -> torch.Tensor:
-    """Per-position cross entropy of the logits `act @ head^T` against `targets`, without keeping the
+                                    ignore_index: int = -100, keep: bool = True) -> torch.Tensor:
+    """Per-position cross entropy of the logits `act @ head^T` against `targets`, without writing the
     logits: what `streamed_position_kl` is to a teacher's distribution. act [..., d], head [V, d] (one
     dtype, bf16 or fp32), targets int32 or int64 [...]. A position whose target is `ignore_index` or
     lies outside [0, V) has loss 0, no gradient and no part in the products. Returns fp32 [...];
-    differentiable in act and head, once: gradients in their dtype, formed over pieces of the vocabulary (bf16:
-    from softmax differences rounded to bf16). `ops.streamed_cross_entropy` gives loss and weighted
+    differentiable in act and head, once: gradients in their dtype (bf16: from softmax differences rounded to bf16).
+
+    With bf16 tensors the softmax is kept in 16 bits for the backward where it and the head take less than 2 GiB each (2 bytes for each
+    position and entry of the vocabulary: 0.8 GB for 8192 over 50277); else, and with `keep` False, the backward forms the logits
+    again, a third of the gradient's products, over pieces of the vocabulary. `ops.streamed_cross_entropy` gives loss and weighted
     gradients in one call."""
     lead, d = act.shape[:-1], act.shape[-1] if act.dim() else 0
     pad = (-d) % 8 if act.dtype == torch.bfloat16 else 0
@@ -375,15 +384,15 @@ def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targe
         raise L.PDError(f"streamed_position_cross_entropy: targets are {tuple(lead)}, got {tuple(targets.shape)}")
     a, h, t = _aligned(act.reshape(-1, d + pad)), _aligned(head), targets.reshape(-1).contiguous()
     if ops.differentiated(a, h):
-        loss = _StreamedCE.apply(a, h, t, int(ignore_index))
+        loss = _StreamedCE.apply(a, h, t, int(ignore_index), bool(keep))
     else:
         loss = ops.streamed_cross_entropy_fwd(a, h, t, ignore_index=ignore_index)[0]
     return loss.reshape(lead)
 
 
 def streamed_cross_entropy(act: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, *,
-                           ignore_index: int = -100) -> torch.Tensor:
+                           ignore_index: int = -100, keep: bool = True) -> torch.Tensor:
     """The mean of `streamed_position_cross_entropy` over the positions that count (0 where none does)."""
-    loss = streamed_position_cross_entropy(act, head, targets, ignore_index=ignore_index)
+    loss = streamed_position_cross_entropy(act, head, targets, ignore_index=ignore_index, keep=keep)
     counts = (targets != ignore_index) & (targets >= 0) & (targets < head.shape[0])
     return loss.sum() / counts.sum().clamp(min=1)

@@ -735,6 +735,44 @@ def streamed_cross_entropy_bwd(act, head, targets, stats, g, *, ignore_index: in
     return da, dh
 
 
+def streamed_cross_entropy_kept_fwd(act, head, targets, *, ignore_index: int = -100):
+    """(loss fp32 [N], kept): the forward that leaves the softmax in 16 bits for
+    `streamed_cross_entropy_kept_bwd`, which then forms no logits again. kept (2 bytes for each
+    position and entry of the vocabulary) is None for fp32 and where it or the head would take 2 GiB:
+    nothing has run then."""
+    name = "streamed_cross_entropy_kept_fwd"
+    device, sizes = _ce_checks(name, act, head, targets)
+    nbytes = L.load().pd_streamed_ce_kept_size(*sizes)
+    if not nbytes:
+        return None, None
+    loss = torch.empty(act.shape[0], dtype=torch.float32, device=device)
+    kept = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = L.workspace(L.load().pd_streamed_ce_kept_workspace_size(*sizes, 0, 0), device)
+    L.launch("pd_streamed_ce_kept_fwd", device, *sizes, *_ce_args(act, head, targets, ignore_index), L.ptr(loss), L.ptr(kept),
+             nbytes, L.ptr(ws), ws.numel())
+    return loss, kept
+
+
+def streamed_cross_entropy_kept_bwd(act, head, targets, kept, g, *, ignore_index: int = -100, want_dact: bool = True,
+                                    want_dhead: bool = True):
+    """(d_act, d_head) of sum g_i loss_i from what the forward kept, g fp32 [N]; None for those not wanted."""
+    name = "streamed_cross_entropy_kept_bwd"
+    device, sizes = _ce_checks(name, act, head, targets)
+    N = act.shape[0]
+    if kept.dtype != torch.uint8 or kept.numel() != L.load().pd_streamed_ce_kept_size(*sizes) or not kept.numel():
+        raise L.PDError(f"{name}: kept is the forward's, got {kept.dtype} {tuple(kept.shape)}")
+    if g.dtype != torch.float32 or tuple(g.shape) != (N,):
+        raise L.PDError(f"{name}: g is float32 [{N}], got {g.dtype} {tuple(g.shape)}")
+    _one_device(name, act, "kept g", kept, g)
+    da = torch.empty_like(act) if want_dact else None
+    dh = torch.empty_like(head) if want_dhead else None
+    if want_dact or want_dhead:
+        ws = L.workspace(L.load().pd_streamed_ce_kept_workspace_size(*sizes, int(want_dact), int(want_dhead)), device)
+        L.launch("pd_streamed_ce_kept_bwd", device, *sizes, *_ce_args(act, head, targets, ignore_index), L.ptr(kept),
+                 kept.numel(), L.ptr(g), L.ptr(da), L.ptr(dh), L.ptr(ws), ws.numel())
+    return da, dh
+
+
 def streamed_cross_entropy(act, head, targets, *, ignore_index: int = -100, row_weight=None, want_dact: bool = False,
                            want_dhead: bool = False):
     """(loss, d_act, d_head): per-position cross entropy (see `losses.streamed_position_cross_entropy`) and

@@ -71,7 +71,14 @@ def _check(got, want, bounds):
 def _both_forms(act, head, t, w, ignore=-100):
     one = ops.streamed_cross_entropy(act, head, t, ignore_index=ignore, row_weight=w, want_dact=True, want_dhead=True)
     loss, stats = ops.streamed_cross_entropy_fwd(act, head, t, ignore_index=ignore, want_stats=True)
-    return one, (loss, *ops.streamed_cross_entropy_bwd(act, head, t, stats, w, ignore_index=ignore))
+    forms = [one, (loss, *ops.streamed_cross_entropy_bwd(act, head, t, stats, w, ignore_index=ignore))]
+    loss, kept = ops.streamed_cross_entropy_kept_fwd(act, head, t, ignore_index=ignore)
+    if kept is not None:
+        ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, 3 * w, ignore_index=ignore)  # leaves it as it is
+        forms.append((loss, *ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, w, ignore_index=ignore)))
+    large = max(2 * act.shape[0] * head.shape[0], 2 * head.numel()) > 2**31 - 2**23
+    assert (kept is None) == (act.dtype == F32 or large)
+    return forms
 
 
 SHAPES = [(1, 8, 1), (1, 64, 7), (2, 16, 129), (33, 72, 1000), (127, 64, 64), (128, 128, 65), (129, 200, 257), (300, 136, 3001),
@@ -96,8 +103,13 @@ def test_odd_widths_through_autograd(device, d):
         act, head = act.requires_grad_(), head.requires_grad_()
         loss = losses.streamed_position_cross_entropy(act.view(7, 10, d), head, t.view(7, 10))
         assert loss.shape == (7, 10)
-        got = (loss.view(-1), *torch.autograd.grad(loss, (act, head), w.view(7, 10)))
-        _check(got, *_expected(act.detach(), head.detach(), t, w))
+        got = (loss.view(-1), *torch.autograd.grad(loss, (act, head), w.view(7, 10), retain_graph=True))
+        want = _expected(act.detach(), head.detach(), t, w)
+        _check(got, *want)
+        for a, b in zip(got[1:], torch.autograd.grad(loss, (act, head), w.view(7, 10))):
+            assert torch.equal(a, b)
+        loss = losses.streamed_position_cross_entropy(act, head, t, keep=False)
+        _check((loss, *torch.autograd.grad(loss, (act, head), w)), *want)
 
 
 def test_mean_and_one_gradient_alone(device):
@@ -271,5 +283,11 @@ def test_refusals(device):
             ops.streamed_cross_entropy_fwd(*bad)
     with pytest.raises(L.PDError, match="row_weight"):
         ops.streamed_cross_entropy(act, head, t, row_weight=w.double(), want_dact=True)
+    kept = ops.streamed_cross_entropy_kept_fwd(act, head, t)[1]
+    for bad in (kept[1:], kept.float(), kept.cpu()):
+        with pytest.raises(L.PDError, match="kept"):
+            ops.streamed_cross_entropy_kept_bwd(act, head, t, bad, w)
+    with pytest.raises(L.PDError, match="g is"):
+        ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, w[:3])
     with pytest.raises(L.PDError, match="stats"):
         ops.streamed_cross_entropy_bwd(act, head, t, w, w)

@@ -71,6 +71,16 @@ def test_cross_entropy_entry_points_refuse():
     assert fwd(N=0) == 0
     size = lib.pd_streamed_ce_train_workspace_size
     assert size(L.BF16, 4, 16, 9, 1, 1) > 0 and size(L.BF16, 0, 16, 9, 1, 1) == 0
+    kept = lib.pd_streamed_ce_kept_size
+    assert kept(L.BF16, 4, 16, 9) > 0 and kept(L.BF16, 0, 16, 9) == 0 and kept(L.F32, 4, 16, 9) == 0
+    assert 8192 * 50277 * 2 <= kept(L.BF16, 8192, 768, 50277) < 1 << 30 and kept(L.BF16, 1 << 18, 16, 131072) == 0
+    a = (b, b, b, 64, -100)
+    assert lib.pd_streamed_ce_kept_fwd(L.F32, 4, 16, 9, *a, b, b, 2**62, b, 2**62, None) == 3  # nothing is kept
+    assert lib.pd_streamed_ce_kept_fwd(L.BF16, 4, 16, 9, *a, b, b, 16, b, 2**62, None) == 4
+    assert lib.pd_streamed_ce_kept_fwd(L.BF16, 4, 16, 9, *a, b, b, 2**62, b, 16, None) == 4
+    assert lib.pd_streamed_ce_kept_fwd(L.BF16, 0, 16, 9, *a, b, b, 2**62, b, 2**62, None) == 1
+    assert lib.pd_streamed_ce_kept_bwd(L.BF16, 4, 16, 9, *a, b, 16, b, b, b, b, 2**62, None) == 4
+    assert lib.pd_streamed_ce_kept_bwd(L.BF16, 4, 16, 9, *a, b, 2**62, None, b, b, b, 2**62, None) == 1
     # the softmax of a chunk, not of all positions: below 2 GiB and what goes with it
     assert size(L.BF16, 1 << 18, 16, 131072, 1, 1) < (3 << 30)
 
@@ -206,6 +216,7 @@ def _refuse_tangents(device):
 
 
 def test_tangents_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "streamed_cross_entropy_kept_fwd", lambda *a, **k: (None, None))
     monkeypatch.setattr(ops, "streamed_cross_entropy_fwd", lambda a, h, t, ignore_index=0, want_stats=False:
                         (a.new_zeros(4), a.new_zeros(4, 2)))
     monkeypatch.setattr(ops, "route_scores_fwd", lambda z, k, **kw: (z.new_zeros(4, k), torch.zeros(4, k, dtype=torch.int32)))
