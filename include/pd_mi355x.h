@@ -765,7 +765,7 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
                        const void* targets, int target_bits, int64_t ignore_index, const float* stats, const float* g,
                        void* d_act, void* d_head, void* workspace, size_t workspace_bytes, void* stream);
 /* Loss and gradients in one call, for weights g that are known before the loss: 6 N d V operations in place of
- * 8 with bf16, where a chunk of positions keeps its softmax in 16 bits (below 2 GiB of workspace) until
+ * 8, where a chunk of positions keeps its softmax in 16 bits (fp32: its logits; below 2 GiB of workspace) until
  * G takes its place (a probability below 2^-28 of the largest of its 64 neighbours loses digits, and is off by
  * 2^-40 of that at most). A position of g = 0 has its loss and no gradient. */
 size_t pd_streamed_ce_train_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead);
@@ -774,8 +774,8 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
                          void* d_act, void* d_head, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same in two calls, for weights g that come after the loss, as autograd's do: the first leaves the softmax in
- * `kept` (pd_streamed_ce_kept_size bytes; 0: bf16 alone, less than 2 GiB of it and of the head, else the pair above), which the
- * second reads and leaves as it is. The workspace is that of want_dact and want_dhead; the first call's of 0 and 0. */
+ * `kept` (fp32: the logits; pd_streamed_ce_kept_size bytes, 0 where that or a bf16 head would take 2 GiB: the pair above is
+ * for those), which the second reads and leaves as it is. The workspace is that of want_dact and want_dhead; the first call's of 0 and 0. */
 size_t pd_streamed_ce_kept_size(int dtype, int64_t N, int64_t d, int64_t V);
 size_t pd_streamed_ce_kept_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead);
 int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,

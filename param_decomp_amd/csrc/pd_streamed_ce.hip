@@ -11,10 +11,11 @@
 // The softmax is formed from the row's maximum and sum, kept apart: the log of the sum alone would
 // round a probability near one to 1e-6.
 //
-// Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep), 6 N d V in all: in one call
+// Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep; fp32: the logits, EpiCEKeepF), 6 N d V in all: in one call
 // for weights known beforehand, or from the loss to its gradients (pd_streamed_ce_kept_*). bf16, loss and both gradients:
 // 8192 x 768 over 50277 2874 us with the logits formed again, 2663 kept (product and epilogue 820, apply 360, d_act 683,
 // d_head 719); three quarters of 4096 x 4096 over 131072 11.7 and 9.0 ms (2735, 300, 2990, 2940: 1.12 PFLOP/s).
+// fp32, 903 of 1003 x 1000 over 32003: 1530 us formed again, 1161 kept (product 427, apply 39, d_act 413, d_head 398).
 //
 // Positions whose target lies outside the vocabulary do not count (nor, backward, those of weight
 // zero): their rows are left out of a dense copy of the activations, so they cost no products and
@@ -474,6 +475,70 @@ struct EpiCEGradF {
   }
 };
 
+// EpiCEStats that writes the logits too, in fp32.
+template <class CFG>
+struct EpiCEKeepF {
+  static constexpr int LDS_BYTES = EpiCEStats<CFG>::LDS_BYTES;
+  struct Args {
+    typename EpiCEStats<CFG>::Args st;
+    float* Z;
+    int64_t ld;  // a multiple of 4
+  };
+  template <class TJ, typename TC>
+  __device__ static void run(const GemmArgs& p, const Args& a, const TileJob& t, int wm, int wn, int tid,
+                             f32x16 (&z)[CFG::TM][CFG::TN], char* smem) {
+    const int lane = tid & 63;
+    const int64_t first = t.n0 + wn * CFG::WTN + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < CFG::TM; ++i) {
+      const int64_t row = t.m0 + wm * CFG::WTM + i * 32 + (lane & 31);
+      if (row >= t.M) continue;
+#pragma unroll
+      for (int j = 0; j < CFG::TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = j * 32 + 8 * q;
+          float* dst = a.Z + row * a.ld + first + c;
+          if (first + c + 3 < p.N) {
+            *(float4*)dst = make_float4(z[i][j][4 * q], z[i][j][4 * q + 1], z[i][j][4 * q + 2], z[i][j][4 * q + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (first + c + e < p.N) dst[e] = z[i][j][4 * q + e];
+          }
+        }
+    }
+    EpiCEStats<CFG>::template run<TJ, TC>(p, a.st, t, wm, wn, tid, z, smem);
+  }
+};
+
+// EpiCEGradF from the logits kept: G (which may be their memory) in fp32. Blocks: a row, 4096 columns of it.
+__global__ __launch_bounds__(256) void k_ce_apply_f32(const float* Z, float* G, int64_t ld, int64_t V, const float2* __restrict__ st,
+                                                      const int32_t* __restrict__ rows, const int32_t* __restrict__ count,
+                                                      CETargets t, const float* __restrict__ g, float* __restrict__ act, int64_t d) {
+  const int64_t row = blockIdx.x;
+  if (row >= *count) return;
+  const int64_t r = rows[row], want = t.at(r);
+  const float2 o = st[row];
+  const float gr = g[r], gs = gr / o.y;
+  if (gr == 0.f && blockIdx.y == 0)
+    for (int64_t c = threadIdx.x; c < d; c += 256) act[row * d + c] = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t c = (int64_t)blockIdx.y * 4096 + k * 1024 + threadIdx.x * 4;
+    if (c >= V) continue;
+    float v[4];  // the row's pitch is a multiple of 4, what lies behind V is not read again
+    const float4 z = *(const float4*)(Z + row * ld + c);
+    v[0] = z.x, v[1] = z.y, v[2] = z.z, v[3] = z.w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = expf(v[e] - o.x);
+      v[e] = gr == 0.f ? 0.f : want == c + e ? -gr * ((o.y - x) / o.y) : x * gs;
+    }
+    *(float4*)(G + row * ld + c) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+
 struct __attribute__((packed, aligned(4))) CEWord {  // at any element's boundary
   float v[4];
 };
@@ -706,47 +771,51 @@ struct CEOnePlan {
   bool big, big_act, big_head;
   int64_t slice;
   int32_t *rows, *pos, *count, *counts;
-  bf16_t *act, *E, *G;
+  bool half;
+  void *act, *E, *G;  // E: bf16 the softmax in 16 bits, fp32 the logits
   float2 *part, *stats;
   float *target, *slabs, *head;
   size_t kept, work;
 };
-// bf16 with a head that one product takes and a softmax whose shortest chunk is below CE_KEPT; else the
+// A head that one product takes and a softmax whose shortest chunk is below CE_KEPT; else the
 // two calls, one after the other.
 bool ce_one_form(int dtype, int64_t d, int64_t V) {
-  return dtype == PD_DTYPE_BF16 && V <= ce_head_rows(d) && (size_t)(256 + 128) * ce_pitch(V) * 2 < CE_KEPT;
+  const bool half = dtype == PD_DTYPE_BF16;
+  return (!half || V <= ce_head_rows(d)) && (size_t)(256 + 128) * ce_pitch(V) * (half ? 2 : 4) < CE_KEPT;
 }
-CEOnePlan ce_one_plan(int64_t N, int64_t d, int64_t V, bool dact, bool dhead, bool apart, char* kept, char* work) {
+CEOnePlan ce_one_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, bool dhead, bool apart, char* kept, char* work) {
   CEOnePlan P{};
   size_t off = 0;
   char* base = kept;
   auto take = [&](size_t bytes) { char* p = base + off; off += up256(bytes); return p; };
+  P.half = dtype == PD_DTYPE_BF16;
+  const size_t esz = P.half ? 2 : 4;
   P.ld = ce_pitch(V);
-  P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * 2)) - 128) & ~(int64_t)255);
+  P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * esz)) - 128) & ~(int64_t)255);
   if (P.R <= 0) P.R = N;
   P.chunks = (int)cdiv(N, P.R);
-  P.big = ce_big(P.R, V);
-  P.n_tiles = tiles_up(V, CE_SPAN);
-  P.big_head = big_tiles(V, d, P.R);
+  P.big = P.half && ce_big(P.R, V);
+  P.n_tiles = tiles_up(V, P.half ? CE_SPAN : 128);
+  P.big_head = P.half && big_tiles(V, d, P.R);
   P.count = (int32_t*)take(4);
   P.counts = (int32_t*)take((size_t)P.chunks * 4);
   P.rows = (int32_t*)take((size_t)N * 4);
   P.pos = (int32_t*)take((size_t)N * 4);
-  P.E = (bf16_t*)take((size_t)P.R * P.ld * 2);
+  P.E = take((size_t)P.R * P.ld * esz);
   P.part = (float2*)take((size_t)P.R * P.n_tiles * 8);
   P.stats = (float2*)take((size_t)P.R * 8);
   P.target = (float*)take((size_t)P.R * 4);
   P.kept = off;
   base = work, off = 0;
-  P.act = (bf16_t*)take((size_t)N * d * 2);
-  P.G = apart && (dact || dhead) ? (bf16_t*)take((size_t)P.R * P.ld * 2) : P.E;
+  P.act = take((size_t)N * d * esz);
+  P.G = apart && (dact || dhead) ? take((size_t)P.R * P.ld * esz) : P.E;
   P.splits = 1;
   if (dact) {
-    ce_dact_form(P.R, d, V, V, true, P.big_act, P.splits);
+    ce_dact_form(P.R, d, V, V, P.half, P.big_act, P.splits);
     P.slabs = (float*)take((size_t)P.splits * P.R * d * 4);
   }
   P.slice = tiles_up(tiles_up(V, P.splits), 64) * 64;
-  if (dhead && P.chunks > 1) P.head = (float*)take((size_t)V * d * 4);
+  if (P.half && dhead && P.chunks > 1) P.head = (float*)take((size_t)V * d * 4);
   P.work = off;
   return P;
 }
@@ -794,41 +863,60 @@ int ce_check(const char* what, int dtype, int64_t N, int64_t d, int64_t V, const
 }
 
 // The logits of chunk c: softmax kept, loss and statistics.
-void ce_one_loss(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const bf16_t* head, const CETargets& t,
+void ce_one_loss(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const void* head, const CETargets& t,
                  float* loss, hipStream_t s) {
   const int64_t R = P.R, M = std::min(R, N - c * R);
   const int32_t *rows = P.rows + c * R, *count = P.counts + c;
   const bool edge = d % 64 != 0;
-  const GemmArgs a{M, V, d, P.act + c * R * d, d, head, d, nullptr, 0, 1.f, 0.f, count, 0, 0, 0, cdiv(d, 64) * 64,
+  const bf16_t* a_c = (const bf16_t*)((const char*)P.act + c * R * d * (P.half ? 2 : 4));
+  const GemmArgs a{M, V, d, a_c, d, (const bf16_t*)head, d, nullptr, 0, 1.f, 0.f, count, 0, 0, 0, cdiv(d, 64) * 64,
                    nullptr, nullptr, nullptr};
-  if (P.big)
+  if (!P.half) {
+    if (M > 128) ce_launch_parts<CfgParts, MODE_COUNTED, EpiCEKeepF<CfgParts>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, (float*)P.E, P.ld}, 1, s);
+    else ce_launch_parts<CfgSmall, MODE_COUNTED, EpiCEKeepF<CfgSmall>, false, false>(a, {{P.part, P.n_tiles, P.target, rows, t}, (float*)P.E, P.ld}, 1, s);
+  } else if (P.big) {
     ce_launch<CfgBig, float, MODE_COUNTED, EpiCEKeep<CfgBig>, false, false>(
-        a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
-  else
+        a, {{P.part, P.n_tiles, P.target, rows, t}, (uint16_t*)P.E, P.ld}, 1, edge, s);
+  } else {
     ce_launch<CfgSmall, float, MODE_COUNTED, EpiCEKeep<CfgSmall>, false, false>(
-        a, {{P.part, P.n_tiles, P.target, rows, t}, P.E, P.ld}, 1, edge, s);
+        a, {{P.part, P.n_tiles, P.target, rows, t}, (uint16_t*)P.E, P.ld}, 1, edge, s);
+  }
   hipLaunchKernelGGL(k_ce_merge, dim3((unsigned)cdiv(M, 4)), dim3(256), 0, s, P.part, P.target, M, P.n_tiles, rows, count, t,
                      loss, nullptr, P.stats);
 }
 // Its gradients.
-void ce_one_grads(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const bf16_t* head, const CETargets& t,
+void ce_one_grads(const CEOnePlan& P, int c, int64_t N, int64_t d, int64_t V, const void* head, const CETargets& t,
                   const float* g, void* d_act, void* d_head, hipStream_t s) {
   const int64_t R = P.R, M = std::min(R, N - c * R);
   const int32_t *rows = P.rows + c * R, *count = P.counts + c;
-  bf16_t* a_c = P.act + c * R * d;
-  hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(V, 8192)), dim3(256), 0, s, P.E, P.G, P.ld,
-                     (V + 7) & ~(int64_t)7, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g, (uint4*)a_c, d / 8);
+  char* a_c = (char*)P.act + c * R * d * (P.half ? 2 : 4);
+  if (P.half)
+    hipLaunchKernelGGL(k_ce_apply, dim3((unsigned)M, (unsigned)cdiv(V, 8192)), dim3(256), 0, s, (const uint16_t*)P.E,
+                       (uint16_t*)P.G, P.ld, (V + 7) & ~(int64_t)7, P.part, P.n_tiles, P.stats, P.target, rows, count, t, g,
+                       (uint4*)a_c, d / 8);
+  else
+    hipLaunchKernelGGL(k_ce_apply_f32, dim3((unsigned)M, (unsigned)cdiv(V, 4096)), dim3(256), 0, s, (const float*)P.E,
+                       (float*)P.G, P.ld, V, P.stats, rows, count, t, g, (float*)a_c, d);
+  const bf16_t* G = (const bf16_t*)P.G;  // k_gemm_parts takes its operands so
   if (d_act) {
-    const GemmArgs b{M, d, V, P.G, P.ld, head, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
-    if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
-    else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
-    hipLaunchKernelGGL(k_ce_scatter<bf16_t>, dim3((unsigned)std::min<int64_t>(cdiv(N * d / 4, 256), 8192)), dim3(256), 0, s,
-                       P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (bf16_t*)d_act);
+    const GemmArgs b{M, d, V, G, P.ld, (const bf16_t*)head, d, P.slabs, d, 1.f, 0.f, count, 0, 0, R * d, P.slice, nullptr, nullptr, nullptr};
+    const dim3 grid((unsigned)std::min<int64_t>(cdiv(P.half ? N * d / 4 : N * d, 256), 8192));
+    if (!P.half) {
+      ce_launch_f32<MODE_COUNTED, EpiCEStore, false, true>(b, P.splits, s);
+      hipLaunchKernelGGL(k_ce_scatter<float>, grid, dim3(256), 0, s, P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (float*)d_act);
+    } else {
+      if (P.big_act) ce_launch<CfgBig, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+      else ce_launch<CfgSmall, float, MODE_COUNTED, EpiStore, false, true>(b, {}, P.splits, V % 64 != 0, s);
+      hipLaunchKernelGGL(k_ce_scatter<bf16_t>, grid, dim3(256), 0, s, P.slabs, P.splits, R * d, N, d, P.pos, c * R, R, (bf16_t*)d_act);
+    }
   }
   if (d_head) {
-    const GemmArgs b{V, d, M, P.G, P.ld, a_c, d, P.chunks > 1 ? (void*)P.head : d_head, d, 1.f, c ? 1.f : 0.f, count, 0, 0, 0, 0,
+    const bool sum = P.half && P.chunks > 1;  // bf16 chunks are added in fp32
+    const GemmArgs b{V, d, M, G, P.ld, (const bf16_t*)a_c, d, sum ? (void*)P.head : d_head, d, 1.f, c ? 1.f : 0.f, count, 0, 0, 0, 0,
                      nullptr, nullptr, nullptr};
-    if (P.chunks > 1) {
+    if (!P.half) {
+      ce_launch_f32<MODE_COUNTED_K, EpiCEStore, true, true>(b, 1, s);
+    } else if (sum) {
       if (P.big_head) ce_launch<CfgBig, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
       else ce_launch<CfgSmall, float, MODE_COUNTED_K, EpiStore, true, true>(b, {}, 1, true, s);
     } else {
@@ -959,7 +1047,7 @@ int pd_streamed_ce_bwd(int dtype, int64_t N, int64_t d, int64_t V, const void* a
 size_t pd_streamed_ce_train_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
   if (N <= 0 || d <= 0 || V <= 0) return 0;
   if (ce_one_form(dtype, d, V)) {
-    const CEOnePlan P = ce_one_plan(N, d, V, want_dact, want_dhead, false, nullptr, nullptr);
+    const CEOnePlan P = ce_one_plan(dtype, N, d, V, want_dact, want_dhead, false, nullptr, nullptr);
     return P.kept + P.work;
   }
   return up256((size_t)N * 8) + std::max(ce_fwd_plan(dtype, N, d, V, nullptr).total,
@@ -984,19 +1072,18 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
     return pd_streamed_ce_bwd(dtype, N, d, V, act, head, targets, target_bits, ignore_index, stats, g, d_act, d_head, ws, left,
                               stream);
   }
-  const size_t kept = ce_one_plan(N, d, V, false, false, false, nullptr, nullptr).kept;
-  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, false, (char*)workspace, (char*)workspace + kept);
-  if (!dtl_fits_mn(P.R, P.ld)) return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
+  const size_t kept = ce_one_plan(dtype, N, d, V, false, false, false, nullptr, nullptr).kept;
+  const CEOnePlan P = ce_one_plan(dtype, N, d, V, d_act != nullptr, d_head != nullptr, false, (char*)workspace, (char*)workspace + kept);
+  if (P.half && !dtl_fits_mn(P.R, P.ld)) return fail(PD_EUNSUPPORTED, std::string(what) + ": too large");
   const CETargets t{targets, target_bits, ignore_index, V};
-  const bf16_t* hd = (const bf16_t*)head;
   hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, P.pos, P.count, loss, nullptr);
-  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
+  ce_gather(P.half, act, N, d, P.rows, P.count, P.act, s);
   hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
   for (int c = 0; c < P.chunks; ++c) {
-    ce_one_loss(P, c, N, d, V, hd, t, loss, s);
-    ce_one_grads(P, c, N, d, V, hd, t, g, d_act, d_head, s);
+    ce_one_loss(P, c, N, d, V, head, t, loss, s);
+    ce_one_grads(P, c, N, d, V, head, t, g, d_act, d_head, s);
   }
-  if (d_head && P.chunks > 1)
+  if (P.half && d_head && P.chunks > 1)
     hipLaunchKernelGGL(k_ce_round, dim3((unsigned)std::min<int64_t>(cdiv(V * d / 4, 256), 16384)), dim3(256), 0, s,
                        (const float4*)P.head, V * d / 4, (uint2*)d_head);
   return check_launch(what);
@@ -1004,13 +1091,13 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
 
 size_t pd_streamed_ce_kept_size(int dtype, int64_t N, int64_t d, int64_t V) {
   if (N <= 0 || d <= 0 || V <= 0 || !ce_one_form(dtype, d, V)) return 0;
-  const CEOnePlan P = ce_one_plan(N, d, V, false, false, true, nullptr, nullptr);
-  return P.chunks == 1 && dtl_fits_mn(P.R, P.ld) ? P.kept : 0;
+  const CEOnePlan P = ce_one_plan(dtype, N, d, V, false, false, true, nullptr, nullptr);
+  return P.chunks == 1 && (!P.half || dtl_fits_mn(P.R, P.ld)) ? P.kept : 0;
 }
 
 size_t pd_streamed_ce_kept_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead) {
   if (!pd_streamed_ce_kept_size(dtype, N, d, V)) return 0;
-  return ce_one_plan(N, d, V, want_dact, want_dhead, true, nullptr, nullptr).work;
+  return ce_one_plan(dtype, N, d, V, want_dact, want_dhead, true, nullptr, nullptr).work;
 }
 
 int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,
@@ -1021,15 +1108,15 @@ int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const vo
   if (!N || !loss) return fail(PD_EINVAL, std::string(what) + ": positions and loss required");
   const size_t need = pd_streamed_ce_kept_size(dtype, N, d, V);
   if (!need) return fail(PD_EUNSUPPORTED, std::string(what) + ": nothing is kept at this size");
-  const CEOnePlan P = ce_one_plan(N, d, V, false, false, true, (char*)kept, (char*)workspace);
+  const CEOnePlan P = ce_one_plan(dtype, N, d, V, false, false, true, (char*)kept, (char*)workspace);
   if (!kept || kept_bytes < need || !workspace || workspace_bytes < P.work)
     return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
   hipStream_t s = (hipStream_t)stream;
   const CETargets t{targets, target_bits, ignore_index, V};
   hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, t, nullptr, N, P.rows, P.pos, P.count, loss, nullptr);
-  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
+  ce_gather(P.half, act, N, d, P.rows, P.count, P.act, s);
   hipLaunchKernelGGL(k_ce_counts, dim3(1), dim3(64), 0, s, P.count, P.R, P.chunks, P.counts);
-  ce_one_loss(P, 0, N, d, V, (const bf16_t*)head, t, loss, s);
+  ce_one_loss(P, 0, N, d, V, head, t, loss, s);
   return check_launch(what);
 }
 
@@ -1043,14 +1130,14 @@ int pd_streamed_ce_kept_bwd(int dtype, int64_t N, int64_t d, int64_t V, const vo
   if (!N || !g) return fail(PD_EINVAL, std::string(what) + ": positions and g required");
   const size_t need = pd_streamed_ce_kept_size(dtype, N, d, V);
   if (!need) return fail(PD_EUNSUPPORTED, std::string(what) + ": nothing is kept at this size");
-  const CEOnePlan P = ce_one_plan(N, d, V, d_act != nullptr, d_head != nullptr, true, (char*)const_cast<void*>(kept),
+  const CEOnePlan P = ce_one_plan(dtype, N, d, V, d_act != nullptr, d_head != nullptr, true, (char*)const_cast<void*>(kept),
                                   (char*)workspace);
   if (!kept || kept_bytes < need || !workspace || workspace_bytes < P.work)
     return fail(PD_EWORKSPACE, std::string(what) + ": workspace");
   hipStream_t s = (hipStream_t)stream;
   const CETargets t{targets, target_bits, ignore_index, V};
-  ce_gather(true, act, N, d, P.rows, P.count, P.act, s);
-  ce_one_grads(P, 0, N, d, V, (const bf16_t*)head, t, g, d_act, d_head, s);
+  ce_gather(P.half, act, N, d, P.rows, P.count, P.act, s);
+  ce_one_grads(P, 0, N, d, V, head, t, g, d_act, d_head, s);
   return check_launch(what);
 }
 

@@ -372,9 +372,9 @@ def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targe
     lies outside [0, V) has loss 0, no gradient and no part in the products. Returns fp32 [...];
     differentiable in act and head, once: gradients in their dtype (bf16: from softmax differences rounded to bf16).
 
-    With bf16 tensors the softmax is kept in 16 bits for the backward where it and the head take less than 2 GiB each (2 bytes for each
-    position and entry of the vocabulary: 0.8 GB for 8192 over 50277); else, and with `keep` False, the backward forms the logits
-    again, a third of the gradient's products, over pieces of the vocabulary. `ops.streamed_cross_entropy` gives loss and weighted
+    The softmax is kept in 16 bits (fp32: the logits) for the backward where it takes less than 2 GiB, 2 or 4 bytes for each
+    position and entry of the vocabulary (0.8 GB for bf16, 8192 over 50277), as has to a bf16 head; else, and with `keep`
+    False, the backward forms the logits again over pieces of the vocabulary, half as much again of its products. `ops.streamed_cross_entropy` gives loss and weighted
     gradients in one call."""
     lead, d = act.shape[:-1], act.shape[-1] if act.dim() else 0
     pad = (-d) % 8 if act.dtype == torch.bfloat16 else 0

@@ -736,10 +736,9 @@ def streamed_cross_entropy_bwd(act, head, targets, stats, g, *, ignore_index: in
 
 
 def streamed_cross_entropy_kept_fwd(act, head, targets, *, ignore_index: int = -100):
-    """(loss fp32 [N], kept): the forward that leaves the softmax in 16 bits for
-    `streamed_cross_entropy_kept_bwd`, which then forms no logits again. kept (2 bytes for each
-    position and entry of the vocabulary) is None for fp32 and where it or the head would take 2 GiB:
-    nothing has run then."""
+    """(loss fp32 [N], kept): the forward that leaves the softmax in 16 bits (fp32: the
+    logits) for `streamed_cross_entropy_kept_bwd`, which then forms no logits again. kept (2 or 4 bytes for each
+    position and entry of the vocabulary) is None where it would take 2 GiB, or a bf16 head does: nothing has run then."""
     name = "streamed_cross_entropy_kept_fwd"
     device, sizes = _ce_checks(name, act, head, targets)
     nbytes = L.load().pd_streamed_ce_kept_size(*sizes)

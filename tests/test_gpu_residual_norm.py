@@ -103,6 +103,13 @@ def test_rows_and_gates(device, rows, gate, d):
         _check(_case(device, rows, d, types, gate, seed=rows, gate_dtype=BF16 if i == 1 else F32))
 
 
+@pytest.mark.parametrize("rows, gate", [(1, 1), (6, 3), (300, 300), (1000, 500), (600, 2), (2000, 1000), (700, 1), (700, 0)])
+def test_gates_of_wide_rows(device, rows, gate):
+    """Whose sums over rows are formed apart from the rows' own gradients."""
+    for i, types in enumerate(TYPES):
+        _check(_case(device, rows, 4104, types, gate, seed=rows, gate_dtype=BF16 if i == 1 else F32))
+
+
 def test_without_weights_and_around_zero(device):
     c = _case(device, 50, 96, (BF16, BF16), gate=5)
     c["pre"] -= 1
@@ -127,8 +134,9 @@ def test_axes_strides_and_gates_of_sequences(device):
     assert d.shape == gate.shape
 
 
-def test_one_result_alone_and_one_gradient_alone(device):
-    c = _case(device, 70, 300, (BF16, BF16), gate=7)
+@pytest.mark.parametrize("d", [300, 5000])
+def test_one_result_alone_and_one_gradient_alone(device, d):
+    c = _case(device, 70, d, (BF16, BF16), gate=7)
     names = ("x", "branch", "post", "gate", "pre")
     leaves = [c[n].requires_grad_() for n in names]
     call = lambda ls: residual_norm(ls[0], ls[1], post_weight=ls[2], gate=ls[3], pre_weight=ls[4], scale=0.7)  # noqa: E731

@@ -76,8 +76,8 @@ def _both_forms(act, head, t, w, ignore=-100):
     if kept is not None:
         ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, 3 * w, ignore_index=ignore)  # leaves it as it is
         forms.append((loss, *ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, w, ignore_index=ignore)))
-    large = max(2 * act.shape[0] * head.shape[0], 2 * head.numel()) > 2**31 - 2**23
-    assert (kept is None) == (act.dtype == F32 or large)
+    large = max(act.element_size() * act.shape[0] * head.shape[0], 2 * head.numel() * (act.dtype == BF16)) > 2**31 - 2**23
+    assert (kept is None) == large
     return forms
 
 

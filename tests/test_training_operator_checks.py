@@ -72,10 +72,10 @@ def test_cross_entropy_entry_points_refuse():
     size = lib.pd_streamed_ce_train_workspace_size
     assert size(L.BF16, 4, 16, 9, 1, 1) > 0 and size(L.BF16, 0, 16, 9, 1, 1) == 0
     kept = lib.pd_streamed_ce_kept_size
-    assert kept(L.BF16, 4, 16, 9) > 0 and kept(L.BF16, 0, 16, 9) == 0 and kept(L.F32, 4, 16, 9) == 0
+    assert kept(L.BF16, 4, 16, 9) > 0 and kept(L.BF16, 0, 16, 9) == 0 and kept(L.F32, 8192, 16, 131072) == 0
     assert 8192 * 50277 * 2 <= kept(L.BF16, 8192, 768, 50277) < 1 << 30 and kept(L.BF16, 1 << 18, 16, 131072) == 0
     a = (b, b, b, 64, -100)
-    assert lib.pd_streamed_ce_kept_fwd(L.F32, 4, 16, 9, *a, b, b, 2**62, b, 2**62, None) == 3  # nothing is kept
+    assert lib.pd_streamed_ce_kept_fwd(L.F32, 8192, 16, 131072, *a, b, b, 2**62, b, 2**62, None) == 3  # nothing is kept
     assert lib.pd_streamed_ce_kept_fwd(L.BF16, 4, 16, 9, *a, b, b, 16, b, 2**62, None) == 4
     assert lib.pd_streamed_ce_kept_fwd(L.BF16, 4, 16, 9, *a, b, b, 2**62, b, 16, None) == 4
     assert lib.pd_streamed_ce_kept_fwd(L.BF16, 0, 16, 9, *a, b, b, 2**62, b, 2**62, None) == 1
