@@ -277,7 +277,7 @@ __device__ __noinline__ void rt_rank_wide(const RtArgs& a, const float* xs, int 
     // without a bias the logits are in the scores' order
     double key = raw || !a.bias ? v : a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - m) / total;
     if (a.bias) key += (double)a.bias[e];
-    lds[i] = key;
+    lds[i] = v == -INFINITY ? v : key;  // masked, whatever its bias
     won[i].y = (uint32_t)e;
   }
   rt_wave_sync();
@@ -447,8 +447,9 @@ __global__ __launch_bounds__(256, J > 8 ? 4 : 8) void k_rt_fwd(RtArgs a) {
     // whether 64 bits may order two words the other way round
     auto close = [&](uint32_t hi, uint32_t lo) {
       if (raw) return (hi & ~LOW) == (lo & ~LOW);
+      if (lo <= LOW + 1u + LOW) return lo != 0u && hi <= LOW + 1u + LOW;  // masked: equal to its like, behind all others
       const float f = rt_unorder(hi & ~LOW), g = rt_unorder(lo & ~LOW);
-      return lo != 0u && !(f - g > 1.5e-6f * smax + (J * 1.2e-7f + 5e-7f) * fmaxf(fabsf(f), fabsf(g)));
+      return !(f - g > 1.5e-6f * smax + (J * 1.2e-7f + 5e-7f) * fmaxf(fabsf(f), fabsf(g)));
     };
     // the rest that may belong to the k best joins them
     int n = a.k;

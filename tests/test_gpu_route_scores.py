@@ -209,3 +209,42 @@ def test_refusals(device):
     _, idx = ops.route_scores_fwd(x, 2)
     with pytest.raises(L.PDError):
         ops.route_scores_bwd(x, idx, torch.zeros(4, 2))
+
+
+def _apart(E, n):
+    """n experts, each in a lane of its own and at another place of it (or, where E is small, the last n)."""
+    return torch.arange(n) * 9 if E >= 64 else torch.arange(E - n, E)
+
+
+@pytest.mark.parametrize("E, masked, groups", [(8, 6, 1), (8, 1, 1), (8, 7, 1), (8, 5, 2), (42, 5, 1), (42, 5, 6), (64, 8, 1), (64, 8, 8),
+                                               (100, 6, 1), (100, 6, 4), (600, 12, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_bias_does_not_bring_masked_experts_back(device, E, masked, groups, dtype):
+    """Masked experts whose words differ, a bias in their favour, and k below, at and above the number that is left."""
+    gone = _apart(E, masked).to(device)
+    bias = torch.linspace(-0.2, 0.2, E, device=device)
+    bias[gone] += 0.9
+    x = _x(device, 30, E, dtype, E + masked)
+    x[:, gone] = -INF
+    for kind in KINDS:
+        for top in sorted({groups, groups - 1 or 1}):
+            size = E // groups
+            for k in {1, 2, E - masked - 1, E - masked, E - masked + 1, E}:
+                if not 1 <= k <= min(64, size * top):
+                    continue
+                kw = dict(kind, bias=bias, n_groups=groups, top_groups=top)
+                w, idx = experts.route_scores(x, k, **kw)
+                want, at = _expected(x, k, **kw)
+                assert torch.equal(idx.long(), at), (kind, top, k)
+                assert ((w.double() - want).abs() <= 64 * U * want.abs() + 1e-37).all()
+                leaf = x.clone().requires_grad_()
+                (d,) = torch.autograd.grad(experts.route_scores(leaf, k, **kw)[0].sum(), leaf)
+                assert torch.isfinite(d).all() and not d[x == -INF].any()
+
+
+def test_one_masked_expert_beside_a_live_one(device):
+    x = torch.full((1, 8), -INF, device=device)
+    x[0, :2] = torch.tensor([1.0, -1.0])
+    bias = torch.tensor([0, 0, 0.9, 0.9, 0.9, 0.9, 0.9, 0.9], device=device)
+    w, idx = experts.route_scores(x, 2, scoring="sigmoid", bias=bias)
+    assert idx.tolist() == [[0, 1]] and (w > 0).all()
