@@ -256,13 +256,13 @@ __device__ __noinline__ void rt_choose_wide(const RtArgs& a, const float* xs, in
   }
 }
 
-// The order of n candidates won[i] (words and their lanes' first experts) by 64-bit scores: the k
-// best of them into won[r].y. Each lane ranks its candidates against all.
+// The order of n candidates won[i] (words and their lanes' first experts) by the scores that rt_choose_wide compares: the
+// k best of them into won[r].y. Each lane ranks its candidates against all.
 template <int NT, int J>
 __device__ __noinline__ void rt_rank_wide(const RtArgs& a, const float* xs, int lane, int n, double* lds, uint2* won) {
   double m = 0.0, total = 1.0;
   const bool raw = !a.bias && a.groups == 1;
-  if (a.bias && !a.sigmoid) {
+  if (!raw && !a.sigmoid) {
     float top = -INFINITY;
     for (int j = 0; j < J; ++j) top = fmaxf(top, xs[lane * J + j]);
     m = (double)rt_max<NT>(top);
@@ -274,8 +274,8 @@ __device__ __noinline__ void rt_rank_wide(const RtArgs& a, const float* xs, int 
   for (int i = lane; i < n; i += NT) {
     const int e = (int)(won[i].y + (J - 1 - (won[i].x & (J - 1))));
     const double v = (double)xs[e];
-    // without a bias the logits are in the scores' order
-    double key = raw || !a.bias ? v : a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - m) / total;
+    // scores, not logits: those of unequal logits may be equal, and the lower index is first then
+    double key = raw ? v : a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - m) / total;
     if (a.bias) key += (double)a.bias[e];
     lds[i] = v == -INFINITY ? v : key;  // masked, whatever its bias
     won[i].y = (uint32_t)e;

@@ -182,7 +182,8 @@ def route_scores(logits: torch.Tensor, k: int, *, scoring: Literal["softmax", "s
     choice alone (a balance that is kept beside training), `n_groups` runs of experts are cut to the
     `top_groups` whose two best keys sum highest (None: all), and the k best keys of those are
     chosen, best first, equal ones by the lower index. weights = scale * scores of the chosen, over
-    their sum with `renormalize`. A logit of -inf masks its expert. Keys are compared in 64 bits;
+    their sum with `renormalize`. A logit of -inf masks its expert. Keys are compared in 64 bits
+    (without a bias and where all groups stay the logits themselves, so equal scores of unequal logits are told apart there);
     differentiable in the logits through the weights, once; the choice and `bias` have no gradient."""
     if scoring not in ("softmax", "sigmoid"):
         raise L.PDError(f"route_scores: scoring is softmax or sigmoid, got {scoring!r}")

@@ -248,3 +248,18 @@ def test_one_masked_expert_beside_a_live_one(device):
     bias = torch.tensor([0, 0, 0.9, 0.9, 0.9, 0.9, 0.9, 0.9], device=device)
     w, idx = experts.route_scores(x, 2, scoring="sigmoid", bias=bias)
     assert idx.tolist() == [[0, 1]] and (w > 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_equal_scores_of_unequal_logits(device, dtype):
+    """Scores that are one number in 64 bits (saturated sigmoids, exponentials of logits next to zero): inside groups the
+    lower index is first, wherever the experts lie in their lanes."""
+    E, groups = 64, 8
+    for places in ([0, 9, 2, 11], [0, 8, 2, 10], [7, 6, 5, 4], [15, 14, 1, 0], [3, 11, 6, 5]):
+        for a, b, kind in ((40.0, 41.0, dict(scoring="sigmoid")), (300.0, 38.0, dict(scoring="sigmoid", renormalize=False)),
+                           (0.0, 1e-20, dict()), (1e-20, -1e-20, dict(renormalize=False))):
+            x = _x(device, 2, E, torch.float32, 11, 0.1) - 6
+            x[0, places] = torch.tensor([a, b, a, b], device=device)
+            x[1, places] = torch.tensor([b, a, b, a], device=device)
+            for k in (1, 2, 3, 4, 6):
+                _check(device, x.to(dtype), k, **dict(kind, n_groups=groups, top_groups=2))
