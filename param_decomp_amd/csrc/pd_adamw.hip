@@ -58,7 +58,7 @@ struct AdamWArgs {
 static_assert(sizeof(AdamWArgs) <= 4096, "kernel arguments");
 
 struct AdamWRates {
-  float a1, a2, size, root, eps, keep, gs;  // size = lr / c1, root = 1 / sqrt(c2), keep = 1 - lr decay
+  float a1, a2, size, root, eps, decay, gs;  // size = lr / c1, root = 1 / sqrt(c2), decay = lr times it
   uint32_t k0, k1;
 };
 
@@ -181,7 +181,8 @@ __device__ inline void adamw_finish(const AdamWTensor& t, const AdamWRates& h, i
     m[e] = fmaf(h.a1, g - m[e], m[e]);
     v[e] = fmaf(h.a2, square_less(g, v[e]), v[e]);
     root[e] = Q8 ? sqrtf(v[e]) : __builtin_amdgcn_sqrtf(v[e]);
-    p[e] = w.p[e] * h.keep - m[e] * h.size * __builtin_amdgcn_rcpf(fmaf(root[e], h.root, h.eps));
+    // taken off with the update: 1 - lr decay would round what lies below 2^-24 away
+    p[e] = w.p[e] - fmaf(h.decay, w.p[e], m[e] * h.size * __builtin_amdgcn_rcpf(fmaf(root[e], h.root, h.eps)));
   }
   const int left = FULL ? 4 : (int)(t.n - i < 0 ? 0 : (t.n - i < 4 ? t.n - i : 4));
   if (FULL) {
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256) void k_adamw(AdamWArgs a) {
   h.gs = a.grad_scale ? *a.grad_scale : 1.f;
   h.size = lr / -expm1f((float)((double)step * a.log_b1));
   h.root = 1.f / sqrtf(-expm1f((float)((double)step * a.log_b2)));
-  h.keep = 1.f - lr * a.decay;
+  h.decay = lr * a.decay;
   h.k0 = 0u, h.k1 = (uint32_t)step;
   threefry2x32(a.k0, a.k1, h.k0, h.k1);
   const int64_t lo = (int64_t)((int)blockIdx.x - t.first) * a.chunk;

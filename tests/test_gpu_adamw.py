@@ -265,3 +265,24 @@ def test_saved_tensors_notice_the_step(device):
     AdamW([p]).step([torch.ones_like(p)])
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("lr, wd", [(1e-3, 1e-2), (1e-6, 1e-2), (1e-7, 1e-1)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_small_decay_is_not_lost(device, lr, wd, bits):
+    """lr * decay below the spacing of fp32 at 1, against the step in 64 bits rounded once. The update is off by 32 2^-24
+    of itself, which moves the mean of the rounded values by as much, and a value that lies so close to a border
+    becomes its neighbour, a step of 2^-23 (p in [1, 2)) up or down: five standard deviations of the mean if all did. (A mean of
+    uniform roundings is not what to compare with: at lr 1e-7 updates are below a step, and p' follows them in steps.)"""
+    n = 1 << 20
+    g = torch.Generator(device=device).manual_seed(1)
+    p = 1 + torch.rand(n, device=device, generator=g)
+    grad = torch.randn(n, device=device, generator=g) * (0.5 + torch.rand(n, device=device, generator=g))
+    before = p.double()
+    opt = AdamW([p], lr=lr, betas=(B1, B2), eps=0.5, weight_decay=wd, state_bits=bits)
+    opt.step([grad])
+    update = lr * grad.double() / (grad.double().abs() + 0.5)
+    off = (p.double() - (before - lr * wd * before - update).float().double()).mean()
+    tol = 32 * U * update.abs().mean() + 5 * 2.0**-23 / math.sqrt(n)
+    assert tol < 0.2 * lr * wd * before.mean()  # what is lost would show
+    assert abs(off) <= tol, (float(off), float(tol))
