@@ -180,7 +180,7 @@ __device__ inline void adamw_finish(const AdamWTensor& t, const AdamWRates& h, i
     const float g = w.g[e] * h.gs;
     m[e] = fmaf(h.a1, g - m[e], m[e]);
     v[e] = fmaf(h.a2, square_less(g, v[e]), v[e]);
-    root[e] = Q8 ? sqrtf(v[e]) : __builtin_amdgcn_sqrtf(v[e]);
+    root[e] = sqrtf(v[e]);  // the hardware's own reads subnormal numbers as zero, and the step would be m / eps
     // taken off with the update: 1 - lr decay would round what lies below 2^-24 away
     p[e] = w.p[e] - fmaf(h.decay, w.p[e], m[e] * h.size * __builtin_amdgcn_rcpf(fmaf(root[e], h.root, h.eps)));
   }

@@ -286,3 +286,18 @@ def test_a_small_decay_is_not_lost(device, lr, wd, bits):
     tol = 32 * U * update.abs().mean() + 5 * 2.0**-23 / math.sqrt(n)
     assert tol < 0.2 * lr * wd * before.mean()  # what is lost would show
     assert abs(off) <= tol, (float(off), float(tol))
+
+
+@pytest.mark.parametrize("size", [1e-19, 1e-20, 1e-21])
+def test_roots_of_subnormal_squares(device, size):
+    """v below fp32's normal numbers and an eps below its root: the step goes by the root of the v that is stored."""
+    n = 3000
+    p = torch.zeros(n, device=device)
+    g = torch.Generator(device=device).manual_seed(2)
+    grad = (1 + torch.rand(n, device=device, generator=g)) * size
+    opt = AdamW([p], lr=LR, betas=(B1, B2), eps=2.0**-126, weight_decay=0.0)
+    opt.step([grad])
+    m, v = opt.state["m"][0].double(), opt.state["v"][0].double()
+    assert (v > 0).all() and (v < 2.0**-100).all()
+    want = -LR * (m / (1 - B1)) / ((v / (1 - B2)).sqrt() + 2.0**-126)
+    _within(p, want, 32 * U * want.abs())
