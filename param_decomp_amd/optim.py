@@ -8,6 +8,7 @@ that the next step computes with, all tensors in one launch.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -16,9 +17,12 @@ from param_decomp_amd.prng import Key
 
 QBLOCK = 256  # values of an 8-bit state that share a scale
 FP8 = torch.float8_e4m3fn
+_ADDRESS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.numel
 
 
 def _plain(name: str, label: str, t: torch.Tensor, numel: int, dtypes, device) -> torch.Tensor:
+    if t is None:
+        raise L.PDError(f"{name}: {label} is missing")
     if t.dtype not in dtypes or t.numel() != numel or t.device != device or not t.is_contiguous():
         raise L.PDError(f"{name}: {label} is a dense {' or '.join(str(d)[6:] for d in dtypes)} tensor of {numel} values "
                         f"on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -36,7 +40,8 @@ class AdamW:
     `state`: {"step" int32 [1], "m", "v": lists} and with 8 bits {"m_scale", "v_scale": lists},
     where a tensor of fp32 states has None; used in place. Default: zeros. `v` holds sqrt(v)
     where it has 8 bits. The step count is in device memory: a captured `step` goes on counting
-    when it is replayed."""
+    when it is replayed. Tensors exchanged in `params`, `state` and `copies` (of the same sizes and types: checked) are those that
+    the next `step` uses; a captured one keeps those that it was captured with."""
 
     def __init__(self, params, *, lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, state_bits: int = 32, key: Key = (0, 0), min_8bit_size: int = 0,
@@ -50,48 +55,57 @@ class AdamW:
         device = self.params[0].device
         if device.type != "cuda":
             raise L.PDError("pd kernels take GPU tensors")
-        for i, p in enumerate(self.params):
-            _plain(name, f"parameter {i}", p, p.numel(), (torch.float32,), device)
         self.device, self.lr, self.betas, self.eps, self.weight_decay = device, lr, betas, eps, weight_decay
         self.key = (int(key[0]), int(key[1]))
-        sizes = [p.numel() for p in self.params]
-        small = [state_bits == 32 or n < min_8bit_size for n in sizes]  # states of 32 bits
-        self.state = self._zeros(sizes, small) if state is None else state
-        self._check_state(sizes, small)
-        if copies is not None:
-            copies = list(copies)
-            if len(copies) != len(sizes):
-                raise L.PDError(f"{name}: {len(copies)} copies for {len(sizes)} parameters")
-            for i, (c, n) in enumerate(zip(copies, sizes)):
-                if c is not None:
-                    _plain(name, f"copy {i}", c, n, (torch.bfloat16,), device)
-        self.copies = copies
+        self._sizes = [p.numel() for p in self.params]
+        self._small = [state_bits == 32 or n < min_8bit_size for n in self._sizes]  # states of 32 bits
+        self.state = self._zeros(self._sizes, self._small) if state is None else state
+        self.copies = None if copies is None else list(copies)
         self._ticket = torch.zeros(1, dtype=torch.int32, device=device)
-        self._sizes, self._shapes = sizes, [p.shape for p in self.params]
-        self._c_sizes = L.host_array(ctypes.c_int64, sizes)
-        n, st = len(sizes), self.state
-        none = [None] * n
-        # the tensors of each argument, in the entry point's order
-        self._held = [list(ts) for ts in (self.params, st["m"], st["v"], st.get("m_scale") or none, st.get("v_scale") or none,
-                                          copies or none)]
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                       for ts in (*self._held, [st["step"]]) for t in ts if t is not None and t.numel())
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-            raise L.PDError(f"{name}: two of the parameters, states and copies share memory")
-        self._written = self._held[0] + [c for c in self._held[5] if c is not None]
-        self._at: list[int] | None = None
+        self._c_sizes = L.host_array(ctypes.c_int64, self._sizes)
+        self._held: list = []
+        self._pointers()
 
     def _pointers(self) -> None:
-        """The arrays of addresses, formed again where a tensor's memory has been exchanged (`p.data = ...`)."""
-        at = [0 if t is None else t.data_ptr() for ts in self._held for t in ts]
-        if at == self._at:
+        """The arrays of addresses, checked and formed again where a tensor is another one than before or its memory has been
+        exchanged (`p.data = ...`): the steps use what `params`, `state` and `copies` hold when they run."""
+        n, st = len(self._sizes), self.state
+        none = [None] * n
+        # the tensors of each argument, in the entry point's order
+        held = [*self.params, *st["m"], *st["v"], *(st.get("m_scale") or none), *(st.get("v_scale") or none),
+                *(none if self.copies is None else self.copies), st["step"]]
+        live = [t for t in held if t is not None]
+        at, sizes = list(map(_ADDRESS, live)), list(map(_NUMEL, live))
+        if len(held) == len(self._held) and all(map(operator.is_, held, self._held)) and at == self._at and sizes == self._at_sizes:
             return
-        n = len(self._sizes)
-        for i, (p, size) in enumerate(zip(self.params, self._sizes)):
-            _plain("AdamW", f"parameter {i}", p, size, (torch.float32,), self.device)
-        arrays = [L.host_array(ctypes.c_void_p, [a or None for a in at[k * n:(k + 1) * n]]) for k in range(6)]
+        self._check()
+        where = [None if t is None else t.data_ptr() or None for t in held]
+        arrays = [L.host_array(ctypes.c_void_p, where[k * n:(k + 1) * n]) for k in range(6)]
         self._p, self._m, self._v, self._ms, self._vs, self._c = arrays
-        self._at = at
+        self._shapes = [p.shape for p in self.params]
+        self._written = self.params + [c for c in self.copies or () if c is not None]
+        self._held, self._at, self._at_sizes = held, at, sizes
+        # the memory is kept, so that nothing else can come to lie at an address that was checked
+        self._memory = [t.detach() for t in live]
+
+    def _check(self) -> None:
+        name, st, sizes = "AdamW", self.state, self._sizes
+        if len(self.params) != len(sizes):
+            raise L.PDError(f"{name}: {len(self.params)} parameters, {len(sizes)} when it was made")
+        for i, (p, n) in enumerate(zip(self.params, sizes)):
+            _plain(name, f"parameter {i}", p, n, (torch.float32,), self.device)
+        self._check_state(sizes, self._small)
+        copies = [None] * len(sizes) if self.copies is None else self.copies
+        if len(copies) != len(sizes):
+            raise L.PDError(f"{name}: {len(copies)} copies for {len(sizes)} parameters")
+        for i, (c, n) in enumerate(zip(copies, sizes)):
+            if c is not None:
+                _plain(name, f"copy {i}", c, n, (torch.bfloat16,), self.device)
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for ts in (self.params, st["m"], st["v"], st.get("m_scale") or (), st.get("v_scale") or (), copies, [st["step"]])
+                       for t in ts if t is not None and t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise L.PDError(f"{name}: two of the parameters, states and copies share memory")
 
     def _zeros(self, sizes, small) -> dict:
         dev = self.device
@@ -127,6 +141,7 @@ class AdamW:
         tensor of one value on the GPU, and `grad_scale` such a tensor that gradients are
         multiplied with: both are read when the step runs, also in a replayed graph."""
         name, n = "AdamW.step", len(self._sizes)
+        self._pointers()
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != n:
             raise L.PDError(f"{name}: {len(grads)} gradients for {n} parameters")
@@ -147,7 +162,6 @@ class AdamW:
         lr = self.lr if lr is None else lr
         lr_dev = self._scalar("lr", lr) if isinstance(lr, torch.Tensor) else None
         scale = None if grad_scale is None else self._scalar("grad_scale", grad_scale)
-        self._pointers()
         L.launch("pd_adamw_step", self.device, n, self._c_sizes, self._p, (ctypes.c_void_p * n)(*ptrs),
                  (ctypes.c_int32 * n)(*types), self._m, self._v, self._ms, self._vs, self._c,
                  self.state["step"].data_ptr(), self._ticket.data_ptr(), 0.0 if lr_dev else float(lr), lr_dev, scale,

@@ -301,3 +301,65 @@ def test_roots_of_subnormal_squares(device, size):
     assert (v > 0).all() and (v < 2.0**-100).all()
     want = -LR * (m / (1 - B1)) / ((v / (1 - B2)).sqrt() + 2.0**-126)
     _within(p, want, 32 * U * want.abs())
+
+
+def test_tensors_that_are_exchanged_are_those_that_the_steps_use(device):
+    sizes, kw = [300, 5000], dict(lr=LR, betas=(B1, B2), eps=EPS, weight_decay=WD, state_bits=8, min_8bit_size=1000, key=(3, 4))
+    a, g = _tensors(device, sizes, 9)
+    b = [x.clone() for x in a]
+    half = lambda: [torch.empty(n, dtype=torch.bfloat16, device=device) for n in sizes]  # noqa: E731
+    one, two = AdamW(a, copies=half(), **kw), AdamW(b, copies=half(), **kw)
+    for opt in (one, two):
+        opt.step(g)
+    own = lambda t: None if t is None else t.clone()  # noqa: E731
+    old = [x.clone() for x in two.params]
+    kept = [(x, own(x)) for k in ("m", "v", "m_scale", "v_scale") for x in two.state[k]] + [(x, own(x)) for x in two.copies]
+    first = two.params[0]
+    two.params[0] = first.clone()
+    for k in ("m", "v", "m_scale", "v_scale"):
+        two.state[k] = [own(x) for x in two.state[k]]  # another list
+    two.state["m"][0] = two.state["m"][0].clone()       # another tensor of it
+    two.state["v"][1].data = two.state["v"][1].data.clone()
+    two.state["step"] = two.state["step"].clone()
+    two.copies[1] = two.copies[1].clone()
+    for opt in (one, two):
+        opt.step(g)
+    assert torch.equal(first, old[0])
+    for x, y in kept[:-2] + kept[-1:]:
+        assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    for x, y in zip(one.params + one.copies, two.params + two.copies):
+        assert torch.equal(x, y)
+    for k in ("m", "v", "m_scale", "v_scale"):
+        for x, y in zip(one.state[k], two.state_dict()[k]):
+            assert (x is None) == (y is None) and (x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8)))
+    assert int(two.state["step"]) == 2
+
+
+def test_exchanged_tensors_are_checked(device):
+    sizes, kw = [2000, 600], dict(state_bits=8, min_8bit_size=1000)
+    p, g = _tensors(device, sizes, 10)
+    other = torch.zeros(40, dtype=torch.int32, device=device)
+
+    def make():
+        return AdamW([x.clone() for x in p], copies=[torch.zeros(n, dtype=torch.bfloat16, device=device) for n in sizes], **kw)
+
+    def shrink(t):
+        t.data = t.data[:t.numel() // 2]
+
+    for change in (lambda o: shrink(o.params[0]), lambda o: shrink(o.state["m"][0]), lambda o: shrink(o.state["v"][1]),
+                   lambda o: shrink(o.state["m_scale"][0]), lambda o: shrink(o.copies[1]),
+                   lambda o: o.state["m"].__setitem__(0, o.state["m"][0][:1000]), lambda o: o.state["v"].__setitem__(0, torch.zeros(2000, device=device)),
+                   lambda o: o.state["v_scale"].__setitem__(0, None), lambda o: o.state["m"].pop(), lambda o: o.copies.pop(),
+                   lambda o: o.copies.__setitem__(0, o.copies[0].float()), lambda o: o.params.pop(), lambda o: o.params.__setitem__(1, p[0]),
+                   lambda o: o.params.__setitem__(0, None), lambda o: o.state["v"].__setitem__(0, None), lambda o: o.copies.clear(),
+                   lambda o: o.state.update(step=other[:2]), lambda o: o.state.update(step=torch.zeros(1, device=device)),
+                   lambda o: o.state["m"].__setitem__(1, o.state["v"][1]), lambda o: o.state.update(v=o.state["m"]),
+                   lambda o: o.params[0].__setattr__("data", o.params[0].data.cpu()), lambda o: o.copies.__setitem__(0, o.copies[0].cpu())):
+        opt = make()
+        opt.step(g)
+        before = [x.clone() for x in opt.params]
+        change(opt)
+        with pytest.raises(L.PDError):
+            opt.step(g)
+        for x, y in zip(before[1:], opt.params[1:]):
+            assert x.shape != y.shape or torch.equal(x, y)
