@@ -178,14 +178,14 @@ class AdamW:
 
     def load_state_dict(self, state: dict) -> None:
         """Copies `state`, of an optimizer over parameters of the same sizes and bits, into this one's."""
-        pairs = []
-        for name, mine in self.state.items():
-            theirs = state.get(name)
-            mine, theirs = ([x] if x is None or isinstance(x, torch.Tensor) else list(x) for x in (mine, theirs))
+        pairs, none = [], [None] * len(self._sizes)
+        for name in ("step", "m", "v", "m_scale", "v_scale"):
+            mine, theirs = self.state.get(name), state.get(name)
+            mine, theirs = ([x] if isinstance(x, torch.Tensor) else list(x or none) for x in (mine, theirs))
             if len(mine) != len(theirs) or any((a is None) != (b is None) or
-                                               (a is not None and (a.dtype != b.dtype or a.shape != b.shape))
+                                               (a is not None and (a.dtype != b.dtype or a.numel() != b.numel()))
                                                for a, b in zip(mine, theirs)):
                 raise L.PDError(f"AdamW.load_state_dict: {name} is of other sizes or bits")
             pairs += [(a, b) for a, b in zip(mine, theirs) if a is not None]
         for a, b in pairs:
-            a.copy_(b)
+            a.copy_(b.reshape(a.shape))

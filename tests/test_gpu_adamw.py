@@ -363,3 +363,25 @@ def test_exchanged_tensors_are_checked(device):
             opt.step(g)
         for x, y in zip(before[1:], opt.params[1:]):
             assert x.shape != y.shape or torch.equal(x, y)
+
+
+def test_states_without_scales_travel(device):
+    """States of 32 bits may come without lists of scales and in any shape, and go to optimizers that have them flat."""
+    a, g = _tensors(device, [30, 40, 50], 11)
+    b = [x.clone() for x in a]
+    plain = dict(step=torch.zeros(1, dtype=torch.int32, device=device), m=[torch.zeros_like(x).view(5, -1) for x in a],
+                 v=[torch.zeros_like(x) for x in a])
+    one, two = AdamW(a, state=plain), AdamW(b)
+    one.step(g)
+    for x, y in zip(b, a):
+        x.copy_(y)
+    two.load_state_dict(one.state_dict())
+    one.step(g)
+    two.step(g)
+    one.load_state_dict(two.state_dict())
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    eight = AdamW([x.clone() for x in a], state_bits=8)
+    for opt, state in ((one, eight.state), (eight, one.state)):
+        with pytest.raises(L.PDError, match="sizes or bits"):
+            opt.load_state_dict(state)
