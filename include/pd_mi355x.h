@@ -749,8 +749,8 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
  *   loss [N] fp32 = logsumexp(z_i) - z_i[target_i], 0 where the target is ignore_index or lies
  *   outside [0, V): such positions do not count, and nothing that they hold reaches a result.
  * targets int32 or int64 [N] (target_bits). stats fp32 [N, 2] (nullable), for the backward: a row's
- * largest logit and its sum of e^(z - that). Products of bf16 operands accumulate in fp32 and
- * logits are not rounded.
+ * largest logit and the sum of e^(z - that) over its other logits, so that loss and 1 - p keep their digits
+ * where p is near 1. Products of bf16 operands accumulate in fp32 and logits are not rounded.
  * The backward gives d_act [N, d] and d_head [V, d] (in dtype, each nullable) of sum g_i loss_i, g
  * fp32 [N]: G = g (softmax(z) - 1_target), d_act = G head, d_head = G^T act, going over the vocabulary
  * in pieces of G of at most 1 GiB. With bf16 G enters both products rounded to bf16. Positions of

@@ -8,8 +8,8 @@
 // sum for every row and the target's logit, and a second kernel merges tiles in a fixed order; the
 // logits stay in registers. The backward goes over the vocabulary in pieces of which G (bf16) fits
 // CE_PIECE bytes of workspace: one product whose epilogue writes G, then both gradients from it.
-// The softmax is formed from the row's maximum and sum, kept apart: the log of the sum alone would
-// round a probability near one to 1e-6.
+// The softmax is formed from the row's maximum and the sum of the others relative to it, kept apart: the log of the sum
+// alone would round a probability near one to 1e-6, and a sum that holds the maximum's 1 what is one less it.
 //
 // Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep; fp32: the logits, EpiCEKeepF), 6 N d V in all: in one call
 // for weights known beforehand, or from the loss to its gradients (pd_streamed_ce_kept_*). bf16, loss and both gradients:
@@ -52,7 +52,7 @@ struct CETargets {
 };
 
 // rows[0 .. count) = the positions that count, in order; pos[i] = position i's place among them or
-// -1. With `loss` those that do not get loss 0 and, with `stats`, statistics (0, 1). One block.
+// -1. With `loss` those that do not get loss 0 and, with `stats`, statistics (0, 0). One block.
 __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* __restrict__ g, int64_t N,
                                                      int32_t* __restrict__ rows, int32_t* __restrict__ pos,
                                                      int32_t* __restrict__ count, float* __restrict__ loss,
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* _
       if (pos) pos[i] = on ? at : -1;
       if (loss && !on) {
         loss[i] = 0.f;
-        if (stats) stats[i] = make_float2(0.f, 1.f);
+        if (stats) stats[i] = make_float2(0.f, 0.f);
       }
     }
   }
@@ -137,14 +137,14 @@ __global__ __launch_bounds__(256) void k_ce_scatter(const float* __restrict__ pa
 
 __device__ inline float ce_exp(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
-// (maximum, sum relative to it) of two sets of columns; (-inf, 0) is none.
+// Of two sets of columns: (maximum m, sum of e^{z - m} less the maximum's own 1); (-inf, -1) is none.
 __device__ inline void ce_merge(float2& o, float2 q) {
-  const float m = fmaxf(o.x, q.x);
-  o.y = o.y * (o.x == m ? 1.f : expf(o.x - m)) + q.y * (q.x == m ? 1.f : expf(q.x - m));
-  o.x = m;
+  const bool first = o.x >= q.x;
+  const float2 hi = first ? o : q, lo = first ? q : o;
+  o = make_float2(hi.x, hi.y + (lo.y + 1.f) * (lo.x == hi.x ? 1.f : expf(lo.x - hi.x)));
 }
 
-// Forward epilogue: each row's maximum and sum over the tile's columns, to part[row][tile], and
+// Forward epilogue: each row's maximum and the others' sum over the tile's columns, to part[row][tile], and
 // the target's logit. A lane holds 16 columns of 32 in its row, its neighbour 32 lanes on the others.
 template <class CFG>
 struct EpiCEStats {
@@ -172,22 +172,23 @@ struct EpiCEStats {
 #pragma unroll
     for (int i = 0; i < CFG::TM; ++i) {
       const int rl = wm * CFG::WTM + i * 32 + (lane & 31);
-      float m, s;
-      row_stats<FULL>(p, a, t, t.m0 + rl, t.n0 + wn * CFG::WTN + 4 * (lane >> 5), z[i], m, s);
-      if (lane < 32) red[wn * CFG::BM + rl] = make_float2(m, s);
+      float m, r;
+      row_stats<FULL>(p, a, t, t.m0 + rl, t.n0 + wn * CFG::WTN + 4 * (lane >> 5), z[i], m, r);
+      if (lane < 32) red[wn * CFG::BM + rl] = make_float2(m, r);
     }
     lds_write_barrier();
     store(a, t, tid, red);
   }
-  // A row's maximum and sum over the wave's columns (`first`: the lane's first one); z becomes
-  // e^{z - m}, and the target's logit is kept.
+  // A row's maximum m and the others' sum r over the wave's columns (`first`: the lane's first one); z becomes
+  // e^{z - m}, and the target's logit is kept. r leaves the maximum's 1 out from the start: added to it, a rest below
+  // 2^-24 would be lost. Entries equal to 1 are counted by what their fractions lack of the sum.
   template <bool FULL>
   __device__ static void row_stats(const GemmArgs& p, const Args& a, const TileJob& t, int64_t row, int64_t first,
-                                   f32x16 (&z)[CFG::TN], float& m, float& s) {
+                                   f32x16 (&z)[CFG::TN], float& m, float& r) {
     int want = -1;  // the target's place in this lane's columns
     if (row < t.M) want = a.t.at(a.rows ? a.rows[row] : row);
     want = want < 0 ? -1 : want - (int)(a.first + first);
-    m = -INFINITY, s = 0.f;
+    m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < CFG::TN; ++j)
 #pragma unroll
@@ -199,6 +200,7 @@ struct EpiCEStats {
         }
       }
     m = fmaxf(m, __shfl_xor(m, 32, 64));
+    float s = 0.f, f = 0.f;
     if (m > -INFINITY) {  // columns there are, and numbers in them
 #pragma unroll
       for (int j = 0; j < CFG::TN; ++j)
@@ -206,12 +208,14 @@ struct EpiCEStats {
         for (int v = 0; v < 16; ++v) {
           const int c = j * 32 + 8 * (v >> 2) + (v & 3);
           z[j][v] = ce_exp(z[j][v] - m);
-          if (FULL || first + c < p.N) s += z[j][v];
+          if (FULL || first + c < p.N) s += z[j][v], f += __builtin_amdgcn_fractf(z[j][v]);
         }
     } else if (FULL || (first & ~(int64_t)7) < p.N) {
       s = NAN;  // NaN or -inf throughout: no softmax
     }
     s += __shfl_xor(s, 32, 64);
+    f += __shfl_xor(f, 32, 64);
+    r = f + (rintf(s - f) - 1.f);
   }
   __device__ static void store(const Args& a, const TileJob& t, int tid, const float2* red) {
     for (int r = tid; r < CFG::BM; r += CFG::NT) {
@@ -255,7 +259,7 @@ struct EpiCEGrad {
       const int rl = wm * CFG::WTM + i * 32 + (lane & 31);
       const int64_t row = t.m0 + rl, r = a.rows[row < t.M ? row : t.m0];
       const float2 st = a.stats[r];
-      const float g = a.g[r], gs = g / st.y;
+      const float gs = a.g[r] / (1.f + st.y);
       const int want = a.t.at(r) - (int)(a.first + t.n0) - (wn * CFG::WTN + 4 * (lane >> 5));
 #pragma unroll
       for (int j = 0; j < CFG::TN; ++j)
@@ -265,8 +269,8 @@ struct EpiCEGrad {
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            v[e] = ce_exp(z[i][j][4 * q + e] - st.x) * gs;
-            if (want == c + e) v[e] -= g;
+            const float x = ce_exp(z[i][j][4 * q + e] - st.x);
+            v[e] = (want == c + e ? (x - 1.f) - st.y : x) * gs;  // p - 1 from the others' sum: p may be near 1
             if (!FULL && t.n0 + wn * CFG::WTN + 4 * (lane >> 5) + c + e >= p.N) v[e] = 0.f;
           }
           *(uint2*)(smem + rl * RSB + (wn * CFG::WTN + c + 4 * (lane >> 5)) * 2) =
@@ -284,7 +288,7 @@ struct EpiCEGrad {
   }
 };
 
-// Epilogue of the one-call form: a row's maximum m and sum over each wave's CE_SPAN columns, and
+// Epilogue of the one-call form: a row's maximum m and the others' sum over each wave's CE_SPAN columns, and
 // 2^15 e^{z - m} in fp16: 11 bits down to 2^-29 of that maximum, 2^-39 at least. (One maximum for the
 // tile would have all its accumulators wait for the others': 66 of them spilled.)
 template <class CFG>
@@ -312,9 +316,9 @@ struct EpiCEKeep {
 #pragma unroll
     for (int i = 0; i < CFG::TM; ++i) {
       const int rl = wm * CFG::WTM + i * 32 + (lane & 31);
-      float m, s;
-      EpiCEStats<CFG>::template row_stats<FULL>(p, a.st, t, t.m0 + rl, first, z[i], m, s);
-      if (lane < 32) red[rl * CFG::WN + wn] = make_float2(m, s);
+      float m, r;
+      EpiCEStats<CFG>::template row_stats<FULL>(p, a.st, t, t.m0 + rl, first, z[i], m, r);
+      if (lane < 32) red[rl * CFG::WN + wn] = make_float2(m, r);
 #pragma unroll
       for (int j = 0; j < CFG::TN; ++j)
 #pragma unroll
@@ -352,15 +356,15 @@ __global__ __launch_bounds__(256) void k_ce_merge(const float2* __restrict__ par
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (count ? (int64_t)*count : N)) return;
-  float2 o = make_float2(-INFINITY, 0.f);
+  float2 o = make_float2(-INFINITY, -1.f);
   for (int64_t i = lane; i < n_tiles; i += 64) ce_merge(o, part[row * n_tiles + i]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) ce_merge(o, make_float2(__shfl_xor(o.x, off, 64), __shfl_xor(o.y, off, 64)));
   if (lane == 0) {
     const int64_t r = rows ? rows[row] : row;
     const bool on = t.at(r) >= 0;
-    loss[r] = on ? (o.x - target[row]) + logf(o.y) : 0.f;
-    if (stats) stats[r] = on ? o : make_float2(0.f, 1.f);
+    loss[r] = on ? (o.x - target[row]) + log1pf(o.y) : 0.f;
+    if (stats) stats[r] = on ? o : make_float2(0.f, 0.f);
     if (row_stats) row_stats[row] = o;
   }
 }
@@ -384,9 +388,8 @@ __global__ __launch_bounds__(256) void k_ce_apply(const uint16_t* E, uint16_t* G
   if (row >= *count) return;
   const int64_t r = rows[row], want = t.at(r);
   const float2 o = st[row];
-  const float gr = g[r], by = gr / o.y * 0x1p-15f;
-  // p - 1 at the target from the sum of the others: p may be near 1
-  const float hit = -gr * ((o.y - ce_exp(target[row] - o.x)) / o.y);
+  const float gr = g[r], gs = gr / (1.f + o.y), by = gs * 0x1p-15f;
+  const float hit = ((ce_exp(target[row] - o.x) - 1.f) - o.y) * gs;  // p - 1 from the others' sum: p may be near 1
   if (gr == 0.f && blockIdx.y == 0)
     for (int64_t c = threadIdx.x; c < words; c += 256) act[row * words + c] = make_uint4(0u, 0u, 0u, 0u);
   const uint16_t* e = E + row * ld;
@@ -448,7 +451,7 @@ struct EpiCEGradF {
       if (row >= t.M) continue;
       const int64_t r = a.rows[row];
       const float2 st = a.stats[r];
-      const float g = a.g[r], gs = g / st.y;
+      const float gs = a.g[r] / (1.f + st.y);
       const int64_t first = t.n0 + wn * CFG::WTN + 4 * (lane >> 5);
       const int want = a.t.at(r) - (int)(a.first + first);
 #pragma unroll
@@ -460,7 +463,7 @@ struct EpiCEGradF {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = expf(z[i][j][4 * q + e] - st.x);
-            v[e] = want == c + e ? -g * ((st.y - x) / st.y) : x * gs;
+            v[e] = (want == c + e ? (x - 1.f) - st.y : x) * gs;
           }
           float* dst = a.G + row * a.ldg + first + c;
           if (first + c + 3 < p.N) {
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256) void k_ce_apply_f32(const float* Z, float* G, 
   if (row >= *count) return;
   const int64_t r = rows[row], want = t.at(r);
   const float2 o = st[row];
-  const float gr = g[r], gs = gr / o.y;
+  const float gr = g[r], gs = gr / (1.f + o.y);
   if (gr == 0.f && blockIdx.y == 0)
     for (int64_t c = threadIdx.x; c < d; c += 256) act[row * d + c] = 0.f;
 #pragma unroll
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(256) void k_ce_apply_f32(const float* Z, float* G, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x = expf(v[e] - o.x);
-      v[e] = gr == 0.f ? 0.f : want == c + e ? -gr * ((o.y - x) / o.y) : x * gs;
+      v[e] = gr == 0.f ? 0.f : (want == c + e ? (x - 1.f) - o.y : x) * gs;
     }
     *(float4*)(G + row * ld + c) = make_float4(v[0], v[1], v[2], v[3]);
   }

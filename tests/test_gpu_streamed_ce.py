@@ -291,3 +291,61 @@ def test_refusals(device):
         ops.streamed_cross_entropy_kept_bwd(act, head, t, kept, w[:3])
     with pytest.raises(L.PDError, match="stats"):
         ops.streamed_cross_entropy_bwd(act, head, t, w, w)
+
+
+def _sure(device, V, dtype, N=64):
+    """Logits that bf16 holds: position i's are row i of head^T. 1 - p of the target from 0.5 to 10^-13, the target at
+    any place, entries of its tile and of others in the rest, two of them as large as the target in the last rows."""
+    g = torch.Generator(device=device).manual_seed(V)
+    z = (torch.randint(-16, 9, (N, V), device=device, generator=g) / 8.0)
+    t = torch.randperm(V, device=device, generator=g)[:N]
+    z[torch.arange(N, device=device), t] = torch.arange(N, device=device) / 2.0
+    # all of the rest in a single entry of the target's 64
+    few, col, other = torch.arange(N, device=device) % 4 == 3, torch.arange(V, device=device), torch.where((t ^ 1) < V, t ^ 1, t - 1)
+    z = torch.where(few[:, None] & (col != other[:, None]) & (col != t[:, None]), torch.full_like(z, -60.0), z)
+    z[-3, (t[-3] + 7) % V] = z[-3, t[-3]]
+    z[-2, (t[-2] + V // 2) % V] = z[-2, t[-2]]
+    return torch.eye(N, device=device).to(dtype), z.t().contiguous().to(dtype), t, z.double()
+
+
+@pytest.mark.parametrize("V", [65, 129, 640, 5000, 20000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_what_is_one_less_a_probability(device, V, dtype):
+    """The loss and the target's gradient relative to 1 - p. Logits are exact, e^x is off by |x| 2^-24 and a few roundings
+    of itself, sums by 2^-24 for each of their additions (a wave's 64 columns, then tiles); bf16 gradients by two
+    roundings more, d_head has one term."""
+    act, head, t, z = _sure(device, V, dtype)
+    N = 64
+    at = torch.arange(N, device=device)
+    w = torch.linspace(-2, 2, N, device=device)
+    w = torch.where(w == 0, torch.ones_like(w), w)
+    rest = torch.where(torch.arange(V, device=device) == t[:, None], torch.zeros_like(z),
+                       (z - z[at, t][:, None]).exp()).sum(-1)  # (1 - p) / p
+    loss, miss = torch.log1p(rest), rest / (1 + rest)
+    rel = (2 * (z.amax(-1) - z.amin(-1).clamp(min=-3)) + 128 + V / 64) * U
+    for got in _both_forms(act, head, t, w):
+        _check_sure(got[0], got[2], t, at, w, loss, miss, rel, dtype)
+
+
+def _check_sure(got, dh, t, at, w, loss, miss, rel, dtype):
+    assert ((got.double() - loss).abs() <= rel * loss + 2**-126).all(), float(((got.double() - loss).abs() / loss).max())
+    d = dh.double()[t, at]  # positions are columns of the identity: G at the target
+    bound = (rel + (2 * HALF[dtype] if dtype == BF16 else 0)) * miss * w.double().abs()
+    assert ((d + miss * w.double()).abs() <= bound + 2**-126).all(), float(((d / -w.double() - miss).abs() / miss).max())
+
+
+@pytest.mark.parametrize("dtype, N, V", [(BF16, 8200, 140000), (BF16, 2100, 300000), (F32, 4000, 80000)])
+def test_what_is_one_less_a_probability_in_pieces(device, dtype, N, V):
+    """The same where the backward forms the logits in pieces of the vocabulary, which may take other tiles: the positions of
+    the identity among others that have no gradient."""
+    few, head, t, z = _sure(device, V, dtype)
+    g = torch.Generator(device=device).manual_seed(N)
+    at, rows = torch.arange(64, device=device), torch.randperm(N, device=device, generator=g)[:64]
+    act = torch.randn(N, 64, device=device, generator=g).to(dtype)
+    targets = torch.randint(V, (N,), device=device, generator=g)
+    w = torch.zeros(N, device=device)
+    act[rows], targets[rows], w[rows] = few, t, torch.linspace(1, 2, 64, device=device)
+    rest = torch.where(torch.arange(V, device=device) == t[:, None], torch.zeros_like(z), (z - z[at, t][:, None]).exp()).sum(-1)
+    rel = (2 * (z.amax(-1) - z.amin(-1).clamp(min=-3)) + 128 + V / 64) * U
+    for got in _both_forms(act, head, targets, w):
+        _check_sure(got[0][rows], got[2], t, at, w[rows], torch.log1p(rest), rest / (1 + rest), rel, dtype)
