@@ -210,8 +210,15 @@ struct EpiCEStats {
           z[j][v] = ce_exp(z[j][v] - m);
           if (FULL || first + c < p.N) s += z[j][v], f += __builtin_amdgcn_fractf(z[j][v]);
         }
-    } else if (FULL || (first & ~(int64_t)7) < p.N) {
-      s = NAN;  // NaN or -inf throughout: no softmax
+    } else {  // no columns, or NaN and -inf throughout: -inf is no part of the sum, a NaN shows
+#pragma unroll
+      for (int j = 0; j < CFG::TN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int c = j * 32 + 8 * (v >> 2) + (v & 3);
+          z[j][v] = z[j][v] == -INFINITY ? 0.f : z[j][v];
+          if (FULL || first + c < p.N) s += z[j][v];
+        }
     }
     s += __shfl_xor(s, 32, 64);
     f += __shfl_xor(f, 32, 64);

@@ -349,3 +349,28 @@ def test_what_is_one_less_a_probability_in_pieces(device, dtype, N, V):
     rel = (2 * (z.amax(-1) - z.amin(-1).clamp(min=-3)) + 128 + V / 64) * U
     for got in _both_forms(act, head, targets, w):
         _check_sure(got[0][rows], got[2], t, at, w[rows], torch.log1p(rest), rest / (1 + rest), rel, dtype)
+
+
+@pytest.mark.parametrize("N, V", [(3, 200), (200, 3000)])
+def test_logits_that_leave_fp32_downwards_are_no_part_of_the_sum(device, N, V):
+    """Whole tiles of entries whose logits are -1e40: their probability is 0, in the loss and in both gradients."""
+    act, head, t, w = _inputs(device, N, 64, V, BF16, V)
+    act[:, 0], head[:, 0] = 1e20, 0
+    head[60:195, 0] = -1e20
+    t[:] = torch.where((t >= 60) & (t < 195), torch.full_like(t, 7), t)
+    # as without those entries
+    rest = torch.cat([head[:60], head[195:]])
+    want, bounds = _expected(act, rest, torch.where(t >= 195, t - 135, t), w)
+    for loss, da, dh in _both_forms(act, head, t, w):
+        assert not dh[60:195].any()
+        _check((loss, da, torch.cat([dh[:60], dh[195:]])), want, bounds)
+
+
+def test_a_row_of_nothing_but_such_logits_is_nan(device):
+    act, head, t, w = _inputs(device, 9, 64, 300, BF16, 3)
+    act[4], head[:, 0] = 0, -1e20
+    act[:, 0] = 0
+    act[4, 0] = 1e20
+    for got in _both_forms(act, head, t, w):
+        bad = torch.arange(9, device=device) == 4
+        assert torch.equal(torch.isnan(got[0]), bad) and torch.isnan(got[1][4]).all() and torch.isfinite(got[1][~bad]).all()
