@@ -812,7 +812,7 @@ int pd_adamw_step(int n_tensors, const int64_t* sizes, void* const* p, const voi
 
 /* ---- routing by scores ------------------------------------------------------------------
  * pd_router_topk's choice with scores of other kinds. logits [T, E] in `dtype` (bf16 or fp32),
- * E up to 1024. s = softmax(logits), or with `sigmoid` 1 / (1 + e^-logits); key = s + bias (fp32
+ * E up to 1024, T up to 2^26 - 4. s = softmax(logits), or with `sigmoid` 1 / (1 + e^-logits); key = s + bias (fp32
  * [E], nullable: it has a part in the choice alone). Of n_groups (up to 64) runs of E / n_groups
  * experts the top_groups best stay, by the sum of the two best keys; top_idx int32 [T, k] are
  * the k best keys of those (k up to 64), best first. Equal keys go to the lower index; keys are

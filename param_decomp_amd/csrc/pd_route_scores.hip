@@ -25,6 +25,7 @@ namespace pd {
 namespace {
 
 constexpr int RT_MAX_E = 1024, RT_MAX_K = 64, RT_MAX_GROUPS = 64;
+constexpr int64_t RT_MAX_T = (((int64_t)1 << 24) - 1) * 4;  // a launch has fewer than 2^32 threads; the widest rows are four to a block
 
 struct RtArgs {
   const void* x;
@@ -691,8 +692,8 @@ int rt_check(const char* what, int dtype, int64_t T, int E, int k, float scale) 
   if (dtype != PD_DTYPE_F32 && dtype != PD_DTYPE_BF16)
     return fail(PD_EUNSUPPORTED, std::string(what) + ": logits are fp32 or bf16");
   if (T < 0 || E < 1 || k < 1 || k > E) return fail(PD_EINVAL, std::string(what) + ": T >= 0 and 1 <= k <= E");
-  if (E > RT_MAX_E || k > RT_MAX_K || T >= ((int64_t)1 << 26))
-    return fail(PD_EUNSUPPORTED, std::string(what) + ": up to 1024 experts, 64 of them chosen, and 2^26 rows");
+  if (E > RT_MAX_E || k > RT_MAX_K || T > RT_MAX_T)
+    return fail(PD_EUNSUPPORTED, std::string(what) + ": up to 1024 experts, 64 of them chosen, and 2^26 - 4 rows");
   if (!std::isfinite(scale)) return fail(PD_EINVAL, std::string(what) + ": scale must be finite");
   return PD_OK;
 }

@@ -123,6 +123,15 @@ def test_route_scores_entry_points_refuse():
     assert f(*args(T=0)) == 0
 
 
+@needs_library
+def test_route_scores_entry_points_refuse_grids_that_a_launch_does_not_take():
+    b = np.zeros(64, np.float32).ctypes.data
+    lib, T = L.load(), (1 << 26) - 3
+    for E in (8, 300, 1024):
+        assert lib.pd_route_scores_fwd(b, 0, T, E, 2, 0, None, 1, 1, 1, 1.0, b, b, None) == 3
+        assert lib.pd_route_scores_bwd(b, 0, T, E, 2, 0, 1, 1.0, b, b, b, None) == 3
+
+
 X = torch.zeros(6, 8)
 
 
