@@ -649,7 +649,7 @@ __global__ __launch_bounds__(256) void k_rt_bwd(RtBwd a) {
     } else {
       c = expf(v - m) / total * g[r] * a.scale;
     }
-    d[e] += c;
+    atomicAdd(&d[e], c);  // a caller's row may hold an index twice
   }
   rt_wave_sync();
   T* out = (T*)a.dx + row * a.E;

@@ -263,3 +263,29 @@ def test_equal_scores_of_unequal_logits(device, dtype):
             x[1, places] = torch.tensor([b, a, b, a], device=device)
             for k in (1, 2, 3, 4, 6):
                 _check(device, x.to(dtype), k, **dict(kind, n_groups=groups, top_groups=2))
+
+
+@pytest.mark.parametrize("E, k", [(8, 2), (42, 8), (256, 8), (600, 40)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_of_an_index_that_a_row_holds_twice(device, E, k, dtype):
+    """A choice of the caller's own: what its places give is added."""
+    x = _x(device, 50, E, dtype, E)
+    g = torch.Generator(device=device).manual_seed(k)
+    at = torch.randint(E, (50, k), device=device, generator=g)
+    at[::2, 1] = at[::2, 0]
+    at[::4] = at[::4, :1]
+    dw = torch.randn(50, k, device=device, generator=g)
+    for sigmoid in (False, True):
+        for renorm in (False, True):
+            d = ops.route_scores_bwd(x, at.int(), dw, sigmoid=sigmoid, renormalize=renorm, scale=1.5)
+            y = x.double().requires_grad_()
+            s = torch.sigmoid(y) if sigmoid else torch.softmax(y, -1)
+            chosen = y.gather(1, at)  # renormalised from these alone: 64-bit roundings of the others are no gradient
+            c = torch.softmax(torch.nn.functional.logsigmoid(chosen) if sigmoid else chosen, -1) if renorm else s.gather(1, at)
+            (want,) = torch.autograd.grad(1.5 * c, y, dw.double())
+            # each place: 64 roundings of its two terms; k of them are added, and those of the row's sum with them
+            per = 1.5 * c.detach() * (dw.double().abs() + (c.detach() * dw.double().abs()).sum(-1, keepdim=True))
+            mag = torch.zeros_like(want).scatter_add(1, at, per) + s.detach() * per.sum(-1, keepdim=True) * (not renorm)
+            half = 2.0**-8 if dtype == torch.bfloat16 else U
+            bound = (64 + k) * U * mag + half * (want.abs() + (64 + k) * U * mag) + 1e-37
+            assert ((d.double() - want).abs() <= bound).all()
