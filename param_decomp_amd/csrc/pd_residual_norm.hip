@@ -29,7 +29,9 @@ namespace pd {
 namespace {
 
 constexpr int RN_MAX_D = 16384;  // largest row held in registers
-constexpr float RN_WIDE = 0x1p-80f;  // rows whose squares leave fp32 are squared again times this
+// Rows whose squares leave fp32 are squared again: those past its end times RN_WIDE, and times RN_NEAR those below
+// RN_LEAST, where squares are subnormal or nothing and eps does not hide it.
+constexpr float RN_WIDE = 0x1p-80f, RN_NEAR = 0x1p80f, RN_LEAST = 0x1p-90f;
 
 // 8 columns of a row as they are stored, loaded at any element's boundary (the hardware takes 16
 // bytes as one access).
@@ -168,16 +170,18 @@ __device__ inline float rn_rstd(const float (&u)[CH][8], float d, float eps, flo
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[0] = fmaf(u[c][e], u[c][e], s[0]);
   rn_sum<NT, 1>(s, part, tid);
-  if (s[0] != INFINITY) return 1.f / sqrtf(s[0] / d + eps);
-  s[0] = 0.f;  // the same way for the team's threads
+  const bool wide = s[0] == INFINITY;  // the same way for the team's threads
+  if (!wide && !(fmaf(eps, d, s[0]) < RN_LEAST)) return 1.f / sqrtf(s[0] / d + eps);
+  const float by = wide ? RN_WIDE : RN_NEAR;
+  s[0] = 0.f;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[0] = fmaf(u[c][e] * RN_WIDE, u[c][e] * RN_WIDE, s[0]);
+    for (int e = 0; e < 8; ++e) s[0] = fmaf(u[c][e] * by, u[c][e] * by, s[0]);
   if constexpr (NT > 64) __syncthreads();
   rn_sum<NT, 1>(s, part + NW, tid);
   if constexpr (NT > 64) __syncthreads();
-  return RN_WIDE / sqrtf(s[0] / d + eps * RN_WIDE * RN_WIDE);
+  return by / sqrtf(s[0] / d + eps * by * by);
 }
 
 // The same in 64 bits, from fp32 sums of two squares (each of bf16 values is exact): 1 neighbour of the right bf16 in
@@ -203,7 +207,7 @@ __device__ inline double rn_rstd_d(const float (&u)[CH][8], int d, float eps, do
     for (int i = 0; i < NT / 64; ++i) t += part[i];
   }
   // the same way for the team's threads
-  if (!(t < (double)__FLT_MAX__)) {
+  if (!(t < (double)__FLT_MAX__ && t + (double)eps * d >= (double)RN_LEAST)) {
     if constexpr (NT > 64) __syncthreads();
     return (double)rn_rstd<NT, CH>(u, (float)d, eps, part_f, tid);
   }

@@ -229,3 +229,34 @@ def test_refusals(device):
         kw = dict(dict(stats=st, d_stream=h, d_y=y), **bad)
         with pytest.raises(L.PDError):
             ops.residual_norm_bwd(h, c["branch"], kw["stats"], kw["d_stream"], kw["d_y"])
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("d", [8, 300, 768, 5000, 9000])
+@pytest.mark.parametrize("eps", [0.0, 1e-38])
+def test_rows_whose_squares_vanish(device, types, d, eps):
+    """Rows whose squares are below fp32's numbers, where eps does not hide them, beside ordinary ones."""
+    c = _case(device, 9, d, types, seed=d)
+    for r, e in ((1, -70), (2, -90), (3, -115), (5, -64)):
+        c["branch"][r] *= 2.0**e
+    for r, e in ((3, -100), (4, -80), (6, -66)):
+        c["x"][r] *= 2.0**e
+    c["post"][:] = 2.0**-60  # so that streams may be small too
+    c["branch"][6] *= 2.0**-70
+    h, y = residual_norm(c["x"], c["branch"], post_weight=c["post"], pre_weight=c["pre"], eps=eps)
+    b = c["branch"].double()
+    n = b * (b.square().mean(-1, keepdim=True) + eps).rsqrt() * c["post"].double()
+    _within("stream", h, c["x"].double() + n, c["x"].double().abs() + n.abs())
+    hs = h.double()
+    want = hs * (hs.square().mean(-1, keepdim=True) + eps).rsqrt() * c["pre"].double()
+    _within("y", y, want, want.abs())
+    for x in (c["x"], c["branch"].to(types[0])):
+        x, w, gy = x.clone().requires_grad_(), c["pre"].clone().requires_grad_(), c["gy"]
+        y = rms_norm(x, w, dtype=types[1], eps=eps)
+        X, W, GY = x.detach().double(), w.detach().double(), gy.double()
+        r = (X.square().mean(-1, keepdim=True) + eps).rsqrt()
+        xh, a = X * r, GY * W
+        _within("rms", y.detach(), xh * W, (xh * W).abs())
+        dx, dw = torch.autograd.grad(y, (x, w), gy)
+        _within("dx", dx, r * (a - xh * (a * xh).mean(-1, keepdim=True)), r * (a.abs() + xh.abs() * (a * xh).abs().mean(-1, keepdim=True)))
+        _within("dw", dw, (GY * xh).sum(0), (GY * xh).abs().sum(0), 9 + 64)
