@@ -731,20 +731,21 @@ struct CEBwdPlan {
 };
 // Tiles and slices of the contraction of d_act = G head (N x d over cw columns a piece): its few tiles
 // fill the chip only in slices, each of which leaves an fp32 slab to write and read. The rounds are
-// those of all positions and, with a quarter of the weight, of three quarters of them, since how many
-// count is not known here. us of 1 / 4 / 5 / 7 / 8 slices of 256x256 tiles: 8192 x 768 over 50277 columns 1466 /
-// 772 / 610 / 682 / 616 (128x128: 824 in 1, 724 in 4); three quarters of 4096 x 4096 over 131072 3921 / 3045 /
-// 3168 / 3446 / 3085, all 4096 3901 / 4009 / 4041 / 4089 / 4135.
+// those of all positions and, with a quarter of the weight, those where a part of them counts, which is not known here:
+// as many as its tiles fill and half a round for the last. us of 1 / 4 / 5 / 8 slices of 256x256 tiles, the slabs' sum with
+// them: 8192 x 768 over 50277 columns 1484 / 920 / 806 / 772, three fifths of it 1454 / 507 / 696 / 548 (8 are taken);
+// 4096 x 4096 over 131072 3952 / 4048 / 4096 / 4196, three quarters of it 3818 / 3169 / 3301 / 3288 (4 are).
 void ce_dact_form(int64_t N, int64_t d, int64_t cw, int64_t V, bool half, bool& big, int& splits) {
   double best = 1e30;
   for (int b = 0; b < (half ? 2 : 1); ++b)
     for (int sp = 1; sp <= 64 && (sp == 1 || cw / sp >= 1024); ++sp) {
       // 256x256 or two 128x128 a CU; fp32 one of 256x128 or 128x128
       const int64_t tm = half ? (b ? 256 : 128) : (N > 128 ? 256 : 128), tn = b ? 256 : 128, round = b || !half ? 256 : 512;
-      auto rounds = [&](int64_t rows) { return (double)tiles_up(tiles_up(rows, tm) * tiles_up(d, tn) * sp, round); };
+      const int64_t tiles = tiles_up(N, tm) * tiles_up(d, tn) * sp;
+      const double rounds = 0.75 * (double)tiles_up(tiles, round) + 0.25 * std::max(1.0, (double)tiles / (double)round + 0.5);
       const double per_round = 2.0 * tm * tn * round * ((double)V / sp) / (b ? 1.2e15 : half ? 1.0e15 : 1.7e14);
       const double slabs = (double)sp * N * d * 4 * 2 * cdiv(V, cw) / 4e12;
-      const double time = (0.75 * rounds(N) + 0.25 * rounds(cdiv(3 * N, 4))) * per_round + slabs;
+      const double time = rounds * per_round + slabs;
       if (time < best) best = time, big = b, splits = sp;
     }
 }
