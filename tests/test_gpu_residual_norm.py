@@ -260,3 +260,31 @@ def test_rows_whose_squares_vanish(device, types, d, eps):
         dx, dw = torch.autograd.grad(y, (x, w), gy)
         _within("dx", dx, r * (a - xh * (a * xh).mean(-1, keepdim=True)), r * (a.abs() + xh.abs() * (a * xh).abs().mean(-1, keepdim=True)))
         _within("dw", dw, (GY * xh).sum(0), (GY * xh).abs().sum(0), 9 + 64)
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [(20000, 768), (6001, 4096), (40, 16384), (100000, 33), (1, 1)])
+def test_rms_norm_of_many_and_of_wide_rows(device, types, shape):
+    g = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn(*shape, device=device, generator=g).to(types[0]).requires_grad_()
+    w = (1 + 0.2 * torch.randn(shape[1], device=device, generator=g)).requires_grad_()
+    gy = torch.randn(*shape, device=device, generator=g).to(types[1])
+    y = rms_norm(x, w, dtype=types[1], eps=EPS)
+    dx, dw = torch.autograd.grad(y, (x, w), gy)
+    X, W, GY = x.detach().double(), w.detach().double(), gy.double()
+    r = (X.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    xh, a = X * r, GY * W
+    _within("y", y.detach(), xh * W, (xh * W).abs())
+    _within("dx", dx, r * (a - xh * (a * xh).mean(-1, keepdim=True)), r * (a.abs() + xh.abs() * (a * xh).abs().mean(-1, keepdim=True)))
+    _within("dw", dw, (GY * xh).sum(0), (GY * xh).abs().sum(0), shape[0] + 64)
+
+
+@pytest.mark.parametrize("rows, d, gate", [(900, 8192, 3), (700, 5000, 700), (300, 9001, 1), (5000, 40, 5000)])
+def test_twice_the_same_in_other_plans(device, rows, d, gate):
+    c = _case(device, rows, d, (BF16, BF16), gate=gate)
+    kw = dict(post_weight=c["post"], gate=c["gate"], pre_weight=c["pre"])
+    h, _, st = ops.residual_norm_fwd(c["x"], c["branch"], want_stats=True, **kw)
+    first = ops.residual_norm_bwd(h, c["branch"], st, c["gh"], c["gy"], **kw)
+    for _ in range(3):
+        for a, b in zip(first, ops.residual_norm_bwd(h, c["branch"], st, c["gh"], c["gy"], **kw)):
+            assert torch.equal(a, b)

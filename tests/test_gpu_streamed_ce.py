@@ -374,3 +374,20 @@ def test_a_row_of_nothing_but_such_logits_is_nan(device):
     for got in _both_forms(act, head, t, w):
         bad = torch.arange(9, device=device) == 4
         assert torch.equal(torch.isnan(got[0]), bad) and torch.isnan(got[1][4]).all() and torch.isfinite(got[1][~bad]).all()
+
+
+@pytest.mark.parametrize("N, d, V", [(1024, 256, 20000), (1500, 1032, 20011), (3000, 264, 40000), (900, 2048, 12000)])
+def test_wide_activations_in_slices(device, N, d, V):
+    """Sums of d_act's slices of the vocabulary, in tiles of either size, whole and with an edge on every side."""
+    act, head, t, w = _inputs(device, N, d, V, BF16, N, 0.2)
+    want, bounds = _expected(act, head, t, w)
+    for got in _both_forms(act, head, t, w):
+        _check(got, want, bounds)
+
+
+def test_chunks_of_fp32_positions(device):
+    """More than 2 GiB of logits in the one-call form: the second chunk's d_head is added to the first's."""
+    act, head, t, w = _inputs(device, 7000, 24, 80000, F32, 15, 0.05)
+    want, bounds = _expected(act, head, t, w)
+    for got in _both_forms(act, head, t, w):
+        _check(got, want, bounds)
