@@ -744,7 +744,8 @@ int pd_top_kl(const void* z, int dtype, int64_t rows, int64_t vocab, const void*
               int idx_bits, int k, const float* clean_lse, double temperature, const float* row_weight, float* kl,
               void* grad, void* workspace, size_t workspace_bytes, void* stream);
 
-/* ---- cross entropy over a vocabulary whose logits are never kept ---------------------------
+/* ---- cross entropy over a vocabulary, logits formed in tiles -------------------------------
+ * pd_streamed_ce_fwd and _bwd keep no logits; _train and _kept_* keep a softmax (below).
  * z = act head^T with act [N, d] and head [V, d] in dtype (bf16 with d a multiple of 8, or fp32):
  *   loss [N] fp32 = logsumexp(z_i) - z_i[target_i], 0 where the target is ignore_index or lies
  *   outside [0, V): such positions do not count, and nothing that they hold reaches a result.
@@ -775,7 +776,8 @@ int pd_streamed_ce_train(int dtype, int64_t N, int64_t d, int64_t V, const void*
 
 /* The same in two calls, for weights g that come after the loss, as autograd's do: the first leaves the softmax in
  * `kept` (fp32: the logits; pd_streamed_ce_kept_size bytes, 0 where that or a bf16 head would take 2 GiB: the pair above is
- * for those), which the second reads and leaves as it is. The workspace is that of want_dact and want_dhead; the first call's of 0 and 0. */
+ * for those), which the second reads and leaves as it is: its workspace holds G, as large again. The workspace is that of want_dact
+ * and want_dhead; the first call's of 0 and 0. */
 size_t pd_streamed_ce_kept_size(int dtype, int64_t N, int64_t d, int64_t V);
 size_t pd_streamed_ce_kept_workspace_size(int dtype, int64_t N, int64_t d, int64_t V, int want_dact, int want_dhead);
 int pd_streamed_ce_kept_fwd(int dtype, int64_t N, int64_t d, int64_t V, const void* act, const void* head,

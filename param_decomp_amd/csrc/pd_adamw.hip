@@ -16,8 +16,8 @@
 // zero keeps the smallest code rather than zero, where the step m / (r + eps) would grow past
 // measure. The update itself uses m' and v' before rounding.
 //
-// Measured: 1.51 10^8 values in 48 tensors, fp32 states and copies, 888 us (5.1 TB/s); 2.64 10^8 in 24, 8-bit states,
-// bf16 gradients and copies, 886 us (4.8 TB/s); a large copy moves 4.84.
+// Measured: 1.51 10^8 values in 48 tensors, fp32 states and copies, 890 us (5.1 TB/s); 2.64 10^8 in 24, 8-bit states,
+// bf16 gradients and copies, 885-905 us (4.7-4.8 TB/s); a large copy moves 4.84.
 #include <algorithm>
 #include <cmath>
 

@@ -19,7 +19,8 @@
 //
 // Measured at 6 10^7 values, both streams and branch (bf16 and bf16; fp32 and fp32), a gate a sequence: forward
 // 106-110 us and 199-224 us from 64 to 4096 columns (4.4-4.8 TB/s; 768 in bf16 123 us, a quarter of its lanes idle and the sums
-// in 64 bits shown), backward with all gradients 156-164 us and 300-325 us (4.4-4.8 TB/s).
+// in 64 bits shown), backward with all gradients 156-164 us and 300-325 us (4.4-4.8 TB/s). Without a branch: forward 47-48 us
+// (768: 61) and 103-115, backward 82-89 us (768: 104) and 152-161 (4.1-5.1 TB/s; 768 in bf16 3.5-3.9).
 #include <algorithm>
 #include <type_traits>
 

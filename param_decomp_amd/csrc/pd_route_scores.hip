@@ -15,7 +15,7 @@
 // exact in 32 bits, and for bf16 logits the word holds the whole index, so equal logits need no second look.
 // Bound by the rounds' vector instructions rather than by memory: several rows share a wave. Measured: 131072 x 128, 8
 // chosen by softmax, fp32: forward 48 us (70 with words compared one by one and every close row chosen again; reading
-// the logits is 14), backward 27 (4.9 TB/s); 8192 x 256, sigmoid with bias, 4 of 8 groups, bf16: 28 and 8.4.
+// the logits is 14), backward 28 (4.8 TB/s); 8192 x 256, sigmoid with bias, 4 of 8 groups, bf16: 28 and 8.4.
 #include <algorithm>
 #include <cmath>
 

@@ -1,4 +1,5 @@
-// Softmax cross entropy over a vocabulary whose logits are never kept, and its gradients.
+// Softmax cross entropy over a vocabulary, from activations and head, and its gradients. The loss keeps no logits;
+// its gradients form them again, or take what a loss kept for them.
 //
 //   z = act head^T, loss_i = log(sum_v e^{z_iv}) - z_i,t_i
 //   G = g (softmax(z) - 1_t), d_act = G head, d_head = G^T act
@@ -11,11 +12,12 @@
 // The softmax is formed from the row's maximum and the sum of the others relative to it, kept apart: the log of the sum
 // alone would round a probability near one to 1e-6, and a sum that holds the maximum's 1 what is one less it.
 //
-// Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep; fp32: the logits, EpiCEKeepF), 6 N d V in all: in one call
-// for weights known beforehand, or from the loss to its gradients (pd_streamed_ce_kept_*). bf16, loss and both gradients:
-// 8192 x 768 over 50277 2874 us with the logits formed again, 2663 kept (product and epilogue 820, apply 360, d_act 683,
-// d_head 719); three quarters of 4096 x 4096 over 131072 11.7 and 9.0 ms (2735, 300, 2990, 2940: 1.12 PFLOP/s).
-// fp32, 903 of 1003 x 1000 over 32003: 1530 us formed again, 1161 kept (product 427, apply 39, d_act 413, d_head 398).
+// Where a chunk of positions' softmax fits CE_KEPT it is kept in 16 bits instead (EpiCEKeep; fp32: the logits, EpiCEKeepF), 6 N d V
+// in all: in one call for weights known beforehand, where G takes its place, or from the loss to its gradients (pd_streamed_ce_kept_*),
+// where G is as large again. bf16, loss and both gradients: 8192 x 768 over 50277 2790 us with the logits formed again (1.1 GB beside
+// inputs), 2590 kept (2.0 GB; product and epilogue 835, apply 360, d_act 662 and its slabs' sum 36, d_head 713); three quarters of
+// 4096 x 4096 over 131072 11.1 and 8.9 ms (2700, 300, 2900, 2900: 1.14 PFLOP/s).
+// fp32, 903 of 1003 x 1000 over 32003: 1515 us formed again, 1190 kept (product 423, apply 39, d_act 421, d_head 393).
 //
 // Positions whose target lies outside the vocabulary do not count (nor, backward, those of weight
 // zero): their rows are left out of a dense copy of the activations, so they cost no products and
@@ -52,7 +54,7 @@ struct CETargets {
 };
 
 // rows[0 .. count) = the positions that count, in order; pos[i] = position i's place among them or
-// -1. With `loss` those that do not get loss 0 and, with `stats`, statistics (0, 0). One block.
+// -1. With `loss` those that do not get loss 0 and, with `stats`, statistics (0, 0). One block, about 1 us for 1024 positions.
 __global__ __launch_bounds__(1024) void k_ce_compact(CETargets t, const float* __restrict__ g, int64_t N,
                                                      int32_t* __restrict__ rows, int32_t* __restrict__ pos,
                                                      int32_t* __restrict__ count, float* __restrict__ loss,
@@ -803,7 +805,6 @@ CEOnePlan ce_one_plan(int dtype, int64_t N, int64_t d, int64_t V, bool dact, boo
   const size_t esz = P.half ? 2 : 4;
   P.ld = ce_pitch(V);
   P.R = std::min<int64_t>(N, std::max<int64_t>(256, (int64_t)(CE_KEPT / ((size_t)P.ld * esz)) - 128) & ~(int64_t)255);
-  if (P.R <= 0) P.R = N;
   P.chunks = (int)cdiv(N, P.R);
   P.big = P.half && ce_big(P.R, V);
   P.n_tiles = tiles_up(V, P.half ? CE_SPAN : 128);

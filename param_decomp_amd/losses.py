@@ -366,16 +366,19 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def streamed_position_cross_entropy(act: torch.Tensor, head: torch.Tensor, targets: torch.Tensor, *,
                                     ignore_index: int = -100, keep: bool = True) -> torch.Tensor:
-    """Per-position cross entropy of the logits `act @ head^T` against `targets`, without writing the
-    logits: what `streamed_position_kl` is to a teacher's distribution. act [..., d], head [V, d] (one
+    """Per-position cross entropy of the logits `act @ head^T` against `targets`, formed in tiles: what
+    `streamed_position_kl` is to a teacher's distribution. act [..., d], head [V, d] (one
     dtype, bf16 or fp32), targets int32 or int64 [...]. A position whose target is `ignore_index` or
     lies outside [0, V) has loss 0, no gradient and no part in the products. Returns fp32 [...];
     differentiable in act and head, once: gradients in their dtype (bf16: from softmax differences rounded to bf16).
 
-    The softmax is kept in 16 bits (fp32: the logits) for the backward where it takes less than 2 GiB, 2 or 4 bytes for each
-    position and entry of the vocabulary (0.8 GB for bf16, 8192 over 50277), as has to a bf16 head; else, and with `keep`
-    False, the backward forms the logits again over pieces of the vocabulary, half as much again of its products. `ops.streamed_cross_entropy` gives loss and weighted
-    gradients in one call."""
+    Without gradients no logits are kept. With them the default keeps the softmax in 16 bits (fp32: the logits) from
+    the loss to the backward where that takes less than 2 GiB (as has to a bf16 head): 2 or 4 bytes for each position and entry of
+    the vocabulary, and as much again while the backward runs; losses that wait for one backward hold theirs each. `keep`
+    False is the form for memory, and what larger ones take: statistics alone are kept and the backward forms the logits again
+    over pieces of the vocabulary of at most 1 GiB, half as much again of its products (8192 of 768 over 50277 in bf16, loss and
+    both gradients: 2.0 GB beside the inputs and 2.6 ms kept, 1.1 GB and 2.8 ms not). A bf16 d that is no multiple of 8 costs a
+    padded copy of act and head. `ops.streamed_cross_entropy` gives loss and weighted gradients in one call."""
     lead, d = act.shape[:-1], act.shape[-1] if act.dim() else 0
     pad = (-d) % 8 if act.dtype == torch.bfloat16 else 0
     if pad:  # zero columns add nothing to the logits; their gradients are cut off

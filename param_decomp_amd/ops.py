@@ -754,7 +754,8 @@ def streamed_cross_entropy_kept_fwd(act, head, targets, *, ignore_index: int = -
 
 def streamed_cross_entropy_kept_bwd(act, head, targets, kept, g, *, ignore_index: int = -100, want_dact: bool = True,
                                     want_dhead: bool = True):
-    """(d_act, d_head) of sum g_i loss_i from what the forward kept, g fp32 [N]; None for those not wanted."""
+    """(d_act, d_head) of sum g_i loss_i from what the forward kept, g fp32 [N]; None for those not wanted. The
+    workspace is as large as kept again."""
     name = "streamed_cross_entropy_kept_bwd"
     device, sizes = _ce_checks(name, act, head, targets)
     N = act.shape[0]
