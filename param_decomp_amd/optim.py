@@ -83,7 +83,7 @@ class AdamW:
         arrays = [L.host_array(ctypes.c_void_p, where[k * n:(k + 1) * n]) for k in range(6)]
         self._p, self._m, self._v, self._ms, self._vs, self._c = arrays
         self._shapes = [p.shape for p in self.params]
-        self._written = self.params + [c for c in self.copies or () if c is not None]
+        self._written = [*self.params, *(c for c in self.copies or () if c is not None)]
         self._held, self._at, self._at_sizes = held, at, sizes
         # the memory is kept, so that nothing else can come to lie at an address that was checked
         self._memory = [t.detach() for t in live]

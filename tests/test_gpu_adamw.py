@@ -385,3 +385,13 @@ def test_states_without_scales_travel(device):
     for opt, state in ((one, eight.state), (eight, one.state)):
         with pytest.raises(L.PDError, match="sizes or bits"):
             opt.load_state_dict(state)
+
+
+def test_parameters_and_copies_may_become_tuples(device):
+    a, g = _tensors(device, [30, 40], 12)
+    opt = AdamW(a, copies=[None, torch.empty(40, dtype=torch.bfloat16, device=device)])
+    opt.params, opt.copies, opt.state = tuple(x.clone() for x in a), tuple(opt.copies), dict(opt.state, m=tuple(opt.state["m"]))
+    before = [x.clone() for x in a]
+    opt.step(g)
+    assert all(torch.equal(x, y) for x, y in zip(a, before)) and not any(torch.equal(x, y) for x, y in zip(a, opt.params))
+    assert torch.equal(opt.copies[1], opt.params[1].bfloat16())
