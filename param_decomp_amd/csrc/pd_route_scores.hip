@@ -495,16 +495,19 @@ __global__ __launch_bounds__(256, J > 8 ? 4 : 8) void k_rt_fwd(RtArgs a) {
   uint32_t live = 0;  // whether one is not masked
   if (a.sigmoid) {
     float sum = 0.f;
+    uint32_t faint = 0;  // a score that leaves fp32, whose weight may not
     for (int r = lane; r < a.k; r += NT) {
       const int e = chosen(r);
       const float s = 1.f / (1.f + expf(-xs[e]));
       won[r] = make_uint2(__float_as_uint(s), (uint32_t)e);
       sum += s;
+      faint |= s < 0x1p-100f && xs[e] != -INFINITY;
     }
     float by = a.scale;
     if (a.renorm) {
       sum = rt_add<NT>(sum);
-      if (sum < 0x1p-60f) {  // the same for the team: scores that may have left fp32, by their logarithms
+      faint = rt_fold<NT>(faint, [](uint32_t p, uint32_t q) { return p | q; });
+      if (sum < 0x1p-60f || faint) {  // the same for the team: by their logarithms
         float lmax = -INFINITY, total = 0.f;
         for (int r = lane; r < a.k; r += NT) {
           const float v = xs[won[r].y], l = fminf(v, 0.f) - log1pf(expf(-fabsf(v)));

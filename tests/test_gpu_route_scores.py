@@ -289,3 +289,18 @@ def test_gradients_of_an_index_that_a_row_holds_twice(device, E, k, dtype):
             half = 2.0**-8 if dtype == torch.bfloat16 else U
             bound = (64 + k) * U * mag + half * (want.abs() + (64 + k) * U * mag) + 1e-37
             assert ((d.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_of_sigmoids_that_leave_fp32_beside_others(device, dtype):
+    """Scores below fp32 whose share of the chosen ones' sum is not, beside masked experts. A logarithm is off by a few
+    2^-24 of itself, and a weight by as much: 110 is the largest here."""
+    x = torch.full((6, 24), -INF, device=device)
+    for r, v in enumerate(([-33.75, -89.5], [-40.0, -90.0, -102.5], [-13.5, -95.0, -88.0], [-99.5, -26.875], [-31.75, -101.0, -31.0], [-60.0, -110.0])):
+        x[r, 7:7 + 5 * len(v):5] = torch.tensor(v, device=device)
+    x = x.to(dtype)
+    for k in (2, 3, 8):
+        w, idx = experts.route_scores(x, k, scoring="sigmoid", scale=1.5)
+        want, at = _expected(x, k, scoring="sigmoid", scale=1.5)
+        assert torch.equal(idx.long(), at) and (want[:, :2] > 1e-37).all()
+        assert ((w.double() - want).abs() <= (64 + 2 * 110) * U * want).all()
